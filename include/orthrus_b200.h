@@ -462,6 +462,33 @@ int orthrus_decode_sample_accept(const float* cand_vals, const int64_t* cand_ids
  * check of the decode's generator. */
 int orthrus_philox4x32_10(const uint32_t* counter_key, int64_t n, uint32_t* out, void* stream);
 
+/* ---- row operators over vocabulary logits ------------------------------------------------ */
+/* Rows are `logits` [R, V] in `dtype` at a pitch of ldl elements (any alignment; rows may overlap or
+ * repeat), V up to 389,000 for fp32 and 778,000 for bf16 (a row lives in the shared memory of eight
+ * SMs); ORTHRUS_EINVAL beyond. Entries that are -inf or NaN are no candidates. Entries are ordered
+ * by descending value, then ascending index; -0 counts as +0. */
+
+/* The k largest candidates of each row (1 <= k <= 1024): values [R, k] fp32 and ids [R, k] in
+ * order, (-inf, -1) past the last candidate, and lse [R] = log(sum exp(x / temperature)) over the
+ * candidates (-inf without any, +inf if one is +inf). temperature > 0. */
+int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
+                      float* values, int64_t* ids, float* lse, int dtype, void* stream);
+
+/* One token per row from its filtered softmax and the row's uniform in [0, 1). With
+ * w_i = exp((x_i - max x) / temperature), kept are the candidates at least as large as the top_k-th
+ * largest (ties kept; top_k < 1 or at least their number: all); of these the ones whose
+ * predecessors in the order above hold at most top_p of their total weight (top_p >= 1: all; the
+ * first always); and of these the ones with w_i >= min_p. The token is the first kept index at
+ * which the running sum of kept weights, in index order, exceeds uniform * total. A uniform below 0
+ * or NaN counts as 0, one of 1 or more picks the last kept token of positive weight. A temperature
+ * below 1e-5 gives the row's first maximum; a row without candidates gives -1. Sums are exact
+ * (integer weights of at least 42 fractional bits), so the token depends on the row and its knobs
+ * alone. Each knob is a device array [R], or NULL and the value beside it for every row. */
+int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
+                          const float* temperature, float temperature1, const int32_t* top_k,
+                          int top_k1, const float* top_p, float top_p1, const float* min_p,
+                          float min_p1, int64_t* tokens, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@
 #include "qkv_prep.cuh"
 #include "rowwise.cuh"
 #include "selftest.cuh"
+#include "vocab_rows.cuh"
 
 using namespace orthrus;
 
@@ -909,6 +910,41 @@ extern "C" int orthrus_swiglu_bwd(const void* gate_up, const void* dout, int64_t
     return ORTHRUS_EINVAL;
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Row operators over vocabulary logits
+// ------------------------------------------------------------------------------------------------
+
+extern "C" int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
+                                 float* values, int64_t* ids, float* lse, int dtype, void* stream) {
+  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V < (1ll << 31) && ldl >= 0 && k >= 1 && k <= kRowMaxK && temperature > 0.f);
+  if (R == 0) return ORTHRUS_OK;
+  ORTHRUS_CHECK_ARG(logits && values && ids && lse);
+  if (dtype == ORTHRUS_F32)
+    return topk_rows_impl(static_cast<const float*>(logits), ldl, R, V, k, temperature, values, ids, lse,
+                          as_stream(stream));
+  if (dtype == ORTHRUS_BF16)
+    return topk_rows_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, k, temperature, values, ids, lse,
+                          as_stream(stream));
+  return ORTHRUS_EINVAL;
+}
+
+extern "C" int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
+                                     const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                                     const float* top_p, float top_p1, const float* min_p, float min_p1,
+                                     int64_t* tokens, int dtype, void* stream) {
+  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V < (1ll << 31) && ldl >= 0);
+  if (R == 0) return ORTHRUS_OK;
+  ORTHRUS_CHECK_ARG(logits && uniform && tokens);
+  const SampleKnobs knobs{temperature, top_k, top_p, min_p, temperature1, top_p1, min_p1, top_k1};
+  if (dtype == ORTHRUS_F32)
+    return sample_logits_impl(static_cast<const float*>(logits), ldl, R, V, uniform, knobs, tokens,
+                              as_stream(stream));
+  if (dtype == ORTHRUS_BF16)
+    return sample_logits_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, uniform, knobs, tokens,
+                              as_stream(stream));
+  return ORTHRUS_EINVAL;
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -47,18 +47,21 @@ inline std::atomic<unsigned long long>& launch_counter() {
     ORTHRUS_CHECK_CUDA(cudaGetLastError());                                     \
   } while (0)
 
-// Opts a kernel into `bytes` of dynamic shared memory once per process and kernel (the attribute
+// Opts a kernel into `bytes` of dynamic shared memory once per device and kernel (the attribute
 // persists; repeating it on every launch would also add a driver call inside stream capture).
 template <typename Kern>
 inline cudaError_t ensure_smem(Kern kernel, int bytes) {
   static std::mutex mu;
-  static std::unordered_map<const void*, int> done;
+  static std::unordered_map<const void*, std::unordered_map<int, int>> done;  // kernel -> device -> bytes
   const void* key = reinterpret_cast<const void*>(kernel);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(mu);
-  auto it = done.find(key);
-  if (it != done.end() && it->second >= bytes) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) done[key] = bytes;
+  int& have = done[key][dev];
+  if (have >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) have = bytes;
   return e;
 }
 

@@ -3,7 +3,9 @@ pointers and the current stream, check the status. No computation happens in Pyt
 
 from __future__ import annotations
 
+import math
 from collections import defaultdict
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -672,6 +674,86 @@ def philox4x32_10(counter_key: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# --- row operators over vocabulary logits --------------------------------------------------------
+
+TOPK_ROWS_MAX_K = 1024
+
+
+def _vocab_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(R, V, row pitch) of 2-D logits whose rows are contiguous."""
+    _require_cuda(logits)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{what} takes logits [R, V] with V >= 1 (got {tuple(logits.shape)})")
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError(f"{what} takes logits with contiguous rows")
+    return logits.shape[0], logits.shape[1], logits.stride(0)
+
+
+def _on_device(device: torch.device):
+    """Makes `device` the current one for the call (kernels launch on the current device)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
+    """The k largest logits of each row [R, V] (fp32 or bf16, rows contiguous at any pitch):
+    (values fp32 [R, k] descending, ids int64 [R, k], lse fp32 [R] = logsumexp(row / temperature)).
+    Among equal values the lower index comes first. -inf and NaN are no candidates; a row with fewer
+    than k of them is padded with (-inf, -1). 1 <= k <= 1024."""
+    R, V, pitch = _vocab_rows(logits, "topk_rows")
+    if not 1 <= k <= TOPK_ROWS_MAX_K:
+        raise ValueError(f"topk_rows takes 1 <= k <= {TOPK_ROWS_MAX_K} (got {k})")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"topk_rows takes a finite temperature > 0 (got {temperature})")
+    code, dev = L.dtype_code(logits.dtype), logits.device
+    values = torch.empty(R, k, dtype=torch.float32, device=dev)
+    ids = torch.empty(R, k, dtype=torch.int64, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        L.check(L.lib().orthrus_topk_rows(logits.data_ptr(), pitch, R, V, k, float(temperature), values.data_ptr(),
+                                          ids.data_ptr(), lse.data_ptr(), code, L.stream_of(dev)), "topk_rows")
+    return values, ids, lse
+
+
+def _knob(value, name: str, rows: int, device, dtype, low, high):
+    """(per-row tensor or None, scalar) of one sampling knob; scalars are checked here, per-row
+    values on the device as orthrus_sample_logits says."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (rows,) or value.device != device:
+            raise ValueError(f"{name} must be a number or a tensor [{rows}] on {device}")
+        return value.to(dtype).contiguous(), low
+    if not low <= value <= high or (name == "top_p" and value == 0):
+        raise ValueError(f"{name} = {value} is out of range")
+    return None, value
+
+
+def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> torch.Tensor:
+    """One token per row of logits [R, V] (fp32 or bf16, rows contiguous at any pitch), int64 [R], from
+    the uniforms fp32 [R] in [0, 1): the inverse of the filtered softmax's running sum in index order.
+
+    The filters, in turn: top_k keeps the entries at least as large as the k-th largest (0: off);
+    top_p the smallest descending prefix whose probability exceeds it (1: off); min_p the entries
+    at least min_p times as probable as the largest (0: off). Each knob is a number or a tensor [R].
+    A temperature of 0 (below 1e-5) is greedy. -inf and NaN logits are never drawn; a row of
+    nothing else gives -1. The sums are exact, so a row's token depends on neither the other rows
+    nor the launch."""
+    R, V, pitch = _vocab_rows(logits, "sample_logits")
+    code, dev = L.dtype_code(logits.dtype), logits.device
+    if uniforms.shape != (R,) or uniforms.dtype != torch.float32 or uniforms.device != dev:
+        raise ValueError(f"uniforms must be fp32 [{R}] on {dev}")
+    uniforms = uniforms.contiguous()
+    t, t1 = _knob(temperature, "temperature", R, dev, torch.float32, 0.0, 3e38)
+    k, k1 = _knob(top_k, "top_k", R, dev, torch.int32, 0, 2 ** 31 - 1)
+    p, p1 = _knob(top_p, "top_p", R, dev, torch.float32, 0.0, 1.0)
+    m, m1 = _knob(min_p, "min_p", R, dev, torch.float32, 0.0, 1.0)
+    tokens = torch.empty(R, dtype=torch.int64, device=dev)
+    with _on_device(dev):
+        L.check(L.lib().orthrus_sample_logits(logits.data_ptr(), pitch, R, V, uniforms.data_ptr(), L.ptr(t), t1,
+                                              L.ptr(k), int(k1), L.ptr(p), p1, L.ptr(m), m1, tokens.data_ptr(), code,
+                                              L.stream_of(dev)), "sample_logits")
+    return tokens
+
+
 # --- row-local elementwise pieces ---------------------------------------------------------------
 
 
@@ -805,5 +887,7 @@ for _name, _label, _work in (
         ("silu_mul_backward", "swiglu_bwd", None),
         ("lmhead_kl_backward", "lmhead_kl_bwd_scale", None),
         ("add", "add", None),
+        ("topk_rows", "topk_rows", None),
+        ("sample_logits", "sample_logits", None),
         ("rope_table", "rope_table", None)):
     globals()[_name] = _timed(globals()[_name], _label, _work)
