@@ -361,6 +361,31 @@ int orthrus_lmhead_kl_fwd(const void* student, int64_t n, const void* teacher, i
 int orthrus_lmhead_kl_bwd(const void* grad, const float* grad_total, void* grad_student,
                           int64_t count, int dtype, void* stream);
 
+/* Distillation from a teacher's top logits through the LM head. Per student row r with teacher row
+ * t = index[r] (index NULL: t = r) and its kept logits (values[t, j], ids[t, j]), j < k <= 1024:
+ *   q_j = softmax over the kept values / temperature, or exp(value_j / temperature - teacher_lse[t])
+ *   p = softmax(weight student[r] / temperature) over all V entries
+ *   kl_rows[r] = sum_j q_j (log q_j - log p[id_j]);  total = sum_r row_weight[r] kl_rows[r];
+ *   grad[r] = (row_weight[r] / temperature) ((sum_j q_j) p - q) weight, the gradient of total;
+ *   agree[r] = 1 when the student's first largest logit is at the id of the first largest value.
+ * Entries with id < 0 or value -inf are padding; a row of padding has kl 0 and gradient 0. An id or
+ * index out of range sets ORTHRUS_ERR_BOUNDS in the device error word and counts as padding; an id
+ * kept twice counts with its whole mass. student [n, d], weight [V, d], grad [n, d] (NULL: not
+ * computed) in dtype, bf16 with d a multiple of 8 and 16-byte alignment; values, teacher_lse and
+ * row_weight fp32, ids and index int64; row_weight, teacher_lse and offsets may be NULL. total and
+ * the per-offset sums as orthrus_lmhead_kl_fwd. The probabilities of chunk_rows rows at a time live
+ * in the workspace. orthrus_lmhead_kl_bwd scales grad by the gradient of total. */
+size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t chunk_rows,
+                                              int dtype);
+int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values,
+                               const int64_t* ids, int64_t m, int k, const int64_t* index,
+                               const float* teacher_lse, const void* weight, int64_t V, int64_t d,
+                               float temperature, const float* row_weight, const int64_t* offsets,
+                               int num_offsets, float* total, float* kl_rows, uint8_t* agree,
+                               void* grad, float* kl_by_offset, int64_t* agree_by_offset,
+                               int64_t chunk_rows, void* workspace, size_t workspace_bytes, int dtype,
+                               void* stream);
+
 /* ---- parallel block decoding ----------------------------------------------------------- */
 /* Row-wise argmax of fp32 logits [R, V] (lowest index on ties, as torch.argmax), R rows at
  * row pitch ldl: out[r] int64. */

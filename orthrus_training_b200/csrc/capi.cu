@@ -18,6 +18,7 @@
 #include "linear_tc.cuh"
 #include "linear_skinny.cuh"
 #include "lmhead_kl.cuh"
+#include "lmhead_topk_kl.cuh"
 #include "qkv_prep.cuh"
 #include "rowwise.cuh"
 #include "selftest.cuh"
@@ -944,6 +945,32 @@ extern "C" int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R,
   if (dtype == ORTHRUS_BF16)
     return sample_logits_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, uniform, knobs, tokens,
                               as_stream(stream));
+  return ORTHRUS_EINVAL;
+}
+
+extern "C" size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t chunk_rows,
+                                                         int dtype) {
+  return topk_kl_plan(n, V, d, chunk_rows, dtype).total;
+}
+
+extern "C" int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values, const int64_t* ids,
+                                          int64_t m, int k, const int64_t* index, const float* teacher_lse,
+                                          const void* weight, int64_t V, int64_t d, float temperature,
+                                          const float* row_weight, const int64_t* offsets, int num_offsets,
+                                          float* total, float* kl_rows, uint8_t* agree, void* grad,
+                                          float* kl_by_offset, int64_t* agree_by_offset, int64_t chunk_rows,
+                                          void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  if (dtype == ORTHRUS_BF16)
+    return lmhead_topk_kl_fwd_impl(static_cast<const __nv_bfloat16*>(student), n, values, ids, m, k, index,
+                                   teacher_lse, static_cast<const __nv_bfloat16*>(weight), V, d, temperature,
+                                   row_weight, offsets, num_offsets, total, kl_rows, agree,
+                                   static_cast<__nv_bfloat16*>(grad), kl_by_offset, agree_by_offset, chunk_rows,
+                                   workspace, workspace_bytes, as_stream(stream));
+  if (dtype == ORTHRUS_F32)
+    return lmhead_topk_kl_fwd_impl(static_cast<const float*>(student), n, values, ids, m, k, index, teacher_lse,
+                                   static_cast<const float*>(weight), V, d, temperature, row_weight, offsets,
+                                   num_offsets, total, kl_rows, agree, static_cast<float*>(grad), kl_by_offset,
+                                   agree_by_offset, chunk_rows, workspace, workspace_bytes, as_stream(stream));
   return ORTHRUS_EINVAL;
 }
 

@@ -556,6 +556,65 @@ class FusedLinearForwardKL:
         return _FusedKL.apply(student, teacher, index, weight, chunk_size, row_weight, None, 0)
 
 
+class _FusedTopKKL(torch.autograd.Function):
+    """LM head + KL to a teacher's top logits, per-offset statistics; gradient computed in the forward."""
+
+    @staticmethod
+    def forward(ctx, student, values, ids, index, weight, chunk_size, row_weight, offsets, num_offsets,
+                temperature, teacher_lse):
+        total, kl_rows, agree, grad, kbo, abo = ops.lmhead_topk_kl(
+            student, values, ids, index, weight, row_weight, offsets, num_offsets, temperature, teacher_lse,
+            need_grad=ctx.needs_input_grad[0], chunk_rows=max(int(chunk_size), 128))
+        ctx.save_for_backward(grad)
+        outs = [kl_rows, agree] + ([kbo, abo] if offsets is not None else [])
+        ctx.mark_non_differentiable(*outs)
+        return (total, *outs)
+
+    @staticmethod
+    def backward(ctx, grad_total, *unused):
+        (grad,) = ctx.saved_tensors
+        return (None if grad is None else ops.lmhead_kl_backward(grad, grad_total),) + (None,) * 10
+
+
+class FusedLinearTopKKL:
+    """FusedLinearForwardKL against a teacher of which only the top logits are kept: sum_r w_r
+    sum_j q_j (log q_j - log softmax(W student[r] / temperature)[ids_j]) over the kept entries
+    values, ids [m, k] of teacher row index[r] (index None: row r; id -1 or value -inf: padding).
+    q is the softmax of the kept values / temperature, or with teacher_lse [m], the log-sum-exp of
+    the teacher's whole row / temperature, the teacher's own probabilities, whose sum falls short
+    of 1 by what was not kept. teacher_top_logits gives all three. Returns (total, kl_rows, agree),
+    total differentiable w.r.t. the student rows (the LM head is frozen). The chunk_size rows whose
+    probabilities are held at a time cost 2 V bytes each for bf16, 4 V for fp32."""
+
+    @staticmethod
+    def apply(student, values, ids, index, weight, chunk_size, row_weight=None, temperature=1.0,
+              teacher_lse=None):
+        return _FusedTopKKL.apply(student, values, ids, index, weight, chunk_size, row_weight, None, 0,
+                                  temperature, teacher_lse)
+
+
+@torch.no_grad()
+def teacher_top_logits(hidden: torch.Tensor, weight: torch.Tensor, k: int, temperature: float = 1.0,
+                       chunk_rows: int = 1024):
+    """What FusedLinearTopKKL keeps of a teacher: the k largest logits of hidden [m, d] @ weight
+    [V, d]^T per row with their ids and the row's log-sum-exp at the temperature (values fp32 and
+    ids int64 [m, k], lse fp32 [m]; ops.topk_rows), the fp32 logits of chunk_rows rows at a time."""
+    m, V = hidden.shape[0], weight.shape[0]
+    values = torch.empty(m, k, dtype=torch.float32, device=hidden.device)
+    ids = torch.empty(m, k, dtype=torch.int64, device=hidden.device)
+    lse = torch.empty(m, dtype=torch.float32, device=hidden.device)
+    pad = (-hidden.shape[1]) % 8
+    hidden, weight = (F.pad(t, (0, pad)) if pad else t.contiguous() for t in (hidden, weight))
+    rows = min(max(int(chunk_rows), 1), max(m, 1))
+    logits = torch.empty(rows, V + (-V) % 8, dtype=torch.float32, device=hidden.device)[:, :V]
+    with torch.cuda.device(hidden.device):
+        for r in range(0, m, rows):
+            part = logits[: min(rows, m - r)]
+            ops.gemm(hidden[r : r + rows], weight, out_dtype=torch.float32, out=part)
+            values[r : r + rows], ids[r : r + rows], lse[r : r + rows] = ops.topk_rows(part, k, temperature)
+    return values, ids, lse
+
+
 class SupervisedLayout:
     """The supervised block positions of a batch, settled before the forward: kept (row, anchor,
     offset) indices ordered by their unique target position, the gather indices of the student
@@ -587,13 +646,14 @@ def orthrus_loss(model: OrthrusLM, input_ids: torch.Tensor, assistant_mask: torc
                  anchors: torch.Tensor, valid: torch.Tensor, kl_chunk_size: int,
                  compiled: bool = False, kernel_options: dict | None = None, gamma: float = 0.0, *,
                  teacher: TeacherPass | None = None, layout: SupervisedLayout | None = None,
-                 document_mask: bool = False):
+                 document_mask: bool = False, teacher_topk: int = 0):
     """Mean (or position-weighted mean) forward KL over supervised block positions and its
     statistics (orthrus/objective.py:395-453). `teacher` (teacher_pass) and `layout`
     (SupervisedLayout) may be prepared by the caller: the training step queues the teacher first
     and settles the layout's host reads on a side stream meanwhile. `document_mask` (off, as in
     the reference) keeps attention inside each packed conversation (document_starts); a prepared
-    teacher carries its own choice."""
+    teacher carries its own choice. `teacher_topk` (0, as in the reference: the whole vocabulary)
+    distils from the teacher's top logits only, renormalised (FusedLinearTopKKL)."""
     K = model.config.block_size
     # The supervised rows depend on the inputs only. Their layout is settled before the forward is
     # queued, so its host reads (the kept-row and unique-target counts, bincount's size) happen
@@ -607,16 +667,17 @@ def orthrus_loss(model: OrthrusLM, input_ids: torch.Tensor, assistant_mask: torc
                                     teacher=teacher, doc_start=doc_start)
     hidden = student.shape[-1]
     row_weight = layout.row_weight
-    total, kl_rows, agree, kl_by_offset, agree_by_offset = _FusedKL.apply(
-        student.reshape(-1, hidden).index_select(0, layout.student_rows),
-        teacher.flatten(0, 1)[layout.positions].to(student.dtype),
-        layout.index,
-        model.lm_head.weight,
-        kl_chunk_size,
-        row_weight,
-        layout.offsets,
-        K - 1,
-    )
+    student_rows = student.reshape(-1, hidden).index_select(0, layout.student_rows)
+    teacher_rows = teacher.flatten(0, 1)[layout.positions].to(student.dtype)
+    if teacher_topk:
+        values, ids, _ = teacher_top_logits(teacher_rows, model.lm_head.weight, teacher_topk)
+        total, kl_rows, agree, kl_by_offset, agree_by_offset = _FusedTopKKL.apply(
+            student_rows, values, ids, layout.index, model.lm_head.weight, kl_chunk_size, row_weight,
+            layout.offsets, K - 1, 1.0, None)
+    else:
+        total, kl_rows, agree, kl_by_offset, agree_by_offset = _FusedKL.apply(
+            student_rows, teacher_rows, layout.index, model.lm_head.weight, kl_chunk_size, row_weight,
+            layout.offsets, K - 1)
     count = layout.count
     norm = row_weight.sum() if row_weight is not None else count.float()
     stats = {

@@ -55,6 +55,11 @@ def _workspace(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
 
 
+def _on_device(device: torch.device):
+    """Makes `device` the current one for the call (kernels launch on the current device)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def gemm(a: torch.Tensor, b: torch.Tensor, *, b_kn: bool = False, out_dtype=None,
          out: torch.Tensor | None = None) -> torch.Tensor:
     """a [M, K] @ (b [N, K])^T (or a @ b for b [K, N] with b_kn). bf16 inputs run on tcgen05 tensor
@@ -320,6 +325,78 @@ def lmhead_kl_backward(grad: torch.Tensor, grad_total: torch.Tensor) -> torch.Te
                                           grad.numel(), L.dtype_code(grad.dtype),
                                           L.stream_of(grad.device)), "lmhead_kl_bwd")
     return out
+
+
+LMHEAD_TOPK_MAX_K = 1024
+
+
+def _kernel_operand(t: torch.Tensor, pad: int = 0) -> torch.Tensor:
+    """t contiguous on a 16-byte boundary, its last dimension padded with zeros."""
+    if pad:
+        return torch.nn.functional.pad(t, (0, pad))
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets=None, num_offsets=0,
+                   temperature=1.0, teacher_lse=None, need_grad=True, chunk_rows=4096):
+    """Distillation from a teacher's top logits through the LM head: sum_r w_r sum_j q_j (log q_j -
+    log p[id_j]) with q = softmax of the kept logits values / temperature [m, k] of teacher row
+    index[r] (index None: row r), or exp(values / temperature - teacher_lse) with the teacher's own
+    log-sum-exp fp32 [m], and p = softmax(student[r] @ weight^T / temperature). Entries with id -1 or
+    value -inf are padding. Returns what lmhead_kl returns: (total, kl_rows, agree, grad,
+    kl_by_offset, agree_by_offset)."""
+    _require_cuda(student, values, ids, index, weight, row_weight, offsets, teacher_lse)
+    code, dev = L.dtype_code(student.dtype), student.device
+    if weight.dtype != student.dtype:
+        raise ValueError("student and weight must share a dtype")
+    if student.dim() != 2 or weight.dim() != 2 or student.shape[1] != weight.shape[1]:
+        raise ValueError(f"lmhead_topk_kl takes student [n, d] and weight [V, d]; got {tuple(student.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if values.dim() != 2 or values.shape != ids.shape or not 1 <= values.shape[1] <= LMHEAD_TOPK_MAX_K:
+        raise ValueError(f"values and ids must be [m, k] with 1 <= k <= {LMHEAD_TOPK_MAX_K}; got "
+                         f"{tuple(values.shape)} and {tuple(ids.shape)}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"lmhead_topk_kl takes a finite temperature > 0 (got {temperature})")
+    (n, d), (m, k), V = student.shape, values.shape, weight.shape[0]
+    if (index.shape != (n,)) if index is not None else n > m:
+        raise ValueError("index must name a teacher row per student row")
+    for name, t, size in (("row_weight", row_weight, n), ("offsets", offsets, n), ("teacher_lse", teacher_lse, m)):
+        if t is not None and t.shape != (size,):
+            raise ValueError(f"{name} must be [{size}]")
+    for t in (values, ids, index, weight, row_weight, offsets, teacher_lse):
+        if t is not None and t.device != dev:
+            raise ValueError("lmhead_topk_kl takes tensors of one device")
+    pad = (-d) % 8 if student.dtype == torch.bfloat16 else 0  # TMA rows are multiples of 16 bytes
+    student, weight = _kernel_operand(student, pad), _kernel_operand(weight, pad)
+    values, ids = values.to(torch.float32).contiguous(), ids.to(torch.int64).contiguous()
+    index = None if index is None else index.to(torch.int64).contiguous()
+    row_weight = None if row_weight is None else row_weight.to(torch.float32).contiguous()
+    teacher_lse = None if teacher_lse is None else teacher_lse.to(torch.float32).contiguous()
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    kl_rows = torch.empty(n, dtype=torch.float32, device=dev)
+    agree = torch.empty(n, dtype=torch.uint8, device=dev)
+    grad = torch.empty(n, d + pad, dtype=student.dtype, device=dev) if need_grad else None
+    kbo = abo = None
+    if offsets is not None:
+        offsets = offsets.to(torch.int64).contiguous()
+        kbo = torch.empty(num_offsets, dtype=torch.float32, device=dev)
+        abo = torch.empty(num_offsets, dtype=torch.int64, device=dev)
+    lib = L.lib()
+    with _on_device(dev):
+        ws = torch.empty(max(lib.orthrus_lmhead_topk_kl_workspace_bytes(n, V, d + pad, chunk_rows, code), 1),
+                         dtype=torch.uint8, device=dev)
+        t0 = TIMER.begin() if TIMER is not None else None
+        L.check(lib.orthrus_lmhead_topk_kl_fwd(
+            L.ptr(student), n, L.ptr(values), L.ptr(ids), m, k, L.ptr(index), L.ptr(teacher_lse), L.ptr(weight), V,
+            d + pad, float(temperature), L.ptr(row_weight), L.ptr(offsets), int(num_offsets), L.ptr(total),
+            L.ptr(kl_rows), L.ptr(agree), L.ptr(grad), L.ptr(kbo), L.ptr(abo), chunk_rows, L.ptr(ws), ws.numel(), code,
+            L.stream_of(dev)), "lmhead_topk_kl_fwd")
+        if t0 is not None:  # student logits + grad GEMM
+            TIMER.end("lmhead_topk_kl", t0, 2.0 * d * V * n * (2 if need_grad else 1))
+    if grad is not None and pad:
+        grad = grad[:, :d]
+    return total, kl_rows, agree.bool(), grad, kbo, abo
 
 
 # --- q/k norm + RoPE ---------------------------------------------------------------------------
@@ -687,11 +764,6 @@ def _vocab_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int]:
     if logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError(f"{what} takes logits with contiguous rows")
     return logits.shape[0], logits.shape[1], logits.stride(0)
-
-
-def _on_device(device: torch.device):
-    """Makes `device` the current one for the call (kernels launch on the current device)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):

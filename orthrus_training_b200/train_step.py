@@ -160,7 +160,7 @@ class Trainer:
                  warmup_ratio=0.05, min_lr_ratio=0.1, max_grad_norm=1.0, num_anchors=32,
                  kl_chunk_size=4096, gamma=0.0, seed=42, world=1, rank=0, group=None,
                  check_device_every=50, monitor: PeerMonitor | None = None,
-                 document_mask: bool = False, layers_per_bucket: int = 4):
+                 document_mask: bool = False, layers_per_bucket: int = 4, teacher_topk: int = 0):
         from orthrus_training_b200.modeling_orthrus import freeze_to_diffusion
 
         self.model = model
@@ -191,6 +191,8 @@ class Trainer:
         # attention kept inside each packed conversation (objective.document_starts); off, as in
         # the reference, whose rows attend across conversation boundaries
         self.document_mask = document_mask
+        # distillation from this many of the teacher's top logits (0, as in the reference: from all)
+        self.teacher_topk = teacher_topk
 
     def _prepare(self, model, ids, mask, rng, ready):
         """Queues the teacher pass (it needs the input ids only) and draws the anchors and
@@ -247,7 +249,8 @@ class Trainer:
             rng = anchor_rng(self.seed, epoch, index, device=ids.device)
             anchors, valid, teacher, layout = self._prepare(model, ids, mask, rng, ready)
             loss, stats = orthrus_loss(model, ids, mask, anchors, valid, self.kl_chunk_size,
-                                       gamma=self.gamma, teacher=teacher, layout=layout)
+                                       gamma=self.gamma, teacher=teacher, layout=layout,
+                                       teacher_topk=self.teacher_topk)
             (loss / accum).backward()
             losses.append(loss.detach())
         self.buckets.wait()

@@ -48,3 +48,30 @@ def test_sample_logits_status(bad):
     f = ctypes.c_float
     assert _lib().lib().orthrus_sample_logits(a["p"], a["ld"], a["R"], a["V"], a["p"], None, f(1), None, 0, None, f(1),
                                               None, f(0), a["p"], a["dtype"], None) == _lib().EINVAL
+
+
+def test_distillation_refuses_cpu_tensors():
+    from orthrus_training_b200 import ops
+
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError):
+        ops.lmhead_topk_kl(x, x, x.long(), None, x)
+
+
+GOOD = dict(student=64, n=4, values=64, ids=64, m=4, k=2, index=64, lse=None, weight=64, V=10, d=8, T=1.0, total=64,
+            kl=64, agree=64, grad=64, offsets=None, num=0, ws=64, ws_bytes=1 << 40, dtype=0)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(n=-1), "EINVAL"), (dict(V=0), "EINVAL"), (dict(d=0), "EINVAL"), (dict(d=12), "EINVAL"), (dict(k=0), "EINVAL"),
+    (dict(k=1025), "EINVAL"), (dict(T=0.0), "EINVAL"), (dict(T=float("nan")), "EINVAL"), (dict(m=0), "EINVAL"),
+    (dict(index=None, m=3), "EINVAL"), (dict(student=None), "EINVAL"), (dict(weight=None), "EINVAL"),
+    (dict(values=None), "EINVAL"), (dict(student=72), "EINVAL"), (dict(offsets=64), "EINVAL"), (dict(dtype=3), "EINVAL"),
+    (dict(n=2 ** 31), "EINVAL"), (dict(ws=None), "EWORKSPACE"), (dict(ws_bytes=16), "EWORKSPACE")])
+def test_distillation_status(bad, status):
+    a = dict(GOOD, **bad)
+    got = _lib().lib().orthrus_lmhead_topk_kl_fwd(
+        a["student"], a["n"], a["values"], a["ids"], a["m"], a["k"], a["index"], a["lse"], a["weight"], a["V"], a["d"],
+        ctypes.c_float(a["T"]), None, a["offsets"], a["num"], a["total"], a["kl"], a["agree"], a["grad"], None, None,
+        4096, a["ws"], a["ws_bytes"], a["dtype"], None)
+    assert got == getattr(_lib(), status)
