@@ -375,8 +375,8 @@ int orthrus_lmhead_kl_bwd(const void* grad, const float* grad_total, void* grad_
  * row_weight fp32, ids and index int64; row_weight, teacher_lse and offsets may be NULL. total and
  * the per-offset sums as orthrus_lmhead_kl_fwd. The probabilities of chunk_rows rows at a time live
  * in the workspace. orthrus_lmhead_kl_bwd scales grad by the gradient of total. */
-size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t chunk_rows,
-                                              int dtype);
+size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,
+                                              int64_t chunk_rows, int dtype);
 int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values,
                                const int64_t* ids, int64_t m, int k, const int64_t* index,
                                const float* teacher_lse, const void* weight, int64_t V, int64_t d,

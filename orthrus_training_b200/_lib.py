@@ -100,7 +100,7 @@ _SIGNATURES = {
     "orthrus_decode_draft_ids": (c_int, [_P, c_int64, c_int, _P, _P, _P, _P]),
     "orthrus_decode_accept_ids": (c_int, [_P, c_int64, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, c_int64,
                                           _P, _P, c_int64, _P]),
-    "orthrus_lmhead_topk_kl_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int]),
+    "orthrus_lmhead_topk_kl_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int64, c_int]),
     "orthrus_lmhead_topk_kl_fwd": (c_int, [_P, c_int64, _P, _P, c_int64, c_int, _P, _P, _P, c_int64, c_int64,
                                            c_float, _P, _P, c_int, _P, _P, _P, _P, _P, _P, c_int64, _P, c_size_t,
                                            c_int, _P]),

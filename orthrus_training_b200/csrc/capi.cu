@@ -948,9 +948,9 @@ extern "C" int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R,
   return ORTHRUS_EINVAL;
 }
 
-extern "C" size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t chunk_rows,
-                                                         int dtype) {
-  return topk_kl_plan(n, V, d, chunk_rows, dtype).total;
+extern "C" size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,
+                                                         int64_t chunk_rows, int dtype) {
+  return topk_kl_plan(n, m, V, d, k, chunk_rows, dtype).total;
 }
 
 extern "C" int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values, const int64_t* ids,
@@ -960,17 +960,16 @@ extern "C" int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const 
                                           float* total, float* kl_rows, uint8_t* agree, void* grad,
                                           float* kl_by_offset, int64_t* agree_by_offset, int64_t chunk_rows,
                                           void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  const TopkKlCall call{n, m, k, values, ids, index, teacher_lse, row_weight, V, d, temperature, kl_rows, agree};
   if (dtype == ORTHRUS_BF16)
-    return lmhead_topk_kl_fwd_impl(static_cast<const __nv_bfloat16*>(student), n, values, ids, m, k, index,
-                                   teacher_lse, static_cast<const __nv_bfloat16*>(weight), V, d, temperature,
-                                   row_weight, offsets, num_offsets, total, kl_rows, agree,
+    return lmhead_topk_kl_fwd_impl(static_cast<const __nv_bfloat16*>(student),
+                                   static_cast<const __nv_bfloat16*>(weight), call, offsets, num_offsets, total,
                                    static_cast<__nv_bfloat16*>(grad), kl_by_offset, agree_by_offset, chunk_rows,
                                    workspace, workspace_bytes, as_stream(stream));
   if (dtype == ORTHRUS_F32)
-    return lmhead_topk_kl_fwd_impl(static_cast<const float*>(student), n, values, ids, m, k, index, teacher_lse,
-                                   static_cast<const float*>(weight), V, d, temperature, row_weight, offsets,
-                                   num_offsets, total, kl_rows, agree, static_cast<float*>(grad), kl_by_offset,
-                                   agree_by_offset, chunk_rows, workspace, workspace_bytes, as_stream(stream));
+    return lmhead_topk_kl_fwd_impl(static_cast<const float*>(student), static_cast<const float*>(weight), call, offsets,
+                                   num_offsets, total, static_cast<float*>(grad), kl_by_offset, agree_by_offset,
+                                   chunk_rows, workspace, workspace_bytes, as_stream(stream));
   return ORTHRUS_EINVAL;
 }
 

@@ -15,7 +15,8 @@
 // Epilogues: store (bf16); residual (bf16 R + acc, one rounding: torch.addmm(R, x, W^T)); and the
 // SwiGLU backward, where acc = dact = dy @ W_down of the MLP and R = [gate | up] [M, 2N] kept by the
 // forward: the epilogue writes C = [dgate | dup] [M, 2N] (the arithmetic and roundings of
-// swiglu_bwd_kernel), so dact never goes through HBM.
+// swiglu_bwd_kernel), so dact never goes through HBM. Row scale: C = s[row] * acc with fp32 factors
+// s [M] (passed in place of R), one rounding (the LM-head gradient of lmhead_topk_kl.cuh).
 //
 // Persistent: one cluster per SM pair loops over pair tiles (n fastest). 320 threads per CTA:
 //   warp 0     TMA producer (both CTAs): this CTA's A and B k-blocks of 64 into a 6-stage ring;
@@ -33,7 +34,7 @@
 
 namespace orthrus {
 
-enum Gemm2Epilogue { kGemm2Store = 0, kGemm2Residual = 1, kGemm2Partial = 2, kGemm2SwiGLUBwd = 3 };
+enum Gemm2Epilogue { kGemm2Store = 0, kGemm2Residual = 1, kGemm2Partial = 2, kGemm2SwiGLUBwd = 3, kGemm2RowScale = 4 };
 
 struct Gemm2Base {
   static constexpr int BM = 128;                  // rows per CTA (256 per pair)
@@ -382,6 +383,11 @@ __global__ void __launch_bounds__(Gemm2Base::THREADS, 1)
           float v[32];
           tmem_ld32(base + c * 32, v);
           tmem_wait_ld();
+          if constexpr (EPI == kGemm2RowScale) {
+            const float f = row < g.M ? reinterpret_cast<const float*>(R)[row] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= f;
+          }
           if constexpr (EPI == kGemm2Residual) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -447,6 +453,31 @@ __global__ void gemm2_reduce_kernel(const float* __restrict__ part, int splits, 
     __nv_bfloat16* c = C + m * ldc + n;
     *reinterpret_cast<__nv_bfloat162*>(c) = __floats2bfloat162_rn(acc.x, acc.y);
     *reinterpret_cast<__nv_bfloat162*>(c + 2) = __floats2bfloat162_rn(acc.z, acc.w);
+  }
+}
+
+// C = bf16(scale[row] * sum over splits of the fp32 partials, in split order): one rounding.
+__global__ void gemm2_reduce_scaled_kernel(const float* __restrict__ part, int splits, int64_t m_pad, int M, int N,
+                                           const float* __restrict__ scale, __nv_bfloat16* __restrict__ C, int64_t ldc) {
+  const int64_t groups = static_cast<int64_t>(M) * (N / 4);
+  griddep_launch_dependents();  // launched as a programmatic dependent
+  griddep_wait();
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < groups;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t m = i / (N / 4);
+    const int n = static_cast<int>(i % (N / 4)) * 4;
+    float4 acc = *reinterpret_cast<const float4*>(part + m * N + n);
+    for (int sp = 1; sp < splits; ++sp) {
+      const float4 p = *reinterpret_cast<const float4*>(part + (sp * m_pad + m) * N + n);
+      acc.x += p.x;
+      acc.y += p.y;
+      acc.z += p.z;
+      acc.w += p.w;
+    }
+    const float f = scale[m];
+    __nv_bfloat16* c = C + m * ldc + n;
+    *reinterpret_cast<__nv_bfloat162*>(c) = __floats2bfloat162_rn(f * acc.x, f * acc.y);
+    *reinterpret_cast<__nv_bfloat162*>(c + 2) = __floats2bfloat162_rn(f * acc.z, f * acc.w);
   }
 }
 
@@ -595,6 +626,68 @@ inline int gemm2_bf16_impl(const void* A, int64_t lda, int a_mn, const void* B, 
     case 5: return gemm2_launch<kGemm2Residual, false, true>(ta, tb, tc, tr, g, r, ldr, stream);
     default: return ORTHRUS_EINVAL;  // a residual needs A in its row-major form
   }
+}
+
+// k-splits of the row-scaled product, with a few tiles (the hidden size over 256 columns) and a long
+// K (the vocabulary): the count up to 16 with the least modelled time, the MMA work at 1.4 PF/s over
+// the share of the cluster waves that the units fill plus the fp32 partials' round trip at 5 TB/s.
+// 7936 x 1024 x 151936: 124 tiles are 1.68 waves of 74 clusters; in 7 splits they are 11.7 waves.
+inline int gemm2_rowscale_splits(int64_t M, int64_t N, int64_t K, int clusters) {
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256), kb = ceil_div(K, 64);
+  auto modelled = [&](int64_t s) {
+    const int64_t units = tiles * s;
+    const double fill = static_cast<double>(units) / static_cast<double>(ceil_div(units, clusters) * clusters);
+    return 2.0 * ceil_div(M, 256) * 256 * ceil_div(N, 256) * 256 * K / 1.4e15 / fill +
+           (s > 1 ? 8.0 * s * M * N / 5e12 + 3e-6 : 0.0);
+  };
+  int best = 1;
+  for (int s = 2; s <= 16 && kb / s >= 16; ++s)
+    if (modelled(s) < modelled(best)) best = s;
+  return best;
+}
+
+inline size_t gemm2_rowscale_ws_bytes(int64_t M, int64_t N, int64_t K) {
+  const int s = gemm2_rowscale_splits(M, N, K, num_sms() / 2);
+  return s > 1 ? static_cast<size_t>(s) * ceil_div(M, 256) * 256 * N * 4 : 0;
+}
+
+// C[M, N] = scale[m] * (A[M, K] @ B[K, N]) in bf16, one rounding; A pitch lda, B and C pitch N, all
+// 16-byte aligned with lda and N multiples of 8.
+inline int gemm2_rowscale_impl(const __nv_bfloat16* A, int64_t lda, const __nv_bfloat16* B, __nv_bfloat16* C,
+                               const float* scale, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes,
+                               cudaStream_t stream) {
+  ORTHRUS_CHECK_ARG(lda % 8 == 0 && N % 8 == 0 && lda >= K && M >= 1 && M < (1ll << 31) && N < (1ll << 30));
+  ORTHRUS_CHECK_ARG(aligned16(A) && aligned16(B) && aligned16(C));
+  CUtensorMap ta, tb, tc, tr{};
+  if (!make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128) || !make_tmap_2d_bf16(&tb, B, N, K, N, 64, 64)) return ORTHRUS_ECUDA;
+  Gemm2Geometry g;
+  g.M = static_cast<int>(M);
+  g.N = static_cast<int>(N);
+  g.K = static_cast<int>(K);
+  g.npairs = static_cast<int>(ceil_div(N, 256));
+  g.splits = gemm2_rowscale_splits(M, N, K, num_sms() / 2);
+  g.kb_split = static_cast<int>(ceil_div(ceil_div(K, 64), g.splits));
+  g.splits = static_cast<int>(ceil_div(ceil_div(K, 64), g.kb_split));  // none of them empty
+  g.m_pad = static_cast<int>(ceil_div(M, 256) * 256);
+  const int64_t tiles = ceil_div(M, 256) * g.npairs * g.splits;
+  ORTHRUS_CHECK_ARG(tiles < (1ll << 31));
+  g.tiles = static_cast<int>(tiles);
+  if (g.splits == 1) {
+    if (!make_tmap_2d_bf16(&tc, C, N, M, N, 64, 32)) return ORTHRUS_ECUDA;
+    return gemm2_launch<kGemm2RowScale, false, true>(ta, tb, tc, tr, g, reinterpret_cast<const __nv_bfloat16*>(scale), 0,
+                                                     stream);
+  }
+  if (ws == nullptr || ws_bytes < static_cast<size_t>(g.splits) * g.m_pad * N * 4) return ORTHRUS_EWORKSPACE;
+  float* part = static_cast<float*>(ws);
+  if (!make_tmap_2d_f32(&tc, part, N, static_cast<uint64_t>(g.splits) * g.m_pad, N, 32, 32)) return ORTHRUS_ECUDA;
+  const int rc = gemm2_launch<kGemm2Partial, false, true>(ta, tb, tc, tr, g, nullptr, 0, stream);
+  if (rc != ORTHRUS_OK) return rc;
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(M * (N / 4), 256), num_sms() * 8));
+  ORTHRUS_CHECK_CUDA(launch_pdl(gemm2_reduce_scaled_kernel, dim3(blocks), dim3(256), 0, stream,
+                                static_cast<const float*>(part), g.splits, static_cast<int64_t>(g.m_pad), g.M, g.N,
+                                scale, C, N));
+  ORTHRUS_CHECK_LAUNCH();
+  return ORTHRUS_OK;
 }
 
 }  // namespace orthrus

@@ -7,20 +7,41 @@
 //   d total / dh = (w / T) (Q p - q) W                Q = sum_j q_j
 //
 // The student's normaliser needs every logit, so forward and gradient are two products of
-// [n, d] x [d, V]; the teacher costs its k entries per row.
+// [n, d] x [d, V]; the teacher costs its k entries per row. With z = sum_i exp(s_i / T - c) for any
+// reference c of the row, e_i = exp(s_i / T - c),
 //
-// Passes, a chunk of rows at a time: logits = student @ W^T (fp32), a row kernel that turns a row of
-// logits into its kl and the difference (w / T) (Q p - q), and grad = difference @ W.
+//   grad = (w Q / (T z)) (e - q z / Q) W
+//
+// so one sweep over the vocabulary can write e before z is known: the row factor is applied to the
+// finished product, and only the k kept entries are rewritten in between. bf16 passes, a chunk of rows
+// at a time:
+//   exp    logits tile in tensor memory (CTA pairs), e in bf16 to the chunk buffer [rows, V],
+//          per-row partial z and maximum, and the fp32 logits at the kept ids picked out of the tile;
+//   finish z, kl, agreement, the kept entries e_j - q_j z / Q (one rounding of the difference, so
+//          the gradient of a student near its teacher is not the difference of rounded numbers),
+//          and the row factor;
+//   grad   row factor * (chunk buffer @ W) on CTA pairs (gemm2_tc.cuh).
+// The reference c is the student's logit at the teacher's first id. bf16 has fp32's exponent range, so
+// a c up to 2^60 below the maximum loses nothing; rows with a larger logit are clamped, noticed by
+// their maximum and swept again with c = maximum (whole tiles of 256 rows; the launch ends at once where
+// there are none).
+//
+// fp32 rows run on CUDA cores: logits = student @ W^T, a row kernel that turns a row of logits into
+// its kl and the difference (w / T) (Q p - q), and grad = difference @ W.
 #pragma once
 
+#include "gemm2_tc.cuh"
 #include "gemm_simt.cuh"
-#include "gemm_tc.cuh"
 #include "lmhead_kl.cuh"
 
 namespace orthrus {
 
 constexpr int kTopkKlMaxK = 1024;
 constexpr int kTopkKlThreads = 512;
+
+// ------------------------------------------------------------------------------------------------
+// fp32 rows
+// ------------------------------------------------------------------------------------------------
 
 // The kept teacher entries of one row in shared memory. Entries with id < 0 or value -inf are
 // padding (q = 0, id = -1); an id past the vocabulary is recorded and counts as padding.
@@ -176,17 +197,526 @@ __global__ void __launch_bounds__(kTopkKlThreads)
 }
 
 // ------------------------------------------------------------------------------------------------
+// bf16 rows
+// ------------------------------------------------------------------------------------------------
+
+constexpr float kTopkExpLimit = 60.f;  // log2 of the largest e: z and Q / z stay normal numbers
+constexpr int kTopkMaxSplits = 64;
+
+// One CTA per teacher row: its entries sorted by id (sid [m, k], padding INT_MAX at the end) with log q
+// beside them, the id of the first largest value and Q. Sorted ids let a sweep over the vocabulary meet
+// them in its own order.
+__global__ void __launch_bounds__(128)
+    topk_teacher_kernel(const float* __restrict__ values, const int64_t* __restrict__ ids, int k, int V, float T,
+                        const float* __restrict__ teacher_lse, int* __restrict__ sid, float* __restrict__ slogq,
+                        int* __restrict__ top_id, float* __restrict__ mass) {
+  __shared__ int id[kTopkKlMaxK];
+  __shared__ float val[kTopkKlMaxK];
+  __shared__ float red[4];
+  __shared__ int redi[4];
+  const int64_t t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int n2 = 1;
+  while (n2 < k) n2 <<= 1;
+  float best = -INFINITY;
+  int at = INT_MAX;
+  for (int j = threadIdx.x; j < n2; j += 128) {
+    const float v = j < k ? values[t * k + j] : -INFINITY;
+    const int64_t i = j < k ? ids[t * k + j] : -1;
+    if (i >= V) record_error(ORTHRUS_ERR_BOUNDS);
+    const bool live = i >= 0 && i < V && v != -INFINITY;
+    id[j] = live ? static_cast<int>(i) : INT_MAX;
+    val[j] = live ? v : -INFINITY;
+    if (live && v > best) {
+      best = v;
+      at = j;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float ov = __shfl_xor_sync(0xffffffffu, best, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, at, o);
+    if (ov > best || (ov == best && oi < at)) {
+      best = ov;
+      at = oi;
+    }
+  }
+  if (lane == 0) {
+    red[warp] = best;
+    redi[warp] = at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    if (red[w] > best || (red[w] == best && redi[w] < at)) {
+      best = red[w];
+      at = redi[w];
+    }
+  const int first = at == INT_MAX ? -1 : id[at];
+  for (int size = 2; size <= n2; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n2 / 2; i += 128) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const int x = id[lo], y = id[hi];
+        if ((x > y) == ((lo & size) == 0)) {
+          const float v = val[lo];
+          id[lo] = y;
+          id[hi] = x;
+          val[lo] = val[hi];
+          val[hi] = v;
+        }
+      }
+    }
+  __syncthreads();
+  auto sum = [&](float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+  };
+  float norm;
+  if (teacher_lse != nullptr) {
+    norm = teacher_lse[t];
+  } else {
+    float z = 0.f;
+    for (int j = threadIdx.x; j < k; j += 128)
+      if (id[j] != INT_MAX) z += expf(val[j] / T - best / T);
+    norm = best / T + logf(sum(z));
+  }
+  float q = 0.f;
+  for (int j = threadIdx.x; j < k; j += 128) {
+    const float lq = id[j] != INT_MAX ? val[j] / T - norm : -INFINITY;
+    sid[t * k + j] = id[j];
+    slogq[t * k + j] = lq;
+    q += expf(lq);
+  }
+  q = sum(q);
+  if (threadIdx.x == 0) {
+    top_id[t] = first;
+    mass[t] = q;
+  }
+}
+
+// One warp per student row: its teacher row (-1 if the index is out of range) and its reference
+// c = log2(e) / T * (student . W[top_id]); clears the tiles' second-sweep flags.
+__global__ void __launch_bounds__(256)
+    topk_student_kernel(const __nv_bfloat16* __restrict__ student, const __nv_bfloat16* __restrict__ W, int64_t n,
+                        int64_t m, int D, const int64_t* __restrict__ index, const int* __restrict__ top_id,
+                        float alpha, int* __restrict__ trow, float* __restrict__ ref, int* __restrict__ again) {
+  const int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= n) return;
+  int64_t t = index ? index[r] : r;
+  if (t < 0 || t >= m) {
+    if (lane == 0) record_error(ORTHRUS_ERR_BOUNDS);
+    t = -1;
+  }
+  const int id = t < 0 ? -1 : top_id[t];
+  float dot = 0.f;
+  if (id >= 0) {
+    const uint4* h4 = reinterpret_cast<const uint4*>(student + r * D);
+    const uint4* w4 = reinterpret_cast<const uint4*>(W + static_cast<int64_t>(id) * D);
+    for (int i = lane; i < D / 8; i += 32) {
+      const uint4 a = h4[i], b = w4[i];
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dot = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), dot);
+        dot = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), dot);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  }
+  if (lane == 0) {
+    trow[r] = static_cast<int>(t);
+    ref[r] = dot * alpha;
+    if (r % 256 == 0) again[r / 256] = 0;
+  }
+}
+
+struct TopkExpTile {
+  static constexpr int BM = 128, BK = 64, BN = 256;  // rows and columns of a pair: 256 x 256
+  static constexpr int A_BYTES = BM * BK * 2;        // this CTA's 128 student rows
+  static constexpr int B_BYTES = 128 * BK * 2;       // this CTA's 128 vocabulary rows of W
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 6;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+};
+
+struct TopkExpArgs {
+  int rows, c0;  // rows of the chunk, its first student row
+  int V, D, k;
+  int vtiles, tiles_per_split, rtiles, units;
+  float alpha;            // log2(e) / T
+  const int* trow;        // [n]
+  const float* ref;       // [n]
+  const int* sid;         // [m, k]
+  const int* again;       // [ceil(n / 256)]: the second sweep takes the flagged tiles only; null: all
+  float* kept;            // [chunk, k] student logits at the sorted ids
+  float* part_z;          // [2 splits, chunk], as part_m and part_i
+  float* part_m;
+  int* part_i;
+  int64_t part_ld;
+  __nv_bfloat16* e;       // [chunk, lde], or null
+  int64_t lde;
+};
+
+// One fp32 column of this warp's 32 TMEM lanes.
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  return __uint_as_float(r);
+}
+
+// The exp sweep: a persistent cluster of two CTAs walks units (tile of 256 student rows, range of the
+// vocabulary). Warp 0 loads, warp 1 of the leader issues the MMAs of the pair, warps 2-9 are the
+// epilogue: thread (quarter, half, lane) owns row quarter * 32 + lane of its CTA and 128 of the
+// tile's 256 columns. Two accumulators of 256 columns let the epilogue of one tile run under the
+// MMAs of the next.
+__global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
+    topk_exp_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
+                    const TopkExpArgs a) {
+  using T = TopkExpTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + T::STAGES * T::A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sB + T::STAGES * T::B_BYTES);
+  uint64_t* empty = full + T::STAGES;
+  uint64_t* acc_full = empty + T::STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;      // [2], leader only: both CTAs' epilogue warps arrive
+  uint64_t* mma_drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  const int KB = (a.D + T::BK - 1) / T::BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < T::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * T::EPI_WARPS);
+    }
+    mbar_init(mma_drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // unit u = (row tile u % rtiles, vocabulary range u / rtiles); the same tiles for every role of
+  // both CTAs (the flags do not change during the launch)
+  auto unit_tiles = [&](int u, int& row0, int& split, int& t0) {
+    const int rt = u % a.rtiles;
+    split = u / a.rtiles;
+    row0 = rt * 256 + static_cast<int>(rank) * T::BM;  // this CTA's first row in the chunk
+    t0 = split * a.tiles_per_split;
+    if (a.again != nullptr && a.again[a.c0 / 256 + rt] == 0) return 0;
+    return max(min(a.vtiles, t0 + a.tiles_per_split) - t0, 0);
+  };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      prefetch_tensormap(&tmH);
+      prefetch_tensormap(&tmW);
+      int it = 0, issued = 0;
+      for (int u = cluster; u < a.units && !*abort_flag; u += nclusters) {
+        int row0, split, t0;
+        const int ntiles = unit_tiles(u, row0, split, t0);
+        for (int t = 0; t < ntiles && !*abort_flag; ++t) {
+          const int v0 = (t0 + t) * T::BN + static_cast<int>(rank) * 128;
+          for (int kb = 0; kb < KB; ++kb, ++it) {
+            const int s = it % T::STAGES;
+            if (!mbar_wait(&empty[s], ((it / T::STAGES) & 1) ^ 1)) {
+              *abort_flag = 1;
+              break;
+            }
+            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+            if (leader) mbar_arrive_expect_tx(&full[s], 2 * T::STAGE_BYTES);
+            tma_load_2d_pair(sA + s * T::A_BYTES, &tmH, bar, kb * T::BK, a.c0 + row0);
+            tma_load_2d_pair(sB + s * T::B_BYTES, &tmW, bar, kb * T::BK, v0);
+            issued = it + 1;
+          }
+        }
+      }
+      if (*abort_flag && leader)
+        for (int i = max(0, issued - T::STAGES); i < issued; ++i)
+          mbar_wait_short(&full[i % T::STAGES], (i / T::STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    if (leader && elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_bf16(256, T::BN, false, false);
+      int it = 0, tt = 0;
+      for (int u = cluster; u < a.units && !*abort_flag; u += nclusters) {
+        int row0, split, t0;
+        const int ntiles = unit_tiles(u, row0, split, t0);
+        for (int t = 0; t < ntiles && !*abort_flag; ++t, ++tt) {
+          const int b = tt & 1;
+          if (!mbar_wait_cluster(&acc_empty[b], ((tt >> 1) & 1) ^ 1)) {
+            *abort_flag = 1;
+            break;
+          }
+          tc_fence_after();
+          for (int kb = 0; kb < KB; ++kb, ++it) {
+            const int s = it % T::STAGES;
+            if (!mbar_wait(&full[s], (it / T::STAGES) & 1)) {
+              *abort_flag = 1;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_base = smem_u32(sA + s * T::A_BYTES);
+            const uint32_t b_base = smem_u32(sB + s * T::B_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < T::BK / 16; ++kk)
+              umma_f16_pair(tmem + b * T::BN, g2_desc_k(a_base, kk), g2_desc_k(b_base, kk), idesc,
+                            (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[s], 3);
+          }
+          umma_commit_pair(&acc_full[b], 3);
+        }
+      }
+      // every MMA issued has completed (in both CTAs' TMEM) before either frees its columns
+      umma_commit_pair(mma_drain, 3);
+      mbar_wait(mma_drain, 0);
+    } else if (!leader && elect_one()) {
+      mbar_wait(mma_drain, 0);  // the leader's last MMAs also wrote this CTA's TMEM
+    }
+  } else {
+    const int quarter = warp & 3;      // TMEM lanes this warp may read
+    const int half = (warp - 2) >> 2;  // which half of the tile's columns it takes
+    int tt = 0;
+    for (int u = cluster; u < a.units && !*abort_flag; u += nclusters) {
+      int row0, split, t0;
+      const int ntiles = unit_tiles(u, row0, split, t0);
+      if (ntiles == 0) continue;
+      const int crow = row0 + quarter * 32 + lane;  // row in the chunk
+      const bool live = crow < a.rows;
+      const float ref = live ? a.ref[a.c0 + crow] : 0.f;
+      const int trow = live ? a.trow[a.c0 + crow] : -1;
+      __nv_bfloat16* erow = a.e != nullptr && live ? a.e + crow * a.lde : nullptr;
+      // the row's sorted ids from this unit's first column on
+      const int* sid = a.sid + static_cast<int64_t>(trow < 0 ? 0 : trow) * a.k;
+      int p = 0;
+      if (trow >= 0)
+        for (int hi = a.k; p < hi;) {
+          const int mid = (p + hi) / 2;
+          if (sid[mid] < t0 * T::BN) p = mid + 1;
+          else hi = mid;
+        }
+      int next = trow >= 0 && p < a.k ? sid[p] : INT_MAX;
+      float z = 0.f, m = -INFINITY;
+      int idx = INT_MAX;
+      for (int t = 0; t < ntiles; ++t, ++tt) {
+        const int b = tt & 1;
+        if (*abort_flag || !mbar_wait(&acc_full[b], (tt >> 1) & 1)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const int v0 = (t0 + t) * T::BN;
+        const int lo = v0 + half * 128;
+        const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * T::BN;
+        // kept ids among these columns: the warp loads one column at a time, the lanes whose id it is
+        // take it
+        while (next < lo) next = ++p < a.k ? sid[p] : INT_MAX;
+        __syncwarp();
+        for (uint32_t todo; (todo = __ballot_sync(0xffffffffu, next < lo + 128)) != 0;) {
+          const int col = __shfl_sync(0xffffffffu, next, __ffs(todo) - 1);
+          const float x = tmem_ld1(base + (col - v0));
+          tmem_wait_ld();
+          while (next == col) {  // an id kept twice stands twice
+            a.kept[static_cast<int64_t>(crow) * a.k + p] = x;
+            next = ++p < a.k ? sid[p] : INT_MAX;
+          }
+          __syncwarp();
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const int col0 = lo + c * 32;
+          const int nvalid = min(32, a.V - col0);
+          if (nvalid <= 0) break;  // uniform over the warp
+          float x[32];
+          tmem_ld32(base + half * 128 + c * 32, x);
+          tmem_wait_ld();
+          // first maximum, four independent chains (column j in chain j % 4), lower columns on ties
+          float cmv[4];
+          int civ[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            cmv[i] = -INFINITY;
+            civ[i] = 32;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < nvalid && x[j] > cmv[j & 3]) {
+              cmv[j & 3] = x[j];
+              civ[j & 3] = j;
+            }
+#pragma unroll
+          for (int i = 1; i < 4; ++i)
+            if (cmv[i] > cmv[0] || (cmv[i] == cmv[0] && civ[i] < civ[0])) {
+              cmv[0] = cmv[i];
+              civ[0] = civ[i];
+            }
+          if (cmv[0] > m) {
+            m = cmv[0];
+            idx = col0 + civ[0];
+          }
+          float zv[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t packed[16];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float y = fmaf(x[j], a.alpha, -ref);
+            y = y > kTopkExpLimit ? kTopkExpLimit : y;  // NaN stays
+            x[j] = j < nvalid ? ex2_approx(y) : 0.f;
+            zv[j & 3] += x[j];
+          }
+          z += (zv[0] + zv[1]) + (zv[2] + zv[3]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) packed[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+          __nv_bfloat16* dst = erow + col0;  // null: a row past the chunk, or no gradient wanted
+          if (erow != nullptr && nvalid == 32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(dst + 8 * q) =
+                  make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+          } else if (erow != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nvalid)
+                dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(packed[j >> 1] >> (16 * (j & 1))));
+          }
+          __syncwarp();  // the tensor-memory loads take the whole warp
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
+      }
+      if (live) {
+        const int64_t o = static_cast<int64_t>(2 * split + half) * a.part_ld + crow;
+        a.part_z[o] = z;
+        a.part_m[o] = m;
+        a.part_i[o] = idx;
+      }
+    }
+  }
+  __syncthreads();
+  cluster_sync_all();  // neither CTA frees TMEM or leaves while the other may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_pair(tmem, 512);
+  }
+}
+
+// Rows whose maximum lies above the exponent limit get it as their reference, and their tile a flag.
+__global__ void topk_again_kernel(const float* __restrict__ part_m, int parts, int64_t part_ld, int rows, int c0,
+                                  float alpha, float* __restrict__ ref, int* __restrict__ again) {
+  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < parts; ++s) m = fmaxf(m, part_m[s * part_ld + r]);
+  if (fmaf(m, alpha, -ref[c0 + r]) > kTopkExpLimit) {
+    ref[c0 + r] = m * alpha;
+    again[(c0 + r) / 256] = 1;
+  }
+}
+
+// One warp per row of the chunk: z and the first maximum from the partials (a fixed order), the row's
+// kl and agreement, the kept entries of the chunk buffer and the row factor of the gradient.
+__global__ void __launch_bounds__(256)
+    topk_finish_kernel(const float* __restrict__ part_z, const float* __restrict__ part_m,
+                       const int* __restrict__ part_i, int parts, int64_t part_ld, int rows, int c0, int k, float alpha,
+                       float T, const int* __restrict__ trow, const float* __restrict__ ref,
+                       const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
+                       const float* __restrict__ mass, const float* __restrict__ kept,
+                       const float* __restrict__ row_weight, float* __restrict__ kl_rows, uint8_t* __restrict__ agree,
+                       __nv_bfloat16* __restrict__ e, int64_t lde, float* __restrict__ scale) {
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  const int64_t g = c0 + r;
+  float z = 0.f, m = -INFINITY;
+  int at = INT_MAX;
+  for (int s = lane; s < parts; s += 32) {
+    z += part_z[s * part_ld + r];
+    const float pm = part_m[s * part_ld + r];
+    const int pi = part_i[s * part_ld + r];
+    if (pm > m || (pm == m && pi < at)) {
+      m = pm;
+      at = pi;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    z += __shfl_xor_sync(0xffffffffu, z, o);
+    const float om = __shfl_xor_sync(0xffffffffu, m, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, at, o);
+    if (om > m || (om == m && oi < at)) {
+      m = om;
+      at = oi;
+    }
+  }
+  const int t = trow[g];
+  const float Q = t >= 0 ? mass[t] : 0.f;
+  const float logz = logf(z), c = ref[g];
+  float kl = 0.f;
+  if (t >= 0 && Q != 0.f) {
+    const int* id = sid + static_cast<int64_t>(t) * k;
+    const float* lq = slogq + static_cast<int64_t>(t) * k;
+    for (int j = lane; j < k; j += 32) {
+      const int i = id[j];
+      if (i == INT_MAX) continue;
+      const float y = fmaf(kept[static_cast<int64_t>(r) * k + j], alpha, -c);
+      const float q = expf(lq[j]);
+      if (q != 0.f) kl += q * (lq[j] - (y * kLn2 - logz));
+      if (e == nullptr || (j > 0 && id[j - 1] == i)) continue;
+      float all = q;  // an id kept twice counts with its whole mass
+      for (int o = j + 1; o < k && id[o] == i; ++o) all += expf(lq[o]);
+      e[r * lde + i] = __float2bfloat16_rn(ex2_approx(y > kTopkExpLimit ? kTopkExpLimit : y) - (all / Q) * z);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
+  if (lane == 0) {
+    kl_rows[g] = kl;
+    agree[g] = t >= 0 && top_id[t] >= 0 && top_id[t] == at;
+    scale[r] = (row_weight ? row_weight[g] : 1.f) / T * (Q / z);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
 // Host orchestration
 // ------------------------------------------------------------------------------------------------
 
 struct TopkKlPlan {
   int64_t chunk, Vp;
-  size_t off_logits, off_diff, off_gemm, gemm_bytes, total;
+  int splits;  // most vocabulary ranges of a chunk's sweep
+  size_t off_buf, off_gemm, gemm_bytes;
+  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_again, off_kept, off_part, off_scale;
+  size_t total;
 };
 
-inline TopkKlPlan topk_kl_plan(int64_t n, int64_t V, int64_t D, int64_t chunk_rows, int dtype) {
+// The chunk buffer holds fp32 logits (fp32 rows) or bf16 exponentials of p.chunk rows.
+inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64_t k, int64_t chunk_rows, int dtype) {
   TopkKlPlan p{};
-  p.chunk = std::min<int64_t>(chunk_rows <= 0 ? 4096 : chunk_rows, std::max<int64_t>(n, 1));
+  const int64_t tile = dtype == ORTHRUS_BF16 ? 256 : 1;
+  const int64_t chunk = std::min<int64_t>(chunk_rows <= 0 ? 4096 : chunk_rows, std::max<int64_t>(n, 1));
+  p.chunk = ceil_div(chunk, tile) * tile;
   p.Vp = ceil_div(V, 8) * 8;
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -194,32 +724,160 @@ inline TopkKlPlan topk_kl_plan(int64_t n, int64_t V, int64_t D, int64_t chunk_ro
     off = align_up(off + bytes, 256);
     return o;
   };
-  p.off_logits = take(static_cast<size_t>(p.chunk) * p.Vp * 4);
-  p.off_diff = dtype == ORTHRUS_BF16 ? take(static_cast<size_t>(p.chunk) * p.Vp * 2) : p.off_logits;
-  p.gemm_bytes = dtype == ORTHRUS_BF16 ? std::max(gemm_ws_bytes(p.chunk, V, D), gemm_ws_bytes(p.chunk, D, V))
-                                       : std::max(simt_ws_bytes(p.chunk, V, D), simt_ws_bytes(p.chunk, D, V));
+  p.off_buf = take(static_cast<size_t>(p.chunk) * p.Vp * (dtype == ORTHRUS_BF16 ? 2 : 4));
+  if (dtype == ORTHRUS_BF16) {
+    // a short last chunk has fewer tiles and may split deeper: the larger of the two
+    p.gemm_bytes = std::max(gemm2_rowscale_ws_bytes(std::min(n, p.chunk), D, V),
+                            n % p.chunk ? gemm2_rowscale_ws_bytes(n % p.chunk, D, V) : size_t(0));
+    p.splits = static_cast<int>(std::min<int64_t>(kTopkMaxSplits, ceil_div(V, 256)));
+    p.off_sid = take(static_cast<size_t>(m) * k * 4);
+    p.off_logq = take(static_cast<size_t>(m) * k * 4);
+    p.off_top = take(static_cast<size_t>(m) * 4);
+    p.off_mass = take(static_cast<size_t>(m) * 4);
+    p.off_trow = take(static_cast<size_t>(n) * 4);
+    p.off_ref = take(static_cast<size_t>(n) * 4);
+    p.off_again = take(static_cast<size_t>(ceil_div(n, 256)) * 4);
+    p.off_kept = take(static_cast<size_t>(p.chunk) * k * 4);
+    p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 12);
+    p.off_scale = take(static_cast<size_t>(p.chunk) * 4);
+  } else {
+    p.gemm_bytes = std::max(simt_ws_bytes(p.chunk, V, D), simt_ws_bytes(p.chunk, D, V));
+  }
   p.off_gemm = take(p.gemm_bytes);
   p.total = off;
   return p;
 }
 
+struct TopkKlCall {
+  int64_t n, m;
+  int k;
+  const float* values;
+  const int64_t *ids, *index;
+  const float *teacher_lse, *row_weight;
+  int64_t V, D;
+  float T;
+  float* kl_rows;
+  uint8_t* agree;
+};
+
+inline int topk_kl_rows_f32(const TopkKlCall& a, const TopkKlPlan& p, const float* student, const float* W, float* grad,
+                            uint8_t* ws, cudaStream_t stream) {
+  float* buf = reinterpret_cast<float*>(ws + p.off_buf);
+  void* gws = ws + p.off_gemm;
+  for (int64_t c0 = 0; c0 < a.n; c0 += p.chunk) {
+    const int64_t rows = std::min<int64_t>(p.chunk, a.n - c0);
+    int rc = gemm_simt_impl<float, false>(student + c0 * a.D, a.D, W, a.D, buf, p.Vp, rows, a.V, a.D, gws, p.gemm_bytes,
+                                          stream);
+    if (rc != ORTHRUS_OK) return rc;
+    topk_kl_rows_kernel<float><<<static_cast<unsigned>(rows), kTopkKlThreads, 0, stream>>>(
+        buf, p.Vp, static_cast<int>(c0), static_cast<int>(a.V), a.values, a.ids, a.k, a.m, a.index, a.teacher_lse,
+        a.row_weight, a.T, a.kl_rows, a.agree, grad ? buf : nullptr, p.Vp);
+    ORTHRUS_CHECK_LAUNCH();
+    if (grad == nullptr) continue;
+    rc = gemm_simt_impl<float, true>(buf, p.Vp, W, a.D, grad + c0 * a.D, a.D, rows, a.D, a.V, gws, p.gemm_bytes, stream);
+    if (rc != ORTHRUS_OK) return rc;
+  }
+  return ORTHRUS_OK;
+}
+
+inline int topk_exp_launch(const CUtensorMap& th, const CUtensorMap& tw, const TopkExpArgs& a, cudaStream_t stream) {
+  ORTHRUS_CHECK_CUDA(ensure_smem(topk_exp_kernel, TopkExpTile::SMEM));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min(a.units, num_sms() / 2)));
+  cfg.blockDim = dim3(TopkExpTile::THREADS);
+  cfg.dynamicSmemBytes = TopkExpTile::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ORTHRUS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, topk_exp_kernel, th, tw, a));
+  ORTHRUS_CHECK_LAUNCH();
+  return ORTHRUS_OK;
+}
+
+inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __nv_bfloat16* student,
+                             const __nv_bfloat16* W, __nv_bfloat16* grad, uint8_t* ws, cudaStream_t stream) {
+  auto* e = reinterpret_cast<__nv_bfloat16*>(ws + p.off_buf);
+  auto f = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
+  auto i = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
+  const float alpha = kLog2e / a.T;
+  const int D = static_cast<int>(a.D), V = static_cast<int>(a.V);
+  topk_teacher_kernel<<<static_cast<unsigned>(a.m), 128, 0, stream>>>(a.values, a.ids, a.k, V, a.T, a.teacher_lse,
+                                                                      i(p.off_sid), f(p.off_logq), i(p.off_top),
+                                                                      f(p.off_mass));
+  ORTHRUS_CHECK_LAUNCH();
+  topk_student_kernel<<<static_cast<unsigned>(ceil_div(a.n, 8)), 256, 0, stream>>>(
+      student, W, a.n, a.m, D, a.index, i(p.off_top), alpha, i(p.off_trow), f(p.off_ref), i(p.off_again));
+  ORTHRUS_CHECK_LAUNCH();
+  CUtensorMap th, tw;
+  if (!make_tmap_2d_bf16(&th, student, a.D, a.n, a.D, 64, 128)) return ORTHRUS_ECUDA;
+  if (!make_tmap_2d_bf16(&tw, W, a.D, a.V, a.D, 64, 128)) return ORTHRUS_ECUDA;
+  TopkExpArgs x{};
+  x.V = V;
+  x.D = D;
+  x.k = a.k;
+  x.vtiles = static_cast<int>(ceil_div(a.V, 256));
+  x.alpha = alpha;
+  x.trow = i(p.off_trow);
+  x.ref = f(p.off_ref);
+  x.sid = i(p.off_sid);
+  x.kept = f(p.off_kept);
+  const size_t part = static_cast<size_t>(p.chunk) * 2 * p.splits;
+  x.part_z = f(p.off_part);
+  x.part_m = x.part_z + part;
+  x.part_i = reinterpret_cast<int*>(x.part_m + part);
+  x.part_ld = p.chunk;
+  x.e = grad ? e : nullptr;
+  x.lde = p.Vp;
+  for (int64_t c0 = 0; c0 < a.n; c0 += p.chunk) {
+    x.rows = static_cast<int>(std::min<int64_t>(p.chunk, a.n - c0));
+    x.c0 = static_cast<int>(c0);
+    x.rtiles = static_cast<int>(ceil_div(x.rows, 256));
+    x.tiles_per_split =
+        static_cast<int>(ceil_div(x.vtiles, pick_splits(x.rtiles, x.vtiles, num_sms() / 2, p.splits)));
+    const int splits = static_cast<int>(ceil_div(x.vtiles, x.tiles_per_split));
+    x.units = x.rtiles * splits;
+    x.again = nullptr;
+    int rc = topk_exp_launch(th, tw, x, stream);
+    if (rc != ORTHRUS_OK) return rc;
+    topk_again_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 128)), 128, 0, stream>>>(
+        x.part_m, 2 * splits, x.part_ld, x.rows, x.c0, alpha, f(p.off_ref), i(p.off_again));
+    ORTHRUS_CHECK_LAUNCH();
+    x.again = i(p.off_again);
+    rc = topk_exp_launch(th, tw, x, stream);
+    if (rc != ORTHRUS_OK) return rc;
+    topk_finish_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 8)), 256, 0, stream>>>(
+        x.part_z, x.part_m, x.part_i, 2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, x.sid,
+        f(p.off_logq), i(p.off_top), f(p.off_mass), x.kept, a.row_weight, a.kl_rows, a.agree, x.e, x.lde,
+        f(p.off_scale));
+    ORTHRUS_CHECK_LAUNCH();
+    if (grad == nullptr) continue;
+    rc = gemm2_rowscale_impl(e, p.Vp, W, grad + c0 * a.D, f(p.off_scale), x.rows, a.D, a.V, ws + p.off_gemm,
+                             p.gemm_bytes, stream);
+    if (rc != ORTHRUS_OK) return rc;
+  }
+  return ORTHRUS_OK;
+}
+
 template <typename E>
-int lmhead_topk_kl_fwd_impl(const E* student, int64_t n, const float* values, const int64_t* ids, int64_t m, int k,
-                            const int64_t* index, const float* teacher_lse, const E* weight, int64_t V, int64_t D,
-                            float temperature, const float* row_weight, const int64_t* offsets, int num_offsets,
-                            float* total, float* kl_rows, uint8_t* agree, E* grad, float* kl_by_offset,
-                            int64_t* agree_by_offset, int64_t chunk_rows, void* ws_raw, size_t ws_bytes,
-                            cudaStream_t stream) {
+int lmhead_topk_kl_fwd_impl(const E* student, const E* weight, const TopkKlCall& a, const int64_t* offsets,
+                            int num_offsets, float* total, E* grad, float* kl_by_offset, int64_t* agree_by_offset,
+                            int64_t chunk_rows, void* ws_raw, size_t ws_bytes, cudaStream_t stream) {
   constexpr bool kBf16 = sizeof(E) == 2;
-  ORTHRUS_CHECK_ARG(n >= 0 && m >= 0 && V >= 1 && D >= 1 && k >= 1 && k <= kTopkKlMaxK && temperature > 0.f);
-  ORTHRUS_CHECK_ARG(n < (1ll << 31) && V < (1ll << 31) && D < (1ll << 31));
-  ORTHRUS_CHECK_ARG(weight && total && (n == 0 || (student && values && ids && kl_rows && agree && m >= 1)));
-  ORTHRUS_CHECK_ARG(index != nullptr || n <= m);
+  ORTHRUS_CHECK_ARG(a.n >= 0 && a.m >= 0 && a.V >= 1 && a.D >= 1 && a.k >= 1 && a.k <= kTopkKlMaxK && a.T > 0.f);
+  ORTHRUS_CHECK_ARG(a.n < (1ll << 31) && a.m < (1ll << 31) && a.V < (1ll << 31) - 256 && a.D < (1ll << 30));
+  ORTHRUS_CHECK_ARG(weight && total);
+  ORTHRUS_CHECK_ARG(a.n == 0 || (student && a.values && a.ids && a.kl_rows && a.agree && a.m >= 1));
+  ORTHRUS_CHECK_ARG(a.index != nullptr || a.n <= a.m);
   ORTHRUS_CHECK_ARG(offsets == nullptr || (kl_by_offset && agree_by_offset && num_offsets > 0));
-  if (kBf16) ORTHRUS_CHECK_ARG(D % 8 == 0 && aligned16(student) && aligned16(weight) && (!grad || aligned16(grad)));
-  const TopkKlPlan p = topk_kl_plan(n, V, D, chunk_rows, kBf16 ? ORTHRUS_BF16 : ORTHRUS_F32);
+  if (kBf16) ORTHRUS_CHECK_ARG(a.D % 8 == 0 && aligned16(student) && aligned16(weight) && (!grad || aligned16(grad)));
+  const TopkKlPlan p = topk_kl_plan(a.n, a.m, a.V, a.D, a.k, chunk_rows, kBf16 ? ORTHRUS_BF16 : ORTHRUS_F32);
   if (ws_raw == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
-  if (n == 0) {
+  if (a.n == 0) {
     ORTHRUS_CHECK_CUDA(cudaMemsetAsync(total, 0, sizeof(float), stream));
     if (kl_by_offset && agree_by_offset) {  // an empty offsets array may be NULL
       ORTHRUS_CHECK_CUDA(cudaMemsetAsync(kl_by_offset, 0, num_offsets * sizeof(float), stream));
@@ -227,31 +885,13 @@ int lmhead_topk_kl_fwd_impl(const E* student, int64_t n, const float* values, co
     }
     return ORTHRUS_OK;
   }
-  uint8_t* ws = static_cast<uint8_t*>(ws_raw);
-  float* logits = reinterpret_cast<float*>(ws + p.off_logits);
-  E* diff = reinterpret_cast<E*>(ws + p.off_diff);
-  void* gws = ws + p.off_gemm;
-  for (int64_t c0 = 0; c0 < n; c0 += p.chunk) {
-    const int64_t rows = std::min<int64_t>(p.chunk, n - c0);
-    int rc;
-    if constexpr (kBf16)
-      rc = gemm_bf16_impl(student + c0 * D, D, weight, D, logits, p.Vp, rows, V, D, 0, 1, gws, p.gemm_bytes, stream);
-    else
-      rc = gemm_simt_impl<E, false>(student + c0 * D, D, weight, D, logits, p.Vp, rows, V, D, gws, p.gemm_bytes, stream);
-    if (rc != ORTHRUS_OK) return rc;
-    topk_kl_rows_kernel<E><<<static_cast<unsigned>(rows), kTopkKlThreads, 0, stream>>>(
-        logits, p.Vp, static_cast<int>(c0), static_cast<int>(V), values, ids, k, m, index, teacher_lse, row_weight,
-        temperature, kl_rows, agree, grad ? diff : nullptr, p.Vp);
-    ORTHRUS_CHECK_LAUNCH();
-    if (grad != nullptr) {
-      if constexpr (kBf16)
-        rc = gemm_bf16_impl(diff, p.Vp, weight, D, grad + c0 * D, D, rows, D, V, 1, 0, gws, p.gemm_bytes, stream, false);
-      else
-        rc = gemm_simt_impl<E, true>(diff, p.Vp, weight, D, grad + c0 * D, D, rows, D, V, gws, p.gemm_bytes, stream);
-      if (rc != ORTHRUS_OK) return rc;
-    }
-  }
-  lmhead_finalize_kernel<<<1, 1024, 0, stream>>>(kl_rows, agree, row_weight, offsets, n, num_offsets, total,
+  int rc;
+  if constexpr (kBf16)
+    rc = topk_kl_rows_bf16(a, p, student, weight, grad, static_cast<uint8_t*>(ws_raw), stream);
+  else
+    rc = topk_kl_rows_f32(a, p, student, weight, grad, static_cast<uint8_t*>(ws_raw), stream);
+  if (rc != ORTHRUS_OK) return rc;
+  lmhead_finalize_kernel<<<1, 1024, 0, stream>>>(a.kl_rows, a.agree, a.row_weight, offsets, a.n, num_offsets, total,
                                                  kl_by_offset, agree_by_offset);
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;

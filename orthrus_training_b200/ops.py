@@ -384,7 +384,7 @@ def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets
         abo = torch.empty(num_offsets, dtype=torch.int64, device=dev)
     lib = L.lib()
     with _on_device(dev):
-        ws = torch.empty(max(lib.orthrus_lmhead_topk_kl_workspace_bytes(n, V, d + pad, chunk_rows, code), 1),
+        ws = torch.empty(max(lib.orthrus_lmhead_topk_kl_workspace_bytes(n, m, V, d + pad, k, chunk_rows, code), 1),
                          dtype=torch.uint8, device=dev)
         t0 = TIMER.begin() if TIMER is not None else None
         L.check(lib.orthrus_lmhead_topk_kl_fwd(
