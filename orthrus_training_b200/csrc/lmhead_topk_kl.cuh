@@ -346,7 +346,8 @@ struct TopkExpTile {
   static constexpr int STAGES = 6;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+  static constexpr int STAGING = 32 * 64 * 2;  // per epilogue warp: 32 rows x 64 bf16 on their way out
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING + 1024 + 256;
 };
 
 struct TopkExpArgs {
@@ -363,8 +364,7 @@ struct TopkExpArgs {
   float* part_m;
   int* part_i;
   int64_t part_ld;
-  __nv_bfloat16* e;       // [chunk, lde], or null
-  int64_t lde;
+  bool write_e;           // the exponentials are wanted (tmE)
 };
 
 // One fp32 column of this warp's 32 TMEM lanes.
@@ -381,13 +381,14 @@ __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
 // MMAs of the next.
 __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
     topk_exp_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
-                    const TopkExpArgs a) {
+                    const __grid_constant__ CUtensorMap tmE, const TopkExpArgs a) {
   using T = TopkExpTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + T::STAGES * T::A_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sB + T::STAGES * T::B_BYTES);
+  uint8_t* staging = sB + T::STAGES * T::B_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + T::EPI_WARPS * T::STAGING);
   uint64_t* empty = full + T::STAGES;
   uint64_t* acc_full = empty + T::STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;      // [2], leader only: both CTAs' epilogue warps arrive
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
   } else {
     const int quarter = warp & 3;      // TMEM lanes this warp may read
     const int half = (warp - 2) >> 2;  // which half of the tile's columns it takes
+    uint8_t* const stage = staging + (warp - 2) * T::STAGING;
     int tt = 0;
     for (int u = cluster; u < a.units && !*abort_flag; u += nclusters) {
       int row0, split, t0;
@@ -509,7 +511,6 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
       const bool live = crow < a.rows;
       const float ref = live ? a.ref[a.c0 + crow] : 0.f;
       const int trow = live ? a.trow[a.c0 + crow] : -1;
-      __nv_bfloat16* erow = a.e != nullptr && live ? a.e + crow * a.lde : nullptr;
       // the row's sorted ids from this unit's first column on
       const int* sid = a.sid + static_cast<int64_t>(trow < 0 ? 0 : trow) * a.k;
       int p = 0;
@@ -551,6 +552,10 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
           const int col0 = lo + c * 32;
           const int nvalid = min(32, a.V - col0);
           if (nvalid <= 0) break;  // uniform over the warp
+          if (a.write_e && !(c & 1)) {  // the previous store has read the staging tile
+            if (lane == 0) tma_store_wait_read_all();
+            __syncwarp();
+          }
           float x[32];
           tmem_ld32(base + half * 128 + c * 32, x);
           tmem_wait_ld();
@@ -590,17 +595,22 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
           z += (zv[0] + zv[1]) + (zv[2] + zv[3]);
 #pragma unroll
           for (int j = 0; j < 16; ++j) packed[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
-          __nv_bfloat16* dst = erow + col0;  // null: a row past the chunk, or no gradient wanted
-          if (erow != nullptr && nvalid == 32) {
+          if (a.write_e) {
+            // 64 columns of the warp's 32 rows leave by one TMA store, which cuts them at the chunk's
+            // rows and at V. Stores straight from registers (16 bytes in each of 32 rows an
+            // instruction) kept the load/store unit 65 % busy and the tensor pipe at 67 %.
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(dst + 8 * q) =
-                  make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
-          } else if (erow != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < nvalid)
-                dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(packed[j >> 1] >> (16 * (j & 1))));
+              st_shared_v4(smem_u32(stage) + sw128_offset(lane, (c & 1) * 4 + q), packed[4 * q], packed[4 * q + 1],
+                           packed[4 * q + 2], packed[4 * q + 3]);
+            if ((c & 1) || col0 + 32 >= a.V) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0 && row0 + quarter * 32 < a.rows) {
+                tma_store_2d(&tmE, stage, col0 - (c & 1) * 32, row0 + quarter * 32);
+                tma_store_commit();
+              }
+            }
           }
           __syncwarp();  // the tensor-memory loads take the whole warp
         }
@@ -615,6 +625,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
         a.part_i[o] = idx;
       }
     }
+    if (lane == 0) tma_store_wait_all();
   }
   __syncthreads();
   cluster_sync_all();  // neither CTA frees TMEM or leaves while the other may still signal it
@@ -780,7 +791,8 @@ inline int topk_kl_rows_f32(const TopkKlCall& a, const TopkKlPlan& p, const floa
   return ORTHRUS_OK;
 }
 
-inline int topk_exp_launch(const CUtensorMap& th, const CUtensorMap& tw, const TopkExpArgs& a, cudaStream_t stream) {
+inline int topk_exp_launch(const CUtensorMap& th, const CUtensorMap& tw, const CUtensorMap& te, const TopkExpArgs& a,
+                           cudaStream_t stream) {
   ORTHRUS_CHECK_CUDA(ensure_smem(topk_exp_kernel, TopkExpTile::SMEM));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min(a.units, num_sms() / 2)));
@@ -794,7 +806,7 @@ inline int topk_exp_launch(const CUtensorMap& th, const CUtensorMap& tw, const T
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ORTHRUS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, topk_exp_kernel, th, tw, a));
+  ORTHRUS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, topk_exp_kernel, th, tw, te, a));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
 }
@@ -804,7 +816,10 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   auto* e = reinterpret_cast<__nv_bfloat16*>(ws + p.off_buf);
   auto f = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   auto i = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
-  const float alpha = kLog2e / a.T;
+  // log2(e) / T, and what the tensor cores' adder takes away: it cuts instead of rounding, so a logit
+  // of d products comes out short by about 8.7e-10 d of itself (measured with normal operands: 9.0e-7
+  // at d = 1024, 6.6e-7 at 768, 2.0e-7 at 256). Left in, that is the larger part of the error of kl.
+  const float alpha = static_cast<float>(1.4426950408889634 / a.T * (1.0 + 8.7e-10 * a.D));
   const int D = static_cast<int>(a.D), V = static_cast<int>(a.V);
   topk_teacher_kernel<<<static_cast<unsigned>(a.m), 128, 0, stream>>>(a.values, a.ids, a.k, V, a.T, a.teacher_lse,
                                                                       i(p.off_sid), f(p.off_logq), i(p.off_top),
@@ -813,7 +828,7 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   topk_student_kernel<<<static_cast<unsigned>(ceil_div(a.n, 8)), 256, 0, stream>>>(
       student, W, a.n, a.m, D, a.index, i(p.off_top), alpha, i(p.off_trow), f(p.off_ref), i(p.off_again));
   ORTHRUS_CHECK_LAUNCH();
-  CUtensorMap th, tw;
+  CUtensorMap th, tw, te{};
   if (!make_tmap_2d_bf16(&th, student, a.D, a.n, a.D, 64, 128)) return ORTHRUS_ECUDA;
   if (!make_tmap_2d_bf16(&tw, W, a.D, a.V, a.D, 64, 128)) return ORTHRUS_ECUDA;
   TopkExpArgs x{};
@@ -831,8 +846,7 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   x.part_m = x.part_z + part;
   x.part_i = reinterpret_cast<int*>(x.part_m + part);
   x.part_ld = p.chunk;
-  x.e = grad ? e : nullptr;
-  x.lde = p.Vp;
+  x.write_e = grad != nullptr;
   for (int64_t c0 = 0; c0 < a.n; c0 += p.chunk) {
     x.rows = static_cast<int>(std::min<int64_t>(p.chunk, a.n - c0));
     x.c0 = static_cast<int>(c0);
@@ -842,17 +856,18 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
     const int splits = static_cast<int>(ceil_div(x.vtiles, x.tiles_per_split));
     x.units = x.rtiles * splits;
     x.again = nullptr;
-    int rc = topk_exp_launch(th, tw, x, stream);
+    if (grad && !make_tmap_2d_bf16(&te, e, a.V, x.rows, p.Vp, 64, 32)) return ORTHRUS_ECUDA;
+    int rc = topk_exp_launch(th, tw, te, x, stream);
     if (rc != ORTHRUS_OK) return rc;
     topk_again_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 128)), 128, 0, stream>>>(
         x.part_m, 2 * splits, x.part_ld, x.rows, x.c0, alpha, f(p.off_ref), i(p.off_again));
     ORTHRUS_CHECK_LAUNCH();
     x.again = i(p.off_again);
-    rc = topk_exp_launch(th, tw, x, stream);
+    rc = topk_exp_launch(th, tw, te, x, stream);
     if (rc != ORTHRUS_OK) return rc;
     topk_finish_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 8)), 256, 0, stream>>>(
         x.part_z, x.part_m, x.part_i, 2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, x.sid,
-        f(p.off_logq), i(p.off_top), f(p.off_mass), x.kept, a.row_weight, a.kl_rows, a.agree, x.e, x.lde,
+        f(p.off_logq), i(p.off_top), f(p.off_mass), x.kept, a.row_weight, a.kl_rows, a.agree, grad ? e : nullptr, p.Vp,
         f(p.off_scale));
     ORTHRUS_CHECK_LAUNCH();
     if (grad == nullptr) continue;

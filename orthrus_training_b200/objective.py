@@ -566,6 +566,7 @@ class _FusedTopKKL(torch.autograd.Function):
             student, values, ids, index, weight, row_weight, offsets, num_offsets, temperature, teacher_lse,
             need_grad=ctx.needs_input_grad[0], chunk_rows=max(int(chunk_size), 128))
         ctx.save_for_backward(grad)
+        ctx.set_materialize_grads(False)  # no zeros for the statistics' gradients
         outs = [kl_rows, agree] + ([kbo, abo] if offsets is not None else [])
         ctx.mark_non_differentiable(*outs)
         return (total, *outs)
@@ -573,7 +574,9 @@ class _FusedTopKKL(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_total, *unused):
         (grad,) = ctx.saved_tensors
-        return (None if grad is None else ops.lmhead_kl_backward(grad, grad_total),) + (None,) * 10
+        if grad is None or grad_total is None:
+            return (None,) * 11
+        return (ops.lmhead_kl_backward(grad, grad_total),) + (None,) * 10
 
 
 class FusedLinearTopKKL:

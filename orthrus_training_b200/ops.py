@@ -375,7 +375,7 @@ def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets
     teacher_lse = None if teacher_lse is None else teacher_lse.to(torch.float32).contiguous()
     total = torch.empty((), dtype=torch.float32, device=dev)
     kl_rows = torch.empty(n, dtype=torch.float32, device=dev)
-    agree = torch.empty(n, dtype=torch.uint8, device=dev)
+    agree = torch.empty(n, dtype=torch.bool, device=dev)  # the kernel writes bytes 0 and 1
     grad = torch.empty(n, d + pad, dtype=student.dtype, device=dev) if need_grad else None
     kbo = abo = None
     if offsets is not None:
@@ -396,7 +396,7 @@ def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets
             TIMER.end("lmhead_topk_kl", t0, 2.0 * d * V * n * (2 if need_grad else 1))
     if grad is not None and pad:
         grad = grad[:, :d]
-    return total, kl_rows, agree.bool(), grad, kbo, abo
+    return total, kl_rows, agree, grad, kbo, abo
 
 
 # --- q/k norm + RoPE ---------------------------------------------------------------------------
