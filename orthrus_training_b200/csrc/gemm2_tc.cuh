@@ -66,6 +66,7 @@ struct Gemm2Geometry {
   int splits;    // k-splits per tile (kGemm2Partial: fp32 partials, reduced by gemm2_reduce_kernel)
   int kb_split;  // k-blocks of 64 per split
   int m_pad;     // rows of one split's partial slab (M rounded up to 256)
+  int tiles_fast;  // pair tiles when the units run through them first (0: through the splits first)
 };
 
 // K-major operand tile of 128 rows: rows of 64 elements (128 B), 8-row groups 1024 B apart.
@@ -128,9 +129,11 @@ __global__ void __launch_bounds__(Gemm2Base::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // unit u = (pair tile u / splits, k-split u % splits)
+  // unit u = (pair tile u / splits, k-split u % splits), or (u % tiles, u / tiles) with tiles_fast:
+  // the units in flight then share one k-range of B, which is read from HBM once per wave
+  auto unit_split = [&](int u) { return g.tiles_fast ? u / g.tiles_fast : u % g.splits; };
   auto tile_coords = [&](int u, int& m0, int& n0, int& kb0, int& nkb) {
-    const int t = u / g.splits, sp = u % g.splits;
+    const int t = g.tiles_fast ? u % g.tiles_fast : u / g.splits, sp = unit_split(u);
     m0 = (t / g.npairs) * 256 + static_cast<int>(rank) * 128;  // this CTA's rows
     n0 = (t % g.npairs) * 256;                                   // the pair's columns
     kb0 = sp * g.kb_split;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(Gemm2Base::THREADS, 1)
       if constexpr (EPI == kGemm2Partial) {
         // fp32 partial of this k-split into rows [split * m_pad + row] of the partial slabs, in
         // 32 x 32 boxes (128-byte rows); rows past M stay inside this split's padded slab
-        const int prow0 = (t % g.splits) * g.m_pad + row0;
+        const int prow0 = unit_split(t) * g.m_pad + row0;
 #pragma unroll 1
         for (int c = 4 * half; c < 4 * half + 4; ++c) {
           reuse();
@@ -582,7 +585,7 @@ inline int gemm2_bf16_impl(const void* A, int64_t lda, int a_mn, const void* B, 
   const bool ok_a = a_mn ? make_tmap_2d_bf16(&ta, A, M, K, lda, 64, 64) : make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128);
   const bool ok_b = b_mn ? make_tmap_2d_bf16(&tb, B, N, K, ldb, 64, 64) : make_tmap_2d_bf16(&tb, B, K, N, ldb, 64, 128);
   if (!ok_a || !ok_b) return ORTHRUS_ECUDA;
-  Gemm2Geometry g;
+  Gemm2Geometry g{};
   g.M = static_cast<int>(M);
   g.N = static_cast<int>(N);
   g.K = static_cast<int>(K);
@@ -660,7 +663,7 @@ inline int gemm2_rowscale_impl(const __nv_bfloat16* A, int64_t lda, const __nv_b
   ORTHRUS_CHECK_ARG(aligned16(A) && aligned16(B) && aligned16(C));
   CUtensorMap ta, tb, tc, tr{};
   if (!make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128) || !make_tmap_2d_bf16(&tb, B, N, K, N, 64, 64)) return ORTHRUS_ECUDA;
-  Gemm2Geometry g;
+  Gemm2Geometry g{};
   g.M = static_cast<int>(M);
   g.N = static_cast<int>(N);
   g.K = static_cast<int>(K);
@@ -672,6 +675,7 @@ inline int gemm2_rowscale_impl(const __nv_bfloat16* A, int64_t lda, const __nv_b
   const int64_t tiles = ceil_div(M, 256) * g.npairs * g.splits;
   ORTHRUS_CHECK_ARG(tiles < (1ll << 31));
   g.tiles = static_cast<int>(tiles);
+  g.tiles_fast = static_cast<int>(tiles / g.splits);
   if (g.splits == 1) {
     if (!make_tmap_2d_bf16(&tc, C, N, M, N, 64, 32)) return ORTHRUS_ECUDA;
     return gemm2_launch<kGemm2RowScale, false, true>(ta, tb, tc, tr, g, reinterpret_cast<const __nv_bfloat16*>(scale), 0,

@@ -23,8 +23,8 @@
 //   grad   row factor * (chunk buffer @ W) on CTA pairs (gemm2_tc.cuh).
 // The reference c is the student's logit at the teacher's first id. bf16 has fp32's exponent range, so
 // a c up to 2^60 below the maximum loses nothing; rows with a larger logit are clamped, noticed by
-// their maximum and swept again with c = maximum (whole tiles of 256 rows; the launch ends at once where
-// there are none).
+// their maximum and swept again with c = maximum (whole tiles of 256 rows; that launch ends at once
+// where there are none).
 //
 // fp32 rows run on CUDA cores: logits = student @ W^T, a row kernel that turns a row of logits into
 // its kl and the difference (w / T) (Q p - q), and grad = difference @ W.
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(128)
   __shared__ int redi[4];
   const int64_t t = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_launch_dependents();
   int n2 = 1;
   while (n2 < k) n2 <<= 1;
   float best = -INFINITY;
@@ -301,13 +302,16 @@ __global__ void __launch_bounds__(128)
 }
 
 // One warp per student row: its teacher row (-1 if the index is out of range) and its reference
-// c = log2(e) / T * (student . W[top_id]); clears the tiles' second-sweep flags.
+// c = log2(e) / T * (student . W[top_id]); clears the second sweep's references and flags.
 __global__ void __launch_bounds__(256)
     topk_student_kernel(const __nv_bfloat16* __restrict__ student, const __nv_bfloat16* __restrict__ W, int64_t n,
                         int64_t m, int D, const int64_t* __restrict__ index, const int* __restrict__ top_id,
-                        float alpha, int* __restrict__ trow, float* __restrict__ ref, int* __restrict__ again) {
+                        float alpha, int* __restrict__ trow, float* __restrict__ ref, unsigned* __restrict__ over,
+                        int* __restrict__ again) {
   const int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  griddep_launch_dependents();
+  griddep_wait();  // launched as a programmatic dependent
   if (r >= n) return;
   int64_t t = index ? index[r] : r;
   if (t < 0 || t >= m) {
@@ -334,8 +338,19 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) {
     trow[r] = static_cast<int>(t);
     ref[r] = dot * alpha;
+    over[r] = 0;
     if (r % 256 == 0) again[r / 256] = 0;
   }
+}
+
+// The reference of a row: its largest logit where the first sweep left one in `over` (as an ordered
+// integer, 0: none), else the logit at the teacher's first id.
+__device__ __forceinline__ unsigned topk_over_key(float x) {
+  const unsigned b = __float_as_uint(x);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float topk_reference(float ref, unsigned over) {
+  return over == 0 ? ref : __uint_as_float((over & 0x80000000u) ? (over & 0x7FFFFFFFu) : ~over);
 }
 
 struct TopkExpTile {
@@ -358,7 +373,9 @@ struct TopkExpArgs {
   const int* trow;        // [n]
   const float* ref;       // [n]
   const int* sid;         // [m, k]
-  const int* again;       // [ceil(n / 256)]: the second sweep takes the flagged tiles only; null: all
+  unsigned* over;         // [n]
+  int* again;             // [ceil(n / 256)]: tiles with a row above the exponent limit
+  bool second;            // the second sweep takes the flagged tiles only
   float* kept;            // [chunk, k] student logits at the sorted ids
   float* part_z;          // [2 splits, chunk], as part_m and part_i
   float* part_m;
@@ -418,17 +435,20 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   __syncthreads();
   cluster_sync_all();  // the peer's barriers are initialised before anyone signals them
+  // launched as a programmatic dependent: the set-up above overlaps the previous kernel's tail
+  griddep_launch_dependents();
+  griddep_wait();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   // unit u = (row tile u % rtiles, vocabulary range u / rtiles); the same tiles for every role of
-  // both CTAs (the flags do not change during the launch)
+  // both CTAs (the flags do not change during the second sweep)
   auto unit_tiles = [&](int u, int& row0, int& split, int& t0) {
     const int rt = u % a.rtiles;
     split = u / a.rtiles;
     row0 = rt * 256 + static_cast<int>(rank) * T::BM;  // this CTA's first row in the chunk
     t0 = split * a.tiles_per_split;
-    if (a.again != nullptr && a.again[a.c0 / 256 + rt] == 0) return 0;
+    if (a.second && a.again[a.c0 / 256 + rt] == 0) return 0;
     return max(min(a.vtiles, t0 + a.tiles_per_split) - t0, 0);
   };
 
@@ -509,7 +529,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
       if (ntiles == 0) continue;
       const int crow = row0 + quarter * 32 + lane;  // row in the chunk
       const bool live = crow < a.rows;
-      const float ref = live ? a.ref[a.c0 + crow] : 0.f;
+      const float ref = live ? topk_reference(a.ref[a.c0 + crow], a.second ? a.over[a.c0 + crow] : 0u) : 0.f;
       const int trow = live ? a.trow[a.c0 + crow] : -1;
       // the row's sorted ids from this unit's first column on
       const int* sid = a.sid + static_cast<int64_t>(trow < 0 ? 0 : trow) * a.k;
@@ -623,6 +643,10 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
         a.part_z[o] = z;
         a.part_m[o] = m;
         a.part_i[o] = idx;
+        if (!a.second && fmaf(m, a.alpha, -ref) > kTopkExpLimit) {
+          atomicMax(&a.over[a.c0 + crow], topk_over_key(m * a.alpha));
+          a.again[(a.c0 + crow) / 256] = 1;
+        }
       }
     }
     if (lane == 0) tma_store_wait_all();
@@ -635,30 +659,19 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
   }
 }
 
-// Rows whose maximum lies above the exponent limit get it as their reference, and their tile a flag.
-__global__ void topk_again_kernel(const float* __restrict__ part_m, int parts, int64_t part_ld, int rows, int c0,
-                                  float alpha, float* __restrict__ ref, int* __restrict__ again) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= rows) return;
-  float m = -INFINITY;
-  for (int s = 0; s < parts; ++s) m = fmaxf(m, part_m[s * part_ld + r]);
-  if (fmaf(m, alpha, -ref[c0 + r]) > kTopkExpLimit) {
-    ref[c0 + r] = m * alpha;
-    again[(c0 + r) / 256] = 1;
-  }
-}
-
 // One warp per row of the chunk: z and the first maximum from the partials (a fixed order), the row's
 // kl and agreement, the kept entries of the chunk buffer and the row factor of the gradient.
 __global__ void __launch_bounds__(256)
     topk_finish_kernel(const float* __restrict__ part_z, const float* __restrict__ part_m,
                        const int* __restrict__ part_i, int parts, int64_t part_ld, int rows, int c0, int k, float alpha,
                        float T, const int* __restrict__ trow, const float* __restrict__ ref,
-                       const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
+                       const unsigned* __restrict__ over, const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
                        const float* __restrict__ mass, const float* __restrict__ kept,
                        const float* __restrict__ row_weight, float* __restrict__ kl_rows, uint8_t* __restrict__ agree,
                        __nv_bfloat16* __restrict__ e, int64_t lde, float* __restrict__ scale) {
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  griddep_launch_dependents();
+  griddep_wait();  // launched as a programmatic dependent
   if (r >= rows) return;
   const int64_t g = c0 + r;
   float z = 0.f, m = -INFINITY;
@@ -684,7 +697,7 @@ __global__ void __launch_bounds__(256)
   }
   const int t = trow[g];
   const float Q = t >= 0 ? mass[t] : 0.f;
-  const float logz = logf(z), c = ref[g];
+  const float logz = logf(z), c = topk_reference(ref[g], over[g]);
   float kl = 0.f;
   if (t >= 0 && Q != 0.f) {
     const int* id = sid + static_cast<int64_t>(t) * k;
@@ -718,7 +731,7 @@ struct TopkKlPlan {
   int64_t chunk, Vp;
   int splits;  // most vocabulary ranges of a chunk's sweep
   size_t off_buf, off_gemm, gemm_bytes;
-  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_again, off_kept, off_part, off_scale;
+  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_over, off_again, off_kept, off_part, off_scale;
   size_t total;
 };
 
@@ -747,6 +760,7 @@ inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64
     p.off_mass = take(static_cast<size_t>(m) * 4);
     p.off_trow = take(static_cast<size_t>(n) * 4);
     p.off_ref = take(static_cast<size_t>(n) * 4);
+    p.off_over = take(static_cast<size_t>(n) * 4);
     p.off_again = take(static_cast<size_t>(ceil_div(n, 256)) * 4);
     p.off_kept = take(static_cast<size_t>(p.chunk) * k * 4);
     p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 12);
@@ -799,13 +813,15 @@ inline int topk_exp_launch(const CUtensorMap& th, const CUtensorMap& tw, const C
   cfg.blockDim = dim3(TopkExpTile::THREADS);
   cfg.dynamicSmemBytes = TopkExpTile::SMEM;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   ORTHRUS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, topk_exp_kernel, th, tw, te, a));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
@@ -825,8 +841,10 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
                                                                       i(p.off_sid), f(p.off_logq), i(p.off_top),
                                                                       f(p.off_mass));
   ORTHRUS_CHECK_LAUNCH();
-  topk_student_kernel<<<static_cast<unsigned>(ceil_div(a.n, 8)), 256, 0, stream>>>(
-      student, W, a.n, a.m, D, a.index, i(p.off_top), alpha, i(p.off_trow), f(p.off_ref), i(p.off_again));
+  auto* over = reinterpret_cast<unsigned*>(ws + p.off_over);
+  ORTHRUS_CHECK_CUDA(launch_pdl(topk_student_kernel, dim3(static_cast<unsigned>(ceil_div(a.n, 8))), dim3(256), 0, stream,
+                                student, W, a.n, a.m, D, a.index, static_cast<const int*>(i(p.off_top)), alpha,
+                                i(p.off_trow), f(p.off_ref), over, i(p.off_again)));
   ORTHRUS_CHECK_LAUNCH();
   CUtensorMap th, tw, te{};
   if (!make_tmap_2d_bf16(&th, student, a.D, a.n, a.D, 64, 128)) return ORTHRUS_ECUDA;
@@ -839,6 +857,8 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   x.alpha = alpha;
   x.trow = i(p.off_trow);
   x.ref = f(p.off_ref);
+  x.over = over;
+  x.again = i(p.off_again);
   x.sid = i(p.off_sid);
   x.kept = f(p.off_kept);
   const size_t part = static_cast<size_t>(p.chunk) * 2 * p.splits;
@@ -855,20 +875,20 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
         static_cast<int>(ceil_div(x.vtiles, pick_splits(x.rtiles, x.vtiles, num_sms() / 2, p.splits)));
     const int splits = static_cast<int>(ceil_div(x.vtiles, x.tiles_per_split));
     x.units = x.rtiles * splits;
-    x.again = nullptr;
+    x.second = false;
     if (grad && !make_tmap_2d_bf16(&te, e, a.V, x.rows, p.Vp, 64, 32)) return ORTHRUS_ECUDA;
     int rc = topk_exp_launch(th, tw, te, x, stream);
     if (rc != ORTHRUS_OK) return rc;
-    topk_again_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 128)), 128, 0, stream>>>(
-        x.part_m, 2 * splits, x.part_ld, x.rows, x.c0, alpha, f(p.off_ref), i(p.off_again));
-    ORTHRUS_CHECK_LAUNCH();
-    x.again = i(p.off_again);
+    x.second = true;
     rc = topk_exp_launch(th, tw, te, x, stream);
     if (rc != ORTHRUS_OK) return rc;
-    topk_finish_kernel<<<static_cast<unsigned>(ceil_div(x.rows, 8)), 256, 0, stream>>>(
-        x.part_z, x.part_m, x.part_i, 2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, x.sid,
-        f(p.off_logq), i(p.off_top), f(p.off_mass), x.kept, a.row_weight, a.kl_rows, a.agree, grad ? e : nullptr, p.Vp,
-        f(p.off_scale));
+    ORTHRUS_CHECK_CUDA(launch_pdl(
+        topk_finish_kernel, dim3(static_cast<unsigned>(ceil_div(x.rows, 8))), dim3(256), 0, stream,
+        static_cast<const float*>(x.part_z), static_cast<const float*>(x.part_m), static_cast<const int*>(x.part_i),
+        2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, static_cast<const unsigned*>(over), x.sid,
+        static_cast<const float*>(f(p.off_logq)), static_cast<const int*>(i(p.off_top)),
+        static_cast<const float*>(f(p.off_mass)), static_cast<const float*>(x.kept), a.row_weight, a.kl_rows, a.agree,
+        grad ? e : nullptr, p.Vp, f(p.off_scale)));
     ORTHRUS_CHECK_LAUNCH();
     if (grad == nullptr) continue;
     rc = gemm2_rowscale_impl(e, p.Vp, W, grad + c0 * a.D, f(p.off_scale), x.rows, a.D, a.V, ws + p.off_gemm,
