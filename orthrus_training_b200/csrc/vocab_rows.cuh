@@ -7,6 +7,13 @@
 // through distributed shared memory. So the bytes moved are the row itself, whatever the filters
 // need.
 //
+// The k largest entries come from a bound: the k-th largest of the threads' own maxima (512 a CTA)
+// is at most the k-th largest entry, and little below it unless the row is arranged against it, so
+// the few entries above that bound are gathered into one CTA and ordered there. A nucleus without a
+// top-k is found by a 512-bin histogram of weights over the values that can hold its border, then
+// exactly among the border bin's entries. Where the gathered entries are too many (rows of equal
+// values), a radix selection over the whole cluster, right for every row, takes over.
+//
 // Candidates are the entries that are neither -inf nor NaN. Entries are ordered by (descending
 // value, ascending index); -0 counts as +0.
 #pragma once
@@ -21,6 +28,8 @@ constexpr int kRowThreads = 512;
 constexpr int kRowBins = 2048;
 constexpr int kRowMaxCluster = 8;  // portable cluster size
 constexpr int kRowMaxK = 1024;     // largest k of topk_rows
+constexpr int kRowList = 2048;     // most entries gathered into one CTA
+constexpr int kRowNucleusBins = 512;
 
 // ------------------------------------------------------------------------------------------------
 // Keys: unsigned integers that order as the values do; 0 marks an entry that is no candidate.
@@ -92,12 +101,15 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t* p, uint32_t rank) {
 }
 
 struct RowShared {
-  uint64_t hist[kRowBins];   // counts (as the low 32-bit words of the first half) or masses
-  uint64_t list[kRowMaxK];   // leader: (key << 32 | ~index) of the chosen entries, then sorted
+  uint64_t hist[kRowBins];   // radix selection: counts (as 32-bit words) or masses; else a second list
+  uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
   double exp_tab[64];        // 2^(-j/64)
   uint64_t warp_u64[kRowThreads / 32];
+  uint64_t warp_count[2][kRowThreads / 32];
   uint64_t slot[8];          // this CTA's published partials, one use each between barriers
   uint64_t found[2];         // result of a block-wide search
+  uint32_t tmax[kRowThreads];  // the threads' largest keys
+  uint32_t listed;           // entries in the list
 };
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -235,6 +247,32 @@ __device__ __forceinline__ void row_stage(const T* __restrict__ p, int n, typena
   if (tail + static_cast<int>(threadIdx.x) < n) scalar(tail + threadIdx.x);  // fewer than VEC
 }
 
+// Visits the entries that row_stage gave this thread: f(index in the slice, key).
+template <typename T, typename F>
+__device__ __forceinline__ void row_own(const typename RowKey<T>::type* keys, int off, int n, F f) {
+  constexpr int VEC = RowKey<T>::VEC;
+  const int head = min(n, (VEC - off) % VEC);
+  const int t = threadIdx.x;
+  if (t < head) f(t, static_cast<uint32_t>(keys[t]));
+  const int nvec = (n - head) / VEC;
+  const uint4* src = reinterpret_cast<const uint4*>(keys + head);
+  for (int v = t; v < nvec; v += kRowThreads) {
+    const uint4 q = src[v];
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 4) {
+        f(head + 4 * v + e, w[e]);
+      } else {
+        f(head + 8 * v + 2 * e, w[e] & 0xFFFFu);
+        f(head + 8 * v + 2 * e + 1, w[e] >> 16);
+      }
+    }
+  }
+  const int tail = head + nvec * VEC;
+  if (tail + t < n) f(tail + t, static_cast<uint32_t>(keys[tail + t]));
+}
+
 // ------------------------------------------------------------------------------------------------
 // Softmax weights as 64-bit integers
 // ------------------------------------------------------------------------------------------------
@@ -362,6 +400,110 @@ __device__ uint32_t row_radix_select(const typename RowKey<T>::type* keys, const
 }
 
 // ------------------------------------------------------------------------------------------------
+// The few largest entries
+// ------------------------------------------------------------------------------------------------
+
+// A key with at least k entries of the cluster's row at or above it, and not many more: between
+// the k-th largest thread maximum and a little below it. Four-way search on counts of the maxima
+// (published in tmax before the last cluster barrier), the same in every CTA.
+__device__ __forceinline__ uint32_t row_bound(int k, uint32_t top_key, RowShared& sh, uint32_t cs) {
+  uint32_t mk[kRowMaxCluster];
+  uint32_t least = 0xFFFFFFFFu, some = 0;
+#pragma unroll
+  for (int c = 0; c < kRowMaxCluster; ++c) {
+    mk[c] = c < static_cast<int>(cs) ? peer_u32(&sh.tmax[threadIdx.x], c) : 0u;
+    if (mk[c]) {
+      least = min(least, mk[c]);
+      ++some;
+    }
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // three counters of 21 bits a word; `buf` alternates, so one barrier an exchange is enough
+  auto total = [&](uint32_t a, uint32_t b, uint32_t c, int buf) {
+    a = __reduce_add_sync(0xffffffffu, a);
+    b = __reduce_add_sync(0xffffffffu, b);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) sh.warp_count[buf][warp] = a | (static_cast<uint64_t>(b) << 21) | (static_cast<uint64_t>(c) << 42);
+    __syncthreads();
+    uint64_t t = 0;
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 32; ++w) t += sh.warp_count[buf][w];
+    return t;
+  };
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (lane == 0) sh.warp_u64[warp] = least;
+  uint32_t have = static_cast<uint32_t>(total(some, 0, 0, 0) & 0x1FFFFF);
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 32; ++w) least = min(least, static_cast<uint32_t>(sh.warp_u64[w]));
+  if (have < static_cast<uint32_t>(k)) return 1u;
+  uint32_t lo = least, hi = top_key + 1;  // at least k maxima at or above lo, fewer at or above hi
+  const uint32_t enough = k + k / 4 + 16;
+  for (int step = 1; have > enough && hi - lo > 1; ++step) {
+    const uint32_t d = hi - lo;
+    const uint32_t t1 = lo + (d + 3) / 4, t2 = lo + (d + 1) / 2, t3 = lo + d - d / 4;
+    uint32_t a = 0, b = 0, c = 0;
+#pragma unroll
+    for (int i = 0; i < kRowMaxCluster; ++i) {
+      a += mk[i] >= t1;
+      b += mk[i] >= t2;
+      c += mk[i] >= t3;
+    }
+    const uint64_t t = total(a, b, c, step & 1);
+    a = static_cast<uint32_t>(t) & 0x1FFFFF;
+    b = static_cast<uint32_t>(t >> 21) & 0x1FFFFF;
+    c = static_cast<uint32_t>(t >> 42);
+    const uint32_t want = k;
+    if (c >= want) {
+      lo = t3;
+      have = c;
+    } else if (b >= want) {
+      lo = t2;
+      hi = t3;
+      have = b;
+    } else if (a >= want) {
+      lo = t1;
+      hi = t2;
+      have = a;
+    } else {
+      hi = t1;
+    }
+  }
+  __syncthreads();  // warp_u64 and warp_count are free again
+  return lo;
+}
+
+// Appends this thread's entries with low <= key < high to the CTA's list (listed counts them, past
+// the list's end too). `listed` is 0 and visible before; a block barrier follows.
+template <typename T>
+__device__ __forceinline__ void row_gather(const typename RowKey<T>::type* keys, int off, const RowSlice& sl,
+                                           uint32_t low, uint32_t high, RowShared& sh) {
+  row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
+    if (key >= low && key < high) {
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i);
+    }
+  });
+}
+
+// Entries listed in the whole cluster (after a cluster barrier).
+__device__ __forceinline__ uint32_t row_listed(RowShared& sh, uint32_t cs) {
+  uint32_t n = 0;
+  for (uint32_t c = 0; c < cs; ++c) n += peer_u32(&sh.listed, c);
+  return n;
+}
+
+// Leader: copies every CTA's list to `out`, at most kRowList entries in all.
+__device__ __forceinline__ void row_collect(uint64_t* out, RowShared& sh, uint32_t cs) {
+  uint32_t at = 0;
+  for (uint32_t c = 0; c < cs; ++c) {
+    const uint32_t n = peer_u32(&sh.listed, c);
+    for (uint32_t j = threadIdx.x; j < n; j += kRowThreads) out[at + j] = peer_u64(&sh.list[j], c);
+    at += n;
+  }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------------------
 // Top-k
 // ------------------------------------------------------------------------------------------------
 
@@ -382,21 +524,34 @@ __device__ __forceinline__ void row_sort_desc(uint64_t* a, int n2) {
   __syncthreads();
 }
 
-// Sum over the thread's staged entries of exp((x - top) / T), `c` = log2(e) / T.
-template <typename T>
-__device__ __forceinline__ float row_exp_sum(const typename RowKey<T>::type* keys, int n, float top, float c) {
-  float s = 0.f;
-  for (int i = threadIdx.x; i < n; i += kRowThreads) {
-    const uint32_t k = keys[i];
-    if (k) s += ex2_approx((RowKey<T>::value(k) - top) * c);
+// Orders `in` (n <= kRowList different entries) descending into `out` (not the same array): by rank
+// counting for a few entries, several threads an entry; else by a sorting network on `in`.
+__device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n, RowShared& sh) {
+  if (n <= kRowThreads) {
+    int parts = 32;
+    while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
+    const int e = threadIdx.x / parts, part = threadIdx.x % parts;
+    const uint64_t x = e < n ? in[e] : 0;
+    int rank = 0;
+    if (e < n)
+      for (int j = part; j < n; j += parts) rank += in[j] > x;
+    for (int o = parts >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (e < n && part == 0) out[rank] = x;
+    __syncthreads();
+    return;
   }
-  return s;
+  int n2 = 1;
+  while (n2 < n) n2 <<= 1;
+  for (int i = n + threadIdx.x; i < n2; i += kRowThreads) in[i] = 0;
+  row_sort_desc(in, n2);
+  for (int i = threadIdx.x; i < n; i += kRowThreads) out[i] = in[i];
+  __syncthreads();
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int per,
-                                                                 int k, float temperature, float* __restrict__ values,
-                                                                 int64_t* __restrict__ ids, float* __restrict__ lse) {
+__global__ void __launch_bounds__(kRowThreads, 2)
+    topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int per, int k, float temperature,
+                     float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   using K = RowKey<T>;
   extern __shared__ __align__(16) uint8_t row_smem[];
   __shared__ RowShared sh;
@@ -406,82 +561,122 @@ __global__ void __launch_bounds__(kRowThreads) topk_rows_kernel(const T* __restr
   const int64_t row = blockIdx.x / cs;
   const RowSlice sl(V, per, rank);
   const T* p = x + row * ldx + sl.lo;
-  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + row_stage_offset(p);
+  const int off = row_stage_offset(p);
+  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + off;
   uint32_t best, count;
+  if (threadIdx.x == 0) sh.listed = 0;
   row_stage<T>(p, sl.n, keys, best, count);
-  const uint64_t bmax = block_max_u64(best, sh), bcount = block_sum_u64(count, sh);
+  sh.tmax[threadIdx.x] = best;
+  // maximum and count of the slice in one exchange: a key of 32 bits over a count of 32
+  const uint32_t wbest = __reduce_max_sync(0xffffffffu, best), wcount = __reduce_add_sync(0xffffffffu, count);
+  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = (static_cast<uint64_t>(wbest) << 32) | wcount;
+  __syncthreads();
+  uint32_t bmax = 0, bcount = 0;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 32; ++w) {
+    bmax = max(bmax, static_cast<uint32_t>(sh.warp_u64[w] >> 32));
+    bcount += static_cast<uint32_t>(sh.warp_u64[w]);
+  }
+  // the slice's sum of exp((x - its maximum) / T)
+  const float btop = K::value(bmax);
+  const float c = kLog2e / temperature;
+  float part = 0.f;
+  if (bmax && btop < INFINITY)
+    row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
+      part += key ? ex2_approx((K::value(key) - btop) * c) : 0.f;
+    });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  if ((threadIdx.x & 31) == 0) sh.warp_count[1][threadIdx.x >> 5] = __float_as_uint(part);
+  __syncthreads();
   if (threadIdx.x == 0) {
-    sh.slot[0] = bmax;
-    sh.slot[1] = bcount;
+    float s = 0.f;
+    for (int w = 0; w < kRowThreads / 32; ++w) s += __uint_as_float(static_cast<uint32_t>(sh.warp_count[1][w]));
+    sh.slot[0] = (static_cast<uint64_t>(bmax) << 32) | bcount;
+    sh.slot[1] = __float_as_uint(s);
   }
   row_cluster_sync();
-  uint32_t top_key = 0;
-  uint64_t candidates = 0;
+  uint32_t top_key = 0, candidates = 0;
   for (uint32_t r = 0; r < cs; ++r) {
-    top_key = max(top_key, static_cast<uint32_t>(peer_u64(&sh.slot[0], r)));
-    candidates += peer_u64(&sh.slot[1], r);
+    const uint64_t e = peer_u64(&sh.slot[0], r);
+    top_key = max(top_key, static_cast<uint32_t>(e >> 32));
+    candidates += static_cast<uint32_t>(e);
   }
-  const float top = K::value(top_key);
-  // the row's exponential sum, published with the tie counts below (64 fractional bits of a double)
-  const float part = top_key && top < INFINITY ? row_exp_sum<T>(keys, sl.n, top, kLog2e / temperature) : 0.f;
-  const uint64_t fixed = block_sum_u64(__double2ull_rn(static_cast<double>(part) * 1099511627776.0), sh);  // 2^40
-  const int kk = static_cast<int>(candidates < static_cast<uint64_t>(k) ? candidates : k);
-  uint32_t cut = 0;
-  uint64_t n_gt = 0;
-  RowWeight none{};
-  if (kk > 0) cut = row_radix_select<T, false>(keys, sl, 1u, kk - 1, none, sh, cs, n_gt);
-  // index-ordered compaction: larger keys first, then the lowest-index equals
-  uint32_t gt = 0, eq = 0;
-  if (kk > 0)
-    for (int i = sl.begin(); i < sl.end(); ++i) {
-      const uint32_t key = keys[i];
-      gt += key > cut;
-      eq += key == cut;
-    }
-  uint64_t total;
-  const uint64_t at = block_exclusive_u64((static_cast<uint64_t>(gt) << 32) | eq, sh, total);
-  if (threadIdx.x == 0) {
-    sh.slot[2] = total;
-    sh.slot[3] = fixed;
+  const int kk = static_cast<int>(min(candidates, static_cast<uint32_t>(k)));
+  if (rank == 0 && threadIdx.x < 32) {  // lane r brings CTA r's sum to the row's maximum
+    const uint32_t r = threadIdx.x;
+    const double top = K::value(top_key);
+    double s = 0.0;
+    const uint32_t m = r < cs ? static_cast<uint32_t>(peer_u64(&sh.slot[0], r) >> 32) : 0u;
+    if (m)
+      s = __uint_as_float(static_cast<uint32_t>(peer_u64(&sh.slot[1], r))) *
+          exp((static_cast<double>(K::value(m)) - top) / temperature);
+#pragma unroll
+    for (int o = kRowMaxCluster / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (r == 0)
+      lse[row] = top_key == 0 ? -INFINITY : !(top < INFINITY) ? INFINITY : static_cast<float>(top / temperature + log(s));
   }
-  row_cluster_sync();
-  uint64_t base = 0;
-  for (uint32_t r = 0; r < rank; ++r) base += peer_u64(&sh.slot[2], r);
-  uint32_t at_gt = static_cast<uint32_t>((base + at) >> 32), at_eq = static_cast<uint32_t>(base + at);
-  const uint32_t room = static_cast<uint32_t>(kk - n_gt);
-  const uint32_t list0 = mapa_shared(smem_u32(sh.list), 0);
-  if (kk > 0 && (gt || eq))
-    for (int i = sl.begin(); i < sl.end(); ++i) {
-      const uint32_t key = keys[i];
-      if (key < cut) continue;
-      uint32_t pos;
-      if (key > cut)
-        pos = at_gt++;
-      else if (at_eq < room)
-        pos = static_cast<uint32_t>(n_gt) + at_eq++;
-      else
-        continue;
-      st_cluster_u64(list0 + pos * 8, (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i));
+  uint64_t* ordered = sh.hist;
+  int have = 0;
+  if (kk > 0) {
+    const uint32_t bound = row_bound(kk, top_key, sh, cs);
+    if (best >= bound) row_gather<T>(keys, off, sl, bound, 0xFFFFFFFFu, sh);
+    row_cluster_sync();
+    const uint32_t n = row_listed(sh, cs);
+    if (n <= kRowList) {
+      have = static_cast<int>(n);
+      if (rank == 0) row_collect(sh.hist, sh, cs);
+      row_cluster_sync();  // nothing of another CTA is read after this
+      if (rank != 0) return;
+      row_order(sh.hist, sh.list, have, sh);
+      ordered = sh.list;
+    } else {
+      uint64_t n_gt;
+      RowWeight none{};
+      const uint32_t cut = row_radix_select<T, false>(keys, sl, 1u, kk - 1, none, sh, cs, n_gt);
+      // index-ordered compaction: larger keys first, then the lowest-index equals
+      uint32_t gt = 0, eq = 0;
+      for (int i = sl.begin(); i < sl.end(); ++i) {
+        const uint32_t key = keys[i];
+        gt += key > cut;
+        eq += key == cut;
+      }
+      uint64_t total;
+      const uint64_t at = block_exclusive_u64((static_cast<uint64_t>(gt) << 32) | eq, sh, total);
+      if (threadIdx.x == 0) sh.slot[2] = total;
+      row_cluster_sync();
+      uint64_t base = at;
+      for (uint32_t r = 0; r < rank; ++r) base += peer_u64(&sh.slot[2], r);
+      uint32_t at_gt = static_cast<uint32_t>(base >> 32), at_eq = static_cast<uint32_t>(base);
+      const uint32_t room = static_cast<uint32_t>(kk - n_gt);
+      const uint32_t list0 = mapa_shared(smem_u32(sh.list), 0);
+      if (gt || eq)
+        for (int i = sl.begin(); i < sl.end(); ++i) {
+          const uint32_t key = keys[i];
+          if (key < cut) continue;
+          uint32_t pos;
+          if (key > cut)
+            pos = at_gt++;
+          else if (at_eq < room)
+            pos = static_cast<uint32_t>(n_gt) + at_eq++;
+          else
+            continue;
+          st_cluster_u64(list0 + pos * 8, (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i));
+        }
+      row_cluster_sync();  // the list is complete; nothing of another CTA is read after this
+      if (rank != 0) return;
+      have = kk;
+      row_order(sh.list, sh.hist, have, sh);
+      ordered = sh.hist;
     }
-  uint64_t sum = 0;
-  if (rank == 0)
-    for (uint32_t r = 0; r < cs; ++r) sum += peer_u64(&sh.slot[3], r);
-  row_cluster_sync();  // the list is complete; nothing of another CTA is read after this
-  if (rank != 0) return;
-  int n2 = 1;
-  while (n2 < kk) n2 <<= 1;
-  for (int i = kk + threadIdx.x; i < n2; i += kRowThreads) sh.list[i] = 0;
-  row_sort_desc(sh.list, n2);
+  } else {
+    row_cluster_sync();  // the leader has read the slots
+    if (rank != 0) return;
+  }
   for (int i = threadIdx.x; i < k; i += kRowThreads) {
-    const uint64_t e = i < kk ? sh.list[i] : 0;
+    const uint64_t e = i < kk ? ordered[i] : 0;
     values[row * k + i] = i < kk ? K::value(static_cast<uint32_t>(e >> 32)) : -INFINITY;
     ids[row * k + i] = i < kk ? static_cast<int64_t>(~static_cast<uint32_t>(e)) : -1;
-  }
-  if (threadIdx.x == 0) {
-    const double s = static_cast<double>(sum) / 1099511627776.0;
-    lse[row] = top_key == 0 ? -INFINITY
-               : !(top < INFINITY) ? INFINITY
-                                   : static_cast<float>(static_cast<double>(top) / temperature + log(s));
   }
 }
 
@@ -498,10 +693,147 @@ struct SampleKnobs {
   int top_k1;
 };
 
+// Order-preserving integer of a number, rounded down to the key's bits: every entry at or above x has a
+// key at or above this.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int per,
-                                                                     int S, const float* __restrict__ uniform,
-                                                                     SampleKnobs knobs, int64_t* __restrict__ tokens) {
+__device__ __forceinline__ uint32_t row_key_floor(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) >> (32 - RowKey<T>::BITS);
+}
+
+// The border of the nucleus among all candidates: the key `cut` of its last entry and how many of
+// the entries with that key are inside (`ties`); `mass` is the weight of all candidates. The entries
+// that weigh at most (mass - target - 1) / V together weigh less than mass - target, so the border
+// lies above them: only the others are counted, in bins even in x. False where the border's bin
+// holds too many entries (the caller then selects by radix).
+template <typename T>
+__device__ bool row_nucleus(const typename RowKey<T>::type* keys, int off, const RowSlice& sl, int V, float T_,
+                            uint64_t mass, uint64_t target, const RowWeight& weight, RowShared& sh, uint32_t cs,
+                            uint32_t& cut, uint64_t& ties) {
+  using K = RowKey<T>;
+  const float top = weight.top;
+  // how far below the maximum (times T) a border can lie, with a margin that covers the fp32 arithmetic;
+  // weights are rounded, so one of light + 1 stands for light + 1/2 or more
+  const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(V);
+  const float depth = (static_cast<float>(weight.S) - log2f(static_cast<float>(light) + 0.5f)) * kLn2 + 1e-3f;
+  const float range = depth * T_ + 1e-5f * fabsf(top);
+  if (!(top < INFINITY) || !(range < INFINITY)) return false;  // the same in every CTA
+  const float inv = static_cast<float>(kRowNucleusBins) / range;
+  const uint32_t low = row_key_floor<T>(top - range);
+  auto bin = [&](uint32_t key) { return min(kRowNucleusBins - 1, static_cast<int>((top - K::value(key)) * inv)); };
+  sh.hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.found[0] = ~0ull;
+  __syncthreads();
+  row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
+    if (key < low || key == 0u) return;
+    const uint64_t w = weight(K::value(key));
+    if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin(key)]), static_cast<unsigned long long>(w));
+  });
+  row_cluster_sync();
+  uint64_t h = 0, total;
+  for (uint32_t c = 0; c < cs; ++c) h += peer_u64(&sh.hist[threadIdx.x], c);
+  const uint64_t run = block_exclusive_u64(h, sh, total);
+  if (run <= target && target < run + h) {
+    sh.found[0] = threadIdx.x;
+    sh.found[1] = run;
+  }
+  __syncthreads();
+  const uint64_t border = sh.found[0];
+  uint64_t before = sh.found[1];
+  if (border != ~0ull)
+    row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
+      if (key < low || key == 0u || bin(key) != static_cast<int>(border)) return;
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i);
+    });
+  row_cluster_sync();
+  const uint32_t n = row_listed(sh, cs);
+  constexpr int MOST = kRowList / 2;
+  if (border == ~0ull || n > MOST) {
+    row_cluster_sync();  // nobody reads the bins any more
+    return false;
+  }
+  // every CTA orders the border bin's entries for itself and finds the entry that holds the target
+  row_collect(sh.hist, sh, cs);
+  uint64_t* sorted = sh.hist + MOST;
+  row_order(sh.hist, sorted, n, sh);
+  constexpr int PER = MOST / kRowThreads;
+  uint64_t w[PER], own = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const uint32_t at = threadIdx.x * PER + j;
+    w[j] = at < n ? weight(K::value(static_cast<uint32_t>(sorted[at] >> 32))) : 0;
+    own += w[j];
+  }
+  before += block_exclusive_u64(own, sh, total);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (before <= target && target < before + w[j]) {
+      const int at = threadIdx.x * PER + j;
+      const uint32_t key = static_cast<uint32_t>(sorted[at] >> 32);
+      int first = at;
+      while (first > 0 && static_cast<uint32_t>(sorted[first - 1] >> 32) == key) --first;
+      sh.found[0] = key;
+      sh.found[1] = at - first + 1;
+    }
+    before += w[j];
+  }
+  __syncthreads();
+  cut = static_cast<uint32_t>(sh.found[0]);
+  ties = sh.found[1];
+  return true;
+}
+
+// The leader's part of a top-k sample: `merged` holds n entries, the top_k largest and every tie of
+// the last among them. Filters them and picks the token.
+template <typename T>
+__device__ void row_pick_listed(uint64_t* merged, uint64_t* sorted, int n, int top_k, float top_p, uint64_t least,
+                                float uniform, const RowWeight& weight, RowShared& sh, int64_t* __restrict__ token) {
+  using K = RowKey<T>;
+  row_order(merged, sorted, n, sh);
+  const uint32_t kth = static_cast<uint32_t>(sorted[top_k - 1] >> 32);
+  constexpr int PER = kRowList / kRowThreads;
+  uint64_t w[PER], own = 0, total;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    const uint32_t key = at < n ? static_cast<uint32_t>(sorted[at] >> 32) : 0u;
+    w[j] = at < n && key >= kth ? weight(K::value(key)) : 0;
+    own += w[j];
+  }
+  uint64_t before = block_exclusive_u64(own, sh, total);
+  const uint64_t target = top_p < 1.f ? floor_share(top_p, total) : ~0ull;
+  own = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    const uint64_t kept = before <= target && w[j] >= least ? w[j] : 0;
+    before += w[j];
+    own += kept;
+    if (at < n) merged[at] = kept;  // merged has been read by row_order
+  }
+  const uint64_t all = block_sum_u64(own, sh);
+  const uint64_t aim = floor_share(uniform, all);
+  // the running sum before an entry in index order is the weight of the kept entries of lower index
+  int parts = 32;
+  while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
+  const int stride = kRowThreads / parts, part = threadIdx.x % parts;
+  for (int e0 = 0; e0 < n; e0 += stride) {
+    const int e = e0 + threadIdx.x / parts;
+    const uint32_t place = e < n ? static_cast<uint32_t>(sorted[e]) : 0u;
+    uint64_t run = 0;
+    if (e < n)
+      for (int j = part; j < n; j += parts)
+        if (static_cast<uint32_t>(sorted[j]) > place) run += merged[j];
+    for (int o = parts >> 1; o > 0; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+    if (e < n && part == 0 && run <= aim && aim < run + merged[e]) *token = ~place;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int per, int S,
+                         const float* __restrict__ uniform, SampleKnobs knobs, int64_t* __restrict__ tokens) {
   using K = RowKey<T>;
   extern __shared__ __align__(16) uint8_t row_smem[];
   __shared__ RowShared sh;
@@ -517,31 +849,48 @@ __global__ void __launch_bounds__(kRowThreads) sample_logits_kernel(const T* __r
 
   const RowSlice sl(V, per, rank);
   const T* p = x + row * ldx + sl.lo;
-  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + row_stage_offset(p);
+  const int off = row_stage_offset(p);
+  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + off;
   uint32_t best, count;
   row_exp_table(sh);
+  if (threadIdx.x == 0) sh.listed = 0;
   row_stage<T>(p, sl.n, keys, best, count);
-  const uint64_t bmax = block_max_u64(best, sh), bcount = block_sum_u64(count, sh);  // both order the staging
-  uint32_t first = 0;  // ~index of the slice's first entry with its largest key
-  if (greedy)
-    for (int i = threadIdx.x; i < sl.n; i += kRowThreads)
-      if (keys[i] == bmax) first = max(first, ~static_cast<uint32_t>(sl.lo + i));
-  const uint64_t bfirst = block_max_u64(first, sh);
+  sh.tmax[threadIdx.x] = best;
+  const uint32_t wbest = __reduce_max_sync(0xffffffffu, best), wcount = __reduce_add_sync(0xffffffffu, count);
+  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = (static_cast<uint64_t>(wbest) << 32) | wcount;
+  __syncthreads();
+  uint32_t bmax = 0, bcount = 0;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 32; ++w) {
+    bmax = max(bmax, static_cast<uint32_t>(sh.warp_u64[w] >> 32));
+    bcount += static_cast<uint32_t>(sh.warp_u64[w]);
+  }
   if (threadIdx.x == 0) {
-    sh.slot[0] = (bmax << 32) | bfirst;
-    sh.slot[1] = bcount;
+    sh.slot[0] = (static_cast<uint64_t>(bmax) << 32) | bcount;
+    sh.slot[1] = 0;
+  }
+  if (greedy) {  // the slice's first entry with its largest key
+    __syncthreads();
+    uint32_t first = 0;
+    if (best == bmax)
+      row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
+        if (key == bmax) first = max(first, ~static_cast<uint32_t>(sl.lo + i));
+      });
+    if (first) atomicMax(reinterpret_cast<unsigned long long*>(&sh.slot[1]), static_cast<unsigned long long>(first));
   }
   row_cluster_sync();
-  uint64_t top_entry = 0, candidates = 0;
+  uint32_t top_key = 0, candidates = 0, top_place = 0;
   for (uint32_t r = 0; r < cs; ++r) {
     const uint64_t e = peer_u64(&sh.slot[0], r);
-    top_entry = e > top_entry ? e : top_entry;
-    candidates += peer_u64(&sh.slot[1], r);
+    const uint32_t key = static_cast<uint32_t>(e >> 32);
+    if (key > top_key) {  // of equal maxima the first CTA's
+      top_key = key;
+      top_place = greedy ? static_cast<uint32_t>(peer_u64(&sh.slot[1], r)) : 0u;
+    }
+    candidates += static_cast<uint32_t>(e);
   }
-  const uint32_t top_key = static_cast<uint32_t>(top_entry >> 32);
   if (greedy || top_key == 0) {  // the same for the whole cluster
-    if (rank == 0 && threadIdx.x == 0)
-      tokens[row] = top_key == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(top_entry));
+    if (rank == 0 && threadIdx.x == 0) tokens[row] = top_key == 0 ? -1 : static_cast<int64_t>(~top_place);
     row_cluster_sync();  // every CTA has read the others' slots
     return;
   }
@@ -550,29 +899,52 @@ __global__ void __launch_bounds__(kRowThreads) sample_logits_kernel(const T* __r
   weight.scale = 92.33248261893567 / static_cast<double>(temperature);  // 64 log2(e) / T
   weight.S = S;
   weight.tab = sh.exp_tab;
+  // min-p: weights below this leave
+  const float floor_p = fminf(fmaxf(min_p, 0.f), 1.f);
+  const uint64_t least = __double2ull_ru(static_cast<double>(floor_p) * (1ull << S));
 
   // top-k: keys below the k-th largest (ties kept) leave
   uint32_t cut = 1;
   uint64_t before;
-  if (top_k >= 1 && static_cast<uint64_t>(top_k) < candidates)
+  if (top_k >= 1 && static_cast<uint32_t>(top_k) < candidates) {
+    if (top_k <= kRowMaxK) {
+      const uint32_t bound = row_bound(top_k, top_key, sh, cs);
+      if (best >= bound) row_gather<T>(keys, off, sl, bound, 0xFFFFFFFFu, sh);
+      row_cluster_sync();
+      const uint32_t n = row_listed(sh, cs);
+      if (n <= kRowList) {  // everything else happens in one CTA
+        if (rank == 0) row_collect(sh.hist, sh, cs);
+        row_cluster_sync();  // nothing of another CTA is read after this
+        if (rank == 0)
+          row_pick_listed<T>(sh.hist, sh.list, n, top_k, top_p, least, uniform[row], weight, sh, tokens + row);
+        return;
+      }
+    }
     cut = row_radix_select<T, false>(keys, sl, 1u, top_k - 1, weight, sh, cs, before);
+  }
   // top-p: the key at the border of the nucleus and how many of its entries are inside
   uint64_t ties = ~0ull;
   if (top_p < 1.f) {
     uint64_t mass = 0;
-    for (int i = threadIdx.x; i < sl.n; i += kRowThreads)
-      if (keys[i] >= cut) mass += weight(K::value(keys[i]));
+    row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
+      if (key >= cut) mass += weight(K::value(key));
+    });
     mass = block_sum_u64(mass, sh);
     if (threadIdx.x == 0) sh.slot[2] = mass;
     row_cluster_sync();
     mass = 0;
     for (uint32_t r = 0; r < cs; ++r) mass += peer_u64(&sh.slot[2], r);
     const uint64_t target = floor_share(top_p, mass);
-    cut = row_radix_select<T, true>(keys, sl, cut, target, weight, sh, cs, before);
-    ties = (target - before) / weight(K::value(cut)) + 1;
+    if (cut > 1 ||
+        !row_nucleus<T>(keys, off, sl, V, temperature, mass, target, weight, sh, cs, cut, ties)) {
+      cut = row_radix_select<T, true>(keys, sl, cut, target, weight, sh, cs, before);
+      ties = (target - before) / weight(K::value(cut)) + 1;
+    }
   }
-  // min-p: weights below this leave
-  const uint64_t least = __double2ull_ru(static_cast<double>(fminf(fmaxf(min_p, 0.f), 1.f)) * (1ull << S));
+  // no entry below this key passes min-p (lower by a margin that covers fp32)
+  uint32_t lowest = cut;
+  if (floor_p > 0.f && weight.top < INFINITY)
+    lowest = max(cut, row_key_floor<T>(weight.top + temperature * (logf(floor_p) - 1e-3f) - 1e-5f * fabsf(weight.top)));
 
   // walk in index order: the thread's kept weight, its offset in the row, the entry that holds u
   const uint64_t cut_weight = weight(K::value(cut));
@@ -580,6 +952,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_logits_kernel(const T* __r
   uint64_t sum = 0;
   for (int i = sl.begin(); i < sl.end(); ++i) {
     const uint32_t key = keys[i];
+    if (key < lowest) continue;
     if (key > cut) {
       const uint64_t w = weight(K::value(key));
       if (w >= least) sum += w;
@@ -609,6 +982,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_logits_kernel(const T* __r
     for (int i = sl.begin(); i < sl.end(); ++i) {
       const uint32_t key = keys[i];
       uint64_t w = 0;
+      if (key < lowest) continue;
       if (key > cut) {
         w = weight(K::value(key));
         if (w < least) w = 0;
@@ -634,16 +1008,16 @@ struct RowLaunch {
   int cs, per, smem;
 };
 
-// Cluster size: the fewest CTAs (a power of two up to 8) whose slices fit `limit` bytes of shared
-// memory each; 0 if the row is too long for a cluster.
+// Cluster size: the fewest CTAs (a power of two up to 8) with at most 20480 entries each, about 40 a
+// thread, so that two CTAs share an SM and a single row is spread wide; longer rows take up to one
+// CTA's shared memory. 0 if the row is too long for a cluster.
 inline RowLaunch row_launch_plan(int64_t V, int elem) {
-  const int64_t limit = 80 * 1024;       // two CTAs per SM beside their static shared memory
-  const int64_t hard = 190 * 1024;       // one CTA per SM
-  for (int64_t cap : {limit, hard})
-    for (int cs = 1; cs <= kRowMaxCluster; cs *= 2) {
-      const int64_t per = ceil_div(ceil_div(V, cs), 8) * 8;
-      if (per * elem + 32 <= cap) return {cs, static_cast<int>(per), static_cast<int>(per * elem + 32)};
-    }
+  for (int cs = 1; cs <= kRowMaxCluster; cs *= 2) {
+    const int64_t per = ceil_div(ceil_div(V, cs), 8) * 8;
+    const int64_t bytes = per * elem + 32;
+    if (per <= 20480 || (cs == kRowMaxCluster && bytes <= 190 * 1024))
+      return {cs, static_cast<int>(per), static_cast<int>(bytes)};
+  }
   return {0, 0, 0};
 }
 
