@@ -489,15 +489,17 @@ int orthrus_philox4x32_10(const uint32_t* counter_key, int64_t n, uint32_t* out,
 
 /* ---- row operators over vocabulary logits ------------------------------------------------ */
 /* Rows are `logits` [R, V] in `dtype` at a pitch of ldl elements (any alignment; rows may overlap or
- * repeat), V up to 389,000 for fp32 and 778,000 for bf16 (a row lives in the shared memory of eight
- * SMs); ORTHRUS_EINVAL beyond. Entries that are -inf or NaN are no candidates. Entries are ordered
- * by descending value, then ascending index; -0 counts as +0. */
+ * repeat), V at most 1048576 (ORTHRUS_EINVAL beyond). Entries that are -inf or NaN are no candidates.
+ * Entries are ordered by descending value, then ascending index; -0 counts as +0. Both operators take
+ * a workspace of orthrus_vocab_rows_workspace_bytes(R, V, dtype) bytes on a 16-byte boundary. */
+size_t orthrus_vocab_rows_workspace_bytes(int64_t R, int64_t V, int dtype);
 
 /* The k largest candidates of each row (1 <= k <= 1024): values [R, k] fp32 and ids [R, k] in
  * order, (-inf, -1) past the last candidate, and lse [R] = log(sum exp(x / temperature)) over the
  * candidates (-inf without any, +inf if one is +inf). temperature > 0. */
 int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
-                      float* values, int64_t* ids, float* lse, int dtype, void* stream);
+                      float* values, int64_t* ids, float* lse, void* workspace,
+                      size_t workspace_bytes, int dtype, void* stream);
 
 /* One token per row from its filtered softmax and the row's uniform in [0, 1). With
  * w_i = exp((x_i - max x) / temperature), kept are the candidates at least as large as the top_k-th
@@ -512,7 +514,8 @@ int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int
 int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
                           const float* temperature, float temperature1, const int32_t* top_k,
                           int top_k1, const float* top_p, float top_p1, const float* min_p,
-                          float min_p1, int64_t* tokens, int dtype, void* stream);
+                          float min_p1, int64_t* tokens, void* workspace, size_t workspace_bytes,
+                          int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -917,35 +917,39 @@ extern "C" int orthrus_swiglu_bwd(const void* gate_up, const void* dout, int64_t
 // Row operators over vocabulary logits
 // ------------------------------------------------------------------------------------------------
 
+extern "C" size_t orthrus_vocab_rows_workspace_bytes(int64_t R, int64_t V, int dtype) {
+  return R < 1 || V < 1 || V > kRowMaxV ? 0 : row_ws_bytes(R, V, dtype == ORTHRUS_BF16 ? 2 : 4);
+}
+
 extern "C" int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
-                                 float* values, int64_t* ids, float* lse, int dtype, void* stream) {
-  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V < (1ll << 31) && ldl >= 0 && k >= 1 && k <= kRowMaxK && temperature > 0.f);
+                                 float* values, int64_t* ids, float* lse, void* workspace, size_t workspace_bytes,
+                                 int dtype, void* stream) {
+  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V <= kRowMaxV && ldl >= 0 && k >= 1 && k <= kRowMaxK && temperature > 0.f);
+  ORTHRUS_CHECK_ARG(R < (1ll << 31) && (dtype == ORTHRUS_F32 || dtype == ORTHRUS_BF16));
   if (R == 0) return ORTHRUS_OK;
   ORTHRUS_CHECK_ARG(logits && values && ids && lse);
   if (dtype == ORTHRUS_F32)
-    return topk_rows_impl(static_cast<const float*>(logits), ldl, R, V, k, temperature, values, ids, lse,
-                          as_stream(stream));
-  if (dtype == ORTHRUS_BF16)
-    return topk_rows_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, k, temperature, values, ids, lse,
-                          as_stream(stream));
-  return ORTHRUS_EINVAL;
+    return topk_rows_impl(static_cast<const float*>(logits), ldl, R, V, k, temperature, values, ids, lse, workspace,
+                          workspace_bytes, as_stream(stream));
+  return topk_rows_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, k, temperature, values, ids, lse,
+                        workspace, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
                                      const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
                                      const float* top_p, float top_p1, const float* min_p, float min_p1,
-                                     int64_t* tokens, int dtype, void* stream) {
-  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V < (1ll << 31) && ldl >= 0);
+                                     int64_t* tokens, void* workspace, size_t workspace_bytes, int dtype,
+                                     void* stream) {
+  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V <= kRowMaxV && ldl >= 0);
+  ORTHRUS_CHECK_ARG(R < (1ll << 31) && (dtype == ORTHRUS_F32 || dtype == ORTHRUS_BF16));
   if (R == 0) return ORTHRUS_OK;
   ORTHRUS_CHECK_ARG(logits && uniform && tokens);
   const SampleKnobs knobs{temperature, top_k, top_p, min_p, temperature1, top_p1, min_p1, top_k1};
   if (dtype == ORTHRUS_F32)
-    return sample_logits_impl(static_cast<const float*>(logits), ldl, R, V, uniform, knobs, tokens,
-                              as_stream(stream));
-  if (dtype == ORTHRUS_BF16)
-    return sample_logits_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, uniform, knobs, tokens,
-                              as_stream(stream));
-  return ORTHRUS_EINVAL;
+    return sample_logits_impl(static_cast<const float*>(logits), ldl, R, V, uniform, knobs, tokens, workspace,
+                              workspace_bytes, as_stream(stream));
+  return sample_logits_impl(static_cast<const __nv_bfloat16*>(logits), ldl, R, V, uniform, knobs, tokens, workspace,
+                            workspace_bytes, as_stream(stream));
 }
 
 extern "C" size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,

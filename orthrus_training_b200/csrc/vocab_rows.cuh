@@ -1,18 +1,19 @@
 // Row operators over vocabulary logits [R, V]: the k largest entries of a row with its
 // log-sum-exp, and sampling from a row's filtered softmax with a given uniform.
 //
-// One cluster of CS CTAs owns one row. Each CTA reads its contiguous slice of the row once from
-// HBM and keeps it in shared memory as order-preserving integer keys (32 bits for fp32, 16 for
-// bf16); every later pass runs on shared memory, and the CTAs exchange maxima, sums and histograms
-// through distributed shared memory. So the bytes moved are the row itself, whatever the filters
-// need.
-//
-// The k largest entries come from a bound: the k-th largest of the threads' own maxima (512 a CTA)
-// is at most the k-th largest entry, and little below it unless the row is arranged against it, so
-// the few entries above that bound are gathered into one CTA and ordered there. A nucleus without a
-// top-k is found by a 512-bin histogram of weights over the values that can hold its border, then
-// exactly among the border bin's entries. Where the gathered entries are too many (rows of equal
-// values), a radix selection over the whole cluster, right for every row, takes over.
+// Two launches. The scan reads every logit once, at HBM speed, over as many CTAs as there are slices:
+// it leaves the largest key of each group of 32 neighbouring entries (3 % of the row's bytes) and per
+// slice its maximum, its candidates and, where it is needed, its softmax weight. Then one CTA per row
+// finishes from those:
+//   - The k largest entries: the k-th largest group maximum is at most the k-th largest entry, and
+//     little below it unless the row is arranged against it, so the few groups at or above it are read
+//     again (from L2) and the entries at or above it, k and a few more, are ordered in shared memory.
+//   - A nucleus without top-k is looked for among the 1024 largest entries first, then by a histogram
+//     of weights over the values that can hold its border, exact among the border bin's entries.
+//   - Without a filter the slices' weights say which slice holds the uniform's share.
+// Where the gathered entries are too many for shared memory (rows of equal values, nuclei of many
+// thousands), the CTA goes over the whole row again: a radix selection that is right for every row, and
+// a walk in index order.
 //
 // Candidates are the entries that are neither -inf nor NaN. Entries are ordered by (descending
 // value, ascending index); -0 counts as +0.
@@ -24,12 +25,14 @@
 
 namespace orthrus {
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 512;          // of the CTA that finishes a row
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kScanThreads = 256;
+constexpr int kRowGroup = 32;             // entries behind one group maximum
 constexpr int kRowBins = 2048;
-constexpr int kRowMaxCluster = 8;  // portable cluster size
-constexpr int kRowMaxK = 1024;     // largest k of topk_rows
-constexpr int kRowList = 2048;     // most entries gathered into one CTA
-constexpr int kRowNucleusBins = 512;
+constexpr int kRowMaxK = 1024;            // largest k of topk_rows
+constexpr int kRowList = 2048;            // most entries gathered into shared memory
+constexpr int kRowMaxV = 1 << 20;         // the group maxima of a longer row do not fit shared memory
 
 // ------------------------------------------------------------------------------------------------
 // Keys: unsigned integers that order as the values do; 0 marks an entry that is no candidate.
@@ -69,47 +72,64 @@ struct RowKey<__nv_bfloat16> {
 };
 
 // ------------------------------------------------------------------------------------------------
-// Cluster and block helpers
+// A row in 16-byte blocks
 // ------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
-}
+// Block b of a row of any alignment covers the entries b * VEC - off .. + VEC - 1, where off is the
+// row's distance in entries from the 16-byte boundary before it; entries outside the row count as no
+// candidates and are never read.
+template <typename T>
+struct RowView {
+  using K = RowKey<T>;
+  static constexpr int VEC = K::VEC;
+  const T* p;
+  int V, off, blocks;
 
-// Cluster barrier of every thread, also after loops whose lanes leave at different iterations.
-__device__ __forceinline__ void row_cluster_sync() {
-  __syncwarp();
-  cluster_sync_all();
-}
+  __device__ __forceinline__ RowView(const T* row, int n)
+      : p(row), V(n), off(static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T))),
+        blocks((n + off + VEC - 1) / VEC) {}
+  __device__ __forceinline__ int first(int b) const { return b * VEC - off; }
+  __device__ __forceinline__ bool whole(int b) const { return first(b) >= 0 && first(b) + VEC <= V; }
+  __device__ __forceinline__ uint4 load(int b) const { return __ldg(reinterpret_cast<const uint4*>(p + first(b))); }
+  // the keys of a block loaded as 16 bytes
+  __device__ __forceinline__ static void keys_of(const uint4& q, uint32_t (&k)[VEC]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      k[e] = sizeof(T) == 4 ? K::of_bits(w[e]) : K::of_bits((e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu);
+  }
+  __device__ __forceinline__ uint32_t key(int i) const {
+    if (i < 0 || i >= V) return 0u;
+    if constexpr (sizeof(T) == 4)
+      return K::of_bits(__ldg(reinterpret_cast<const uint32_t*>(p) + i));
+    else
+      return K::of_bits(__ldg(reinterpret_cast<const uint16_t*>(p) + i));
+  }
+  __device__ __forceinline__ void edge(int b, uint32_t (&k)[VEC]) const {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) k[e] = b < blocks ? key(first(b) + e) : 0u;
+  }
+  __device__ __forceinline__ void keys(int b, uint32_t (&k)[VEC]) const {
+    if (b < blocks && whole(b))
+      keys_of(load(b), k);
+    else
+      edge(b, k);
+  }
+};
 
-// The same object's value in CTA `rank` of the cluster.
-__device__ __forceinline__ uint64_t peer_u64(const uint64_t* p, uint32_t rank) {
-  return ld_cluster_u64(mapa_shared(smem_u32(p), rank));
-}
-__device__ __forceinline__ uint32_t peer_u32(const uint32_t* p, uint32_t rank) {
-  return ld_cluster_u32(mapa_shared(smem_u32(p), rank));
-}
+// ------------------------------------------------------------------------------------------------
+// Block helpers
+// ------------------------------------------------------------------------------------------------
 
-struct RowShared {
-  uint64_t hist[kRowBins];   // radix selection: counts (as 32-bit words) or masses; else a second list
+struct RowScratch {
+  uint64_t hist[kRowBins];   // radix selection and nucleus: counts (32-bit words) or weights; else a list
   uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
   double exp_tab[64];        // 2^(-j/64)
-  uint64_t warp_u64[kRowThreads / 32];
-  uint64_t warp_count[2][kRowThreads / 32];
-  uint64_t slot[8];          // this CTA's published partials, one use each between barriers
+  uint64_t warp[kRowWarps];
+  uint64_t warp_count[2][kRowWarps];
   uint64_t found[2];         // result of a block-wide search
-  uint32_t tmax[kRowThreads];  // the threads' largest keys
-  uint32_t listed;           // entries in the list
+  uint32_t groups[kRowList]; // numbers of the groups to read again
+  uint32_t ngroups, listed;
 };
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -119,34 +139,19 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
 }
 
 // Block-wide sum; every thread gets it. Leaves warp_u64 free for reuse.
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, RowShared& sh) {
+__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, RowScratch& sh) {
   v = warp_sum_u64(v);
-  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
   __syncthreads();
   uint64_t t = 0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) t += sh.warp_u64[w];
-  __syncthreads();
-  return t;
-}
-
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, RowShared& sh) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
-  }
-  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint64_t t = 0;
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) t = sh.warp_u64[w] > t ? sh.warp_u64[w] : t;
+  for (int w = 0; w < kRowWarps; ++w) t += sh.warp[w];
   __syncthreads();
   return t;
 }
 
 // Exclusive prefix sum over the block's threads; `total` is the block's sum.
-__device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowShared& sh, uint64_t& total) {
+__device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowScratch& sh, uint64_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t inc = v;
 #pragma unroll
@@ -154,13 +159,13 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowShared& s
     const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += u;
   }
-  if (lane == 31) sh.warp_u64[warp] = inc;
+  if (lane == 31) sh.warp[warp] = inc;
   __syncthreads();
   uint64_t before = 0, t = 0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) {
+  for (int w = 0; w < kRowWarps; ++w) {
     if (w == warp) before = t;
-    t += sh.warp_u64[w];
+    t += sh.warp[w];
   }
   __syncthreads();
   total = t;
@@ -168,118 +173,12 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowShared& s
 }
 
 // ------------------------------------------------------------------------------------------------
-// The row slice of a CTA
-// ------------------------------------------------------------------------------------------------
-
-// Index arithmetic of a slice: `lo` its first index in the row, `n` its entries, `chunk` the
-// contiguous entries of one thread in the index-ordered passes (odd, so that neighbouring threads
-// read different banks).
-struct RowSlice {
-  int lo, n, chunk;
-  __device__ __forceinline__ RowSlice(int V, int per, uint32_t rank) {
-    const int64_t a = static_cast<int64_t>(per) * rank;
-    lo = static_cast<int>(a < V ? a : V);
-    n = V - lo < per ? V - lo : per;
-    chunk = ((n + kRowThreads - 1) / kRowThreads) | 1;
-  }
-  __device__ __forceinline__ int begin() const { return min(n, static_cast<int>(threadIdx.x) * chunk); }
-  __device__ __forceinline__ int end() const { return min(n, (static_cast<int>(threadIdx.x) + 1) * chunk); }
-};
-
-// Loads the slice into shared memory as keys. The keys start `off` elements into the buffer so that
-// the 16-byte vectors of the (arbitrarily aligned) row land on 16-byte boundaries. Returns the
-// thread's largest key and its number of candidates.
-template <typename T>
-__device__ __forceinline__ int row_stage_offset(const T* p) {
-  return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
-}
-
-template <typename T>
-__device__ __forceinline__ void row_stage(const T* __restrict__ p, int n, typename RowKey<T>::type* keys,
-                                          uint32_t& best, uint32_t& count) {
-  using K = RowKey<T>;
-  constexpr int VEC = K::VEC;
-  const int off = row_stage_offset(p);
-  const int head = min(n, (VEC - off) % VEC);
-  best = 0;
-  count = 0;
-  auto take = [&](uint32_t bits) {
-    const uint32_t k = K::of_bits(bits);
-    best = max(best, k);
-    count += k != 0u;
-    return k;
-  };
-  auto scalar = [&](int i) {
-    uint32_t bits;
-    if constexpr (sizeof(T) == 4)
-      bits = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-    else
-      bits = __ldg(reinterpret_cast<const uint16_t*>(p) + i);
-    keys[i] = static_cast<typename K::type>(take(bits));
-  };
-  if (static_cast<int>(threadIdx.x) < head) scalar(threadIdx.x);
-  const int nvec = (n - head) / VEC;
-  const uint4* src = reinterpret_cast<const uint4*>(p + head);
-  uint4* dst = reinterpret_cast<uint4*>(keys + head);
-  constexpr int UNROLL = 4;
-  for (int v0 = threadIdx.x; v0 < nvec; v0 += UNROLL * kRowThreads) {
-    uint4 q[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * kRowThreads < nvec) q[u] = __ldg(src + v0 + u * kRowThreads);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * kRowThreads < nvec) {
-        uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(T) == 4)
-            w[e] = take(w[e]);
-          else {
-            const uint32_t a = take(w[e] & 0xFFFFu), b = take(w[e] >> 16);
-            w[e] = a | (b << 16);
-          }
-        }
-        dst[v0 + u * kRowThreads] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-  }
-  const int tail = head + nvec * VEC;
-  if (tail + static_cast<int>(threadIdx.x) < n) scalar(tail + threadIdx.x);  // fewer than VEC
-}
-
-// Visits the entries that row_stage gave this thread: f(index in the slice, key).
-template <typename T, typename F>
-__device__ __forceinline__ void row_own(const typename RowKey<T>::type* keys, int off, int n, F f) {
-  constexpr int VEC = RowKey<T>::VEC;
-  const int head = min(n, (VEC - off) % VEC);
-  const int t = threadIdx.x;
-  if (t < head) f(t, static_cast<uint32_t>(keys[t]));
-  const int nvec = (n - head) / VEC;
-  const uint4* src = reinterpret_cast<const uint4*>(keys + head);
-  for (int v = t; v < nvec; v += kRowThreads) {
-    const uint4 q = src[v];
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 4) {
-        f(head + 4 * v + e, w[e]);
-      } else {
-        f(head + 8 * v + 2 * e, w[e] & 0xFFFFu);
-        f(head + 8 * v + 2 * e + 1, w[e] >> 16);
-      }
-    }
-  }
-  const int tail = head + nvec * VEC;
-  if (tail + t < n) f(tail + t, static_cast<uint32_t>(keys[tail + t]));
-}
-
-// ------------------------------------------------------------------------------------------------
 // Softmax weights as 64-bit integers
 // ------------------------------------------------------------------------------------------------
 
-// w(x) = round(2^S exp((x - max) / T)). Integer weights make every sum exact, so running sums do
-// not depend on how a row is split over threads and CTAs, and comparisons with a uniform's share of
-// the total fall the same way on every path. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
+// w(x) = round(2^S exp((x - top) / T)). Integer weights make every sum exact, so running sums do not
+// depend on how a row is split over threads, and comparisons with a uniform's share of the total
+// fall the same way on every path. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
 // 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
 //
 // The exponential is the table method (P. T. P. Tang, "Table-driven implementation of the
@@ -313,8 +212,12 @@ __host__ __device__ inline int row_weight_bits(int V) {
   return 62 - b < 44 ? 62 - b : 44;
 }
 
-__device__ __forceinline__ void row_exp_table(RowShared& sh) {
-  if (threadIdx.x < 64) sh.exp_tab[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+__device__ __forceinline__ void row_exp_table(double* tab) {
+  if (threadIdx.x < 64) tab[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+}
+
+__device__ __forceinline__ RowWeight row_weight(float top, float temperature, int S, const double* tab) {
+  return {top, 92.33248261893567 / static_cast<double>(temperature), S, tab};  // 64 log2(e) / T
 }
 
 // floor(f * z) for f in [0, 1) and z < 2^62, exactly (f is an integer of 24 bits times a power of
@@ -333,91 +236,187 @@ __device__ __forceinline__ uint64_t floor_share(float f, uint64_t z) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Radix selection over the cluster
+// The scan
 // ------------------------------------------------------------------------------------------------
 
-// Finds, among the cluster's entries with key >= floor_key in descending order of key, the key
-// whose entries hold position `target` of the running measure: the measure (MASS: the sum of
-// weights; otherwise the count) of all larger keys is `before` <= target < before + its own. The
-// caller makes sure that target is below the total. Every thread of the cluster gets the result.
-template <typename T, bool MASS>
-__device__ uint32_t row_radix_select(const typename RowKey<T>::type* keys, const RowSlice& sl, uint32_t floor_key,
-                                     uint64_t target, const RowWeight& weight, RowShared& sh, uint32_t cs,
-                                     uint64_t& before) {
-  constexpr int BITS = RowKey<T>::BITS;
-  uint32_t prefix = 0;
-  int shift = BITS;
-  before = 0;
-  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
-  while (shift > 0) {
-    const int width = shift < 11 ? shift : 11;
-    const int next = shift - width;
-    const uint32_t mask = (1u << width) - 1u;
-    for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) {
-      if constexpr (MASS) sh.hist[i] = 0;
-      else counts[i] = 0;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < sl.n; i += kRowThreads) {
-      const uint32_t k = keys[i];
-      if (k < floor_key || k == 0u || (shift < BITS && (k >> shift) != prefix)) continue;
-      const uint32_t d = (k >> next) & mask;
-      if constexpr (MASS) {
-        const uint64_t w = weight(RowKey<T>::value(k));
-        if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[d]), static_cast<unsigned long long>(w));
-      } else {
-        atomicAdd(&counts[d], 1u);
-      }
-    }
-    row_cluster_sync();
-    // thread t sums the cluster's bins 2047 - 4t .. 2044 - 4t
-    constexpr int PER = kRowBins / kRowThreads;
-    uint64_t h[PER], own = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int b = kRowBins - 1 - (static_cast<int>(threadIdx.x) * PER + j);
-      h[j] = 0;
-      for (uint32_t c = 0; c < cs; ++c) h[j] += MASS ? peer_u64(&sh.hist[b], c) : peer_u32(&counts[b], c);
-      own += h[j];
-    }
-    uint64_t total;
-    uint64_t run = before + block_exclusive_u64(own, sh, total);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (run <= target && target < run + h[j]) {
-        sh.found[0] = kRowBins - 1 - (threadIdx.x * PER + j);
-        sh.found[1] = run;
-      }
-      run += h[j];
-    }
-    row_cluster_sync();  // found is set; no CTA clears its bins while another still reads them
-    prefix = (prefix << width) | static_cast<uint32_t>(sh.found[0]);
-    before = sh.found[1];
-    shift = next;
-    __syncthreads();  // found is read before the next level sets it
+struct RowSlice {
+  uint32_t top;    // largest key
+  uint32_t count;  // candidates
+  uint64_t mass;   // sum of exp((x - slice's largest) / T): a float's bits (top-k), or 2^S fold (sampling)
+};
+
+// What the scan leaves of R rows: group maxima [R, groups] and slices [R, slices].
+struct RowScan {
+  uint32_t* group;
+  RowSlice* slice;
+  int groups, slices;
+};
+
+struct SampleKnobs {
+  const float* temperature;  // [R], or null: one value for every row
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature1, top_p1, min_p1;
+  int top_k1;
+};
+
+// How a row is sampled, from its knobs.
+struct SampleRow {
+  float temperature, top_p, min_p;
+  int top_k;
+  bool greedy;
+  __device__ __forceinline__ SampleRow(const SampleKnobs& k, int64_t row)
+      : temperature(k.temperature ? k.temperature[row] : k.temperature1),
+        top_p(k.top_p ? k.top_p[row] : k.top_p1),
+        min_p(k.min_p ? k.min_p[row] : k.min_p1),
+        top_k(k.top_k ? k.top_k[row] : k.top_k1),
+        greedy(temperature < 1e-5f) {}
+  // whether the slices' weights are asked for: no filter, or a nucleus of the whole row
+  __device__ __forceinline__ bool wants_mass() const { return !greedy && top_k < 1 && (top_p < 1.f || !(min_p > 0.f)); }
+};
+
+// One slice of BLOCKS * 256 16-byte blocks per CTA (slices of a row first), every load issued before the
+// first is used. The slice's weight is the fp32 sum of exponentials, or, to SAMPLE, integer weights
+// for the rows that want them.
+template <typename T, int BLOCKS, bool SAMPLE>
+__global__ void __launch_bounds__(kScanThreads)
+    row_scan_kernel(const T* __restrict__ x, int64_t ldx, int V, float temperature, int S, SampleKnobs knobs,
+                    RowScan out) {
+  using View = RowView<T>;
+  constexpr int VEC = View::VEC;
+  constexpr int LANES = kRowGroup / VEC;  // neighbouring lanes of a group
+  __shared__ double tab[64];
+  __shared__ uint32_t wtop[kScanThreads / 32], wcount[kScanThreads / 32];
+  __shared__ uint64_t wmass[kScanThreads / 32];
+  griddep_launch_dependents();
+  const int64_t row = blockIdx.x / static_cast<unsigned>(out.slices);
+  const int slice = static_cast<int>(blockIdx.x % static_cast<unsigned>(out.slices));
+  const View v(x + row * ldx, V);
+  const int b0 = slice * BLOCKS * kScanThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool mass_wanted = true;
+  if constexpr (SAMPLE) {
+    const SampleRow knob(knobs, row);
+    temperature = knob.temperature;
+    mass_wanted = knob.wants_mass();
+    if (mass_wanted) row_exp_table(tab);
   }
-  return prefix;
+  uint32_t key[BLOCKS][VEC];
+  if (v.whole(b0) && v.whole(b0 + BLOCKS * kScanThreads - 1)) {
+    uint4 q[BLOCKS];
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) q[j] = v.load(b0 + j * kScanThreads + threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) View::keys_of(q[j], key[j]);
+  } else {  // the row's ends
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) v.keys(b0 + j * kScanThreads + threadIdx.x, key[j]);
+  }
+  uint32_t top = 0, count = 0;
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      m = max(m, key[j][e]);
+      count += key[j][e] != 0u;
+    }
+    top = max(top, m);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int g = (b0 + j * kScanThreads + static_cast<int>(threadIdx.x)) / LANES;
+    if (lane % LANES == 0 && g < out.groups) out.group[row * out.groups + g] = m;
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane == 0) {
+    wtop[warp] = top;
+    wcount[warp] = count;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kScanThreads / 32; ++w) top = max(top, wtop[w]);
+  const float ftop = RowKey<T>::value(top);
+  uint64_t mass = 0;
+  if constexpr (SAMPLE) {
+    if (mass_wanted && top) {
+      const RowWeight weight = row_weight(ftop, temperature, S, tab);
+#pragma unroll
+      for (int j = 0; j < BLOCKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (key[j][e]) mass += weight(RowKey<T>::value(key[j][e]));
+    }
+    mass = warp_sum_u64(mass);
+  } else {
+    const float c = kLog2e / temperature;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top && ftop < INFINITY) {
+#pragma unroll
+      for (int j = 0; j < BLOCKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          sum[e & 3] += key[j][e] ? ex2_approx((RowKey<T>::value(key[j][e]) - ftop) * c) : 0.f;
+    }
+    float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    mass = __float_as_uint(s);
+  }
+  if (lane == 0) wmass[warp] = mass;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    RowSlice r{top, 0u, 0ull};
+    float s = 0.f;
+    for (int w = 0; w < kScanThreads / 32; ++w) {
+      r.count += wcount[w];
+      if constexpr (SAMPLE) r.mass += wmass[w];
+      else s += __uint_as_float(static_cast<uint32_t>(wmass[w]));
+    }
+    if constexpr (!SAMPLE) r.mass = __float_as_uint(s);
+    out.slice[row * out.slices + slice] = r;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
 // The few largest entries
 // ------------------------------------------------------------------------------------------------
 
-// A key with at least k entries of the cluster's row at or above it, and not many more: between
-// the k-th largest thread maximum and a little below it. Four-way search on counts of the maxima
-// (published in tmax before the last cluster barrier), the same in every CTA.
-__device__ __forceinline__ uint32_t row_bound(int k, uint32_t top_key, RowShared& sh, uint32_t cs) {
-  uint32_t mk[kRowMaxCluster];
-  uint32_t least = 0xFFFFFFFFu, some = 0;
-#pragma unroll
-  for (int c = 0; c < kRowMaxCluster; ++c) {
-    mk[c] = c < static_cast<int>(cs) ? peer_u32(&sh.tmax[threadIdx.x], c) : 0u;
-    if (mk[c]) {
-      least = min(least, mk[c]);
-      ++some;
-    }
+// The row's group maxima into shared memory (padded with zeros to a multiple of four), its largest
+// key and its candidates. Every thread gets both.
+__device__ __forceinline__ void row_open(const RowScan& scan, int64_t row, uint32_t* maxima, RowScratch& sh,
+                                         uint32_t& top_key, uint32_t& candidates) {
+  const uint32_t* g = scan.group + row * scan.groups;
+  for (int i = threadIdx.x; i < (scan.groups + 3) / 4 * 4; i += kRowThreads) maxima[i] = i < scan.groups ? g[i] : 0u;
+  uint32_t top = 0, count = 0;
+  for (int i = threadIdx.x; i < scan.slices; i += kRowThreads) {
+    const RowSlice s = scan.slice[row * scan.slices + i];
+    top = max(top, s.top);
+    count += s.count;
   }
+  top = __reduce_max_sync(0xffffffffu, top);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = (static_cast<uint64_t>(top) << 32) | count;
+  if (threadIdx.x == 0) sh.ngroups = sh.listed = 0;
+  __syncthreads();
+  top_key = candidates = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) {
+    top_key = max(top_key, static_cast<uint32_t>(sh.warp[w] >> 32));
+    candidates += static_cast<uint32_t>(sh.warp[w]);
+  }
+  __syncthreads();
+}
+
+// A key with at least k entries of the row at or above it, and not many more: between the k-th largest
+// group maximum and a little below it; 1 if fewer than k groups hold a candidate. Four-way search
+// on counts of the maxima.
+__device__ __forceinline__ uint32_t row_bound(const uint32_t* maxima, int groups, int k, uint32_t top_key,
+                                              RowScratch& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint4* m4 = reinterpret_cast<const uint4*>(maxima);
+  const int n4 = (groups + 3) / 4;
   // three counters of 21 bits a word; `buf` alternates, so one barrier an exchange is enough
   auto total = [&](uint32_t a, uint32_t b, uint32_t c, int buf) {
     a = __reduce_add_sync(0xffffffffu, a);
@@ -427,32 +426,49 @@ __device__ __forceinline__ uint32_t row_bound(int k, uint32_t top_key, RowShared
     __syncthreads();
     uint64_t t = 0;
 #pragma unroll
-    for (int w = 0; w < kRowThreads / 32; ++w) t += sh.warp_count[buf][w];
+    for (int w = 0; w < kRowWarps; ++w) t += sh.warp_count[buf][w];
     return t;
   };
+  uint32_t least = 0xFFFFFFFFu, some = 0;
+  for (int i = threadIdx.x; i < n4; i += kRowThreads) {
+    const uint4 q = m4[i];
+    const uint32_t m[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (m[e]) {
+        least = min(least, m[e]);
+        ++some;
+      }
+  }
   least = __reduce_min_sync(0xffffffffu, least);
-  if (lane == 0) sh.warp_u64[warp] = least;
+  if (lane == 0) sh.warp[warp] = least;
   uint32_t have = static_cast<uint32_t>(total(some, 0, 0, 0) & 0x1FFFFF);
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) least = min(least, static_cast<uint32_t>(sh.warp_u64[w]));
-  if (have < static_cast<uint32_t>(k)) return 1u;
+  for (int w = 0; w < kRowWarps; ++w) least = min(least, static_cast<uint32_t>(sh.warp[w]));
+  const uint32_t want = k, enough = k + k / 4 + 16;
   uint32_t lo = least, hi = top_key + 1;  // at least k maxima at or above lo, fewer at or above hi
-  const uint32_t enough = k + k / 4 + 16;
+  if (have < want) {
+    lo = 1u;
+    hi = 2u;
+  }
   for (int step = 1; have > enough && hi - lo > 1; ++step) {
     const uint32_t d = hi - lo;
     const uint32_t t1 = lo + (d + 3) / 4, t2 = lo + (d + 1) / 2, t3 = lo + d - d / 4;
     uint32_t a = 0, b = 0, c = 0;
+    for (int i = threadIdx.x; i < n4; i += kRowThreads) {
+      const uint4 q = m4[i];
+      const uint32_t m[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < kRowMaxCluster; ++i) {
-      a += mk[i] >= t1;
-      b += mk[i] >= t2;
-      c += mk[i] >= t3;
+      for (int e = 0; e < 4; ++e) {
+        a += m[e] >= t1;
+        b += m[e] >= t2;
+        c += m[e] >= t3;
+      }
     }
     const uint64_t t = total(a, b, c, step & 1);
     a = static_cast<uint32_t>(t) & 0x1FFFFF;
     b = static_cast<uint32_t>(t >> 21) & 0x1FFFFF;
     c = static_cast<uint32_t>(t >> 42);
-    const uint32_t want = k;
     if (c >= want) {
       lo = t3;
       have = c;
@@ -468,46 +484,56 @@ __device__ __forceinline__ uint32_t row_bound(int k, uint32_t top_key, RowShared
       hi = t1;
     }
   }
-  __syncthreads();  // warp_u64 and warp_count are free again
+  __syncthreads();  // warp and warp_count are free again
   return lo;
 }
 
-// Appends this thread's entries with low <= key < high to the CTA's list (listed counts them, past
-// the list's end too). `listed` is 0 and visible before; a block barrier follows.
+// Reads the groups at or above `low` again and lists their entries with low <= key; returns their
+// number, or more than kRowList if they do not fit. Ends with a barrier; listed is left at 0.
 template <typename T>
-__device__ __forceinline__ void row_gather(const typename RowKey<T>::type* keys, int off, const RowSlice& sl,
-                                           uint32_t low, uint32_t high, RowShared& sh) {
-  row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
-    if (key >= low && key < high) {
-      const uint32_t at = atomicAdd(&sh.listed, 1u);
-      if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i);
+__device__ int row_gather(const RowView<T>& v, const uint32_t* maxima, int groups, uint32_t low, RowScratch& sh) {
+  constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC;
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < groups; i += kRowThreads)
+    if (maxima[i] >= low) {
+      const uint32_t at = atomicAdd(&sh.ngroups, 1u);
+      if (at < kRowList) sh.groups[at] = i;
     }
-  });
-}
-
-// Entries listed in the whole cluster (after a cluster barrier).
-__device__ __forceinline__ uint32_t row_listed(RowShared& sh, uint32_t cs) {
-  uint32_t n = 0;
-  for (uint32_t c = 0; c < cs; ++c) n += peer_u32(&sh.listed, c);
+  __syncthreads();
+  const int ng = static_cast<int>(sh.ngroups);
+  if (ng > kRowList) {  // every group holds at least one entry
+    __syncthreads();
+    if (threadIdx.x == 0) sh.ngroups = 0;
+    __syncthreads();
+    return kRowList + 1;
+  }
+  // LANES neighbouring lanes a group
+  for (int i0 = 0; i0 < ng; i0 += kRowThreads / LANES) {
+    const int i = i0 + static_cast<int>(threadIdx.x) / LANES;
+    uint32_t k[VEC];
+    int b = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) k[e] = 0u;
+    if (i < ng) {
+      b = static_cast<int>(sh.groups[i]) * LANES + lane % LANES;
+      v.keys(b, k);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (k[e] >= low) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e);
+      }
+  }
+  __syncthreads();
+  const int n = static_cast<int>(sh.listed);
+  __syncthreads();
+  if (threadIdx.x == 0) sh.ngroups = sh.listed = 0;
+  __syncthreads();
   return n;
 }
 
-// Leader: copies every CTA's list to `out`, at most kRowList entries in all.
-__device__ __forceinline__ void row_collect(uint64_t* out, RowShared& sh, uint32_t cs) {
-  uint32_t at = 0;
-  for (uint32_t c = 0; c < cs; ++c) {
-    const uint32_t n = peer_u32(&sh.listed, c);
-    for (uint32_t j = threadIdx.x; j < n; j += kRowThreads) out[at + j] = peer_u64(&sh.list[j], c);
-    at += n;
-  }
-  __syncthreads();
-}
-
-// ------------------------------------------------------------------------------------------------
-// Top-k
-// ------------------------------------------------------------------------------------------------
-
-// Descending bitonic sort of sh.list[0, n2), n2 a power of two.
+// Descending bitonic sort of a[0, n2), n2 a power of two.
 __device__ __forceinline__ void row_sort_desc(uint64_t* a, int n2) {
   for (int size = 2; size <= n2; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -526,7 +552,7 @@ __device__ __forceinline__ void row_sort_desc(uint64_t* a, int n2) {
 
 // Orders `in` (n <= kRowList different entries) descending into `out` (not the same array): by rank
 // counting for a few entries, several threads an entry; else by a sorting network on `in`.
-__device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n, RowShared& sh) {
+__device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n) {
   if (n <= kRowThreads) {
     int parts = 32;
     while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
@@ -548,133 +574,178 @@ __device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n, Ro
   __syncthreads();
 }
 
+// ------------------------------------------------------------------------------------------------
+// Going over the whole row
+// ------------------------------------------------------------------------------------------------
+
+// f(index, key) for every candidate of the row, each by one thread.
+template <typename T, typename F>
+__device__ __forceinline__ void row_visit(const RowView<T>& v, F f) {
+  constexpr int VEC = RowView<T>::VEC, UNROLL = 4;
+  for (int b0 = threadIdx.x; b0 < v.blocks; b0 += UNROLL * kRowThreads) {
+    uint32_t k[UNROLL][VEC];
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) v.keys(b0 + j * kRowThreads, k[j]);
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (k[j][e]) f(v.first(b0 + j * kRowThreads) + e, k[j][e]);
+  }
+}
+
+// Finds, among the candidates with key >= floor_key in descending order of key, the key whose
+// entries hold position `target` of the running measure: the measure (MASS: the sum of weights;
+// otherwise the count) of all larger keys is `before` <= target < before + its own. The caller
+// makes sure that target is below the total. Every thread gets the result.
+template <typename T, bool MASS>
+__device__ uint32_t row_radix_select(const RowView<T>& v, uint32_t floor_key, uint64_t target, const RowWeight& weight,
+                                     RowScratch& sh, uint64_t& before) {
+  constexpr int BITS = RowKey<T>::BITS;
+  uint32_t prefix = 0;
+  int shift = BITS;
+  before = 0;
+  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
+  while (shift > 0) {
+    const int width = shift < 11 ? shift : 11;
+    const int next = shift - width;
+    const uint32_t mask = (1u << width) - 1u;
+    for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) {
+      if constexpr (MASS) sh.hist[i] = 0;
+      else counts[i] = 0;
+    }
+    __syncthreads();
+    row_visit<T>(v, [&](int, uint32_t k) {
+      if (k < floor_key || (shift < BITS && (k >> shift) != prefix)) return;
+      const uint32_t d = (k >> next) & mask;
+      if constexpr (MASS) {
+        const uint64_t w = weight(RowKey<T>::value(k));
+        if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[d]), static_cast<unsigned long long>(w));
+      } else {
+        atomicAdd(&counts[d], 1u);
+      }
+    });
+    __syncthreads();
+    // thread t takes the bins 2047 - 4t .. 2044 - 4t
+    constexpr int PER = kRowBins / kRowThreads;
+    uint64_t h[PER], own = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int b = kRowBins - 1 - (static_cast<int>(threadIdx.x) * PER + j);
+      h[j] = MASS ? sh.hist[b] : counts[b];
+      own += h[j];
+    }
+    uint64_t total;
+    uint64_t run = before + block_exclusive_u64(own, sh, total);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (run <= target && target < run + h[j]) {
+        sh.found[0] = kRowBins - 1 - (threadIdx.x * PER + j);
+        sh.found[1] = run;
+      }
+      run += h[j];
+    }
+    __syncthreads();
+    prefix = (prefix << width) | static_cast<uint32_t>(sh.found[0]);
+    before = sh.found[1];
+    shift = next;
+    __syncthreads();  // found is read before the next level sets it
+  }
+  return prefix;
+}
+
+// Blocks of the row in index order, a contiguous range per warp: f(block, keys of this lane's block)
+// with 32 neighbouring blocks a step, by every lane of the warp (keys of 0 past the end).
+template <typename T, typename F>
+__device__ __forceinline__ void row_warp_walk(const RowView<T>& v, F f) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int steps = (v.blocks + 31) / 32, per = (steps + kRowWarps - 1) / kRowWarps;
+  for (int s = warp * per; s < min(steps, (warp + 1) * per); ++s) {
+    uint32_t k[RowView<T>::VEC];
+    const int b = s * 32 + lane;
+    v.keys(b, k);
+    if (!f(b, k)) break;  // the same in every lane
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Top-k
+// ------------------------------------------------------------------------------------------------
+
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2)
-    topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int per, int k, float temperature,
+    topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int k, float temperature, RowScan scan,
                      float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   using K = RowKey<T>;
-  extern __shared__ __align__(16) uint8_t row_smem[];
-  __shared__ RowShared sh;
-  uint32_t cs, rank;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cs));
-  rank = cluster_ctarank();
-  const int64_t row = blockIdx.x / cs;
-  const RowSlice sl(V, per, rank);
-  const T* p = x + row * ldx + sl.lo;
-  const int off = row_stage_offset(p);
-  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + off;
-  uint32_t best, count;
-  if (threadIdx.x == 0) sh.listed = 0;
-  row_stage<T>(p, sl.n, keys, best, count);
-  sh.tmax[threadIdx.x] = best;
-  // maximum and count of the slice in one exchange: a key of 32 bits over a count of 32
-  const uint32_t wbest = __reduce_max_sync(0xffffffffu, best), wcount = __reduce_add_sync(0xffffffffu, count);
-  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = (static_cast<uint64_t>(wbest) << 32) | wcount;
-  __syncthreads();
-  uint32_t bmax = 0, bcount = 0;
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) {
-    bmax = max(bmax, static_cast<uint32_t>(sh.warp_u64[w] >> 32));
-    bcount += static_cast<uint32_t>(sh.warp_u64[w]);
-  }
-  // the slice's sum of exp((x - its maximum) / T)
-  const float btop = K::value(bmax);
-  const float c = kLog2e / temperature;
-  float part = 0.f;
-  if (bmax && btop < INFINITY)
-    row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
-      part += key ? ex2_approx((K::value(key) - btop) * c) : 0.f;
-    });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  if ((threadIdx.x & 31) == 0) sh.warp_count[1][threadIdx.x >> 5] = __float_as_uint(part);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float s = 0.f;
-    for (int w = 0; w < kRowThreads / 32; ++w) s += __uint_as_float(static_cast<uint32_t>(sh.warp_count[1][w]));
-    sh.slot[0] = (static_cast<uint64_t>(bmax) << 32) | bcount;
-    sh.slot[1] = __float_as_uint(s);
-  }
-  row_cluster_sync();
-  uint32_t top_key = 0, candidates = 0;
-  for (uint32_t r = 0; r < cs; ++r) {
-    const uint64_t e = peer_u64(&sh.slot[0], r);
-    top_key = max(top_key, static_cast<uint32_t>(e >> 32));
-    candidates += static_cast<uint32_t>(e);
-  }
+  extern __shared__ __align__(16) uint32_t row_maxima[];
+  __shared__ RowScratch sh;
+  griddep_wait();  // launched as a programmatic dependent of the scan
+  const int64_t row = blockIdx.x;
+  const RowView<T> v(x + row * ldx, V);
+  uint32_t top_key, candidates;
+  row_open(scan, row, row_maxima, sh, top_key, candidates);
   const int kk = static_cast<int>(min(candidates, static_cast<uint32_t>(k)));
-  if (rank == 0 && threadIdx.x < 32) {  // lane r brings CTA r's sum to the row's maximum
-    const uint32_t r = threadIdx.x;
+  if (threadIdx.x >= kRowThreads - 32) {  // the last warp joins the slices' sums at the row's maximum
     const double top = K::value(top_key);
     double s = 0.0;
-    const uint32_t m = r < cs ? static_cast<uint32_t>(peer_u64(&sh.slot[0], r) >> 32) : 0u;
-    if (m)
-      s = __uint_as_float(static_cast<uint32_t>(peer_u64(&sh.slot[1], r))) *
-          exp((static_cast<double>(K::value(m)) - top) / temperature);
+    for (int i = threadIdx.x & 31; i < scan.slices; i += 32) {
+      const RowSlice a = scan.slice[row * scan.slices + i];
+      if (a.top)
+        s += __uint_as_float(static_cast<uint32_t>(a.mass)) *
+             exp((static_cast<double>(K::value(a.top)) - top) / temperature);
+    }
 #pragma unroll
-    for (int o = kRowMaxCluster / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (r == 0)
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0)
       lse[row] = top_key == 0 ? -INFINITY : !(top < INFINITY) ? INFINITY : static_cast<float>(top / temperature + log(s));
   }
-  uint64_t* ordered = sh.hist;
-  int have = 0;
   if (kk > 0) {
-    const uint32_t bound = row_bound(kk, top_key, sh, cs);
-    if (best >= bound) row_gather<T>(keys, off, sl, bound, 0xFFFFFFFFu, sh);
-    row_cluster_sync();
-    const uint32_t n = row_listed(sh, cs);
-    if (n <= kRowList) {
-      have = static_cast<int>(n);
-      if (rank == 0) row_collect(sh.hist, sh, cs);
-      row_cluster_sync();  // nothing of another CTA is read after this
-      if (rank != 0) return;
-      row_order(sh.hist, sh.list, have, sh);
-      ordered = sh.list;
-    } else {
+    const uint32_t bound = row_bound(row_maxima, scan.groups, kk, top_key, sh);
+    int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+    if (n > kRowList) {
+      // the kk-th largest key, then the larger ones and of its equals the first in index order
       uint64_t n_gt;
-      RowWeight none{};
-      const uint32_t cut = row_radix_select<T, false>(keys, sl, 1u, kk - 1, none, sh, cs, n_gt);
-      // index-ordered compaction: larger keys first, then the lowest-index equals
-      uint32_t gt = 0, eq = 0;
-      for (int i = sl.begin(); i < sl.end(); ++i) {
-        const uint32_t key = keys[i];
-        gt += key > cut;
-        eq += key == cut;
-      }
+      const RowWeight none{};
+      const uint32_t cut = row_radix_select<T, false>(v, 1u, kk - 1, none, sh, n_gt);
+      uint32_t eq = 0;
+      row_warp_walk<T>(v, [&](int, const uint32_t(&key)[RowView<T>::VEC]) {
+#pragma unroll
+        for (int e = 0; e < RowView<T>::VEC; ++e) eq += key[e] == cut;
+        return true;
+      });
+      // equals of the warps before this one
       uint64_t total;
-      const uint64_t at = block_exclusive_u64((static_cast<uint64_t>(gt) << 32) | eq, sh, total);
-      if (threadIdx.x == 0) sh.slot[2] = total;
-      row_cluster_sync();
-      uint64_t base = at;
-      for (uint32_t r = 0; r < rank; ++r) base += peer_u64(&sh.slot[2], r);
-      uint32_t at_gt = static_cast<uint32_t>(base >> 32), at_eq = static_cast<uint32_t>(base);
-      const uint32_t room = static_cast<uint32_t>(kk - n_gt);
-      const uint32_t list0 = mapa_shared(smem_u32(sh.list), 0);
-      if (gt || eq)
-        for (int i = sl.begin(); i < sl.end(); ++i) {
-          const uint32_t key = keys[i];
-          if (key < cut) continue;
-          uint32_t pos;
-          if (key > cut)
-            pos = at_gt++;
-          else if (at_eq < room)
-            pos = static_cast<uint32_t>(n_gt) + at_eq++;
-          else
-            continue;
-          st_cluster_u64(list0 + pos * 8, (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i));
+      uint64_t rank = block_exclusive_u64(eq, sh, total);
+      rank = __shfl_sync(0xffffffffu, rank, 0);
+      const uint64_t room = kk - n_gt;
+      const int lane = threadIdx.x & 31;
+      row_warp_walk<T>(v, [&](int b, const uint32_t(&key)[RowView<T>::VEC]) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < RowView<T>::VEC; ++e) mine += key[e] == cut;
+        uint32_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += u;
         }
-      row_cluster_sync();  // the list is complete; nothing of another CTA is read after this
-      if (rank != 0) return;
-      have = kk;
-      row_order(sh.list, sh.hist, have, sh);
-      ordered = sh.hist;
+        uint64_t r = rank + inc - mine;
+        rank += __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+        for (int e = 0; e < RowView<T>::VEC; ++e)
+          if (key[e] > cut || (key[e] == cut && r++ < room)) {
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            sh.list[at] = (static_cast<uint64_t>(key[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e);
+          }
+        return true;
+      });
+      __syncthreads();
+      n = kk;
     }
-  } else {
-    row_cluster_sync();  // the leader has read the slots
-    if (rank != 0) return;
+    row_order(sh.list, sh.hist, n);
   }
   for (int i = threadIdx.x; i < k; i += kRowThreads) {
-    const uint64_t e = i < kk ? ordered[i] : 0;
+    const uint64_t e = i < kk ? sh.hist[i] : 0;
     values[row * k + i] = i < kk ? K::value(static_cast<uint32_t>(e >> 32)) : -INFINITY;
     ids[row * k + i] = i < kk ? static_cast<int64_t>(~static_cast<uint32_t>(e)) : -1;
   }
@@ -684,15 +755,6 @@ __global__ void __launch_bounds__(kRowThreads, 2)
 // Sampling
 // ------------------------------------------------------------------------------------------------
 
-struct SampleKnobs {
-  const float* temperature;  // [R], or null: one value for every row
-  const int* top_k;
-  const float* top_p;
-  const float* min_p;
-  float temperature1, top_p1, min_p1;
-  int top_k1;
-};
-
 // Order-preserving integer of a number, rounded down to the key's bits: every entry at or above x has a
 // key at or above this.
 template <typename T>
@@ -701,67 +763,127 @@ __device__ __forceinline__ uint32_t row_key_floor(float x) {
   return ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) >> (32 - RowKey<T>::BITS);
 }
 
+
+// Filters the n listed entries and picks the token: the kept ones among the top_k largest and the ties
+// of the last (top_k 0: among all). `mass` is the total that top-p refers to (0: the list's own); then
+// the list is the head of the row's order, and the result is false if the border lies beyond it.
+template <typename T>
+__device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, uint64_t least, float uniform,
+                                const RowWeight& weight, RowScratch& sh, int64_t* __restrict__ token) {
+  using K = RowKey<T>;
+  uint64_t* sorted = sh.hist;
+  row_order(sh.list, sorted, n);
+  const uint32_t kth = top_k ? static_cast<uint32_t>(sorted[top_k - 1] >> 32) : 0u;
+  constexpr int PER = kRowList / kRowThreads;
+  uint64_t w[PER], own = 0, total;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    const uint32_t key = at < n ? static_cast<uint32_t>(sorted[at] >> 32) : 0u;
+    w[j] = at < n && key >= kth ? weight(K::value(key)) : 0;
+    own += w[j];
+  }
+  uint64_t before = block_exclusive_u64(own, sh, total);
+  const uint64_t target = top_p < 1.f ? floor_share(top_p, mass ? mass : total) : ~0ull;
+  if (mass && target >= total) return false;
+  uint64_t* kept = sh.list;  // row_order has read the list
+  own = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    const uint64_t keep = before <= target && w[j] >= least ? w[j] : 0;
+    before += w[j];
+    own += keep;
+    if (at < n) kept[at] = keep;
+  }
+  const uint64_t aim = floor_share(uniform, block_sum_u64(own, sh));
+  // the running sum before an entry in index order is the weight of the kept entries of lower index
+  int parts = 32;
+  while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
+  const int stride = kRowThreads / parts, part = threadIdx.x % parts;
+  for (int e0 = 0; e0 < n; e0 += stride) {
+    const int e = e0 + threadIdx.x / parts;
+    const uint32_t place = e < n ? static_cast<uint32_t>(sorted[e]) : 0u;
+    const uint64_t mine = e < n ? kept[e] : 0;
+    uint64_t run = 0;
+    if (mine)
+      for (int j = part; j < n; j += parts)
+        if (static_cast<uint32_t>(sorted[j]) > place) run += kept[j];
+    for (int o = parts >> 1; o > 0; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+    if (mine && part == 0 && run <= aim && aim < run + mine) *token = ~place;
+  }
+  return true;
+}
+
+// A slice's weight at the row's maximum: as it is where the slice holds that maximum, else brought down.
+__device__ __forceinline__ uint64_t row_slice_mass(const RowSlice& a, uint32_t top_key, float slice_top,
+                                                   const RowWeight& weight, float temperature) {
+  if (a.top == top_key || a.top == 0) return a.mass;
+  return __double2ull_rn(static_cast<double>(a.mass) *
+                         exp((static_cast<double>(slice_top) - static_cast<double>(weight.top)) / temperature));
+}
+
 // The border of the nucleus among all candidates: the key `cut` of its last entry and how many of
 // the entries with that key are inside (`ties`); `mass` is the weight of all candidates. The entries
 // that weigh at most (mass - target - 1) / V together weigh less than mass - target, so the border
 // lies above them: only the others are counted, in bins even in x. False where the border's bin
 // holds too many entries (the caller then selects by radix).
 template <typename T>
-__device__ bool row_nucleus(const typename RowKey<T>::type* keys, int off, const RowSlice& sl, int V, float T_,
-                            uint64_t mass, uint64_t target, const RowWeight& weight, RowShared& sh, uint32_t cs,
-                            uint32_t& cut, uint64_t& ties) {
+__device__ bool row_nucleus(const RowView<T>& v, float temperature, uint64_t mass, uint64_t target,
+                            const RowWeight& weight, RowScratch& sh, uint32_t& cut, uint64_t& ties) {
   using K = RowKey<T>;
   const float top = weight.top;
   // how far below the maximum (times T) a border can lie, with a margin that covers the fp32 arithmetic;
   // weights are rounded, so one of light + 1 stands for light + 1/2 or more
-  const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(V);
+  const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(v.V);
   const float depth = (static_cast<float>(weight.S) - log2f(static_cast<float>(light) + 0.5f)) * kLn2 + 1e-3f;
-  const float range = depth * T_ + 1e-5f * fabsf(top);
-  if (!(top < INFINITY) || !(range < INFINITY)) return false;  // the same in every CTA
-  const float inv = static_cast<float>(kRowNucleusBins) / range;
+  const float range = depth * temperature + 1e-5f * fabsf(top);
+  if (!(top < INFINITY) || !(range < INFINITY)) return false;
+  const float inv = static_cast<float>(kRowBins) / range;
   const uint32_t low = row_key_floor<T>(top - range);
-  auto bin = [&](uint32_t key) { return min(kRowNucleusBins - 1, static_cast<int>((top - K::value(key)) * inv)); };
-  sh.hist[threadIdx.x] = 0;
+  auto bin = [&](uint32_t key) { return min(kRowBins - 1, static_cast<int>((top - K::value(key)) * inv)); };
+  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) sh.hist[i] = 0;
   if (threadIdx.x == 0) sh.found[0] = ~0ull;
   __syncthreads();
-  row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
-    if (key < low || key == 0u) return;
+  row_visit<T>(v, [&](int, uint32_t key) {
+    if (key < low) return;
     const uint64_t w = weight(K::value(key));
     if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin(key)]), static_cast<unsigned long long>(w));
   });
-  row_cluster_sync();
-  uint64_t h = 0, total;
-  for (uint32_t c = 0; c < cs; ++c) h += peer_u64(&sh.hist[threadIdx.x], c);
-  const uint64_t run = block_exclusive_u64(h, sh, total);
-  if (run <= target && target < run + h) {
-    sh.found[0] = threadIdx.x;
-    sh.found[1] = run;
+  __syncthreads();
+  constexpr int BINS = kRowBins / kRowThreads;
+  uint64_t h[BINS], own = 0, total;
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) own += h[j] = sh.hist[threadIdx.x * BINS + j];
+  uint64_t run = block_exclusive_u64(own, sh, total);
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) {
+    if (run <= target && target < run + h[j]) {
+      sh.found[0] = threadIdx.x * BINS + j;
+      sh.found[1] = run;
+    }
+    run += h[j];
   }
   __syncthreads();
-  const uint64_t border = sh.found[0];
+  if (sh.found[0] == ~0ull) return false;
+  const int border = static_cast<int>(sh.found[0]);
   uint64_t before = sh.found[1];
-  if (border != ~0ull)
-    row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
-      if (key < low || key == 0u || bin(key) != static_cast<int>(border)) return;
-      const uint32_t at = atomicAdd(&sh.listed, 1u);
-      if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(sl.lo + i);
-    });
-  row_cluster_sync();
-  const uint32_t n = row_listed(sh, cs);
-  constexpr int MOST = kRowList / 2;
-  if (border == ~0ull || n > MOST) {
-    row_cluster_sync();  // nobody reads the bins any more
-    return false;
-  }
-  // every CTA orders the border bin's entries for itself and finds the entry that holds the target
-  row_collect(sh.hist, sh, cs);
-  uint64_t* sorted = sh.hist + MOST;
-  row_order(sh.hist, sorted, n, sh);
-  constexpr int PER = MOST / kRowThreads;
-  uint64_t w[PER], own = 0;
+  row_visit<T>(v, [&](int i, uint32_t key) {
+    if (key < low || bin(key) != border) return;
+    const uint32_t at = atomicAdd(&sh.listed, 1u);
+    if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(i);
+  });
+  __syncthreads();
+  const int n = static_cast<int>(min(sh.listed, static_cast<uint32_t>(kRowList) + 1));
+  if (n > kRowList) return false;
+  uint64_t* sorted = sh.hist;
+  row_order(sh.list, sorted, n);
+  constexpr int PER = kRowList / kRowThreads;
+  uint64_t w[PER];
+  own = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const uint32_t at = threadIdx.x * PER + j;
+    const int at = threadIdx.x * PER + j;
     w[j] = at < n ? weight(K::value(static_cast<uint32_t>(sorted[at] >> 32))) : 0;
     own += w[j];
   }
@@ -784,278 +906,337 @@ __device__ bool row_nucleus(const typename RowKey<T>::type* keys, int off, const
   return true;
 }
 
-// The leader's part of a top-k sample: `merged` holds n entries, the top_k largest and every tie of
-// the last among them. Filters them and picks the token.
+// Picks the token by going over the row in index order: kept are the entries above `cut` and the first
+// `ties` equal to it, as far as they weigh `least`; no entry below the key `lowest` does.
 template <typename T>
-__device__ void row_pick_listed(uint64_t* merged, uint64_t* sorted, int n, int top_k, float top_p, uint64_t least,
-                                float uniform, const RowWeight& weight, RowShared& sh, int64_t* __restrict__ token) {
+__device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, uint32_t lowest, uint64_t least,
+                              float uniform, const RowWeight& weight, RowScratch& sh, int64_t* __restrict__ token) {
   using K = RowKey<T>;
-  row_order(merged, sorted, n, sh);
-  const uint32_t kth = static_cast<uint32_t>(sorted[top_k - 1] >> 32);
-  constexpr int PER = kRowList / kRowThreads;
-  uint64_t w[PER], own = 0, total;
+  constexpr int VEC = RowView<T>::VEC;
+  const int lane = threadIdx.x & 31;
+  const uint64_t cut_weight = weight(K::value(cut));
+  if (cut_weight < least) ties = 0;
+  auto above = [&](uint32_t key) -> uint64_t {
+    if (key <= cut || key < lowest) return 0;
+    const uint64_t w = weight(K::value(key));
+    return w >= least ? w : 0;
+  };
+  uint64_t sum = 0;
+  uint32_t eq = 0;
+  row_warp_walk<T>(v, [&](int, const uint32_t(&key)[VEC]) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int at = threadIdx.x * PER + j;
-    const uint32_t key = at < n ? static_cast<uint32_t>(sorted[at] >> 32) : 0u;
-    w[j] = at < n && key >= kth ? weight(K::value(key)) : 0;
-    own += w[j];
-  }
-  uint64_t before = block_exclusive_u64(own, sh, total);
-  const uint64_t target = top_p < 1.f ? floor_share(top_p, total) : ~0ull;
-  own = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int at = threadIdx.x * PER + j;
-    const uint64_t kept = before <= target && w[j] >= least ? w[j] : 0;
-    before += w[j];
-    own += kept;
-    if (at < n) merged[at] = kept;  // merged has been read by row_order
-  }
-  const uint64_t all = block_sum_u64(own, sh);
+    for (int e = 0; e < VEC; ++e) {
+      sum += above(key[e]);
+      eq += key[e] == cut;
+    }
+    return true;
+  });
+  // of each warp's range: its equals inside, its weight, the weight before it
+  uint64_t all;
+  uint64_t rank = __shfl_sync(0xffffffffu, block_exclusive_u64(eq, sh, all), 0);
+  const uint64_t equals = __reduce_add_sync(0xffffffffu, eq);
+  const uint64_t inside = rank < ties ? min(ties - rank, equals) : 0;
+  sum = warp_sum_u64(sum) + inside * cut_weight;
+  uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? sum : 0, sh, all), 0);
   const uint64_t aim = floor_share(uniform, all);
-  // the running sum before an entry in index order is the weight of the kept entries of lower index
-  int parts = 32;
-  while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
-  const int stride = kRowThreads / parts, part = threadIdx.x % parts;
-  for (int e0 = 0; e0 < n; e0 += stride) {
-    const int e = e0 + threadIdx.x / parts;
-    const uint32_t place = e < n ? static_cast<uint32_t>(sorted[e]) : 0u;
-    uint64_t run = 0;
-    if (e < n)
-      for (int j = part; j < n; j += parts)
-        if (static_cast<uint32_t>(sorted[j]) > place) run += merged[j];
-    for (int o = parts >> 1; o > 0; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
-    if (e < n && part == 0 && run <= aim && aim < run + merged[e]) *token = ~place;
-  }
+  if (run > aim || aim >= run + sum) return;
+  row_warp_walk<T>(v, [&](int b, const uint32_t(&key)[VEC]) {
+    uint32_t same = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) same += key[e] == cut;
+    uint32_t se = same;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, se, o);
+      if (lane >= o) se += u;
+    }
+    uint64_t r = rank + se - same;
+    rank += __shfl_sync(0xffffffffu, se, 31);
+    uint64_t w[VEC], mine = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[e] = key[e] == cut ? (r++ < ties ? cut_weight : 0) : above(key[e]);
+      mine += w[e];
+    }
+    uint64_t si = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t u = __shfl_up_sync(0xffffffffu, si, o);
+      if (lane >= o) si += u;
+    }
+    uint64_t at = run + si - mine;
+    run += __shfl_sync(0xffffffffu, si, 31);
+    if (at <= aim && aim < at + mine)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (at <= aim && aim < at + w[e]) *token = v.first(b) + e;
+        at += w[e];
+      }
+    return run <= aim;
+  });
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 2)
-    sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int per, int S,
-                         const float* __restrict__ uniform, SampleKnobs knobs, int64_t* __restrict__ tokens) {
+// Picks the token of an unfiltered row from the slices' weights: the slice that holds the uniform's
+// share, and in it the entry, by the slice's own weights.
+template <typename T, int BLOCKS>
+__device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t row, uint32_t top_key,
+                               float temperature, float uniform, const RowWeight& weight, RowScratch& sh,
+                               int64_t* __restrict__ token) {
   using K = RowKey<T>;
-  extern __shared__ __align__(16) uint8_t row_smem[];
-  __shared__ RowShared sh;
-  uint32_t cs, rank;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cs));
-  rank = cluster_ctarank();
-  const int64_t row = blockIdx.x / cs;
-  const float temperature = knobs.temperature ? knobs.temperature[row] : knobs.temperature1;
-  const int top_k = knobs.top_k ? knobs.top_k[row] : knobs.top_k1;
-  const float top_p = knobs.top_p ? knobs.top_p[row] : knobs.top_p1;
-  const float min_p = knobs.min_p ? knobs.min_p[row] : knobs.min_p1;
-  const bool greedy = temperature < 1e-5f;
-
-  const RowSlice sl(V, per, rank);
-  const T* p = x + row * ldx + sl.lo;
-  const int off = row_stage_offset(p);
-  auto* keys = reinterpret_cast<typename K::type*>(row_smem) + off;
-  uint32_t best, count;
-  row_exp_table(sh);
-  if (threadIdx.x == 0) sh.listed = 0;
-  row_stage<T>(p, sl.n, keys, best, count);
-  sh.tmax[threadIdx.x] = best;
-  const uint32_t wbest = __reduce_max_sync(0xffffffffu, best), wcount = __reduce_add_sync(0xffffffffu, count);
-  if ((threadIdx.x & 31) == 0) sh.warp_u64[threadIdx.x >> 5] = (static_cast<uint64_t>(wbest) << 32) | wcount;
-  __syncthreads();
-  uint32_t bmax = 0, bcount = 0;
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) {
-    bmax = max(bmax, static_cast<uint32_t>(sh.warp_u64[w] >> 32));
-    bcount += static_cast<uint32_t>(sh.warp_u64[w]);
+  constexpr int VEC = RowView<T>::VEC, SLICE = BLOCKS * kScanThreads;
+  RowSlice a{0u, 0u, 0ull};
+  uint64_t own = 0, total;
+  if (static_cast<int>(threadIdx.x) < scan.slices) {
+    a = scan.slice[row * scan.slices + threadIdx.x];
+    own = row_slice_mass(a, top_key, K::value(a.top), weight, temperature);
   }
-  if (threadIdx.x == 0) {
-    sh.slot[0] = (static_cast<uint64_t>(bmax) << 32) | bcount;
-    sh.slot[1] = 0;
-  }
-  if (greedy) {  // the slice's first entry with its largest key
-    __syncthreads();
-    uint32_t first = 0;
-    if (best == bmax)
-      row_own<T>(keys, off, sl.n, [&](int i, uint32_t key) {
-        if (key == bmax) first = max(first, ~static_cast<uint32_t>(sl.lo + i));
-      });
-    if (first) atomicMax(reinterpret_cast<unsigned long long*>(&sh.slot[1]), static_cast<unsigned long long>(first));
-  }
-  row_cluster_sync();
-  uint32_t top_key = 0, candidates = 0, top_place = 0;
-  for (uint32_t r = 0; r < cs; ++r) {
-    const uint64_t e = peer_u64(&sh.slot[0], r);
-    const uint32_t key = static_cast<uint32_t>(e >> 32);
-    if (key > top_key) {  // of equal maxima the first CTA's
-      top_key = key;
-      top_place = greedy ? static_cast<uint32_t>(peer_u64(&sh.slot[1], r)) : 0u;
+  const uint64_t run = block_exclusive_u64(own, sh, total);
+  uint64_t aim = floor_share(uniform, total);
+  if (run <= aim && aim < run + own) {
+    aim -= run;
+    if (own != a.mass) {  // the share of the slice's own weight
+      const double f = static_cast<double>(aim) / static_cast<double>(own) * static_cast<double>(a.mass);
+      aim = min(static_cast<uint64_t>(__double2ull_rd(f)), a.mass - 1);
     }
-    candidates += static_cast<uint32_t>(e);
+    sh.found[0] = (static_cast<uint64_t>(a.top) << 32) | threadIdx.x;
+    sh.found[1] = aim;
   }
-  if (greedy || top_key == 0) {  // the same for the whole cluster
-    if (rank == 0 && threadIdx.x == 0) tokens[row] = top_key == 0 ? -1 : static_cast<int64_t>(~top_place);
-    row_cluster_sync();  // every CTA has read the others' slots
+  __syncthreads();
+  const RowWeight local = row_weight(K::value(static_cast<uint32_t>(sh.found[0] >> 32)), temperature, weight.S, sh.exp_tab);
+  const int b0 = static_cast<int>(sh.found[0] & 0xFFFFFFFFu) * SLICE;
+  aim = sh.found[1];
+  constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;  // blocks of a thread, neighbours
+  uint32_t key[PER][VEC];
+  uint64_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    if (at < SLICE) {
+      v.keys(b0 + at, key[j]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) key[j][e] = 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (key[j][e]) mine += local(K::value(key[j][e]));
+  }
+  uint64_t at = block_exclusive_u64(mine, sh, total);
+  if (at <= aim && aim < at + mine)
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint64_t w = key[j][e] ? local(K::value(key[j][e])) : 0;
+        if (at <= aim && aim < at + w) *token = v.first(b0 + threadIdx.x * PER + j) + e;
+        at += w;
+      }
+}
+
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, const float* __restrict__ uniform,
+                         SampleKnobs knobs, RowScan scan, int64_t* __restrict__ tokens) {
+  using K = RowKey<T>;
+  constexpr int LANES = kRowGroup / RowView<T>::VEC;
+  extern __shared__ __align__(16) uint32_t row_maxima[];
+  __shared__ RowScratch sh;
+  const int64_t row = blockIdx.x;
+  const RowView<T> v(x + row * ldx, V);
+  row_exp_table(sh.exp_tab);
+  griddep_wait();  // launched as a programmatic dependent of the scan
+  const SampleRow knob(knobs, row);
+  const float u = uniform[row], T_ = knob.temperature;
+  uint32_t top_key, candidates;
+  row_open(scan, row, row_maxima, sh, top_key, candidates);
+  if (top_key == 0) {
+    if (threadIdx.x == 0) tokens[row] = -1;
     return;
   }
-  RowWeight weight;
-  weight.top = K::value(top_key);
-  weight.scale = 92.33248261893567 / static_cast<double>(temperature);  // 64 log2(e) / T
-  weight.S = S;
-  weight.tab = sh.exp_tab;
-  // min-p: weights below this leave
-  const float floor_p = fminf(fmaxf(min_p, 0.f), 1.f);
-  const uint64_t least = __double2ull_ru(static_cast<double>(floor_p) * (1ull << S));
-
-  // top-k: keys below the k-th largest (ties kept) leave
-  uint32_t cut = 1;
-  uint64_t before;
-  if (top_k >= 1 && static_cast<uint32_t>(top_k) < candidates) {
-    if (top_k <= kRowMaxK) {
-      const uint32_t bound = row_bound(top_k, top_key, sh, cs);
-      if (best >= bound) row_gather<T>(keys, off, sl, bound, 0xFFFFFFFFu, sh);
-      row_cluster_sync();
-      const uint32_t n = row_listed(sh, cs);
-      if (n <= kRowList) {  // everything else happens in one CTA
-        if (rank == 0) row_collect(sh.hist, sh, cs);
-        row_cluster_sync();  // nothing of another CTA is read after this
-        if (rank == 0)
-          row_pick_listed<T>(sh.hist, sh.list, n, top_k, top_p, least, uniform[row], weight, sh, tokens + row);
-        return;
-      }
+  if (knob.greedy) {  // the first group with the largest key, its first entry
+    uint32_t g = 0xFFFFFFFFu;
+    for (int i = threadIdx.x; i < scan.groups; i += kRowThreads)
+      if (row_maxima[i] == top_key) g = min(g, static_cast<uint32_t>(i));
+    g = __reduce_min_sync(0xffffffffu, g);
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = g;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    for (int w = 0; w < kRowWarps; ++w) g = min(g, static_cast<uint32_t>(sh.warp[w]));
+    uint32_t at = 0xFFFFFFFFu;
+    if (threadIdx.x < LANES) {
+      uint32_t k[RowView<T>::VEC];
+      const int b = static_cast<int>(g) * LANES + threadIdx.x;
+      v.keys(b, k);
+#pragma unroll
+      for (int e = RowView<T>::VEC - 1; e >= 0; --e)
+        if (k[e] == top_key) at = v.first(b) + e;
     }
-    cut = row_radix_select<T, false>(keys, sl, 1u, top_k - 1, weight, sh, cs, before);
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (threadIdx.x == 0) tokens[row] = at;
+    return;
   }
-  // top-p: the key at the border of the nucleus and how many of its entries are inside
-  uint64_t ties = ~0ull;
-  if (top_p < 1.f) {
+  const RowWeight weight = row_weight(K::value(top_key), T_, S, sh.exp_tab);
+  // min-p: weights below `least` leave; no entry below the key `lowest` passes (lower by a margin that
+  // covers fp32)
+  const float floor_p = fminf(fmaxf(knob.min_p, 0.f), 1.f);
+  const uint64_t least = __double2ull_ru(static_cast<double>(floor_p) * (1ull << S));
+  uint32_t lowest = 1u;
+  if (floor_p > 0.f)
+    lowest = weight.top < INFINITY
+                 ? max(1u, row_key_floor<T>(weight.top + T_ * (logf(floor_p) - 1e-3f) - 1e-5f * fabsf(weight.top)))
+                 : top_key;
+
+  if (knob.top_k >= 1 && knob.top_k <= kRowMaxK) {
+    const int k = static_cast<int>(min(candidates, static_cast<uint32_t>(knob.top_k)));
+    const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
+    const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+    if (n <= kRowList) {
+      row_pick_listed<T>(n, k, knob.top_p, 0, least, u, weight, sh, tokens + row);
+      return;
+    }
+  }
+  uint32_t cut = 1u;
+  uint64_t before, ties = ~0ull;
+  const bool filtered = knob.top_k >= 1 && static_cast<uint32_t>(knob.top_k) < candidates;
+  if (filtered) cut = row_radix_select<T, false>(v, 1u, knob.top_k - 1, weight, sh, before);
+  if (knob.top_p < 1.f) {
     uint64_t mass = 0;
-    row_own<T>(keys, off, sl.n, [&](int, uint32_t key) {
-      if (key >= cut) mass += weight(K::value(key));
-    });
+    if (knob.wants_mass()) {
+      if (static_cast<int>(threadIdx.x) < scan.slices) {
+        const RowSlice a = scan.slice[row * scan.slices + threadIdx.x];
+        mass = row_slice_mass(a, top_key, K::value(a.top), weight, T_);
+      }
+    } else {
+      row_visit<T>(v, [&](int, uint32_t key) {
+        if (key >= cut) mass += weight(K::value(key));
+      });
+    }
     mass = block_sum_u64(mass, sh);
-    if (threadIdx.x == 0) sh.slot[2] = mass;
-    row_cluster_sync();
-    mass = 0;
-    for (uint32_t r = 0; r < cs; ++r) mass += peer_u64(&sh.slot[2], r);
-    const uint64_t target = floor_share(top_p, mass);
-    if (cut > 1 ||
-        !row_nucleus<T>(keys, off, sl, V, temperature, mass, target, weight, sh, cs, cut, ties)) {
-      cut = row_radix_select<T, true>(keys, sl, cut, target, weight, sh, cs, before);
+    if (!filtered) {
+      // the head of the order first: a nucleus is usually a few hundred entries
+      const int k = static_cast<int>(min(candidates, static_cast<uint32_t>(kRowMaxK)));
+      const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
+      const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+      if (n <= kRowList &&
+          row_pick_listed<T>(n, 0, knob.top_p, static_cast<uint32_t>(n) == candidates ? 0 : mass, least, u, weight, sh,
+                             tokens + row))
+        return;
+      __syncthreads();
+    }
+    const uint64_t target = floor_share(knob.top_p, mass);
+    if (filtered || !row_nucleus<T>(v, T_, mass, target, weight, sh, cut, ties)) {
+      __syncthreads();
+      cut = row_radix_select<T, true>(v, cut, target, weight, sh, before);
       ties = (target - before) / weight(K::value(cut)) + 1;
     }
-  }
-  // no entry below this key passes min-p (lower by a margin that covers fp32)
-  uint32_t lowest = cut;
-  if (floor_p > 0.f && weight.top < INFINITY)
-    lowest = max(cut, row_key_floor<T>(weight.top + temperature * (logf(floor_p) - 1e-3f) - 1e-5f * fabsf(weight.top)));
-
-  // walk in index order: the thread's kept weight, its offset in the row, the entry that holds u
-  const uint64_t cut_weight = weight(K::value(cut));
-  uint32_t eq = 0;
-  uint64_t sum = 0;
-  for (int i = sl.begin(); i < sl.end(); ++i) {
-    const uint32_t key = keys[i];
-    if (key < lowest) continue;
-    if (key > cut) {
-      const uint64_t w = weight(K::value(key));
-      if (w >= least) sum += w;
-    } else if (key == cut) {
-      ++eq;
+  } else if (!filtered && floor_p > 0.f) {
+    const int n = row_gather<T>(v, row_maxima, scan.groups, lowest, sh);
+    if (n <= kRowList) {
+      row_pick_listed<T>(n, 0, 1.f, 0, least, u, weight, sh, tokens + row);
+      return;
     }
+  } else if (!filtered && knob.wants_mass()) {
+    row_pick_slice<T, BLOCKS>(v, scan, row, top_key, T_, u, weight, sh, tokens + row);
+    return;
   }
-  uint64_t eq_total = 0, eq_before = block_exclusive_u64(eq, sh, eq_total);
-  if (threadIdx.x == 0) sh.slot[3] = eq_total;
-  row_cluster_sync();
-  for (uint32_t r = 0; r < rank; ++r) eq_before += peer_u64(&sh.slot[3], r);
-  uint64_t eq_kept = eq_before < ties ? min(ties - eq_before, static_cast<uint64_t>(eq)) : 0;
-  if (cut_weight < least) eq_kept = 0;
-  sum += eq_kept * cut_weight;
-  uint64_t cta_total;
-  uint64_t run = block_exclusive_u64(sum, sh, cta_total);
-  if (threadIdx.x == 0) sh.slot[4] = cta_total;
-  row_cluster_sync();
-  uint64_t total = 0;
-  for (uint32_t r = 0; r < cs; ++r) {
-    const uint64_t t = peer_u64(&sh.slot[4], r);
-    if (r < rank) run += t;
-    total += t;
-  }
-  const uint64_t target = floor_share(uniform[row], total);
-  if (run <= target && target < run + sum) {
-    for (int i = sl.begin(); i < sl.end(); ++i) {
-      const uint32_t key = keys[i];
-      uint64_t w = 0;
-      if (key < lowest) continue;
-      if (key > cut) {
-        w = weight(K::value(key));
-        if (w < least) w = 0;
-      } else if (key == cut && eq_kept > 0) {
-        w = cut_weight;
-        --eq_kept;
-      }
-      run += w;
-      if (run > target) {
-        tokens[row] = sl.lo + i;
-        break;
-      }
-    }
-  }
-  row_cluster_sync();  // no CTA leaves while another reads its shared memory
+  row_pick_walk<T>(v, cut, ties, lowest, least, u, weight, sh, tokens + row);
 }
 
 // ------------------------------------------------------------------------------------------------
 // Launch
 // ------------------------------------------------------------------------------------------------
 
-struct RowLaunch {
-  int cs, per, smem;
+struct RowPlan {
+  int groups, slices, blocks;  // blocks: 16-byte blocks of a scan thread
+  size_t off_slice, total;
 };
 
-// Cluster size: the fewest CTAs (a power of two up to 8) with at most 20480 entries each, about 40 a
-// thread, so that two CTAs share an SM and a single row is spread wide; longer rows take up to one
-// CTA's shared memory. 0 if the row is too long for a cluster.
-inline RowLaunch row_launch_plan(int64_t V, int elem) {
-  for (int cs = 1; cs <= kRowMaxCluster; cs *= 2) {
-    const int64_t per = ceil_div(ceil_div(V, cs), 8) * 8;
-    const int64_t bytes = per * elem + 32;
-    if (per <= 20480 || (cs == kRowMaxCluster && bytes <= 190 * 1024))
-      return {cs, static_cast<int>(per), static_cast<int>(bytes)};
-  }
-  return {0, 0, 0};
+// Slices of 8192 entries, 32 a thread in flight; of 2048 where that leaves SMs without a slice (a
+// few rows). `aligned`: every row starts on a 16-byte boundary.
+inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned) {
+  RowPlan p{};
+  const int vec = 16 / elem;
+  p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), kRowGroup));
+  const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 19);
+  p.blocks = (small ? 2048 : 8192) / vec / kScanThreads;
+  p.slices = static_cast<int>(ceil_div(static_cast<int64_t>(p.groups) * kRowGroup, static_cast<int64_t>(p.blocks) * kScanThreads * vec));
+  p.off_slice = (static_cast<size_t>(R) * p.groups * 4 + 255) / 256 * 256;
+  p.total = p.off_slice + static_cast<size_t>(R) * p.slices * sizeof(RowSlice);
+  return p;
 }
 
-template <typename Kern, typename... Args>
-inline int row_launch(Kern kernel, const RowLaunch& lp, int64_t rows, cudaStream_t stream, Args... args) {
-  ORTHRUS_CHECK_CUDA(ensure_smem(kernel, 192 * 1024));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * lp.cs));
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = lp.smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = lp.cs;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  ORTHRUS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+// Bytes that do for any alignment.
+inline size_t row_ws_bytes(int64_t R, int64_t V, int elem) {
+  return std::max(row_plan(R, V, elem, true).total, row_plan(R, V, elem, false).total);
+}
+
+template <typename T, bool SAMPLE>
+int row_scan_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, int V, float temperature, int S,
+                    const SampleKnobs& knobs, const RowScan& scan, cudaStream_t stream) {
+  constexpr int BIG = 8192 / RowView<T>::VEC / kScanThreads, SMALL = 2048 / RowView<T>::VEC / kScanThreads;
+  const unsigned grid = static_cast<unsigned>(R * p.slices);
+  if (p.blocks == BIG)
+    row_scan_kernel<T, BIG, SAMPLE><<<grid, kScanThreads, 0, stream>>>(x, ldx, V, temperature, S, knobs, scan);
+  else
+    row_scan_kernel<T, SMALL, SAMPLE><<<grid, kScanThreads, 0, stream>>>(x, ldx, V, temperature, S, knobs, scan);
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
 }
 
 template <typename T>
+inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, void* ws, size_t ws_bytes, RowPlan& p,
+                       RowScan& scan) {
+  p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0);
+  ORTHRUS_CHECK_ARG(R * p.slices < (1ll << 31) && (reinterpret_cast<uintptr_t>(x) & (sizeof(T) - 1)) == 0);
+  if (ws == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
+  scan = {static_cast<uint32_t*>(ws), reinterpret_cast<RowSlice*>(static_cast<uint8_t*>(ws) + p.off_slice), p.groups,
+          p.slices};
+  return ORTHRUS_OK;
+}
+
+constexpr int kRowSmem = (kRowMaxV + 8) / kRowGroup * 4 + 32;  // the group maxima of the longest row
+
+template <typename T>
 int topk_rows_impl(const T* x, int64_t ldx, int64_t R, int64_t V, int k, float temperature, float* values, int64_t* ids,
-                   float* lse, cudaStream_t stream) {
-  const RowLaunch lp = row_launch_plan(V, sizeof(T));
-  ORTHRUS_CHECK_ARG(lp.cs > 0 && R <= (1ll << 31) / kRowMaxCluster - 1);
-  return row_launch(topk_rows_kernel<T>, lp, R, stream, x, ldx, static_cast<int>(V), lp.per, k, temperature, values, ids, lse);
+                   float* lse, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  RowPlan p;
+  RowScan scan;
+  int rc = row_prepare(x, ldx, R, V, ws, ws_bytes, p, scan);
+  if (rc != ORTHRUS_OK) return rc;
+  rc = row_scan_launch<T, false>(p, x, ldx, R, static_cast<int>(V), temperature, 0, SampleKnobs{}, scan, stream);
+  if (rc != ORTHRUS_OK) return rc;
+  ORTHRUS_CHECK_CUDA(ensure_smem(topk_rows_kernel<T>, kRowSmem));
+  ORTHRUS_CHECK_CUDA(launch_pdl(topk_rows_kernel<T>, dim3(static_cast<unsigned>(R)), dim3(kRowThreads),
+                                (p.groups + 3) / 4 * 16, stream, x, ldx, static_cast<int>(V), k, temperature, scan, values,
+                                ids, lse));
+  ORTHRUS_CHECK_LAUNCH();
+  return ORTHRUS_OK;
+}
+
+template <typename T, int BLOCKS>
+int sample_finish_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, int V, int S, const float* uniform,
+                         const SampleKnobs& knobs, const RowScan& scan, int64_t* tokens, cudaStream_t stream) {
+  auto kernel = sample_logits_kernel<T, BLOCKS>;
+  ORTHRUS_CHECK_CUDA(ensure_smem(kernel, kRowSmem));
+  ORTHRUS_CHECK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(R)), dim3(kRowThreads), (p.groups + 3) / 4 * 16,
+                                stream, x, ldx, V, S, uniform, knobs, scan, tokens));
+  ORTHRUS_CHECK_LAUNCH();
+  return ORTHRUS_OK;
 }
 
 template <typename T>
 int sample_logits_impl(const T* x, int64_t ldx, int64_t R, int64_t V, const float* uniform, const SampleKnobs& knobs,
-                       int64_t* tokens, cudaStream_t stream) {
-  const RowLaunch lp = row_launch_plan(V, sizeof(T));
-  ORTHRUS_CHECK_ARG(lp.cs > 0 && R <= (1ll << 31) / kRowMaxCluster - 1);
-  return row_launch(sample_logits_kernel<T>, lp, R, stream, x, ldx, static_cast<int>(V), lp.per,
-                    row_weight_bits(static_cast<int>(V)), uniform, knobs, tokens);
+                       int64_t* tokens, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  RowPlan p;
+  RowScan scan;
+  int rc = row_prepare(x, ldx, R, V, ws, ws_bytes, p, scan);
+  if (rc != ORTHRUS_OK) return rc;
+  const int n = static_cast<int>(V), S = row_weight_bits(n);
+  rc = row_scan_launch<T, true>(p, x, ldx, R, n, 1.f, S, knobs, scan, stream);
+  if (rc != ORTHRUS_OK) return rc;
+  constexpr int BIG = 8192 / RowView<T>::VEC / kScanThreads, SMALL = 2048 / RowView<T>::VEC / kScanThreads;
+  return p.blocks == BIG ? sample_finish_launch<T, BIG>(p, x, ldx, R, n, S, uniform, knobs, scan, tokens, stream)
+                         : sample_finish_launch<T, SMALL>(p, x, ldx, R, n, S, uniform, knobs, scan, tokens, stream);
 }
 
 }  // namespace orthrus

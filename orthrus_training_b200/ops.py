@@ -780,9 +780,13 @@ def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
     values = torch.empty(R, k, dtype=torch.float32, device=dev)
     ids = torch.empty(R, k, dtype=torch.int64, device=dev)
     lse = torch.empty(R, dtype=torch.float32, device=dev)
+    lib = L.lib()
+    nbytes = lib.orthrus_vocab_rows_workspace_bytes(R, V, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
-        L.check(L.lib().orthrus_topk_rows(logits.data_ptr(), pitch, R, V, k, float(temperature), values.data_ptr(),
-                                          ids.data_ptr(), lse.data_ptr(), code, L.stream_of(dev)), "topk_rows")
+        L.check(lib.orthrus_topk_rows(logits.data_ptr(), pitch, R, V, k, float(temperature), values.data_ptr(),
+                                      ids.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, code, L.stream_of(dev)),
+                "topk_rows")
     return values, ids, lse
 
 
@@ -819,10 +823,13 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     p, p1 = _knob(top_p, "top_p", R, dev, torch.float32, 0.0, 1.0)
     m, m1 = _knob(min_p, "min_p", R, dev, torch.float32, 0.0, 1.0)
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
+    lib = L.lib()
+    nbytes = lib.orthrus_vocab_rows_workspace_bytes(R, V, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
-        L.check(L.lib().orthrus_sample_logits(logits.data_ptr(), pitch, R, V, uniforms.data_ptr(), L.ptr(t), t1,
-                                              L.ptr(k), int(k1), L.ptr(p), p1, L.ptr(m), m1, tokens.data_ptr(), code,
-                                              L.stream_of(dev)), "sample_logits")
+        L.check(lib.orthrus_sample_logits(logits.data_ptr(), pitch, R, V, uniforms.data_ptr(), L.ptr(t), t1, L.ptr(k),
+                                          int(k1), L.ptr(p), p1, L.ptr(m), m1, tokens.data_ptr(), ws.data_ptr(), nbytes,
+                                          code, L.stream_of(dev)), "sample_logits")
     return tokens
 
 

@@ -23,31 +23,45 @@ def test_wrappers_refuse_cpu_tensors():
         ops.sample_logits(x, torch.zeros(2))
 
 
-def _topk(R=2, V=8, ld=8, k=2, temperature=1.0, dtype=1, p=64):
-    return _lib().lib().orthrus_topk_rows(p, ld, R, V, k, ctypes.c_float(temperature), p, p, p, dtype, None)
+def _topk(R=2, V=8, ld=8, k=2, temperature=1.0, dtype=1, p=64, ws=64, ws_bytes=1 << 50):
+    return _lib().lib().orthrus_topk_rows(p, ld, R, V, k, ctypes.c_float(temperature), p, p, p, ws, ws_bytes, dtype,
+                                          None)
 
 
 @pytest.mark.parametrize("bad", [dict(R=-1), dict(V=0), dict(ld=-1), dict(k=0), dict(k=1025), dict(temperature=0.0),
-                                 dict(temperature=float("nan")), dict(dtype=2), dict(p=None), dict(V=400_000),
-                                 dict(V=2 ** 31), dict(R=2 ** 40)])
+                                 dict(temperature=float("nan")), dict(dtype=2), dict(p=None), dict(V=2 ** 20 + 1),
+                                 dict(V=2 ** 31), dict(R=2 ** 40), dict(R=2 ** 28, V=2 ** 20), dict(p=66)])
 def test_topk_rows_status(bad):
     assert _topk(**bad) == _lib().EINVAL
+
+
+def test_row_workspace():
+    lib, L = _lib().lib(), _lib()
+    assert _topk(ws=None) == L.EWORKSPACE and _topk(ws_bytes=8) == L.EWORKSPACE
+    for dtype in (L.F32, L.BF16):
+        assert lib.orthrus_vocab_rows_workspace_bytes(0, 100, dtype) == 0
+        for R, V in ((1, 1), (3, 1000), (1024, 151936), (2, 2 ** 20)):
+            # a maximum for 32 entries, and a record of 16 bytes for 2048 or 8192
+            assert R * V / 8 <= lib.orthrus_vocab_rows_workspace_bytes(R, V, dtype) <= R * (V / 8 + V / 128 + 64) + 256
 
 
 def test_no_rows_are_no_work():
     assert _topk(R=0) == _lib().OK
     f = ctypes.c_float
     assert _lib().lib().orthrus_sample_logits(None, 8, 0, 8, None, None, f(1), None, 0, None, f(1), None, f(0), None,
-                                              1, None) == _lib().OK
+                                              None, 0, 1, None) == _lib().OK
 
 
-@pytest.mark.parametrize("bad", [dict(R=-1), dict(V=0), dict(ld=-1), dict(dtype=7), dict(p=None), dict(V=400_000),
-                                 dict(R=2 ** 40)])
-def test_sample_logits_status(bad):
-    a = dict(dict(R=2, V=8, ld=8, dtype=1, p=64), **bad)
+@pytest.mark.parametrize("bad,status", [
+    (dict(R=-1), "EINVAL"), (dict(V=0), "EINVAL"), (dict(ld=-1), "EINVAL"), (dict(dtype=7), "EINVAL"),
+    (dict(p=None), "EINVAL"), (dict(V=2 ** 20 + 1), "EINVAL"), (dict(R=2 ** 40), "EINVAL"),
+    (dict(ws=None), "EWORKSPACE"), (dict(ws_bytes=8), "EWORKSPACE")])
+def test_sample_logits_status(bad, status):
+    a = dict(dict(R=2, V=8, ld=8, dtype=1, p=64, ws=64, ws_bytes=1 << 50), **bad)
     f = ctypes.c_float
     assert _lib().lib().orthrus_sample_logits(a["p"], a["ld"], a["R"], a["V"], a["p"], None, f(1), None, 0, None, f(1),
-                                              None, f(0), a["p"], a["dtype"], None) == _lib().EINVAL
+                                              None, f(0), a["p"], a["ws"], a["ws_bytes"], a["dtype"],
+                                              None) == getattr(_lib(), status)
 
 
 def test_distillation_refuses_cpu_tensors():

@@ -74,7 +74,7 @@ def _check_topk(x, k, T):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 1024, 5003, 32003, 151936])
+@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 1024, 5003, 32003, 151936, 2 ** 20])
 def test_topk_sizes(dtype, V):
     for k in sorted({1, min(V, 5), 64, 1024}):
         _check_topk(_rows("normal", 3, V, dtype, seed=V + k), k, 1.0)
@@ -153,7 +153,7 @@ FILTERS = [dict(), dict(top_k=1), dict(top_k=40), dict(top_p=0.9), dict(top_p=0.
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 5003, 32003, 151936])
+@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 5003, 32003, 151936, 2 ** 20])
 def test_sample_sizes(dtype, V):
     g = torch.Generator().manual_seed(V)
     x = _rows("normal", 6, V, dtype, seed=V)
@@ -273,7 +273,7 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.topk_rows(x[0], 2)
     with pytest.raises(ValueError):
-        ops.topk_rows(torch.zeros(1, 400_000, device=DEV), 2)  # a row longer than a cluster holds
+        ops.topk_rows(torch.zeros(1, 2 ** 20 + 1, device=DEV), 2)  # a row longer than the operators take
     for bad in (u[:1], u.double(), u.cpu()):
         with pytest.raises(ValueError):
             ops.sample_logits(x, bad)
