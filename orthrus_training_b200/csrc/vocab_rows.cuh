@@ -3,13 +3,13 @@
 //
 // Two launches. The scan reads every logit once, at HBM speed, over as many CTAs as there are slices:
 // it leaves the largest key of each group of 32 neighbouring entries (3 % of the row's bytes) and per
-// slice its maximum, its candidates and, where it is needed, its softmax weight. Then one CTA per row
+// slice its maximum and, where it is needed, its softmax weight. Then one CTA per row
 // finishes from those:
 //   - The k largest entries: the k-th largest group maximum is at most the k-th largest entry, and
 //     little below it unless the row is arranged against it, so the few groups at or above it are read
 //     again (from L2) and the entries at or above it, k and a few more, are ordered in shared memory.
-//   - A nucleus without top-k is looked for among the 1024 largest entries first, then by a histogram
-//     of weights over the values that can hold its border, exact among the border bin's entries.
+//   - A nucleus without top-k is looked for among the 1024 largest entries first; a wider one's border
+//     is bracketed by a histogram and found exactly among the entries in the bracket.
 //   - Without a filter the slices' weights say which slice holds the uniform's share.
 // Where the gathered entries are too many for shared memory (rows of equal values, nuclei of many
 // thousands), the CTA goes over the whole row again: a radix selection that is right for every row, and
@@ -46,6 +46,7 @@ struct RowKey<float> {
   using type = uint32_t;
   static constexpr int BITS = 32;
   static constexpr int VEC = 4;  // elements per 16-byte load
+  __device__ static __forceinline__ uint32_t of(float x) { return of_bits(__float_as_uint(x)); }
   __device__ static __forceinline__ uint32_t of_bits(uint32_t b) {
     if ((b << 1) == 0u) b = 0u;                                       // -0 as +0
     if ((b << 1) > 0xFF000000u || b == 0xFF800000u) return 0u;        // NaN, -inf
@@ -61,6 +62,7 @@ struct RowKey<__nv_bfloat16> {
   using type = uint16_t;
   static constexpr int BITS = 16;
   static constexpr int VEC = 8;
+  __device__ static __forceinline__ uint32_t of(float x) { return of_bits(__float_as_uint(x) >> 16); }  // x is a bf16
   __device__ static __forceinline__ uint32_t of_bits(uint32_t b) {
     if ((b & 0x7FFFu) == 0u) b = 0u;
     if ((b & 0x7FFFu) > 0x7F80u || b == 0xFF80u) return 0u;
@@ -98,6 +100,23 @@ struct RowView {
     for (int e = 0; e < VEC; ++e)
       k[e] = sizeof(T) == 4 ? K::of_bits(w[e]) : K::of_bits((e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu);
   }
+  // its values, with -inf for what is no candidate
+  __device__ __forceinline__ static void values_of(const uint4& q, float (&x)[VEC]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint32_t b = sizeof(T) == 4 ? w[e] : (e & 1) ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16;
+      x[e] = fmaxf(__uint_as_float(b), -INFINITY);  // NaN gives way
+    }
+  }
+  __device__ __forceinline__ void values(int b, float (&x)[VEC]) const {
+    if (b < blocks && whole(b)) {
+      values_of(load(b), x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[e] = b < blocks ? K::value(key(first(b) + e)) : -INFINITY;
+    }
+  }
   __device__ __forceinline__ uint32_t key(int i) const {
     if (i < 0 || i >= V) return 0u;
     if constexpr (sizeof(T) == 4)
@@ -126,7 +145,7 @@ struct RowScratch {
   uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
   double exp_tab[64];        // 2^(-j/64)
   uint64_t warp[kRowWarps];
-  uint64_t warp_count[2][kRowWarps];
+  uint32_t top[kRowWarps];
   uint64_t found[2];         // result of a block-wide search
   uint32_t groups[kRowList]; // numbers of the groups to read again
   uint32_t ngroups, listed;
@@ -186,22 +205,23 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowScratch& 
 // = n + f with |f| <= 1/2, exp = 2^-(n >> 6) * tab[n & 63] * e^(-f ln2 / 64), the last factor by
 // its Taylor polynomial of degree 4 (error below (0.0055)^5 / 120 = 4e-14).
 struct RowWeight {
-  float top;     // the row's maximum
-  double scale;  // 64 log2(e) / T
+  float top;         // the maximum the weights refer to
   int S;
+  double scale, at;  // 64 log2(e) / T; top * scale
   const double* tab;
 
   __device__ __forceinline__ uint64_t operator()(float x) const {
-    constexpr double kRound = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to an integer
-    constexpr double kInt = 4503599627370496.0;     // 2^52
-    const double y = x == top ? 0.0 : (static_cast<double>(top) - static_cast<double>(x)) * scale;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    constexpr double kInt = 4503599627370496.0;    // 2^52
+    constexpr double c = -0.6931471805599453 / 64.0;
+    const double y = x == top ? 0.0 : fma(-static_cast<double>(x), scale, at);
     if (!(y < 64.0 * (S + 2))) return 0;  // rounds to 0; also an infinite maximum's other entries
     const double r = y + kRound;
     const int n = __double2loint(r);
-    const double z = (y - (r - kRound)) * (-0.6931471805599453 / 64.0);
-    const double p = fma(fma(fma(fma(z, 1.0 / 24.0, 1.0 / 6.0), z, 0.5), z, 1.0), z, 1.0);
-    const double s = __hiloint2double((1023 + S - (n >> 6)) << 20, 0);  // 2^(S - n/64)
-    const double w = fma(p * tab[n & 63], s, kInt);
+    const double f = y - (r - kRound);
+    const double p = fma(fma(fma(fma(f, c * c * c * c / 24.0, c * c * c / 6.0), f, c * c / 2.0), f, c), f, 1.0) * tab[n & 63];
+    // times 2^(S - n / 64), by the exponent
+    const double w = __hiloint2double(__double2hiint(p) + ((S - (n >> 6)) << 20), __double2loint(p)) + kInt;
     return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
   }
 };
@@ -217,7 +237,8 @@ __device__ __forceinline__ void row_exp_table(double* tab) {
 }
 
 __device__ __forceinline__ RowWeight row_weight(float top, float temperature, int S, const double* tab) {
-  return {top, 92.33248261893567 / static_cast<double>(temperature), S, tab};  // 64 log2(e) / T
+  const double scale = 92.33248261893567 / static_cast<double>(temperature);  // 64 log2(e) / T
+  return {top, S, scale, static_cast<double>(top) * scale, tab};
 }
 
 // floor(f * z) for f in [0, 1) and z < 2^62, exactly (f is an integer of 24 bits times a power of
@@ -241,11 +262,12 @@ __device__ __forceinline__ uint64_t floor_share(float f, uint64_t z) {
 
 struct RowSlice {
   uint32_t top;    // largest key
-  uint32_t count;  // candidates
-  uint64_t mass;   // sum of exp((x - slice's largest) / T): a float's bits (top-k), or 2^S fold (sampling)
+  float sum;       // sum of exp((x - slice's largest) / T) (top-k)
+  uint64_t mass;   // the same, 2^S fold (sampling)
 };
 
-// What the scan leaves of R rows: group maxima [R, groups] and slices [R, slices].
+// What the scan leaves of R rows: group maxima [R, groups] (groups a multiple of four, so that a row's
+// are read as vectors) and slices [R, slices].
 struct RowScan {
   uint32_t* group;
   RowSlice* slice;
@@ -284,10 +306,11 @@ __global__ void __launch_bounds__(kScanThreads)
     row_scan_kernel(const T* __restrict__ x, int64_t ldx, int V, float temperature, int S, SampleKnobs knobs,
                     RowScan out) {
   using View = RowView<T>;
+  using K = RowKey<T>;
   constexpr int VEC = View::VEC;
   constexpr int LANES = kRowGroup / VEC;  // neighbouring lanes of a group
   __shared__ double tab[64];
-  __shared__ uint32_t wtop[kScanThreads / 32], wcount[kScanThreads / 32];
+  __shared__ float wtop[kScanThreads / 32], wsum[kScanThreads / 32];
   __shared__ uint64_t wmass[kScanThreads / 32];
   griddep_launch_dependents();
   const int64_t row = blockIdx.x / static_cast<unsigned>(out.slices);
@@ -302,79 +325,68 @@ __global__ void __launch_bounds__(kScanThreads)
     mass_wanted = knob.wants_mass();
     if (mass_wanted) row_exp_table(tab);
   }
-  uint32_t key[BLOCKS][VEC];
+  float val[BLOCKS][VEC];
   if (v.whole(b0) && v.whole(b0 + BLOCKS * kScanThreads - 1)) {
     uint4 q[BLOCKS];
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) q[j] = v.load(b0 + j * kScanThreads + threadIdx.x);
 #pragma unroll
-    for (int j = 0; j < BLOCKS; ++j) View::keys_of(q[j], key[j]);
+    for (int j = 0; j < BLOCKS; ++j) View::values_of(q[j], val[j]);
   } else {  // the row's ends
 #pragma unroll
-    for (int j = 0; j < BLOCKS; ++j) v.keys(b0 + j * kScanThreads + threadIdx.x, key[j]);
+    for (int j = 0; j < BLOCKS; ++j) v.values(b0 + j * kScanThreads + threadIdx.x, val[j]);
   }
-  uint32_t top = 0, count = 0;
+  float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < BLOCKS; ++j) {
-    uint32_t m = 0;
+    float m = val[j][0];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      m = max(m, key[j][e]);
-      count += key[j][e] != 0u;
-    }
-    top = max(top, m);
+    for (int e = 1; e < VEC; ++e) m = fmaxf(m, val[j][e]);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    top = fmaxf(top, m);
     const int g = (b0 + j * kScanThreads + static_cast<int>(threadIdx.x)) / LANES;
-    if (lane % LANES == 0 && g < out.groups) out.group[row * out.groups + g] = m;
+    if (lane % LANES == 0 && g < out.groups) out.group[row * out.groups + g] = K::of(m);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  count = __reduce_add_sync(0xffffffffu, count);
-  if (lane == 0) {
-    wtop[warp] = top;
-    wcount[warp] = count;
-  }
+#pragma unroll
+  for (int o = 16; o >= LANES; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) wtop[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kScanThreads / 32; ++w) top = max(top, wtop[w]);
-  const float ftop = RowKey<T>::value(top);
+  for (int w = 0; w < kScanThreads / 32; ++w) top = fmaxf(top, wtop[w]);
   uint64_t mass = 0;
+  float sum = 0.f;
   if constexpr (SAMPLE) {
-    if (mass_wanted && top) {
-      const RowWeight weight = row_weight(ftop, temperature, S, tab);
+    if (mass_wanted && top > -INFINITY) {
+      const RowWeight weight = row_weight(top, temperature, S, tab);
 #pragma unroll
       for (int j = 0; j < BLOCKS; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (key[j][e]) mass += weight(RowKey<T>::value(key[j][e]));
+        for (int e = 0; e < VEC; ++e) mass += weight(val[j][e]);
+      mass = warp_sum_u64(mass);
     }
-    mass = warp_sum_u64(mass);
+    if (lane == 0) wmass[warp] = mass;
   } else {
     const float c = kLog2e / temperature;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (top && ftop < INFINITY) {
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top > -INFINITY && top < INFINITY) {
 #pragma unroll
       for (int j = 0; j < BLOCKS; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          sum[e & 3] += key[j][e] ? ex2_approx((RowKey<T>::value(key[j][e]) - ftop) * c) : 0.f;
+        for (int e = 0; e < VEC; ++e) part[e & 3] += ex2_approx((val[j][e] - top) * c);
     }
-    float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    sum = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    mass = __float_as_uint(s);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) wsum[warp] = sum;
   }
-  if (lane == 0) wmass[warp] = mass;
   __syncthreads();
   if (threadIdx.x == 0) {
-    RowSlice r{top, 0u, 0ull};
-    float s = 0.f;
+    RowSlice r{K::of(top), 0.f, 0ull};
     for (int w = 0; w < kScanThreads / 32; ++w) {
-      r.count += wcount[w];
       if constexpr (SAMPLE) r.mass += wmass[w];
-      else s += __uint_as_float(static_cast<uint32_t>(wmass[w]));
+      else r.sum += wsum[w];
     }
-    if constexpr (!SAMPLE) r.mass = __float_as_uint(s);
     out.slice[row * out.slices + slice] = r;
   }
 }
@@ -383,109 +395,106 @@ __global__ void __launch_bounds__(kScanThreads)
 // The few largest entries
 // ------------------------------------------------------------------------------------------------
 
-// The row's group maxima into shared memory (padded with zeros to a multiple of four), its largest
-// key and its candidates. Every thread gets both.
-__device__ __forceinline__ void row_open(const RowScan& scan, int64_t row, uint32_t* maxima, RowScratch& sh,
-                                         uint32_t& top_key, uint32_t& candidates) {
-  const uint32_t* g = scan.group + row * scan.groups;
-  for (int i = threadIdx.x; i < (scan.groups + 3) / 4 * 4; i += kRowThreads) maxima[i] = i < scan.groups ? g[i] : 0u;
-  uint32_t top = 0, count = 0;
-  for (int i = threadIdx.x; i < scan.slices; i += kRowThreads) {
-    const RowSlice s = scan.slice[row * scan.slices + i];
-    top = max(top, s.top);
-    count += s.count;
-  }
+// The row's group maxima into shared memory and its largest key (0: no candidates), for every thread.
+__device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row, uint32_t* maxima, RowScratch& sh) {
+  const uint4* g = reinterpret_cast<const uint4*>(scan.group + row * scan.groups);
+  uint4* m = reinterpret_cast<uint4*>(maxima);
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < scan.slices; i += kRowThreads) top = max(top, scan.slice[row * scan.slices + i].top);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < scan.groups / 4; i += kRowThreads) m[i] = g[i];
   top = __reduce_max_sync(0xffffffffu, top);
-  count = __reduce_add_sync(0xffffffffu, count);
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = (static_cast<uint64_t>(top) << 32) | count;
+  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = top;
   if (threadIdx.x == 0) sh.ngroups = sh.listed = 0;
   __syncthreads();
-  top_key = candidates = 0;
 #pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) {
-    top_key = max(top_key, static_cast<uint32_t>(sh.warp[w] >> 32));
-    candidates += static_cast<uint32_t>(sh.warp[w]);
-  }
-  __syncthreads();
+  for (int w = 0; w < kRowWarps; ++w) top = max(top, sh.top[w]);
+  return top;
 }
 
 // A key with at least k entries of the row at or above it, and not many more: between the k-th largest
-// group maximum and a little below it; 1 if fewer than k groups hold a candidate. Four-way search
-// on counts of the maxima.
+// group maximum and a little below it; 1 if fewer than k groups hold a candidate. Histograms of the
+// maxima over the range of keys that can hold the bound, 1024 bins at a time.
 __device__ __forceinline__ uint32_t row_bound(const uint32_t* maxima, int groups, int k, uint32_t top_key,
                                               RowScratch& sh) {
+  constexpr int BINS = 2 * kRowThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
   const uint4* m4 = reinterpret_cast<const uint4*>(maxima);
-  const int n4 = (groups + 3) / 4;
-  // three counters of 21 bits a word; `buf` alternates, so one barrier an exchange is enough
-  auto total = [&](uint32_t a, uint32_t b, uint32_t c, int buf) {
-    a = __reduce_add_sync(0xffffffffu, a);
-    b = __reduce_add_sync(0xffffffffu, b);
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) sh.warp_count[buf][warp] = a | (static_cast<uint64_t>(b) << 21) | (static_cast<uint64_t>(c) << 42);
-    __syncthreads();
-    uint64_t t = 0;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) t += sh.warp_count[buf][w];
-    return t;
-  };
-  uint32_t least = 0xFFFFFFFFu, some = 0;
-  for (int i = threadIdx.x; i < n4; i += kRowThreads) {
+  // the smallest candidate maximum
+  uint32_t least = top_key;
+  for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
     const uint4 q = m4[i];
-    const uint32_t m[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (m[e]) {
-        least = min(least, m[e]);
-        ++some;
-      }
+    least = min(min(least, q.x ? q.x : top_key), min(min(q.y ? q.y : top_key, q.z ? q.z : top_key), q.w ? q.w : top_key));
   }
   least = __reduce_min_sync(0xffffffffu, least);
-  if (lane == 0) sh.warp[warp] = least;
-  uint32_t have = static_cast<uint32_t>(total(some, 0, 0, 0) & 0x1FFFFF);
+  if (lane == 0) sh.top[warp] = least;
+  counts[threadIdx.x] = counts[threadIdx.x + kRowThreads] = 0;
+  if (threadIdx.x == 0) sh.found[0] = ~0ull;
+  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) least = min(least, static_cast<uint32_t>(sh.warp[w]));
+  for (int w = 0; w < kRowWarps; ++w) least = min(least, sh.top[w]);
+  uint32_t lo = least, hi = top_key;  // the bound is in [lo, hi]
+  uint32_t above = 0;                 // maxima above hi
   const uint32_t want = k, enough = k + k / 4 + 16;
-  uint32_t lo = least, hi = top_key + 1;  // at least k maxima at or above lo, fewer at or above hi
-  if (have < want) {
-    lo = 1u;
-    hi = 2u;
-  }
-  for (int step = 1; have > enough && hi - lo > 1; ++step) {
-    const uint32_t d = hi - lo;
-    const uint32_t t1 = lo + (d + 3) / 4, t2 = lo + (d + 1) / 2, t3 = lo + d - d / 4;
-    uint32_t a = 0, b = 0, c = 0;
-    for (int i = threadIdx.x; i < n4; i += kRowThreads) {
+  while (true) {
+    int shift = 0;
+    while (((hi - lo) >> shift) >= BINS) ++shift;
+    for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
       const uint4 q = m4[i];
       const uint32_t m[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a += m[e] >= t1;
-        b += m[e] >= t2;
-        c += m[e] >= t3;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (m[e] >= lo && m[e] <= hi) atomicAdd(&counts[(hi - m[e]) >> shift], 1u);
     }
-    const uint64_t t = total(a, b, c, step & 1);
-    a = static_cast<uint32_t>(t) & 0x1FFFFF;
-    b = static_cast<uint32_t>(t >> 21) & 0x1FFFFF;
-    c = static_cast<uint32_t>(t >> 42);
-    if (c >= want) {
-      lo = t3;
-      have = c;
-    } else if (b >= want) {
-      lo = t2;
-      hi = t3;
-      have = b;
-    } else if (a >= want) {
-      lo = t1;
-      hi = t2;
-      have = a;
-    } else {
-      hi = t1;
+    __syncthreads();
+    // bin b holds the keys hi - (b << shift) downwards; thread t has the bins 2t and 2t + 1
+    const uint32_t c0 = counts[2 * threadIdx.x], c1 = counts[2 * threadIdx.x + 1];
+    uint32_t inc = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
     }
+    if (lane == 31) sh.top[warp] = inc;
+    __syncthreads();
+    uint32_t run = above + inc - c0 - c1;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) run += w < warp ? sh.top[w] : 0u;
+    if (run < want && want <= run + c0) {
+      sh.found[0] = 2 * threadIdx.x;
+      sh.found[1] = (static_cast<uint64_t>(run) << 32) | (run + c0);
+    } else if (run + c0 < want && want <= run + c0 + c1) {
+      sh.found[0] = 2 * threadIdx.x + 1;
+      sh.found[1] = (static_cast<uint64_t>(run + c0) << 32) | (run + c0 + c1);
+    }
+    counts[2 * threadIdx.x] = counts[2 * threadIdx.x + 1] = 0;
+    __syncthreads();
+    if (sh.found[0] == ~0ull) {  // fewer than k groups hold a candidate
+      lo = 1u;
+      break;
+    }
+    const uint32_t b = static_cast<uint32_t>(sh.found[0]), have = static_cast<uint32_t>(sh.found[1]);
+    const uint32_t from = hi - (b << shift), depth = (1u << shift) - 1u;
+    above = static_cast<uint32_t>(sh.found[1] >> 32);
+    lo = from - lo > depth ? from - depth : lo;
+    hi = from;
+    if (have <= enough || shift == 0) break;
   }
-  __syncthreads();  // warp and warp_count are free again
+  __syncthreads();  // found and the counts are free again
   return lo;
+}
+
+// Appends the entries of the lanes with `take` to the list, one atomic a warp. Every lane calls it.
+template <typename E>
+__device__ __forceinline__ void row_append(bool take, E entry, E* list, uint32_t* count) {
+  const uint32_t who = __ballot_sync(0xffffffffu, take);
+  if (who == 0) return;
+  const int lane = threadIdx.x & 31, first = __ffs(who) - 1;
+  uint32_t at = 0;
+  if (lane == first) at = atomicAdd(count, static_cast<uint32_t>(__popc(who)));
+  at = __shfl_sync(0xffffffffu, at, first) + __popc(who & ((1u << lane) - 1u));
+  if (take && at < kRowList) list[at] = entry;
 }
 
 // Reads the groups at or above `low` again and lists their entries with low <= key; returns their
@@ -494,39 +503,32 @@ template <typename T>
 __device__ int row_gather(const RowView<T>& v, const uint32_t* maxima, int groups, uint32_t low, RowScratch& sh) {
   constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC;
   const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < groups; i += kRowThreads)
-    if (maxima[i] >= low) {
-      const uint32_t at = atomicAdd(&sh.ngroups, 1u);
-      if (at < kRowList) sh.groups[at] = i;
-    }
-  __syncthreads();
-  const int ng = static_cast<int>(sh.ngroups);
-  if (ng > kRowList) {  // every group holds at least one entry
-    __syncthreads();
-    if (threadIdx.x == 0) sh.ngroups = 0;
-    __syncthreads();
-    return kRowList + 1;
+  for (int i0 = 0; i0 < groups; i0 += kRowThreads) {
+    const int i = i0 + static_cast<int>(threadIdx.x);
+    row_append(i < groups && maxima[i] >= low, static_cast<uint32_t>(i), sh.groups, &sh.ngroups);
   }
+  __syncthreads();
+  const int ng = static_cast<int>(sh.ngroups);  // every group holds at least one entry
   // LANES neighbouring lanes a group
-  for (int i0 = 0; i0 < ng; i0 += kRowThreads / LANES) {
-    const int i = i0 + static_cast<int>(threadIdx.x) / LANES;
-    uint32_t k[VEC];
-    int b = 0;
+  if (ng <= kRowList)
+    for (int i0 = 0; i0 < ng; i0 += kRowThreads / LANES) {
+      const int i = i0 + static_cast<int>(threadIdx.x) / LANES;
+      uint32_t k[VEC];
+      int b = 0;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) k[e] = 0u;
-    if (i < ng) {
-      b = static_cast<int>(sh.groups[i]) * LANES + lane % LANES;
-      v.keys(b, k);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (k[e] >= low) {
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e);
+      for (int e = 0; e < VEC; ++e) k[e] = 0u;
+      if (i < ng) {
+        b = static_cast<int>(sh.groups[i]) * LANES + lane % LANES;
+        v.keys(b, k);
       }
-  }
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        row_append(k[e] >= low, (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e), sh.list,
+                   &sh.listed);
+    }
   __syncthreads();
-  const int n = static_cast<int>(sh.listed);
+  const int n = ng <= kRowList ? static_cast<int>(sh.listed) : kRowList + 1;
   __syncthreads();
   if (threadIdx.x == 0) sh.ngroups = sh.listed = 0;
   __syncthreads();
@@ -581,16 +583,24 @@ __device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n) {
 // f(index, key) for every candidate of the row, each by one thread.
 template <typename T, typename F>
 __device__ __forceinline__ void row_visit(const RowView<T>& v, F f) {
-  constexpr int VEC = RowView<T>::VEC, UNROLL = 4;
+  constexpr int VEC = RowView<T>::VEC, UNROLL = 32 / VEC;
   for (int b0 = threadIdx.x; b0 < v.blocks; b0 += UNROLL * kRowThreads) {
-    uint32_t k[UNROLL][VEC];
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) v.keys(b0 + j * kRowThreads, k[j]);
+    uint4 q[UNROLL];
+    const bool inside = v.whole(b0) && v.whole(b0 + (UNROLL - 1) * kRowThreads);
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j)
+      if (inside) q[j] = v.load(b0 + j * kRowThreads);
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      uint32_t k[VEC];
+      if (inside)
+        RowView<T>::keys_of(q[j], k);
+      else
+        v.keys(b0 + j * kRowThreads, k);
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (k[j][e]) f(v.first(b0 + j * kRowThreads) + e, k[j][e]);
+        if (k[e]) f(v.first(b0 + j * kRowThreads) + e, k[e]);
+    }
   }
 }
 
@@ -654,17 +664,43 @@ __device__ uint32_t row_radix_select(const RowView<T>& v, uint32_t floor_key, ui
   return prefix;
 }
 
-// Blocks of the row in index order, a contiguous range per warp: f(block, keys of this lane's block)
-// with 32 neighbouring blocks a step, by every lane of the warp (keys of 0 past the end).
+// Steps of 32 blocks (512 bytes) that a warp goes through in index order: warp w has the steps from
+// w * row_warp_steps on.
+__device__ __forceinline__ int row_warp_steps(int blocks) { return ((blocks + 31) / 32 + kRowWarps - 1) / kRowWarps; }
+
+// f(block, keys of this lane's block) for each step, by every lane of the warp, until f returns false
+// (the same in every lane). Blocks whose group lies below `low` are not read (maxima null: all are);
+// their keys are 0, as past the end. Loads run four steps ahead.
 template <typename T, typename F>
-__device__ __forceinline__ void row_warp_walk(const RowView<T>& v, F f) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int steps = (v.blocks + 31) / 32, per = (steps + kRowWarps - 1) / kRowWarps;
-  for (int s = warp * per; s < min(steps, (warp + 1) * per); ++s) {
-    uint32_t k[RowView<T>::VEC];
-    const int b = s * 32 + lane;
-    v.keys(b, k);
-    if (!f(b, k)) break;  // the same in every lane
+__device__ __forceinline__ void row_warp_walk(const RowView<T>& v, const uint32_t* maxima, uint32_t low, F f) {
+  constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC, AHEAD = 4;
+  const int lane = threadIdx.x & 31, per = row_warp_steps(v.blocks);
+  const int s0 = static_cast<int>(threadIdx.x >> 5) * per, s1 = min((v.blocks + 31) / 32, s0 + per);
+  for (int s = s0; s < s1; s += AHEAD) {
+    uint4 q[AHEAD];
+    bool whole[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int b = (s + j) * 32 + lane;
+      whole[j] = s + j < s1 && v.whole(b) && (maxima == nullptr || maxima[b / LANES] >= low);
+      if (whole[j]) q[j] = v.load(b);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (s + j >= s1) return;
+      const int b = (s + j) * 32 + lane;
+      uint32_t k[VEC];
+      if (whole[j]) {
+        RowView<T>::keys_of(q[j], k);
+      } else if (b < v.blocks && !v.whole(b)) {
+        v.edge(b, k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) k[e] = 0u;
+      }
+      __syncwarp();
+      if (!f(b, k)) return;
+    }
   }
 }
 
@@ -682,33 +718,31 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   griddep_wait();  // launched as a programmatic dependent of the scan
   const int64_t row = blockIdx.x;
   const RowView<T> v(x + row * ldx, V);
-  uint32_t top_key, candidates;
-  row_open(scan, row, row_maxima, sh, top_key, candidates);
-  const int kk = static_cast<int>(min(candidates, static_cast<uint32_t>(k)));
+  const uint32_t top_key = row_open(scan, row, row_maxima, sh);
   if (threadIdx.x >= kRowThreads - 32) {  // the last warp joins the slices' sums at the row's maximum
     const double top = K::value(top_key);
     double s = 0.0;
     for (int i = threadIdx.x & 31; i < scan.slices; i += 32) {
       const RowSlice a = scan.slice[row * scan.slices + i];
-      if (a.top)
-        s += __uint_as_float(static_cast<uint32_t>(a.mass)) *
-             exp((static_cast<double>(K::value(a.top)) - top) / temperature);
+      if (a.top) s += a.sum * exp((static_cast<double>(K::value(a.top)) - top) / temperature);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) == 0)
       lse[row] = top_key == 0 ? -INFINITY : !(top < INFINITY) ? INFINITY : static_cast<float>(top / temperature + log(s));
   }
-  if (kk > 0) {
-    const uint32_t bound = row_bound(row_maxima, scan.groups, kk, top_key, sh);
+  int kk = 0;  // entries given
+  if (top_key > 0) {
+    const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
     int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+    kk = min(n, k);
     if (n > kRowList) {
       // the kk-th largest key, then the larger ones and of its equals the first in index order
       uint64_t n_gt;
       const RowWeight none{};
       const uint32_t cut = row_radix_select<T, false>(v, 1u, kk - 1, none, sh, n_gt);
       uint32_t eq = 0;
-      row_warp_walk<T>(v, [&](int, const uint32_t(&key)[RowView<T>::VEC]) {
+      row_warp_walk<T>(v, nullptr, 0u, [&](int, const uint32_t(&key)[RowView<T>::VEC]) {
 #pragma unroll
         for (int e = 0; e < RowView<T>::VEC; ++e) eq += key[e] == cut;
         return true;
@@ -719,7 +753,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       rank = __shfl_sync(0xffffffffu, rank, 0);
       const uint64_t room = kk - n_gt;
       const int lane = threadIdx.x & 31;
-      row_warp_walk<T>(v, [&](int b, const uint32_t(&key)[RowView<T>::VEC]) {
+      row_warp_walk<T>(v, nullptr, 0u, [&](int b, const uint32_t(&key)[RowView<T>::VEC]) {
         uint32_t mine = 0;
 #pragma unroll
         for (int e = 0; e < RowView<T>::VEC; ++e) mine += key[e] == cut;
@@ -771,11 +805,19 @@ template <typename T>
 __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, uint64_t least, float uniform,
                                 const RowWeight& weight, RowScratch& sh, int64_t* __restrict__ token) {
   using K = RowKey<T>;
+  constexpr int PER = kRowList / kRowThreads;
+  uint64_t w[PER], own = 0, total;
+  if (mass) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (threadIdx.x + j * kRowThreads < n)
+        own += weight(K::value(static_cast<uint32_t>(sh.list[threadIdx.x + j * kRowThreads] >> 32)));
+    if (floor_share(top_p, mass) >= block_sum_u64(own, sh)) return false;
+    own = 0;
+  }
   uint64_t* sorted = sh.hist;
   row_order(sh.list, sorted, n);
   const uint32_t kth = top_k ? static_cast<uint32_t>(sorted[top_k - 1] >> 32) : 0u;
-  constexpr int PER = kRowList / kRowThreads;
-  uint64_t w[PER], own = 0, total;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int at = threadIdx.x * PER + j;
@@ -785,7 +827,6 @@ __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, ui
   }
   uint64_t before = block_exclusive_u64(own, sh, total);
   const uint64_t target = top_p < 1.f ? floor_share(top_p, mass ? mass : total) : ~0ull;
-  if (mass && target >= total) return false;
   uint64_t* kept = sh.list;  // row_order has read the list
   own = 0;
 #pragma unroll
@@ -823,64 +864,127 @@ __device__ __forceinline__ uint64_t row_slice_mass(const RowSlice& a, uint32_t t
                          exp((static_cast<double>(slice_top) - static_cast<double>(weight.top)) / temperature));
 }
 
-// The border of the nucleus among all candidates: the key `cut` of its last entry and how many of
-// the entries with that key are inside (`ties`); `mass` is the weight of all candidates. The entries
-// that weigh at most (mass - target - 1) / V together weigh less than mass - target, so the border
-// lies above them: only the others are counted, in bins even in x. False where the border's bin
-// holds too many entries (the caller then selects by radix).
+// One step of a warp's walk to the token: the weights of each lane's block, in index order, on top of
+// `run`; writes the token where `aim` falls and returns whether it lies further on.
+template <int VEC>
+__device__ __forceinline__ bool row_warp_find(const uint64_t (&w)[VEC], uint64_t& run, uint64_t aim, int first,
+                                              int64_t* __restrict__ token) {
+  const int lane = threadIdx.x & 31;
+  uint64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) mine += w[e];
+  uint64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  uint64_t at = run + inc - mine;
+  run += __shfl_sync(0xffffffffu, inc, 31);
+  if (at <= aim && aim < at + mine)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (at <= aim && aim < at + w[e]) *token = first + e;
+      at += w[e];
+    }
+  return run <= aim;
+}
+
+// Samples from the nucleus of the whole row; `mass` is the weight of all candidates and `target` top-p's
+// share of it. Entries that weigh at most (mass - target - 1) / V together weigh less than
+// mass - target, so the border lies above them. The others are counted (32-bit counts, no weights) in
+// 2048 bins even in x; as the entries of a bin weigh the same within a percent, the counts bound the
+// running weight from both sides and leave a few bins that can hold the border. A second pass, in
+// index order, sums what lies above those bins exactly and lists what lies in them. False where that
+// list is too long (the caller then selects by radix).
 template <typename T>
-__device__ bool row_nucleus(const RowView<T>& v, float temperature, uint64_t mass, uint64_t target,
-                            const RowWeight& weight, RowScratch& sh, uint32_t& cut, uint64_t& ties) {
+__device__ bool row_pick_nucleus(const RowView<T>& v, const uint32_t* maxima, float temperature, uint64_t mass,
+                                 uint64_t target, uint64_t least, float uniform, const RowWeight& weight,
+                                 RowScratch& sh, int64_t* __restrict__ token) {
   using K = RowKey<T>;
+  constexpr int VEC = RowView<T>::VEC;
   const float top = weight.top;
-  // how far below the maximum (times T) a border can lie, with a margin that covers the fp32 arithmetic;
+  // how far below the maximum (times T) the border can lie, with a margin that covers the fp32 arithmetic;
   // weights are rounded, so one of light + 1 stands for light + 1/2 or more
   const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(v.V);
   const float depth = (static_cast<float>(weight.S) - log2f(static_cast<float>(light) + 0.5f)) * kLn2 + 1e-3f;
   const float range = depth * temperature + 1e-5f * fabsf(top);
   if (!(top < INFINITY) || !(range < INFINITY)) return false;
-  const float inv = static_cast<float>(kRowBins) / range;
+  const float inv = static_cast<float>(kRowBins) / range, step = range / (temperature * kRowBins);
   const uint32_t low = row_key_floor<T>(top - range);
   auto bin = [&](uint32_t key) { return min(kRowBins - 1, static_cast<int>((top - K::value(key)) * inv)); };
-  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) sh.hist[i] = 0;
-  if (threadIdx.x == 0) sh.found[0] = ~0ull;
+  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
+  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) counts[i] = 0;
+  if (threadIdx.x == 0) {
+    sh.found[0] = ~0ull;
+    sh.found[1] = kRowBins - 1;
+    sh.listed = 0;
+  }
   __syncthreads();
   row_visit<T>(v, [&](int, uint32_t key) {
-    if (key < low) return;
-    const uint64_t w = weight(K::value(key));
-    if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin(key)]), static_cast<unsigned long long>(w));
+    if (key >= low) atomicAdd(&counts[bin(key)], 1u);
   });
   __syncthreads();
+  // bounds of an entry's weight at a bin's ends, 2e-4 wider than the fp32 arithmetic needs, and of the
+  // running weight
   constexpr int BINS = kRowBins / kRowThreads;
-  uint64_t h[BINS], own = 0, total;
-#pragma unroll
-  for (int j = 0; j < BINS; ++j) own += h[j] = sh.hist[threadIdx.x * BINS + j];
-  uint64_t run = block_exclusive_u64(own, sh, total);
+  uint32_t c[BINS];
+  uint64_t most[BINS], fewest[BINS], sum_most = 0, sum_fewest = 0, total;
 #pragma unroll
   for (int j = 0; j < BINS; ++j) {
-    if (run <= target && target < run + h[j]) {
-      sh.found[0] = threadIdx.x * BINS + j;
-      sh.found[1] = run;
-    }
-    run += h[j];
+    const int b = threadIdx.x * BINS + j;
+    c[j] = counts[b];
+    const double one = static_cast<double>(1ull << weight.S);
+    most[j] = c[j] * (__double2ull_ru(expf(-step * b) * 1.0002 * one) + 1);
+    fewest[j] = b == kRowBins - 1 ? 0 : c[j] * __double2ull_rd(expf(-step * (b + 1)) * 0.9998 * one);
+    sum_most += most[j];
+    sum_fewest += fewest[j];
+  }
+  uint64_t hi = block_exclusive_u64(sum_most, sh, total), lo = block_exclusive_u64(sum_fewest, sh, total);
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) {
+    if (hi <= target && target < hi + most[j]) sh.found[0] = threadIdx.x * BINS + j;
+    if (lo <= target && target < lo + fewest[j]) sh.found[1] = threadIdx.x * BINS + j;
+    hi += most[j];
+    lo += fewest[j];
   }
   __syncthreads();
   if (sh.found[0] == ~0ull) return false;
-  const int border = static_cast<int>(sh.found[0]);
-  uint64_t before = sh.found[1];
-  row_visit<T>(v, [&](int i, uint32_t key) {
-    if (key < low || bin(key) != border) return;
-    const uint32_t at = atomicAdd(&sh.listed, 1u);
-    if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(i);
+  const int b1 = static_cast<int>(sh.found[0]), b2 = static_cast<int>(sh.found[1]);  // bins that can hold the border
+  uint64_t inside = 0;
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) {
+    const int b = threadIdx.x * BINS + j;
+    if (b >= b1 && b <= b2) inside += c[j];
+  }
+  if (block_sum_u64(inside, sh) > kRowList) return false;
+  // no entry of those bins or above lies below this key
+  const uint32_t floor_key = b2 == kRowBins - 1 ? low : max(low, row_key_floor<T>(top - (b2 + 1) * 1.00001f / inv - 1e-6f * fabsf(top)));
+  uint64_t above = 0, kept = 0;
+  row_warp_walk<T>(v, maxima, floor_key, [&](int b, const uint32_t(&key)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int at = key[e] >= floor_key ? bin(key[e]) : kRowBins;
+      if (at < b1) {
+        const uint64_t w = weight(K::value(key[e]));
+        above += w;
+        kept += w >= least ? w : 0;
+      }
+      row_append(at >= b1 && at <= b2, (static_cast<uint64_t>(key[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e),
+                 sh.list, &sh.listed);
+    }
+    return true;
   });
   __syncthreads();
-  const int n = static_cast<int>(min(sh.listed, static_cast<uint32_t>(kRowList) + 1));
-  if (n > kRowList) return false;
+  const int n = static_cast<int>(sh.listed);
+  uint64_t before = block_sum_u64(above, sh);
+  if (n == 0 || target < before) return false;
+  // the border: the listed entry at which the running weight passes the target
   uint64_t* sorted = sh.hist;
+  if (threadIdx.x == 0) sh.found[0] = ~0ull;
   row_order(sh.list, sorted, n);
   constexpr int PER = kRowList / kRowThreads;
-  uint64_t w[PER];
-  own = 0;
+  uint64_t w[PER], own = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int at = threadIdx.x * PER + j;
@@ -890,32 +994,50 @@ __device__ bool row_nucleus(const RowView<T>& v, float temperature, uint64_t mas
   before += block_exclusive_u64(own, sh, total);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    if (before <= target && target < before + w[j]) {
-      const int at = threadIdx.x * PER + j;
-      const uint32_t key = static_cast<uint32_t>(sorted[at] >> 32);
-      int first = at;
-      while (first > 0 && static_cast<uint32_t>(sorted[first - 1] >> 32) == key) --first;
-      sh.found[0] = key;
-      sh.found[1] = at - first + 1;
-    }
+    if (before <= target && target < before + w[j]) sh.found[0] = threadIdx.x * PER + j;
     before += w[j];
   }
   __syncthreads();
-  cut = static_cast<uint32_t>(sh.found[0]);
-  ties = sh.found[1];
+  if (sh.found[0] == ~0ull) return false;
+  const int last = static_cast<int>(sh.found[0]);
+  const uint64_t border = sorted[last];
+  // the kept weight of each warp's range of the row
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = row_warp_steps(v.blocks);
+  for (int j = lane; j <= last; j += 32) {
+    const int i = static_cast<int>(~static_cast<uint32_t>(sorted[j]));
+    if ((i + v.off) / VEC / 32 / per != warp) continue;
+    const uint64_t wj = weight(K::value(static_cast<uint32_t>(sorted[j] >> 32)));
+    kept += wj >= least ? wj : 0;
+  }
+  kept = warp_sum_u64(kept);
+  uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? kept : 0, sh, total), 0);
+  const uint64_t aim = floor_share(uniform, total);
+  if (run > aim || aim >= run + kept) return true;
+  row_warp_walk<T>(v, maxima, floor_key, [&](int b, const uint32_t(&key)[VEC]) {
+    uint64_t we[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint64_t entry = (static_cast<uint64_t>(key[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e);
+      we[e] = entry >= border && key[e] ? weight(K::value(key[e])) : 0;
+      we[e] = we[e] >= least ? we[e] : 0;
+    }
+    return row_warp_find<VEC>(we, run, aim, v.first(b), token);
+  });
   return true;
 }
 
 // Picks the token by going over the row in index order: kept are the entries above `cut` and the first
 // `ties` equal to it, as far as they weigh `least`; no entry below the key `lowest` does.
 template <typename T>
-__device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, uint32_t lowest, uint64_t least,
-                              float uniform, const RowWeight& weight, RowScratch& sh, int64_t* __restrict__ token) {
+__device__ void row_pick_walk(const RowView<T>& v, const uint32_t* maxima, uint32_t cut, uint64_t ties, uint32_t lowest,
+                              uint64_t least, float uniform, const RowWeight& weight, RowScratch& sh,
+                              int64_t* __restrict__ token) {
   using K = RowKey<T>;
   constexpr int VEC = RowView<T>::VEC;
   const int lane = threadIdx.x & 31;
   const uint64_t cut_weight = weight(K::value(cut));
   if (cut_weight < least) ties = 0;
+  const uint32_t low = max(cut, lowest);
   auto above = [&](uint32_t key) -> uint64_t {
     if (key <= cut || key < lowest) return 0;
     const uint64_t w = weight(K::value(key));
@@ -923,7 +1045,7 @@ __device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, 
   };
   uint64_t sum = 0;
   uint32_t eq = 0;
-  row_warp_walk<T>(v, [&](int, const uint32_t(&key)[VEC]) {
+  row_warp_walk<T>(v, maxima, low, [&](int, const uint32_t(&key)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       sum += above(key[e]);
@@ -940,7 +1062,7 @@ __device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, 
   uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? sum : 0, sh, all), 0);
   const uint64_t aim = floor_share(uniform, all);
   if (run > aim || aim >= run + sum) return;
-  row_warp_walk<T>(v, [&](int b, const uint32_t(&key)[VEC]) {
+  row_warp_walk<T>(v, maxima, low, [&](int b, const uint32_t(&key)[VEC]) {
     uint32_t same = 0;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) same += key[e] == cut;
@@ -952,27 +1074,10 @@ __device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, 
     }
     uint64_t r = rank + se - same;
     rank += __shfl_sync(0xffffffffu, se, 31);
-    uint64_t w[VEC], mine = 0;
+    uint64_t w[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[e] = key[e] == cut ? (r++ < ties ? cut_weight : 0) : above(key[e]);
-      mine += w[e];
-    }
-    uint64_t si = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, si, o);
-      if (lane >= o) si += u;
-    }
-    uint64_t at = run + si - mine;
-    run += __shfl_sync(0xffffffffu, si, 31);
-    if (at <= aim && aim < at + mine)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (at <= aim && aim < at + w[e]) *token = v.first(b) + e;
-        at += w[e];
-      }
-    return run <= aim;
+    for (int e = 0; e < VEC; ++e) w[e] = key[e] == cut ? (r++ < ties ? cut_weight : 0) : above(key[e]);
+    return row_warp_find<VEC>(w, run, aim, v.first(b), token);
   });
 }
 
@@ -1047,8 +1152,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   griddep_wait();  // launched as a programmatic dependent of the scan
   const SampleRow knob(knobs, row);
   const float u = uniform[row], T_ = knob.temperature;
-  uint32_t top_key, candidates;
-  row_open(scan, row, row_maxima, sh, top_key, candidates);
+  const uint32_t top_key = row_open(scan, row, row_maxima, sh);
   if (top_key == 0) {
     if (threadIdx.x == 0) tokens[row] = -1;
     return;
@@ -1086,18 +1190,23 @@ __global__ void __launch_bounds__(kRowThreads, 2)
                  ? max(1u, row_key_floor<T>(weight.top + T_ * (logf(floor_p) - 1e-3f) - 1e-5f * fabsf(weight.top)))
                  : top_key;
 
-  if (knob.top_k >= 1 && knob.top_k <= kRowMaxK) {
-    const int k = static_cast<int>(min(candidates, static_cast<uint32_t>(knob.top_k)));
-    const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
+  // a top-k that is smaller than the number of candidates
+  bool filtered = false;
+  if (knob.top_k > kRowMaxK) {
+    uint64_t candidates = 0;
+    row_visit<T>(v, [&](int, uint32_t) { ++candidates; });
+    filtered = static_cast<uint64_t>(knob.top_k) < block_sum_u64(candidates, sh);
+  } else if (knob.top_k >= 1) {
+    const uint32_t bound = row_bound(row_maxima, scan.groups, knob.top_k, top_key, sh);
     const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
-    if (n <= kRowList) {
-      row_pick_listed<T>(n, k, knob.top_p, 0, least, u, weight, sh, tokens + row);
+    if (n <= kRowList) {  // with fewer than top_k entries, all there are
+      row_pick_listed<T>(n, min(n, knob.top_k), knob.top_p, 0, least, u, weight, sh, tokens + row);
       return;
     }
+    filtered = true;
   }
   uint32_t cut = 1u;
   uint64_t before, ties = ~0ull;
-  const bool filtered = knob.top_k >= 1 && static_cast<uint32_t>(knob.top_k) < candidates;
   if (filtered) cut = row_radix_select<T, false>(v, 1u, knob.top_k - 1, weight, sh, before);
   if (knob.top_p < 1.f) {
     uint64_t mass = 0;
@@ -1112,23 +1221,20 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       });
     }
     mass = block_sum_u64(mass, sh);
+    const uint64_t target = floor_share(knob.top_p, mass);
     if (!filtered) {
       // the head of the order first: a nucleus is usually a few hundred entries
-      const int k = static_cast<int>(min(candidates, static_cast<uint32_t>(kRowMaxK)));
-      const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
+      const uint32_t bound = row_bound(row_maxima, scan.groups, kRowMaxK, top_key, sh);
       const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
-      if (n <= kRowList &&
-          row_pick_listed<T>(n, 0, knob.top_p, static_cast<uint32_t>(n) == candidates ? 0 : mass, least, u, weight, sh,
-                             tokens + row))
+      const bool whole_row = n < kRowMaxK || bound == 1u;
+      if (n <= kRowList && row_pick_listed<T>(n, 0, knob.top_p, whole_row ? 0 : mass, least, u, weight, sh, tokens + row))
         return;
       __syncthreads();
-    }
-    const uint64_t target = floor_share(knob.top_p, mass);
-    if (filtered || !row_nucleus<T>(v, T_, mass, target, weight, sh, cut, ties)) {
+      if (row_pick_nucleus<T>(v, row_maxima, T_, mass, target, least, u, weight, sh, tokens + row)) return;
       __syncthreads();
-      cut = row_radix_select<T, true>(v, cut, target, weight, sh, before);
-      ties = (target - before) / weight(K::value(cut)) + 1;
     }
+    cut = row_radix_select<T, true>(v, cut, target, weight, sh, before);
+    ties = (target - before) / weight(K::value(cut)) + 1;
   } else if (!filtered && floor_p > 0.f) {
     const int n = row_gather<T>(v, row_maxima, scan.groups, lowest, sh);
     if (n <= kRowList) {
@@ -1139,7 +1245,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     row_pick_slice<T, BLOCKS>(v, scan, row, top_key, T_, u, weight, sh, tokens + row);
     return;
   }
-  row_pick_walk<T>(v, cut, ties, lowest, least, u, weight, sh, tokens + row);
+  row_pick_walk<T>(v, row_maxima, cut, ties, lowest, least, u, weight, sh, tokens + row);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1156,7 +1262,7 @@ struct RowPlan {
 inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned) {
   RowPlan p{};
   const int vec = 16 / elem;
-  p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), kRowGroup));
+  p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), 4 * kRowGroup)) * 4;
   const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 19);
   p.blocks = (small ? 2048 : 8192) / vec / kScanThreads;
   p.slices = static_cast<int>(ceil_div(static_cast<int64_t>(p.groups) * kRowGroup, static_cast<int64_t>(p.blocks) * kScanThreads * vec));
@@ -1207,7 +1313,7 @@ int topk_rows_impl(const T* x, int64_t ldx, int64_t R, int64_t V, int k, float t
   if (rc != ORTHRUS_OK) return rc;
   ORTHRUS_CHECK_CUDA(ensure_smem(topk_rows_kernel<T>, kRowSmem));
   ORTHRUS_CHECK_CUDA(launch_pdl(topk_rows_kernel<T>, dim3(static_cast<unsigned>(R)), dim3(kRowThreads),
-                                (p.groups + 3) / 4 * 16, stream, x, ldx, static_cast<int>(V), k, temperature, scan, values,
+                                p.groups * 4, stream, x, ldx, static_cast<int>(V), k, temperature, scan, values,
                                 ids, lse));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
@@ -1218,7 +1324,7 @@ int sample_finish_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, i
                          const SampleKnobs& knobs, const RowScan& scan, int64_t* tokens, cudaStream_t stream) {
   auto kernel = sample_logits_kernel<T, BLOCKS>;
   ORTHRUS_CHECK_CUDA(ensure_smem(kernel, kRowSmem));
-  ORTHRUS_CHECK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(R)), dim3(kRowThreads), (p.groups + 3) / 4 * 16,
+  ORTHRUS_CHECK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(R)), dim3(kRowThreads), p.groups * 4,
                                 stream, x, ldx, V, S, uniform, knobs, scan, tokens));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
