@@ -490,9 +490,9 @@ int orthrus_philox4x32_10(const uint32_t* counter_key, int64_t n, uint32_t* out,
 /* ---- row operators over vocabulary logits ------------------------------------------------ */
 /* Rows are `logits` [R, V] in `dtype` at a pitch of ldl elements (any alignment; rows may overlap or
  * repeat), V at most 1048576 (ORTHRUS_EINVAL beyond). Entries that are -inf or NaN are no candidates.
- * Entries are ordered by descending value, then ascending index; -0 counts as +0. Both operators take
- * a workspace of orthrus_vocab_rows_workspace_bytes(R, V, dtype) bytes on a 16-byte boundary. */
-size_t orthrus_vocab_rows_workspace_bytes(int64_t R, int64_t V, int dtype);
+ * Entries are ordered by descending value, then ascending index; -0 counts as +0. Workspaces start on
+ * a 16-byte boundary. */
+size_t orthrus_topk_rows_workspace_bytes(int64_t R, int64_t V, int dtype);
 
 /* The k largest candidates of each row (1 <= k <= 1024): values [R, k] fp32 and ids [R, k] in
  * order, (-inf, -1) past the last candidate, and lse [R] = log(sum exp(x / temperature)) over the
@@ -510,7 +510,11 @@ int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int
  * or NaN counts as 0, one of 1 or more picks the last kept token of positive weight. A temperature
  * below 1e-5 gives the row's first maximum; a row without candidates gives -1. Sums are exact
  * (integer weights of at least 42 fractional bits), so the token depends on the row and its knobs
- * alone. Each knob is a device array [R], or NULL and the value beside it for every row. */
+ * alone. Each knob is a device array [R], or NULL and the value beside it for every row. The workspace
+ * is asked for with `filters` = 1 when top_p or min_p can filter a row whose top_k is off or above 1024
+ * (either array given, or top_p1 < 1 or min_p1 > 0; top_k given, or top_k1 < 1 or > 1024): rows that
+ * keep thousands of entries need about V bytes each, for up to 2048 of them. */
+size_t orthrus_sample_logits_workspace_bytes(int64_t R, int64_t V, int filters, int dtype);
 int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
                           const float* temperature, float temperature1, const int32_t* top_k,
                           int top_k1, const float* top_p, float top_p1, const float* min_p,

@@ -104,7 +104,8 @@ _SIGNATURES = {
     "orthrus_lmhead_topk_kl_fwd": (c_int, [_P, c_int64, _P, _P, c_int64, c_int, _P, _P, _P, c_int64, c_int64,
                                            c_float, _P, _P, c_int, _P, _P, _P, _P, _P, _P, c_int64, _P, c_size_t,
                                            c_int, _P]),
-    "orthrus_vocab_rows_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "orthrus_topk_rows_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "orthrus_sample_logits_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "orthrus_topk_rows": (c_int, [_P, c_int64, c_int64, c_int64, c_int, c_float, _P, _P, _P, _P, c_size_t, c_int,
                                   _P]),
     "orthrus_sample_logits": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P, c_float, _P, c_int, _P, c_float,

@@ -8,12 +8,13 @@
 //   - The k largest entries: the k-th largest group maximum is at most the k-th largest entry, and
 //     little below it unless the row is arranged against it, so the few groups at or above it are read
 //     again (from L2) and the entries at or above it, k and a few more, are ordered in shared memory.
-//   - A nucleus without top-k is looked for among the 1024 largest entries first; a wider one's border
-//     is bracketed by a histogram and found exactly among the entries in the bracket.
+//   - A nucleus without top-k is looked for among the 256 largest entries.
 //   - Without a filter the slices' weights say which slice holds the uniform's share.
-// Where the gathered entries are too many for shared memory (rows of equal values, nuclei of many
-// thousands), the CTA goes over the whole row again: a radix selection that is right for every row, and
-// a walk in index order.
+// Sampled rows that keep more than fits a CTA's shared memory (wide rows: nuclei of thousands of entries)
+// get more launches: a scan that bins their weights and so finds a narrow window of values with the
+// nucleus' border, one that sums what lies above the window and lists what lies in it, and a pick. Where
+// even that does not do (rows of equal values), a CTA goes over the whole row again: a radix selection
+// that is right for every row, and a walk in index order.
 //
 // Candidates are the entries that are neither -inf nor NaN. Entries are ordered by (descending
 // value, ascending index); -0 counts as +0.
@@ -32,6 +33,10 @@ constexpr int kRowGroup = 32;             // entries behind one group maximum
 constexpr int kRowBins = 2048;
 constexpr int kRowMaxK = 1024;            // largest k of topk_rows
 constexpr int kRowList = 2048;            // most entries gathered into shared memory
+constexpr int kRowWideShare = 8;          // a wide row's window lists at most one in so many of a slice's entries
+constexpr int kRowWideBins = 512;         // weight bins of a wide row
+constexpr int kRowWideRows = 2048;        // most wide rows of a call
+constexpr int kRowHead = 256;             // entries among which a nucleus is looked for first
 constexpr int kRowMaxV = 1 << 20;         // the group maxima of a longer row do not fit shared memory
 
 // ------------------------------------------------------------------------------------------------
@@ -77,6 +82,17 @@ struct RowKey<__nv_bfloat16> {
 // A row in 16-byte blocks
 // ------------------------------------------------------------------------------------------------
 
+// Key of entry i, 0 outside the row. Out of line: only a row's ends need it, and in line it would be most
+// of the code of every loop over a row (whose instruction fetches are what such a loop waits for).
+template <typename T>
+__device__ __noinline__ uint32_t row_key_at(const T* p, int V, int i) {
+  if (i < 0 || i >= V) return 0u;
+  if constexpr (sizeof(T) == 4)
+    return RowKey<T>::of_bits(__ldg(reinterpret_cast<const uint32_t*>(p) + i));
+  else
+    return RowKey<T>::of_bits(__ldg(reinterpret_cast<const uint16_t*>(p) + i));
+}
+
 // Block b of a row of any alignment covers the entries b * VEC - off .. + VEC - 1, where off is the
 // row's distance in entries from the 16-byte boundary before it; entries outside the row count as no
 // candidates and are never read.
@@ -117,13 +133,7 @@ struct RowView {
       for (int e = 0; e < VEC; ++e) x[e] = b < blocks ? K::value(key(first(b) + e)) : -INFINITY;
     }
   }
-  __device__ __forceinline__ uint32_t key(int i) const {
-    if (i < 0 || i >= V) return 0u;
-    if constexpr (sizeof(T) == 4)
-      return K::of_bits(__ldg(reinterpret_cast<const uint32_t*>(p) + i));
-    else
-      return K::of_bits(__ldg(reinterpret_cast<const uint16_t*>(p) + i));
-  }
+  __device__ __forceinline__ uint32_t key(int i) const { return row_key_at<T>(p, V, i); }
   __device__ __forceinline__ void edge(int b, uint32_t (&k)[VEC]) const {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) k[e] = b < blocks ? key(first(b) + e) : 0u;
@@ -141,15 +151,28 @@ struct RowView {
 // ------------------------------------------------------------------------------------------------
 
 struct RowScratch {
-  uint64_t hist[kRowBins];   // radix selection and nucleus: counts (32-bit words) or weights; else a list
   uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
-  double exp_tab[64];        // 2^(-j/64)
+  uint32_t counts[kRowBins]; // histograms
   uint64_t warp[kRowWarps];
   uint32_t top[kRowWarps];
   uint64_t found[2];         // result of a block-wide search
-  uint32_t groups[kRowList]; // numbers of the groups to read again
+  union {
+    uint64_t hist[kRowBins];           // weights of a radix selection
+    uint64_t sorted[kRowList];         // the list in order
+    uint32_t groups[kRowList];         // numbers of the groups to read again
+  };
   uint32_t ngroups, listed;
 };
+
+// The finishing CTA's shared memory: the scratch, then the row's group maxima. The functions below
+// reach it by name rather than through a reference, so that those kept out of line (the finish is
+// long, and mostly run once per row: instruction fetches are what it waits for most) still use
+// shared-memory instructions.
+extern __shared__ __align__(16) uint8_t row_smem[];
+__device__ __forceinline__ RowScratch& row_scratch() { return *reinterpret_cast<RowScratch*>(row_smem); }
+__device__ __forceinline__ uint32_t* row_maxima() {
+  return reinterpret_cast<uint32_t*>(row_smem + (sizeof(RowScratch) + 15) / 16 * 16);
+}
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
 #pragma unroll
@@ -157,20 +180,25 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
   return v;
 }
 
+struct uint2x64 {
+  uint64_t x, y;
+};
+
 // Block-wide sum; every thread gets it. Leaves warp_u64 free for reuse.
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, RowScratch& sh) {
+__device__ __noinline__ uint64_t block_sum_u64(uint64_t v) {
+  RowScratch& sh = row_scratch();
   v = warp_sum_u64(v);
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) sh.warp[threadIdx.x >> 5] = v;
   __syncthreads();
-  uint64_t t = 0;
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) t += sh.warp[w];
+  v = lane < kRowWarps ? sh.warp[lane] : 0;
   __syncthreads();
-  return t;
+  return warp_sum_u64(v);
 }
 
-// Exclusive prefix sum over the block's threads; `total` is the block's sum.
-__device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowScratch& sh, uint64_t& total) {
+// Exclusive prefix sum over the block's threads, and the block's sum.
+__device__ __noinline__ uint2x64 block_exclusive2(uint64_t v) {
+  RowScratch& sh = row_scratch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t inc = v;
 #pragma unroll
@@ -180,15 +208,14 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowScratch& 
   }
   if (lane == 31) sh.warp[warp] = inc;
   __syncthreads();
-  uint64_t before = 0, t = 0;
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) {
-    if (w == warp) before = t;
-    t += sh.warp[w];
-  }
+  const uint64_t w = lane < kRowWarps ? sh.warp[lane] : 0;
   __syncthreads();
-  total = t;
-  return before + inc - v;
+  return {inc - v + warp_sum_u64(lane < warp ? w : 0), warp_sum_u64(w)};
+}
+__device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& total) {
+  const uint2x64 r = block_exclusive2(v);
+  total = r.y;
+  return r.x;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -200,28 +227,35 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, RowScratch& 
 // fall the same way on every path. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
 // 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
 //
-// The exponential is the table method (P. T. P. Tang, "Table-driven implementation of the
-// exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989): y = 64 (max - x) log2(e) / T
-// = n + f with |f| <= 1/2, exp = 2^-(n >> 6) * tab[n & 63] * e^(-f ln2 / 64), the last factor by
-// its Taylor polynomial of degree 4 (error below (0.0055)^5 / 120 = 4e-14).
+// The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f by its Taylor polynomial of
+// degree 10 (error below (ln2 / 2)^11 / 11! = 2.2e-13), 2^(S - n) by the exponent. A table would save
+// six of the fp64 products, but its lookups, of random banks, take longer.
 struct RowWeight {
   float top;         // the maximum the weights refer to
   int S;
-  double scale, at;  // 64 log2(e) / T; top * scale
-  const double* tab;
+  double scale, at;  // log2(e) / T; top * scale
 
   __device__ __forceinline__ uint64_t operator()(float x) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     constexpr double kInt = 4503599627370496.0;    // 2^52
-    constexpr double c = -0.6931471805599453 / 64.0;
+    constexpr double c = 0.6931471805599453;
+    constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5, c6 = c5 * c / 6, c7 = c6 * c / 7,
+                     c8 = c7 * c / 8, c9 = c8 * c / 9, c10 = c9 * c / 10;
     const double y = x == top ? 0.0 : fma(-static_cast<double>(x), scale, at);
-    if (!(y < 64.0 * (S + 2))) return 0;  // rounds to 0; also an infinite maximum's other entries
+    if (!(y < S + 2.0)) return 0;  // rounds to 0; also an infinite maximum's other entries
     const double r = y + kRound;
-    const int n = __double2loint(r);
-    const double f = y - (r - kRound);
-    const double p = fma(fma(fma(fma(f, c * c * c * c / 24.0, c * c * c / 6.0), f, c * c / 2.0), f, c), f, 1.0) * tab[n & 63];
-    // times 2^(S - n / 64), by the exponent
-    const double w = __hiloint2double(__double2hiint(p) + ((S - (n >> 6)) << 20), __double2loint(p)) + kInt;
+    const double f = (r - kRound) - y;
+    double p = fma(c10, f, c9);
+    p = fma(p, f, c8);
+    p = fma(p, f, c7);
+    p = fma(p, f, c6);
+    p = fma(p, f, c5);
+    p = fma(p, f, c4);
+    p = fma(p, f, c3);
+    p = fma(p, f, c2);
+    p = fma(p, f, c);
+    p = fma(p, f, 1.0);
+    const double w = __hiloint2double(__double2hiint(p) + ((S - __double2loint(r)) << 20), __double2loint(p)) + kInt;
     return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
   }
 };
@@ -232,14 +266,22 @@ __host__ __device__ inline int row_weight_bits(int V) {
   return 62 - b < 44 ? 62 - b : 44;
 }
 
-__device__ __forceinline__ void row_exp_table(double* tab) {
-  if (threadIdx.x < 64) tab[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+__device__ __forceinline__ RowWeight row_weight(float top, float temperature, int S) {
+  const double scale = 1.4426950408889634 / static_cast<double>(temperature);
+  return {top, S, scale, static_cast<double>(top) * scale};
 }
 
-__device__ __forceinline__ RowWeight row_weight(float top, float temperature, int S, const double* tab) {
-  const double scale = 92.33248261893567 / static_cast<double>(temperature);  // 64 log2(e) / T
-  return {top, S, scale, static_cast<double>(top) * scale, tab};
+// The same out of line, for the finish, which has many places that weigh an entry.
+__device__ __noinline__ uint64_t row_weigh(float x, float top, int S, double scale, double at) {
+  return RowWeight{top, S, scale, at}(x);
 }
+struct RowWeigher {
+  float top;
+  int S;
+  double scale, at;
+  __device__ __forceinline__ explicit RowWeigher(const RowWeight& w) : top(w.top), S(w.S), scale(w.scale), at(w.at) {}
+  __device__ __forceinline__ uint64_t operator()(float x) const { return row_weigh(x, top, S, scale, at); }
+};
 
 // floor(f * z) for f in [0, 1) and z < 2^62, exactly (f is an integer of 24 bits times a power of
 // two). Negative or NaN f count as 0; f >= 1 gives z - 1 (z > 0).
@@ -272,6 +314,34 @@ struct RowScan {
   uint32_t* group;
   RowSlice* slice;
   int groups, slices;
+  uint32_t* wide_count;  // cleared by the scan; may be null
+};
+
+// What a wide row's slice leaves: the weight above the window, the part of it that passes min-p, and the
+// number of entries in the window.
+struct RowSums {
+  uint64_t above, kept;
+  uint32_t listed;
+};
+
+// A wide row: the border of its nucleus lies in the window [lo, hi) of values, or (nucleus false) all
+// entries from lo = hi on are kept. `bins`: the weights from the maximum down to lo, for the window.
+struct RowWideRow {
+  int64_t row;
+  float top, lo, hi;
+  uint64_t target;  // the weight at which the border lies
+  bool nucleus;
+  uint64_t bins[kRowWideBins];
+  __device__ __forceinline__ float per_value() const { return static_cast<float>(kRowWideBins) / fmaxf(top - lo, 1e-30f); }
+};
+
+// The wide rows of a call: their records, sums [most, slices] and lists [most, slices, room].
+struct RowWideRows {
+  uint32_t* count;
+  RowWideRow* rows;
+  RowSums* sums;
+  uint64_t* lists;
+  int most, room;
 };
 
 struct SampleKnobs {
@@ -282,6 +352,11 @@ struct SampleKnobs {
   float temperature1, top_p1, min_p1;
   int top_k1;
 };
+
+// min-p as the least weight that passes.
+__device__ __forceinline__ uint64_t row_least(float min_p, int S) {
+  return __double2ull_ru(static_cast<double>(fminf(fmaxf(min_p, 0.f), 1.f)) * static_cast<double>(1ull << S));
+}
 
 // How a row is sampled, from its knobs.
 struct SampleRow {
@@ -309,10 +384,10 @@ __global__ void __launch_bounds__(kScanThreads)
   using K = RowKey<T>;
   constexpr int VEC = View::VEC;
   constexpr int LANES = kRowGroup / VEC;  // neighbouring lanes of a group
-  __shared__ double tab[64];
   __shared__ float wtop[kScanThreads / 32], wsum[kScanThreads / 32];
   __shared__ uint64_t wmass[kScanThreads / 32];
   griddep_launch_dependents();
+  if (SAMPLE && blockIdx.x == 0 && threadIdx.x == 0 && out.wide_count) *out.wide_count = 0;
   const int64_t row = blockIdx.x / static_cast<unsigned>(out.slices);
   const int slice = static_cast<int>(blockIdx.x % static_cast<unsigned>(out.slices));
   const View v(x + row * ldx, V);
@@ -323,7 +398,6 @@ __global__ void __launch_bounds__(kScanThreads)
     const SampleRow knob(knobs, row);
     temperature = knob.temperature;
     mass_wanted = knob.wants_mass();
-    if (mass_wanted) row_exp_table(tab);
   }
   float val[BLOCKS][VEC];
   if (v.whole(b0) && v.whole(b0 + BLOCKS * kScanThreads - 1)) {
@@ -357,12 +431,16 @@ __global__ void __launch_bounds__(kScanThreads)
   uint64_t mass = 0;
   float sum = 0.f;
   if constexpr (SAMPLE) {
+    // the slice again, from L1: weighing it from registers would take 32 copies of the weight's code
     if (mass_wanted && top > -INFINITY) {
-      const RowWeight weight = row_weight(top, temperature, S, tab);
+      const RowWeight weight = row_weight(top, temperature, S);
+#pragma unroll 1
+      for (int j = 0; j < BLOCKS; ++j) {
+        float x[VEC];
+        v.values(b0 + j * kScanThreads + threadIdx.x, x);
 #pragma unroll
-      for (int j = 0; j < BLOCKS; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) mass += weight(val[j][e]);
+        for (int e = 0; e < VEC; ++e) mass += weight(x[e]);
+      }
       mass = warp_sum_u64(mass);
     }
     if (lane == 0) wmass[warp] = mass;
@@ -396,7 +474,9 @@ __global__ void __launch_bounds__(kScanThreads)
 // ------------------------------------------------------------------------------------------------
 
 // The row's group maxima into shared memory and its largest key (0: no candidates), for every thread.
-__device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row, uint32_t* maxima, RowScratch& sh) {
+__device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row) {
+  RowScratch& sh = row_scratch();
+  uint32_t* maxima = row_maxima();
   const uint4* g = reinterpret_cast<const uint4*>(scan.group + row * scan.groups);
   uint4* m = reinterpret_cast<uint4*>(maxima);
   uint32_t top = 0;
@@ -407,24 +487,31 @@ __device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row, u
   if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = top;
   if (threadIdx.x == 0) sh.ngroups = sh.listed = 0;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) top = max(top, sh.top[w]);
-  return top;
+  return __reduce_max_sync(0xffffffffu, sh.top[threadIdx.x % kRowWarps]);
 }
 
 // A key with at least k entries of the row at or above it, and not many more: between the k-th largest
-// group maximum and a little below it; 1 if fewer than k groups hold a candidate. Histograms of the
-// maxima over the range of keys that can hold the bound, 1024 bins at a time.
-__device__ __forceinline__ uint32_t row_bound(const uint32_t* maxima, int groups, int k, uint32_t top_key,
-                                              RowScratch& sh) {
-  constexpr int BINS = 2 * kRowThreads;
+// maximum of a group (of four groups where k is a small part of their number) and a little below it;
+// 1 if fewer than k of them hold a candidate. Histograms of the maxima over the range of keys that
+// can hold the bound, 1024 bins at a time.
+__device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) {
+  RowScratch& sh = row_scratch();
+  const uint32_t* maxima = row_maxima();
+  constexpr int BIN_BITS = 10;  // two bins a thread
+  static_assert(1 << BIN_BITS == 2 * kRowThreads, "");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
+  uint32_t* counts = sh.counts;
   const uint4* m4 = reinterpret_cast<const uint4*>(maxima);
+  const bool quads = k <= groups / 16;
   // the smallest candidate maximum
   uint32_t least = top_key;
   for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
     const uint4 q = m4[i];
+    if (quads) {
+      const uint32_t m = max(max(q.x, q.y), max(q.z, q.w));
+      least = min(least, m ? m : top_key);
+      continue;
+    }
     least = min(min(least, q.x ? q.x : top_key), min(min(q.y ? q.y : top_key, q.z ? q.z : top_key), q.w ? q.w : top_key));
   }
   least = __reduce_min_sync(0xffffffffu, least);
@@ -432,17 +519,16 @@ __device__ __forceinline__ uint32_t row_bound(const uint32_t* maxima, int groups
   counts[threadIdx.x] = counts[threadIdx.x + kRowThreads] = 0;
   if (threadIdx.x == 0) sh.found[0] = ~0ull;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) least = min(least, sh.top[w]);
+  least = __reduce_min_sync(0xffffffffu, sh.top[lane % kRowWarps]);
   uint32_t lo = least, hi = top_key;  // the bound is in [lo, hi]
   uint32_t above = 0;                 // maxima above hi
   const uint32_t want = k, enough = k + k / 4 + 16;
   while (true) {
-    int shift = 0;
-    while (((hi - lo) >> shift) >= BINS) ++shift;
+    const int shift = max(0, 32 - __clz(hi - lo) - BIN_BITS);
     for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
       const uint4 q = m4[i];
-      const uint32_t m[4] = {q.x, q.y, q.z, q.w};
+      const uint32_t m[4] = {quads ? max(max(q.x, q.y), max(q.z, q.w)) : q.x, quads ? 0u : q.y, quads ? 0u : q.z,
+                             quads ? 0u : q.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (m[e] >= lo && m[e] <= hi) atomicAdd(&counts[(hi - m[e]) >> shift], 1u);
@@ -458,9 +544,7 @@ __device__ __forceinline__ uint32_t row_bound(const uint32_t* maxima, int groups
     }
     if (lane == 31) sh.top[warp] = inc;
     __syncthreads();
-    uint32_t run = above + inc - c0 - c1;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) run += w < warp ? sh.top[w] : 0u;
+    const uint32_t run = above + inc - c0 - c1 + __reduce_add_sync(0xffffffffu, lane < warp ? sh.top[lane] : 0u);
     if (run < want && want <= run + c0) {
       sh.found[0] = 2 * threadIdx.x;
       sh.found[1] = (static_cast<uint64_t>(run) << 32) | (run + c0);
@@ -497,36 +581,68 @@ __device__ __forceinline__ void row_append(bool take, E entry, E* list, uint32_t
   if (take && at < kRowList) list[at] = entry;
 }
 
+// The same for the keys at or above `low` of each lane's block, whose first entry has index `first`.
+template <int VEC>
+__device__ __forceinline__ void row_append_block(const uint32_t (&k)[VEC], uint32_t low, int first, uint64_t* list,
+                                                 uint32_t* count) {
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1u;
+  uint32_t who[VEC], total = 0;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    who[e] = __ballot_sync(0xffffffffu, k[e] >= low);
+    total += __popc(who[e]);
+  }
+  if (total == 0) return;
+  uint32_t at = 0;
+  if ((threadIdx.x & 31) == 0) at = atomicAdd(count, total);
+  at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const uint32_t mine = at + __popc(who[e] & below);
+    if (k[e] >= low && mine < kRowList) list[mine] = (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(first + e);
+    at += __popc(who[e]);
+  }
+}
+
 // Reads the groups at or above `low` again and lists their entries with low <= key; returns their
 // number, or more than kRowList if they do not fit. Ends with a barrier; listed is left at 0.
 template <typename T>
-__device__ int row_gather(const RowView<T>& v, const uint32_t* maxima, int groups, uint32_t low, RowScratch& sh) {
+__device__ __noinline__ int row_gather(const T* row, int V, int groups, uint32_t low) {
+  RowScratch& sh = row_scratch();
+  const uint32_t* maxima = row_maxima();
+  const RowView<T> v(row, V);
   constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC;
   const int lane = threadIdx.x & 31;
-  for (int i0 = 0; i0 < groups; i0 += kRowThreads) {
-    const int i = i0 + static_cast<int>(threadIdx.x);
-    row_append(i < groups && maxima[i] >= low, static_cast<uint32_t>(i), sh.groups, &sh.ngroups);
+  for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
+    const uint4 q = reinterpret_cast<const uint4*>(maxima)[i];
+    if (max(max(q.x, q.y), max(q.z, q.w)) < low) continue;
+    const uint32_t m[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (m[e] >= low) {
+        const uint32_t at = atomicAdd(&sh.ngroups, 1u);
+        if (at < kRowList) sh.groups[at] = 4 * i + e;
+      }
   }
   __syncthreads();
   const int ng = static_cast<int>(sh.ngroups);  // every group holds at least one entry
-  // LANES neighbouring lanes a group
-  if (ng <= kRowList)
+  // LANES neighbouring lanes a group, the next load ahead of the one in hand
+  if (ng <= kRowList) {
+    auto block = [&](int i) { return i < ng ? static_cast<int>(sh.groups[i]) * LANES + lane % LANES : v.blocks; };
+    int i = static_cast<int>(threadIdx.x) / LANES, b = block(i);
+    uint32_t k[VEC], next[VEC];
+    v.keys(b, k);
+#pragma unroll 1
     for (int i0 = 0; i0 < ng; i0 += kRowThreads / LANES) {
-      const int i = i0 + static_cast<int>(threadIdx.x) / LANES;
-      uint32_t k[VEC];
-      int b = 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) k[e] = 0u;
-      if (i < ng) {
-        b = static_cast<int>(sh.groups[i]) * LANES + lane % LANES;
-        v.keys(b, k);
-      }
+      const int bn = block(i += kRowThreads / LANES);
+      v.keys(bn, next);
       __syncwarp();
+      row_append_block<VEC>(k, low, v.first(b), sh.list, &sh.listed);
+      b = bn;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        row_append(k[e] >= low, (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e), sh.list,
-                   &sh.listed);
+      for (int e = 0; e < VEC; ++e) k[e] = next[e];
     }
+  }
   __syncthreads();
   const int n = ng <= kRowList ? static_cast<int>(sh.listed) : kRowList + 1;
   __syncthreads();
@@ -552,9 +668,10 @@ __device__ __forceinline__ void row_sort_desc(uint64_t* a, int n2) {
   __syncthreads();
 }
 
-// Orders `in` (n <= kRowList different entries) descending into `out` (not the same array): by rank
-// counting for a few entries, several threads an entry; else by a sorting network on `in`.
-__device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n) {
+// Orders the scratch's list (n <= kRowList different entries) descending into `sorted`: by rank
+// counting for a few entries, several threads an entry; else by a sorting network.
+__device__ __noinline__ void row_order(int n) {
+  uint64_t *in = row_scratch().list, *out = row_scratch().sorted;
   if (n <= kRowThreads) {
     int parts = 32;
     while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
@@ -580,27 +697,20 @@ __device__ __forceinline__ void row_order(uint64_t* in, uint64_t* out, int n) {
 // Going over the whole row
 // ------------------------------------------------------------------------------------------------
 
-// f(index, key) for every candidate of the row, each by one thread.
+// f(index, key) for every candidate of the row, each by one thread, four loads at a time.
 template <typename T, typename F>
 __device__ __forceinline__ void row_visit(const RowView<T>& v, F f) {
-  constexpr int VEC = RowView<T>::VEC, UNROLL = 32 / VEC;
-  for (int b0 = threadIdx.x; b0 < v.blocks; b0 += UNROLL * kRowThreads) {
-    uint4 q[UNROLL];
-    const bool inside = v.whole(b0) && v.whole(b0 + (UNROLL - 1) * kRowThreads);
+  constexpr int VEC = RowView<T>::VEC, AHEAD = 4;
+#pragma unroll 1
+  for (int b0 = threadIdx.x; b0 < v.blocks; b0 += AHEAD * kRowThreads) {
+    uint32_t k[AHEAD][VEC];
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j)
-      if (inside) q[j] = v.load(b0 + j * kRowThreads);
+    for (int j = 0; j < AHEAD; ++j) v.keys(b0 + j * kRowThreads, k[j]);
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      uint32_t k[VEC];
-      if (inside)
-        RowView<T>::keys_of(q[j], k);
-      else
-        v.keys(b0 + j * kRowThreads, k);
+    for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (k[e]) f(v.first(b0 + j * kRowThreads) + e, k[e]);
-    }
+        if (k[j][e]) f(v.first(b0 + j * kRowThreads) + e, k[j][e]);
   }
 }
 
@@ -609,13 +719,14 @@ __device__ __forceinline__ void row_visit(const RowView<T>& v, F f) {
 // otherwise the count) of all larger keys is `before` <= target < before + its own. The caller
 // makes sure that target is below the total. Every thread gets the result.
 template <typename T, bool MASS>
-__device__ uint32_t row_radix_select(const RowView<T>& v, uint32_t floor_key, uint64_t target, const RowWeight& weight,
-                                     RowScratch& sh, uint64_t& before) {
+__device__ __noinline__ uint32_t row_radix_select(const RowView<T> v, uint32_t floor_key, uint64_t target,
+                                                  const RowWeigher weight, uint64_t& before) {
+  RowScratch& sh = row_scratch();
   constexpr int BITS = RowKey<T>::BITS;
   uint32_t prefix = 0;
   int shift = BITS;
   before = 0;
-  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
+  uint32_t* counts = sh.counts;
   while (shift > 0) {
     const int width = shift < 11 ? shift : 11;
     const int next = shift - width;
@@ -646,7 +757,7 @@ __device__ uint32_t row_radix_select(const RowView<T>& v, uint32_t floor_key, ui
       own += h[j];
     }
     uint64_t total;
-    uint64_t run = before + block_exclusive_u64(own, sh, total);
+    uint64_t run = before + block_exclusive_u64(own, total);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (run <= target && target < run + h[j]) {
@@ -669,38 +780,22 @@ __device__ uint32_t row_radix_select(const RowView<T>& v, uint32_t floor_key, ui
 __device__ __forceinline__ int row_warp_steps(int blocks) { return ((blocks + 31) / 32 + kRowWarps - 1) / kRowWarps; }
 
 // f(block, keys of this lane's block) for each step, by every lane of the warp, until f returns false
-// (the same in every lane). Blocks whose group lies below `low` are not read (maxima null: all are);
-// their keys are 0, as past the end. Loads run four steps ahead.
+// (the same in every lane); keys of 0 past the end. The next step's load is ahead of the one in hand.
 template <typename T, typename F>
-__device__ __forceinline__ void row_warp_walk(const RowView<T>& v, const uint32_t* maxima, uint32_t low, F f) {
-  constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC, AHEAD = 4;
+__device__ __forceinline__ void row_key_walk(const RowView<T>& v, F f) {
+  constexpr int VEC = RowView<T>::VEC;
   const int lane = threadIdx.x & 31, per = row_warp_steps(v.blocks);
   const int s0 = static_cast<int>(threadIdx.x >> 5) * per, s1 = min((v.blocks + 31) / 32, s0 + per);
-  for (int s = s0; s < s1; s += AHEAD) {
-    uint4 q[AHEAD];
-    bool whole[AHEAD];
+  uint32_t k[VEC], next[VEC];
+  if (s0 < s1) v.keys(s0 * 32 + lane, k);
+#pragma unroll 1
+  for (int s = s0; s < s1; ++s) {
+    const int b = s * 32 + lane;
+    v.keys(s + 1 < s1 ? b + 32 : v.blocks, next);
+    __syncwarp();
+    if (!f(b, k)) return;
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int b = (s + j) * 32 + lane;
-      whole[j] = s + j < s1 && v.whole(b) && (maxima == nullptr || maxima[b / LANES] >= low);
-      if (whole[j]) q[j] = v.load(b);
-    }
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (s + j >= s1) return;
-      const int b = (s + j) * 32 + lane;
-      uint32_t k[VEC];
-      if (whole[j]) {
-        RowView<T>::keys_of(q[j], k);
-      } else if (b < v.blocks && !v.whole(b)) {
-        v.edge(b, k);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) k[e] = 0u;
-      }
-      __syncwarp();
-      if (!f(b, k)) return;
-    }
+    for (int e = 0; e < VEC; ++e) k[e] = next[e];
   }
 }
 
@@ -713,12 +808,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int k, float temperature, RowScan scan,
                      float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   using K = RowKey<T>;
-  extern __shared__ __align__(16) uint32_t row_maxima[];
-  __shared__ RowScratch sh;
+  RowScratch& sh = row_scratch();
   griddep_wait();  // launched as a programmatic dependent of the scan
   const int64_t row = blockIdx.x;
   const RowView<T> v(x + row * ldx, V);
-  const uint32_t top_key = row_open(scan, row, row_maxima, sh);
+  const uint32_t top_key = row_open(scan, row);
   if (threadIdx.x >= kRowThreads - 32) {  // the last warp joins the slices' sums at the row's maximum
     const double top = K::value(top_key);
     double s = 0.0;
@@ -733,27 +827,27 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   }
   int kk = 0;  // entries given
   if (top_key > 0) {
-    const uint32_t bound = row_bound(row_maxima, scan.groups, k, top_key, sh);
-    int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+    const uint32_t bound = row_bound(scan.groups, k, top_key);
+    int n = row_gather<T>(v.p, V, scan.groups, bound);
     kk = min(n, k);
     if (n > kRowList) {
       // the kk-th largest key, then the larger ones and of its equals the first in index order
       uint64_t n_gt;
-      const RowWeight none{};
-      const uint32_t cut = row_radix_select<T, false>(v, 1u, kk - 1, none, sh, n_gt);
+      const RowWeigher none{RowWeight{}};
+      const uint32_t cut = row_radix_select<T, false>(v, 1u, kk - 1, none, n_gt);
       uint32_t eq = 0;
-      row_warp_walk<T>(v, nullptr, 0u, [&](int, const uint32_t(&key)[RowView<T>::VEC]) {
+      row_key_walk<T>(v, [&](int, const uint32_t(&key)[RowView<T>::VEC]) {
 #pragma unroll
         for (int e = 0; e < RowView<T>::VEC; ++e) eq += key[e] == cut;
         return true;
       });
       // equals of the warps before this one
       uint64_t total;
-      uint64_t rank = block_exclusive_u64(eq, sh, total);
+      uint64_t rank = block_exclusive_u64(eq, total);
       rank = __shfl_sync(0xffffffffu, rank, 0);
       const uint64_t room = kk - n_gt;
       const int lane = threadIdx.x & 31;
-      row_warp_walk<T>(v, nullptr, 0u, [&](int b, const uint32_t(&key)[RowView<T>::VEC]) {
+      row_key_walk<T>(v, [&](int b, const uint32_t(&key)[RowView<T>::VEC]) {
         uint32_t mine = 0;
 #pragma unroll
         for (int e = 0; e < RowView<T>::VEC; ++e) mine += key[e] == cut;
@@ -776,10 +870,10 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       __syncthreads();
       n = kk;
     }
-    row_order(sh.list, sh.hist, n);
+    row_order(n);
   }
   for (int i = threadIdx.x; i < k; i += kRowThreads) {
-    const uint64_t e = i < kk ? sh.hist[i] : 0;
+    const uint64_t e = i < kk ? sh.sorted[i] : 0;
     values[row * k + i] = i < kk ? K::value(static_cast<uint32_t>(e >> 32)) : -INFINITY;
     ids[row * k + i] = i < kk ? static_cast<int64_t>(~static_cast<uint32_t>(e)) : -1;
   }
@@ -802,8 +896,9 @@ __device__ __forceinline__ uint32_t row_key_floor(float x) {
 // of the last (top_k 0: among all). `mass` is the total that top-p refers to (0: the list's own); then
 // the list is the head of the row's order, and the result is false if the border lies beyond it.
 template <typename T>
-__device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, uint64_t least, float uniform,
-                                const RowWeight& weight, RowScratch& sh, int64_t* __restrict__ token) {
+__device__ __noinline__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, uint64_t least, float uniform,
+                                             const RowWeigher weight, int64_t* __restrict__ token) {
+  RowScratch& sh = row_scratch();
   using K = RowKey<T>;
   constexpr int PER = kRowList / kRowThreads;
   uint64_t w[PER], own = 0, total;
@@ -812,11 +907,12 @@ __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, ui
     for (int j = 0; j < PER; ++j)
       if (threadIdx.x + j * kRowThreads < n)
         own += weight(K::value(static_cast<uint32_t>(sh.list[threadIdx.x + j * kRowThreads] >> 32)));
-    if (floor_share(top_p, mass) >= block_sum_u64(own, sh)) return false;
+    own = block_sum_u64(own);
+    if (floor_share(top_p, mass) >= own) return false;
     own = 0;
   }
-  uint64_t* sorted = sh.hist;
-  row_order(sh.list, sorted, n);
+  uint64_t* sorted = sh.sorted;
+  row_order(n);
   const uint32_t kth = top_k ? static_cast<uint32_t>(sorted[top_k - 1] >> 32) : 0u;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -825,7 +921,7 @@ __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, ui
     w[j] = at < n && key >= kth ? weight(K::value(key)) : 0;
     own += w[j];
   }
-  uint64_t before = block_exclusive_u64(own, sh, total);
+  uint64_t before = block_exclusive_u64(own, total);
   const uint64_t target = top_p < 1.f ? floor_share(top_p, mass ? mass : total) : ~0ull;
   uint64_t* kept = sh.list;  // row_order has read the list
   own = 0;
@@ -837,7 +933,7 @@ __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, ui
     own += keep;
     if (at < n) kept[at] = keep;
   }
-  const uint64_t aim = floor_share(uniform, block_sum_u64(own, sh));
+  const uint64_t aim = floor_share(uniform, block_sum_u64(own));
   // the running sum before an entry in index order is the weight of the kept entries of lower index
   int parts = 32;
   while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
@@ -858,7 +954,7 @@ __device__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, ui
 
 // A slice's weight at the row's maximum: as it is where the slice holds that maximum, else brought down.
 __device__ __forceinline__ uint64_t row_slice_mass(const RowSlice& a, uint32_t top_key, float slice_top,
-                                                   const RowWeight& weight, float temperature) {
+                                                   const RowWeigher& weight, float temperature) {
   if (a.top == top_key || a.top == 0) return a.mass;
   return __double2ull_rn(static_cast<double>(a.mass) *
                          exp((static_cast<double>(slice_top) - static_cast<double>(weight.top)) / temperature));
@@ -890,154 +986,27 @@ __device__ __forceinline__ bool row_warp_find(const uint64_t (&w)[VEC], uint64_t
   return run <= aim;
 }
 
-// Samples from the nucleus of the whole row; `mass` is the weight of all candidates and `target` top-p's
-// share of it. Entries that weigh at most (mass - target - 1) / V together weigh less than
-// mass - target, so the border lies above them. The others are counted (32-bit counts, no weights) in
-// 2048 bins even in x; as the entries of a bin weigh the same within a percent, the counts bound the
-// running weight from both sides and leave a few bins that can hold the border. A second pass, in
-// index order, sums what lies above those bins exactly and lists what lies in them. False where that
-// list is too long (the caller then selects by radix).
-template <typename T>
-__device__ bool row_pick_nucleus(const RowView<T>& v, const uint32_t* maxima, float temperature, uint64_t mass,
-                                 uint64_t target, uint64_t least, float uniform, const RowWeight& weight,
-                                 RowScratch& sh, int64_t* __restrict__ token) {
-  using K = RowKey<T>;
-  constexpr int VEC = RowView<T>::VEC;
-  const float top = weight.top;
-  // how far below the maximum (times T) the border can lie, with a margin that covers the fp32 arithmetic;
-  // weights are rounded, so one of light + 1 stands for light + 1/2 or more
-  const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(v.V);
-  const float depth = (static_cast<float>(weight.S) - log2f(static_cast<float>(light) + 0.5f)) * kLn2 + 1e-3f;
-  const float range = depth * temperature + 1e-5f * fabsf(top);
-  if (!(top < INFINITY) || !(range < INFINITY)) return false;
-  const float inv = static_cast<float>(kRowBins) / range, step = range / (temperature * kRowBins);
-  const uint32_t low = row_key_floor<T>(top - range);
-  auto bin = [&](uint32_t key) { return min(kRowBins - 1, static_cast<int>((top - K::value(key)) * inv)); };
-  uint32_t* counts = reinterpret_cast<uint32_t*>(sh.hist);
-  for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) counts[i] = 0;
-  if (threadIdx.x == 0) {
-    sh.found[0] = ~0ull;
-    sh.found[1] = kRowBins - 1;
-    sh.listed = 0;
-  }
-  __syncthreads();
-  row_visit<T>(v, [&](int, uint32_t key) {
-    if (key >= low) atomicAdd(&counts[bin(key)], 1u);
-  });
-  __syncthreads();
-  // bounds of an entry's weight at a bin's ends, 2e-4 wider than the fp32 arithmetic needs, and of the
-  // running weight
-  constexpr int BINS = kRowBins / kRowThreads;
-  uint32_t c[BINS];
-  uint64_t most[BINS], fewest[BINS], sum_most = 0, sum_fewest = 0, total;
-#pragma unroll
-  for (int j = 0; j < BINS; ++j) {
-    const int b = threadIdx.x * BINS + j;
-    c[j] = counts[b];
-    const double one = static_cast<double>(1ull << weight.S);
-    most[j] = c[j] * (__double2ull_ru(expf(-step * b) * 1.0002 * one) + 1);
-    fewest[j] = b == kRowBins - 1 ? 0 : c[j] * __double2ull_rd(expf(-step * (b + 1)) * 0.9998 * one);
-    sum_most += most[j];
-    sum_fewest += fewest[j];
-  }
-  uint64_t hi = block_exclusive_u64(sum_most, sh, total), lo = block_exclusive_u64(sum_fewest, sh, total);
-#pragma unroll
-  for (int j = 0; j < BINS; ++j) {
-    if (hi <= target && target < hi + most[j]) sh.found[0] = threadIdx.x * BINS + j;
-    if (lo <= target && target < lo + fewest[j]) sh.found[1] = threadIdx.x * BINS + j;
-    hi += most[j];
-    lo += fewest[j];
-  }
-  __syncthreads();
-  if (sh.found[0] == ~0ull) return false;
-  const int b1 = static_cast<int>(sh.found[0]), b2 = static_cast<int>(sh.found[1]);  // bins that can hold the border
-  uint64_t inside = 0;
-#pragma unroll
-  for (int j = 0; j < BINS; ++j) {
-    const int b = threadIdx.x * BINS + j;
-    if (b >= b1 && b <= b2) inside += c[j];
-  }
-  if (block_sum_u64(inside, sh) > kRowList) return false;
-  // no entry of those bins or above lies below this key
-  const uint32_t floor_key = b2 == kRowBins - 1 ? low : max(low, row_key_floor<T>(top - (b2 + 1) * 1.00001f / inv - 1e-6f * fabsf(top)));
-  uint64_t above = 0, kept = 0;
-  row_warp_walk<T>(v, maxima, floor_key, [&](int b, const uint32_t(&key)[VEC]) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int at = key[e] >= floor_key ? bin(key[e]) : kRowBins;
-      if (at < b1) {
-        const uint64_t w = weight(K::value(key[e]));
-        above += w;
-        kept += w >= least ? w : 0;
-      }
-      row_append(at >= b1 && at <= b2, (static_cast<uint64_t>(key[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e),
-                 sh.list, &sh.listed);
-    }
-    return true;
-  });
-  __syncthreads();
-  const int n = static_cast<int>(sh.listed);
-  uint64_t before = block_sum_u64(above, sh);
-  if (n == 0 || target < before) return false;
-  // the border: the listed entry at which the running weight passes the target
-  uint64_t* sorted = sh.hist;
-  if (threadIdx.x == 0) sh.found[0] = ~0ull;
-  row_order(sh.list, sorted, n);
-  constexpr int PER = kRowList / kRowThreads;
-  uint64_t w[PER], own = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int at = threadIdx.x * PER + j;
-    w[j] = at < n ? weight(K::value(static_cast<uint32_t>(sorted[at] >> 32))) : 0;
-    own += w[j];
-  }
-  before += block_exclusive_u64(own, sh, total);
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    if (before <= target && target < before + w[j]) sh.found[0] = threadIdx.x * PER + j;
-    before += w[j];
-  }
-  __syncthreads();
-  if (sh.found[0] == ~0ull) return false;
-  const int last = static_cast<int>(sh.found[0]);
-  const uint64_t border = sorted[last];
-  // the kept weight of each warp's range of the row
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = row_warp_steps(v.blocks);
-  for (int j = lane; j <= last; j += 32) {
-    const int i = static_cast<int>(~static_cast<uint32_t>(sorted[j]));
-    if ((i + v.off) / VEC / 32 / per != warp) continue;
-    const uint64_t wj = weight(K::value(static_cast<uint32_t>(sorted[j] >> 32)));
-    kept += wj >= least ? wj : 0;
-  }
-  kept = warp_sum_u64(kept);
-  uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? kept : 0, sh, total), 0);
-  const uint64_t aim = floor_share(uniform, total);
-  if (run > aim || aim >= run + kept) return true;
-  row_warp_walk<T>(v, maxima, floor_key, [&](int b, const uint32_t(&key)[VEC]) {
-    uint64_t we[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const uint64_t entry = (static_cast<uint64_t>(key[e]) << 32) | ~static_cast<uint32_t>(v.first(b) + e);
-      we[e] = entry >= border && key[e] ? weight(K::value(key[e])) : 0;
-      we[e] = we[e] >= least ? we[e] : 0;
-    }
-    return row_warp_find<VEC>(we, run, aim, v.first(b), token);
-  });
-  return true;
+// A value that the border of a row's nucleus does not lie below. `mass` is the weight of all candidates,
+// `target` top-p's share of it. Entries that weigh at most (mass - target - 1) / V together weigh less than
+// mass - target, so the border lies above them; weights are rounded, so one of light + 1 stands for
+// light + 1/2 or more. The margin covers the fp32 arithmetic.
+__device__ __forceinline__ float row_border_floor(int V, float temperature, uint64_t mass, uint64_t target, float top,
+                                                  int S) {
+  const uint64_t light = (mass - target - 1) / static_cast<uint64_t>(V);
+  const float depth = (static_cast<float>(S) - log2f(static_cast<float>(light) + 0.5f)) * kLn2 + 1e-3f;
+  return fmaxf(top - depth * temperature - 1e-5f * fabsf(top), -3.4e38f);
 }
 
 // Picks the token by going over the row in index order: kept are the entries above `cut` and the first
 // `ties` equal to it, as far as they weigh `least`; no entry below the key `lowest` does.
 template <typename T>
-__device__ void row_pick_walk(const RowView<T>& v, const uint32_t* maxima, uint32_t cut, uint64_t ties, uint32_t lowest,
-                              uint64_t least, float uniform, const RowWeight& weight, RowScratch& sh,
-                              int64_t* __restrict__ token) {
+__device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, uint32_t lowest, uint64_t least,
+                              float uniform, const RowWeigher& weight, int64_t* __restrict__ token) {
   using K = RowKey<T>;
   constexpr int VEC = RowView<T>::VEC;
   const int lane = threadIdx.x & 31;
   const uint64_t cut_weight = weight(K::value(cut));
   if (cut_weight < least) ties = 0;
-  const uint32_t low = max(cut, lowest);
   auto above = [&](uint32_t key) -> uint64_t {
     if (key <= cut || key < lowest) return 0;
     const uint64_t w = weight(K::value(key));
@@ -1045,7 +1014,7 @@ __device__ void row_pick_walk(const RowView<T>& v, const uint32_t* maxima, uint3
   };
   uint64_t sum = 0;
   uint32_t eq = 0;
-  row_warp_walk<T>(v, maxima, low, [&](int, const uint32_t(&key)[VEC]) {
+  row_key_walk<T>(v, [&](int, const uint32_t(&key)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       sum += above(key[e]);
@@ -1055,14 +1024,14 @@ __device__ void row_pick_walk(const RowView<T>& v, const uint32_t* maxima, uint3
   });
   // of each warp's range: its equals inside, its weight, the weight before it
   uint64_t all;
-  uint64_t rank = __shfl_sync(0xffffffffu, block_exclusive_u64(eq, sh, all), 0);
+  uint64_t rank = __shfl_sync(0xffffffffu, block_exclusive_u64(eq, all), 0);
   const uint64_t equals = __reduce_add_sync(0xffffffffu, eq);
   const uint64_t inside = rank < ties ? min(ties - rank, equals) : 0;
   sum = warp_sum_u64(sum) + inside * cut_weight;
-  uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? sum : 0, sh, all), 0);
+  uint64_t run = __shfl_sync(0xffffffffu, block_exclusive_u64(lane == 0 ? sum : 0, all), 0);
   const uint64_t aim = floor_share(uniform, all);
   if (run > aim || aim >= run + sum) return;
-  row_warp_walk<T>(v, maxima, low, [&](int b, const uint32_t(&key)[VEC]) {
+  row_key_walk<T>(v, [&](int b, const uint32_t(&key)[VEC]) {
     uint32_t same = 0;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) same += key[e] == cut;
@@ -1085,8 +1054,9 @@ __device__ void row_pick_walk(const RowView<T>& v, const uint32_t* maxima, uint3
 // share, and in it the entry, by the slice's own weights.
 template <typename T, int BLOCKS>
 __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t row, uint32_t top_key,
-                               float temperature, float uniform, const RowWeight& weight, RowScratch& sh,
+                               float temperature, float uniform, const RowWeigher& weight,
                                int64_t* __restrict__ token) {
+  RowScratch& sh = row_scratch();
   using K = RowKey<T>;
   constexpr int VEC = RowView<T>::VEC, SLICE = BLOCKS * kScanThreads;
   RowSlice a{0u, 0u, 0ull};
@@ -1095,7 +1065,7 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
     a = scan.slice[row * scan.slices + threadIdx.x];
     own = row_slice_mass(a, top_key, K::value(a.top), weight, temperature);
   }
-  const uint64_t run = block_exclusive_u64(own, sh, total);
+  const uint64_t run = block_exclusive_u64(own, total);
   uint64_t aim = floor_share(uniform, total);
   if (run <= aim && aim < run + own) {
     aim -= run;
@@ -1107,7 +1077,7 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
     sh.found[1] = aim;
   }
   __syncthreads();
-  const RowWeight local = row_weight(K::value(static_cast<uint32_t>(sh.found[0] >> 32)), temperature, weight.S, sh.exp_tab);
+  const RowWeigher local{row_weight(K::value(static_cast<uint32_t>(sh.found[0] >> 32)), temperature, weight.S)};
   const int b0 = static_cast<int>(sh.found[0] & 0xFFFFFFFFu) * SLICE;
   aim = sh.found[1];
   constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;  // blocks of a thread, neighbours
@@ -1126,7 +1096,7 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
     for (int e = 0; e < VEC; ++e)
       if (key[j][e]) mine += local(K::value(key[j][e]));
   }
-  uint64_t at = block_exclusive_u64(mine, sh, total);
+  uint64_t at = block_exclusive_u64(mine, total);
   if (at <= aim && aim < at + mine)
 #pragma unroll
     for (int j = 0; j < PER; ++j)
@@ -1141,18 +1111,17 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kRowThreads, 2)
     sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, const float* __restrict__ uniform,
-                         SampleKnobs knobs, RowScan scan, int64_t* __restrict__ tokens) {
+                         SampleKnobs knobs, RowScan scan, RowWideRows wide, int64_t* __restrict__ tokens) {
   using K = RowKey<T>;
   constexpr int LANES = kRowGroup / RowView<T>::VEC;
-  extern __shared__ __align__(16) uint32_t row_maxima[];
-  __shared__ RowScratch sh;
+  RowScratch& sh = row_scratch();
   const int64_t row = blockIdx.x;
   const RowView<T> v(x + row * ldx, V);
-  row_exp_table(sh.exp_tab);
+  griddep_launch_dependents();
   griddep_wait();  // launched as a programmatic dependent of the scan
   const SampleRow knob(knobs, row);
   const float u = uniform[row], T_ = knob.temperature;
-  const uint32_t top_key = row_open(scan, row, row_maxima, sh);
+  const uint32_t top_key = row_open(scan, row);
   if (top_key == 0) {
     if (threadIdx.x == 0) tokens[row] = -1;
     return;
@@ -1160,7 +1129,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   if (knob.greedy) {  // the first group with the largest key, its first entry
     uint32_t g = 0xFFFFFFFFu;
     for (int i = threadIdx.x; i < scan.groups; i += kRowThreads)
-      if (row_maxima[i] == top_key) g = min(g, static_cast<uint32_t>(i));
+      if (row_maxima()[i] == top_key) g = min(g, static_cast<uint32_t>(i));
     g = __reduce_min_sync(0xffffffffu, g);
     if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = g;
     __syncthreads();
@@ -1179,11 +1148,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     if (threadIdx.x == 0) tokens[row] = at;
     return;
   }
-  const RowWeight weight = row_weight(K::value(top_key), T_, S, sh.exp_tab);
+  const RowWeigher weight{row_weight(K::value(top_key), T_, S)};
   // min-p: weights below `least` leave; no entry below the key `lowest` passes (lower by a margin that
   // covers fp32)
   const float floor_p = fminf(fmaxf(knob.min_p, 0.f), 1.f);
-  const uint64_t least = __double2ull_ru(static_cast<double>(floor_p) * (1ull << S));
+  const uint64_t least = row_least(floor_p, S);
   uint32_t lowest = 1u;
   if (floor_p > 0.f)
     lowest = weight.top < INFINITY
@@ -1195,19 +1164,40 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   if (knob.top_k > kRowMaxK) {
     uint64_t candidates = 0;
     row_visit<T>(v, [&](int, uint32_t) { ++candidates; });
-    filtered = static_cast<uint64_t>(knob.top_k) < block_sum_u64(candidates, sh);
+    filtered = static_cast<uint64_t>(knob.top_k) < block_sum_u64(candidates);
   } else if (knob.top_k >= 1) {
-    const uint32_t bound = row_bound(row_maxima, scan.groups, knob.top_k, top_key, sh);
-    const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
+    const uint32_t bound = row_bound(scan.groups, knob.top_k, top_key);
+    const int n = row_gather<T>(v.p, V, scan.groups, bound);
     if (n <= kRowList) {  // with fewer than top_k entries, all there are
-      row_pick_listed<T>(n, min(n, knob.top_k), knob.top_p, 0, least, u, weight, sh, tokens + row);
+      row_pick_listed<T>(n, min(n, knob.top_k), knob.top_p, 0, least, u, weight, tokens + row);
       return;
     }
     filtered = true;
   }
+  // the row's number among the wide rows, or -1: no room
+  auto enlist = [&](float lo, float hi, uint64_t target, bool nucleus) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const uint32_t slot = wide.count ? atomicAdd(wide.count, 1u) : 0xFFFFFFFFu;
+      if (slot < static_cast<uint32_t>(wide.most)) {
+        RowWideRow& r = wide.rows[slot];
+        r.row = row;
+        r.top = weight.top;
+        r.lo = lo;
+        r.hi = hi;
+        r.target = target;
+        r.nucleus = nucleus;
+      }
+      sh.found[0] = slot;
+    }
+    __syncthreads();
+    if (sh.found[0] >= static_cast<uint64_t>(wide.most)) return false;
+    for (int i = threadIdx.x; i < kRowWideBins; i += kRowThreads) wide.rows[sh.found[0]].bins[i] = 0;
+    return true;
+  };
   uint32_t cut = 1u;
   uint64_t before, ties = ~0ull;
-  if (filtered) cut = row_radix_select<T, false>(v, 1u, knob.top_k - 1, weight, sh, before);
+  if (filtered) cut = row_radix_select<T, false>(v, 1u, knob.top_k - 1, weight, before);
   if (knob.top_p < 1.f) {
     uint64_t mass = 0;
     if (knob.wants_mass()) {
@@ -1220,32 +1210,378 @@ __global__ void __launch_bounds__(kRowThreads, 2)
         if (key >= cut) mass += weight(K::value(key));
       });
     }
-    mass = block_sum_u64(mass, sh);
+    mass = block_sum_u64(mass);
     const uint64_t target = floor_share(knob.top_p, mass);
     if (!filtered) {
-      // the head of the order first: a nucleus is usually a few hundred entries
-      const uint32_t bound = row_bound(row_maxima, scan.groups, kRowMaxK, top_key, sh);
-      const int n = row_gather<T>(v, row_maxima, scan.groups, bound, sh);
-      const bool whole_row = n < kRowMaxK || bound == 1u;
-      if (n <= kRowList && row_pick_listed<T>(n, 0, knob.top_p, whole_row ? 0 : mass, least, u, weight, sh, tokens + row))
-        return;
-      __syncthreads();
-      if (row_pick_nucleus<T>(v, row_maxima, T_, mass, target, least, u, weight, sh, tokens + row)) return;
+      // the head of the order first: most nuclei are a few hundred entries at most
+      const uint32_t bound = row_bound(scan.groups, kRowHead, top_key);
+      const int n = row_gather<T>(v.p, V, scan.groups, bound);
+      if (n <= kRowList) {
+        const bool whole_row = n < kRowHead || bound == 1u;
+        if (row_pick_listed<T>(n, 0, knob.top_p, whole_row ? 0 : mass, least, u, weight, tokens + row)) return;
+        if (weight.top < INFINITY &&
+            enlist(row_border_floor(V, T_, mass, target, weight.top, S), INFINITY, target, true))
+          return;
+      }
       __syncthreads();
     }
-    cut = row_radix_select<T, true>(v, cut, target, weight, sh, before);
+    cut = row_radix_select<T, true>(v, cut, target, weight, before);
     ties = (target - before) / weight(K::value(cut)) + 1;
   } else if (!filtered && floor_p > 0.f) {
-    const int n = row_gather<T>(v, row_maxima, scan.groups, lowest, sh);
+    const int n = row_gather<T>(v.p, V, scan.groups, lowest);
     if (n <= kRowList) {
-      row_pick_listed<T>(n, 0, 1.f, 0, least, u, weight, sh, tokens + row);
+      row_pick_listed<T>(n, 0, 1.f, 0, least, u, weight, tokens + row);
       return;
     }
+    if (weight.top < INFINITY && enlist(K::value(lowest), K::value(lowest), 0, false)) return;
   } else if (!filtered && knob.wants_mass()) {
-    row_pick_slice<T, BLOCKS>(v, scan, row, top_key, T_, u, weight, sh, tokens + row);
+    row_pick_slice<T, BLOCKS>(v, scan, row, top_key, T_, u, weight, tokens + row);
     return;
   }
-  row_pick_walk<T>(v, row_maxima, cut, ties, lowest, least, u, weight, sh, tokens + row);
+  row_pick_walk<T>(v, cut, ties, lowest, least, u, weight, tokens + row);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Wide rows
+// ------------------------------------------------------------------------------------------------
+
+// f(index, value, live) for the entries at or above `lo` of a slice, 32 at a time by a whole warp: a warp
+// queues its entries, so that the few that matter do not each cost a warp's arithmetic.
+template <typename T, int BLOCKS, typename F>
+__device__ __forceinline__ void row_slice_entries(const RowView<T>& v, int b0, float lo, uint2* queue, F f) {
+  constexpr int VEC = RowView<T>::VEC;
+  const int lane = threadIdx.x & 31;
+  const uint32_t below = (1u << lane) - 1u;
+  int queued = 0;
+#pragma unroll 1
+  for (int j = 0; j < BLOCKS; ++j) {
+    const int b = b0 + j * kScanThreads + static_cast<int>(threadIdx.x);
+    float xs[VEC];
+    v.values(b, xs);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint32_t who = __ballot_sync(0xffffffffu, xs[e] >= lo);
+      if (xs[e] >= lo) queue[queued + __popc(who & below)] = make_uint2(v.first(b) + e, __float_as_uint(xs[e]));
+      queued += __popc(who);
+    }
+    __syncwarp();
+#pragma unroll 1
+    while (queued >= 32) {
+      queued -= 32;
+      const uint2 e = queue[queued + lane];
+      f(e.x, __uint_as_float(e.y), true);
+      __syncwarp();
+    }
+  }
+  if (queued) {
+    const uint2 e = queue[lane];
+    f(e.x, __uint_as_float(e.y), lane < queued);
+  }
+}
+
+// Persistent over the slices of the wide rows with a nucleus: the weights from the maximum down to lo, in
+// bins even in x.
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kScanThreads)
+    row_wide_bins_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, SampleKnobs knobs, int slices,
+                         RowWideRows wide) {
+  __shared__ uint2 queues[kScanThreads / 32][32 * (RowView<T>::VEC + 1)];  // (index, value)
+  __shared__ unsigned long long bins[kRowWideBins];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int64_t units = static_cast<int64_t>(min(*wide.count, static_cast<uint32_t>(wide.most))) * slices;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    RowWideRow& r = wide.rows[unit / slices];
+    if (!r.nucleus) continue;
+    for (int i = threadIdx.x; i < kRowWideBins; i += kScanThreads) bins[i] = 0;
+    __syncthreads();
+    const RowView<T> v(x + r.row * ldx, V);
+    const SampleRow knob(knobs, r.row);
+    const RowWeight weight = row_weight(r.top, knob.temperature, S);
+    const float top = r.top, inv = r.per_value();
+    row_slice_entries<T, BLOCKS>(v, static_cast<int>(unit % slices) * BLOCKS * kScanThreads, r.lo, queues[threadIdx.x >> 5],
+                                 [&](uint32_t, float xe, bool live) {
+                                   const uint64_t w = live ? weight(xe) : 0;
+                                   if (w) atomicAdd(&bins[min(kRowWideBins - 1, static_cast<int>((top - xe) * inv))], w);
+                                 });
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRowWideBins; i += kScanThreads)
+      if (bins[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&r.bins[i]), bins[i]);
+    __syncthreads();
+  }
+}
+
+// One warp per wide row: the window becomes the bin that holds the border, a little wider than the fp32
+// arithmetic needs.
+__global__ void __launch_bounds__(256) row_wide_window_kernel(RowWideRows wide) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const uint32_t count = min(*wide.count, static_cast<uint32_t>(wide.most));
+  for (uint32_t slot = blockIdx.x * 8 + (threadIdx.x >> 5); slot < count; slot += gridDim.x * 8) {
+    RowWideRow& r = wide.rows[slot];
+    if (!r.nucleus) continue;
+    constexpr int PER = kRowWideBins / 32;
+    uint64_t sum = 0;
+    for (int j = 0; j < PER; ++j) sum += r.bins[lane * PER + j];
+    uint64_t run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
+    }
+    run -= sum;
+    const float lo = r.lo, inv = r.per_value();
+    __syncwarp();
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t h = r.bins[lane * PER + j];
+      if (run <= r.target && r.target < run + h) {
+        const int b = lane * PER + j;
+        const float slack = 1e-6f * (fabsf(r.top) + (r.top - lo));
+        r.hi = b == 0 ? INFINITY : r.top - static_cast<float>(b) / inv + slack;
+        r.lo = b == kRowWideBins - 1 ? lo : fmaxf(lo, r.top - static_cast<float>(b + 1) / inv - slack);
+      }
+      run += h;
+    }
+  }
+}
+
+// Persistent over the slices of the wide rows: per slice the weight of the entries above the window, all
+// of them and those that pass min-p, and the window's entries.
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kScanThreads)
+    row_wide_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, SampleKnobs knobs, int slices,
+                    RowWideRows wide) {
+  using K = RowKey<T>;
+  constexpr int WARPS = kScanThreads / 32;
+  __shared__ uint2 queues[WARPS][32 * (RowView<T>::VEC + 1)];  // (index, value)
+  __shared__ uint64_t wabove[WARPS], wkept[WARPS];
+  __shared__ uint32_t listed;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t below = (1u << lane) - 1u;
+  const int64_t units = static_cast<int64_t>(min(*wide.count, static_cast<uint32_t>(wide.most))) * slices;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const RowWideRow& r = wide.rows[unit / slices];
+    uint64_t* const list = wide.lists + unit * wide.room;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    const float hi = r.hi;
+    const RowView<T> v(x + r.row * ldx, V);
+    const SampleRow knob(knobs, r.row);
+    const RowWeight weight = row_weight(r.top, knob.temperature, S);
+    const uint64_t least = row_least(knob.min_p, S);
+    uint64_t above = 0, kept = 0;
+    row_slice_entries<T, BLOCKS>(
+        v, static_cast<int>(unit % slices) * BLOCKS * kScanThreads, r.lo, queues[warp], [&](uint32_t i, float xe, bool live) {
+          const bool inside = live && !(xe >= hi);
+          if (live && !inside) {
+            const uint64_t w = weight(xe);
+            above += w;
+            kept += w >= least ? w : 0;
+          }
+          const uint32_t who = __ballot_sync(0xffffffffu, inside);
+          if (who == 0) return;
+          uint32_t at = 0;
+          if (lane == 0) at = atomicAdd(&listed, static_cast<uint32_t>(__popc(who)));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & below);
+          if (inside && at < static_cast<uint32_t>(wide.room)) list[at] = (static_cast<uint64_t>(K::of(xe)) << 32) | ~i;
+        });
+    above = warp_sum_u64(above);
+    kept = warp_sum_u64(kept);
+    if (lane == 0) {
+      wabove[warp] = above;
+      wkept[warp] = kept;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      RowSums s{0, 0, listed};
+      for (int w = 0; w < WARPS; ++w) {
+        s.above += wabove[w];
+        s.kept += wkept[w];
+      }
+      wide.sums[unit] = s;
+    }
+    __syncthreads();
+  }
+}
+
+// Per slice, after the scratch: its kept weight and the entries that it listed.
+struct RowWideSlices {
+  uint64_t kept[kRowThreads];
+  uint32_t listed[kRowThreads];
+};
+
+// One CTA per wide row at a time: the border among the window's entries, the slice that holds the
+// uniform's share of the kept weight, and in it the entry.
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    row_wide_pick_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, const float* __restrict__ uniform,
+                         SampleKnobs knobs, int slices, RowWideRows wide, int64_t* __restrict__ tokens) {
+  using K = RowKey<T>;
+  constexpr int VEC = RowView<T>::VEC, SLICE = BLOCKS * kScanThreads;
+  RowScratch& sh = row_scratch();
+  RowWideSlices& win = *reinterpret_cast<RowWideSlices*>(row_smem + (sizeof(RowScratch) + 15) / 16 * 16);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_wait();
+  const uint32_t count = min(*wide.count, static_cast<uint32_t>(wide.most));
+  for (uint32_t slot = blockIdx.x; slot < count; slot += gridDim.x) {
+    __syncthreads();
+    const RowWideRow& r = wide.rows[slot];
+    const RowView<T> v(x + r.row * ldx, V);
+    const SampleRow knob(knobs, r.row);
+    const RowWeigher weight{row_weight(r.top, knob.temperature, S)};
+    const uint64_t least = row_least(knob.min_p, S);
+    const float u = uniform[r.row];
+    uint64_t total;
+    RowSums own{0, 0, 0};
+    if (static_cast<int>(threadIdx.x) < slices) own = wide.sums[static_cast<int64_t>(slot) * slices + threadIdx.x];
+    win.kept[threadIdx.x] = own.kept;
+    win.listed[threadIdx.x] = own.listed;
+    if (threadIdx.x == 0) {
+      sh.listed = 0;
+      sh.found[0] = ~0ull;
+    }
+    for (int i = threadIdx.x; i < kRowBins; i += kRowThreads) sh.hist[i] = 0;
+    uint64_t border = 0;  // of the kept entries the last in the order; 0: all are kept
+    // f(entry or 0) for the listed entries of the warp's slices, 32 at a time; then g(slice)
+    auto each = [&](auto f, auto g) {
+      for (int s = warp; s < slices; s += kRowWarps) {
+        const uint64_t* list = wide.lists + (static_cast<int64_t>(slot) * slices + s) * wide.room;
+        const int n = static_cast<int>(win.listed[s]);
+#pragma unroll 1
+        for (int i = lane; i - lane < n; i += 128) {  // four loads at a time
+          uint64_t e[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) e[j] = i + 32 * j < n ? list[i + 32 * j] : 0ull;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f(e[j]);
+        }
+        g(s);
+      }
+    };
+    if (r.nucleus) {
+      const uint64_t above = block_sum_u64(own.above);
+      bool ok = !__syncthreads_or(own.listed > static_cast<uint32_t>(wide.room)) && above <= r.target;
+      if (ok) {
+        // weights in 2048 bins even in x, the bin that holds the target, its entries in order
+        const float xhi = fminf(r.hi, r.top), inv = static_cast<float>(kRowBins) / fmaxf(xhi - r.lo, 1e-30f);
+        auto bin = [&](float x) { return min(kRowBins - 1, max(0, static_cast<int>((xhi - x) * inv))); };
+        each(
+            [&](uint64_t e) {
+              if (e == 0) return;
+              const float x = K::value(static_cast<uint32_t>(e >> 32));
+              atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin(x)]), static_cast<unsigned long long>(weight(x)));
+            },
+            [](int) {});
+        __syncthreads();
+        constexpr int BINS = kRowBins / kRowThreads;
+        uint64_t h[BINS], sum = 0;
+#pragma unroll
+        for (int j = 0; j < BINS; ++j) sum += h[j] = sh.hist[threadIdx.x * BINS + j];
+        uint64_t run = above + block_exclusive_u64(sum, total);
+#pragma unroll
+        for (int j = 0; j < BINS; ++j) {
+          if (run <= r.target && r.target < run + h[j]) {
+            sh.found[0] = threadIdx.x * BINS + j;
+            sh.found[1] = run;
+          }
+          run += h[j];
+        }
+        __syncthreads();
+        ok = sh.found[0] != ~0ull;
+        if (ok) {
+          const int at = static_cast<int>(sh.found[0]);
+          const uint64_t before = sh.found[1];
+          each(
+              [&](uint64_t e) {
+                row_append(e && bin(K::value(static_cast<uint32_t>(e >> 32))) == at, e, sh.list, &sh.listed);
+              },
+              [](int) {});
+          __syncthreads();
+          const int m = static_cast<int>(min(sh.listed, static_cast<uint32_t>(kRowList) + 1u));
+          ok = m <= kRowList;
+          if (ok) {
+            row_order(m);
+            constexpr int PER = kRowList / kRowThreads;
+            uint64_t w[PER], mine = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              const int k = threadIdx.x * PER + j;
+              w[j] = k < m ? weight(K::value(static_cast<uint32_t>(sh.sorted[k] >> 32))) : 0;
+              mine += w[j];
+            }
+            run = before + block_exclusive_u64(mine, total);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              if (run <= r.target && r.target < run + w[j]) sh.found[0] = sh.sorted[threadIdx.x * PER + j];
+              run += w[j];
+            }
+            __syncthreads();
+            border = sh.found[0];
+          }
+        }
+      }
+      if (!ok) {  // the border is not in the window, or the window holds too much: the whole row
+        __syncthreads();
+        uint64_t before;
+        const uint32_t cut = row_radix_select<T, true>(v, 1u, r.target, weight, before);
+        const uint64_t ties = (r.target - before) / weight(K::value(cut)) + 1;
+        row_pick_walk<T>(v, cut, ties, 1u, least, u, weight, tokens + r.row);
+        continue;
+      }
+      // the kept entries of the window join their slices
+      uint64_t sum = 0;
+      each(
+          [&](uint64_t e) {
+            if (e < border || e == 0) return;
+            const uint64_t w = weight(K::value(static_cast<uint32_t>(e >> 32)));
+            sum += w >= least ? w : 0;
+          },
+          [&](int s) {
+            sum = warp_sum_u64(sum);
+            if (lane == 0) win.kept[s] += sum;
+            sum = 0;
+          });
+    }
+    __syncthreads();
+    const uint64_t mine = win.kept[threadIdx.x];
+    uint64_t run = block_exclusive_u64(mine, total);
+    const uint64_t aim = floor_share(u, total);
+    if (run <= aim && aim < run + mine) {
+      sh.found[0] = threadIdx.x;
+      sh.found[1] = aim - run;
+    }
+    __syncthreads();
+    const int b0 = static_cast<int>(sh.found[0]) * SLICE;
+    const uint64_t rest = sh.found[1];
+    // the slice, a thread its neighbouring blocks
+    constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;
+    uint64_t sum = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      uint64_t at = pass ? block_exclusive_u64(sum, total) : 0;
+      if (pass && !(at <= rest && rest < at + sum)) break;
+#pragma unroll 1
+      for (int j = 0; j < PER; ++j) {
+        const int k = threadIdx.x * PER + j;
+        float xs[VEC];
+        v.values(k < SLICE ? b0 + k : v.blocks, xs);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (!(xs[e] >= r.lo)) continue;
+          const uint32_t i = v.first(b0 + k) + e;
+          if (((static_cast<uint64_t>(K::of(xs[e])) << 32) | ~i) < border) continue;
+          uint64_t w = weight(xs[e]);
+          w = w >= least ? w : 0;
+          if (pass && at <= rest && rest < at + w) tokens[r.row] = i;
+          at += w;
+        }
+      }
+      if (!pass) sum = at;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1254,26 +1590,40 @@ __global__ void __launch_bounds__(kRowThreads, 2)
 
 struct RowPlan {
   int groups, slices, blocks;  // blocks: 16-byte blocks of a scan thread
-  size_t off_slice, total;
+  int wide, room;              // most wide rows; entries a slice of one may list
+  size_t off_slice, off_count, off_rows, off_sums, off_lists, total;
 };
 
 // Slices of 8192 entries, 32 a thread in flight; of 2048 where that leaves SMs without a slice (a
-// few rows). `aligned`: every row starts on a 16-byte boundary.
-inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned) {
+// few rows). `aligned`: every row starts on a 16-byte boundary. `wide`: rows can turn out wide.
+inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned, bool wide) {
   RowPlan p{};
   const int vec = 16 / elem;
   p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), 4 * kRowGroup)) * 4;
   const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 19);
   p.blocks = (small ? 2048 : 8192) / vec / kScanThreads;
   p.slices = static_cast<int>(ceil_div(static_cast<int64_t>(p.groups) * kRowGroup, static_cast<int64_t>(p.blocks) * kScanThreads * vec));
-  p.off_slice = (static_cast<size_t>(R) * p.groups * 4 + 255) / 256 * 256;
-  p.total = p.off_slice + static_cast<size_t>(R) * p.slices * sizeof(RowSlice);
+  p.wide = wide ? static_cast<int>(std::min<int64_t>(R, kRowWideRows)) : 0;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = (off + bytes + 255) / 256 * 256;
+    return o;
+  };
+  take(static_cast<size_t>(R) * p.groups * 4);
+  p.off_slice = take(static_cast<size_t>(R) * p.slices * sizeof(RowSlice));
+  p.off_count = take(wide ? 4 : 0);
+  p.off_rows = take(static_cast<size_t>(p.wide) * sizeof(RowWideRow));
+  p.off_sums = take(static_cast<size_t>(p.wide) * p.slices * sizeof(RowSums));
+  p.room = p.blocks * kScanThreads * vec / kRowWideShare;
+  p.off_lists = take(static_cast<size_t>(p.wide) * p.slices * p.room * 8);
+  p.total = off;
   return p;
 }
 
 // Bytes that do for any alignment.
-inline size_t row_ws_bytes(int64_t R, int64_t V, int elem) {
-  return std::max(row_plan(R, V, elem, true).total, row_plan(R, V, elem, false).total);
+inline size_t row_ws_bytes(int64_t R, int64_t V, int elem, bool wide) {
+  return std::max(row_plan(R, V, elem, true, wide).total, row_plan(R, V, elem, false, wide).total);
 }
 
 template <typename T, bool SAMPLE>
@@ -1290,42 +1640,76 @@ int row_scan_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, int V,
 }
 
 template <typename T>
-inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, void* ws, size_t ws_bytes, RowPlan& p,
+inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, bool wide, void* ws, size_t ws_bytes, RowPlan& p,
                        RowScan& scan) {
-  p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0);
+  p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0, wide);
   ORTHRUS_CHECK_ARG(R * p.slices < (1ll << 31) && (reinterpret_cast<uintptr_t>(x) & (sizeof(T) - 1)) == 0);
   if (ws == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
-  scan = {static_cast<uint32_t*>(ws), reinterpret_cast<RowSlice*>(static_cast<uint8_t*>(ws) + p.off_slice), p.groups,
-          p.slices};
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  scan = {reinterpret_cast<uint32_t*>(w), reinterpret_cast<RowSlice*>(w + p.off_slice), p.groups, p.slices,
+          wide ? reinterpret_cast<uint32_t*>(w + p.off_count) : nullptr};
   return ORTHRUS_OK;
 }
 
-constexpr int kRowSmem = (kRowMaxV + 8) / kRowGroup * 4 + 32;  // the group maxima of the longest row
+// The scratch and the group maxima, of the longest row or of these; the scratch and a window.
+constexpr int kRowScratch = (sizeof(RowScratch) + 15) / 16 * 16;
+constexpr int kRowSmem = kRowScratch + (kRowMaxV + 8) / kRowGroup * 4 + 512;
+constexpr int kRowWideSmem = kRowScratch + static_cast<int>(sizeof(RowWideSlices));
 
 template <typename T>
 int topk_rows_impl(const T* x, int64_t ldx, int64_t R, int64_t V, int k, float temperature, float* values, int64_t* ids,
                    float* lse, void* ws, size_t ws_bytes, cudaStream_t stream) {
   RowPlan p;
   RowScan scan;
-  int rc = row_prepare(x, ldx, R, V, ws, ws_bytes, p, scan);
+  int rc = row_prepare(x, ldx, R, V, false, ws, ws_bytes, p, scan);
   if (rc != ORTHRUS_OK) return rc;
   rc = row_scan_launch<T, false>(p, x, ldx, R, static_cast<int>(V), temperature, 0, SampleKnobs{}, scan, stream);
   if (rc != ORTHRUS_OK) return rc;
   ORTHRUS_CHECK_CUDA(ensure_smem(topk_rows_kernel<T>, kRowSmem));
   ORTHRUS_CHECK_CUDA(launch_pdl(topk_rows_kernel<T>, dim3(static_cast<unsigned>(R)), dim3(kRowThreads),
-                                p.groups * 4, stream, x, ldx, static_cast<int>(V), k, temperature, scan, values,
+                                kRowScratch + p.groups * 4, stream, x, ldx, static_cast<int>(V), k, temperature, scan, values,
                                 ids, lse));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
 }
 
+// Whether rows can turn out wide: a nucleus or min-p without a top-k that fits a list.
+inline bool sample_can_be_wide(const SampleKnobs& k) {
+  return (k.top_k || k.top_k1 < 1 || k.top_k1 > kRowMaxK) && (k.top_p || k.top_p1 < 1.f || k.min_p || k.min_p1 > 0.f);
+}
+
 template <typename T, int BLOCKS>
 int sample_finish_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, int V, int S, const float* uniform,
-                         const SampleKnobs& knobs, const RowScan& scan, int64_t* tokens, cudaStream_t stream) {
-  auto kernel = sample_logits_kernel<T, BLOCKS>;
-  ORTHRUS_CHECK_CUDA(ensure_smem(kernel, kRowSmem));
-  ORTHRUS_CHECK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(R)), dim3(kRowThreads), p.groups * 4,
-                                stream, x, ldx, V, S, uniform, knobs, scan, tokens));
+                         const SampleKnobs& knobs, const RowScan& scan, uint8_t* ws, int64_t* tokens,
+                         cudaStream_t stream) {
+  const RowWideRows wide{scan.wide_count, reinterpret_cast<RowWideRow*>(ws + p.off_rows),
+                         reinterpret_cast<RowSums*>(ws + p.off_sums), reinterpret_cast<uint64_t*>(ws + p.off_lists),
+                         p.wide, p.room};
+  auto finish = sample_logits_kernel<T, BLOCKS>;
+  ORTHRUS_CHECK_CUDA(ensure_smem(finish, kRowSmem));
+  ORTHRUS_CHECK_CUDA(launch_pdl(finish, dim3(static_cast<unsigned>(R)), dim3(kRowThreads), kRowScratch + p.groups * 4,
+                                stream, x, ldx, V, S, uniform, knobs, scan, wide, tokens));
+  ORTHRUS_CHECK_LAUNCH();
+  if (p.wide == 0) return ORTHRUS_OK;
+  const int64_t units = static_cast<int64_t>(p.wide) * p.slices;
+  if (knobs.top_p || knobs.top_p1 < 1.f) {
+    ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_bins_kernel<T, BLOCKS>,
+                                  dim3(static_cast<unsigned>(std::min<int64_t>(units, 6 * num_sms()))), dim3(kScanThreads),
+                                  0, stream, x, ldx, V, S, knobs, p.slices, wide));
+    ORTHRUS_CHECK_LAUNCH();
+    ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_window_kernel,
+                                  dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(p.wide, 8), num_sms()))),
+                                  dim3(256), 0, stream, wide));
+    ORTHRUS_CHECK_LAUNCH();
+  }
+  ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_kernel<T, BLOCKS>,
+                                dim3(static_cast<unsigned>(std::min<int64_t>(units, 6 * num_sms()))), dim3(kScanThreads), 0,
+                                stream, x, ldx, V, S, knobs, p.slices, wide));
+  ORTHRUS_CHECK_LAUNCH();
+  auto pick = row_wide_pick_kernel<T, BLOCKS>;
+  ORTHRUS_CHECK_CUDA(ensure_smem(pick, kRowWideSmem));
+  ORTHRUS_CHECK_CUDA(launch_pdl(pick, dim3(static_cast<unsigned>(std::min(p.wide, 2 * num_sms()))), dim3(kRowThreads),
+                                kRowWideSmem, stream, x, ldx, V, S, uniform, knobs, p.slices, wide, tokens));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
 }
@@ -1335,14 +1719,15 @@ int sample_logits_impl(const T* x, int64_t ldx, int64_t R, int64_t V, const floa
                        int64_t* tokens, void* ws, size_t ws_bytes, cudaStream_t stream) {
   RowPlan p;
   RowScan scan;
-  int rc = row_prepare(x, ldx, R, V, ws, ws_bytes, p, scan);
+  int rc = row_prepare(x, ldx, R, V, sample_can_be_wide(knobs), ws, ws_bytes, p, scan);
   if (rc != ORTHRUS_OK) return rc;
   const int n = static_cast<int>(V), S = row_weight_bits(n);
   rc = row_scan_launch<T, true>(p, x, ldx, R, n, 1.f, S, knobs, scan, stream);
   if (rc != ORTHRUS_OK) return rc;
   constexpr int BIG = 8192 / RowView<T>::VEC / kScanThreads, SMALL = 2048 / RowView<T>::VEC / kScanThreads;
-  return p.blocks == BIG ? sample_finish_launch<T, BIG>(p, x, ldx, R, n, S, uniform, knobs, scan, tokens, stream)
-                         : sample_finish_launch<T, SMALL>(p, x, ldx, R, n, S, uniform, knobs, scan, tokens, stream);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  return p.blocks == BIG ? sample_finish_launch<T, BIG>(p, x, ldx, R, n, S, uniform, knobs, scan, w, tokens, stream)
+                         : sample_finish_launch<T, SMALL>(p, x, ldx, R, n, S, uniform, knobs, scan, w, tokens, stream);
 }
 
 }  // namespace orthrus

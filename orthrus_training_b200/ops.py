@@ -781,7 +781,7 @@ def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
     ids = torch.empty(R, k, dtype=torch.int64, device=dev)
     lse = torch.empty(R, dtype=torch.float32, device=dev)
     lib = L.lib()
-    nbytes = lib.orthrus_vocab_rows_workspace_bytes(R, V, code)
+    nbytes = lib.orthrus_topk_rows_workspace_bytes(R, V, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
         L.check(lib.orthrus_topk_rows(logits.data_ptr(), pitch, R, V, k, float(temperature), values.data_ptr(),
@@ -824,7 +824,9 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     m, m1 = _knob(min_p, "min_p", R, dev, torch.float32, 0.0, 1.0)
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
     lib = L.lib()
-    nbytes = lib.orthrus_vocab_rows_workspace_bytes(R, V, code)
+    filters = (k is not None or not 1 <= k1 <= TOPK_ROWS_MAX_K) and (
+        p is not None or p1 < 1 or m is not None or m1 > 0)
+    nbytes = lib.orthrus_sample_logits_workspace_bytes(R, V, int(filters), code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
         L.check(lib.orthrus_sample_logits(logits.data_ptr(), pitch, R, V, uniforms.data_ptr(), L.ptr(t), t1, L.ptr(k),

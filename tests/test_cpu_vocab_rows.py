@@ -39,10 +39,15 @@ def test_row_workspace():
     lib, L = _lib().lib(), _lib()
     assert _topk(ws=None) == L.EWORKSPACE and _topk(ws_bytes=8) == L.EWORKSPACE
     for dtype in (L.F32, L.BF16):
-        assert lib.orthrus_vocab_rows_workspace_bytes(0, 100, dtype) == 0
+        assert lib.orthrus_topk_rows_workspace_bytes(0, 100, dtype) == 0
         for R, V in ((1, 1), (3, 1000), (1024, 151936), (2, 2 ** 20)):
             # a maximum for 32 entries, and a record of 16 bytes for 2048 or 8192
-            assert R * V / 8 <= lib.orthrus_vocab_rows_workspace_bytes(R, V, dtype) <= R * (V / 8 + V / 128 + 80) + 256
+            small = lib.orthrus_topk_rows_workspace_bytes(R, V, dtype)
+            assert R * V / 8 <= small <= R * (V / 8 + V / 128 + 80) + 512
+            assert lib.orthrus_sample_logits_workspace_bytes(R, V, 0, dtype) == small
+            # and the lists of up to 2048 rows that keep much, an eighth of the row at 8 bytes
+            more = lib.orthrus_sample_logits_workspace_bytes(R, V, 1, dtype) - small
+            assert min(R, 2048) * V <= more <= min(R, 2048) * (V + 8192 + V / 64 + 8192) + 2048
 
 
 def test_no_rows_are_no_work():
