@@ -156,6 +156,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(device: torch.device | None = None) -> int:
+    if device is not None and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -26,7 +26,7 @@
 
 namespace orthrus {
 
-constexpr int kRowThreads = 512;          // of the CTA that finishes a row
+constexpr int kRowThreads = 256;          // of the CTA that finishes a row
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kScanThreads = 256;
 constexpr int kRowGroup = 32;             // entries behind one group maximum
@@ -497,7 +497,7 @@ __device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row) {
 __device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) {
   RowScratch& sh = row_scratch();
   const uint32_t* maxima = row_maxima();
-  constexpr int BIN_BITS = 10;  // two bins a thread
+  constexpr int BIN_BITS = 9;  // two bins a thread
   static_assert(1 << BIN_BITS == 2 * kRowThreads, "");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t* counts = sh.counts;
@@ -804,7 +804,7 @@ __device__ __forceinline__ void row_key_walk(const RowView<T>& v, F f) {
 // ------------------------------------------------------------------------------------------------
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 2)
+__global__ void __launch_bounds__(kRowThreads, 4)
     topk_rows_kernel(const T* __restrict__ x, int64_t ldx, int V, int k, float temperature, RowScan scan,
                      float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   using K = RowKey<T>;
@@ -896,8 +896,8 @@ __device__ __forceinline__ uint32_t row_key_floor(float x) {
 // of the last (top_k 0: among all). `mass` is the total that top-p refers to (0: the list's own); then
 // the list is the head of the row's order, and the result is false if the border lies beyond it.
 template <typename T>
-__device__ __noinline__ bool row_pick_listed(int n, int top_k, float top_p, uint64_t mass, uint64_t least, float uniform,
-                                             const RowWeigher weight, int64_t* __restrict__ token) {
+__device__ __noinline__ bool row_pick_listed(int n, int V, int top_k, float top_p, uint64_t mass, uint64_t least,
+                                             float uniform, const RowWeigher weight, int64_t* __restrict__ token) {
   RowScratch& sh = row_scratch();
   using K = RowKey<T>;
   constexpr int PER = kRowList / kRowThreads;
@@ -911,44 +911,60 @@ __device__ __noinline__ bool row_pick_listed(int n, int top_k, float top_p, uint
     if (floor_share(top_p, mass) >= own) return false;
     own = 0;
   }
-  uint64_t* sorted = sh.sorted;
-  row_order(n);
-  const uint32_t kth = top_k ? static_cast<uint32_t>(sorted[top_k - 1] >> 32) : 0u;
+  // only top-k and top-p ask for the order
+  const bool order = top_k || top_p < 1.f;
+  if (order) row_order(n);
+  const uint64_t* entries = order ? sh.sorted : sh.list;
+  const uint32_t kth = top_k ? static_cast<uint32_t>(entries[top_k - 1] >> 32) : 0u;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int at = threadIdx.x * PER + j;
-    const uint32_t key = at < n ? static_cast<uint32_t>(sorted[at] >> 32) : 0u;
+    const uint32_t key = at < n ? static_cast<uint32_t>(entries[at] >> 32) : 0u;
     w[j] = at < n && key >= kth ? weight(K::value(key)) : 0;
     own += w[j];
   }
   uint64_t before = block_exclusive_u64(own, total);
   const uint64_t target = top_p < 1.f ? floor_share(top_p, mass ? mass : total) : ~0ull;
-  uint64_t* kept = sh.list;  // row_order has read the list
   own = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const int at = threadIdx.x * PER + j;
     const uint64_t keep = before <= target && w[j] >= least ? w[j] : 0;
     before += w[j];
-    own += keep;
-    if (at < n) kept[at] = keep;
+    own += w[j] = keep;
   }
   const uint64_t aim = floor_share(uniform, block_sum_u64(own));
-  // the running sum before an entry in index order is the weight of the kept entries of lower index
-  int parts = 32;
-  while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
-  const int stride = kRowThreads / parts, part = threadIdx.x % parts;
-  for (int e0 = 0; e0 < n; e0 += stride) {
-    const int e = e0 + threadIdx.x / parts;
-    const uint32_t place = e < n ? static_cast<uint32_t>(sorted[e]) : 0u;
-    const uint64_t mine = e < n ? kept[e] : 0;
+  // the token: the lowest index up to which the kept entries weigh more than `aim`
+  if (n <= kRowThreads / 2) {  // a few: the running sum before each, two threads an entry
+    uint64_t* kept = order ? sh.list : sh.sorted;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (threadIdx.x * PER + j < n) kept[threadIdx.x * PER + j] = w[j];
+    __syncthreads();
+    const int e = min(static_cast<int>(threadIdx.x) / 2, n - 1);
+    const uint32_t place = static_cast<uint32_t>(entries[e]);
     uint64_t run = 0;
-    if (mine)
-      for (int j = part; j < n; j += parts)
-        if (static_cast<uint32_t>(sorted[j]) > place) run += kept[j];
-    for (int o = parts >> 1; o > 0; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
-    if (mine && part == 0 && run <= aim && aim < run + mine) *token = ~place;
+    for (int j = threadIdx.x % 2; j < n; j += 2) run += static_cast<uint32_t>(entries[j]) > place ? kept[j] : 0;
+    run += __shfl_xor_sync(0xffffffffu, run, 1);
+    if (run <= aim && aim < run + kept[e]) *token = ~place;
+    return true;
   }
+  uint32_t place[PER];  // more: by bisection
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int at = threadIdx.x * PER + j;
+    place[j] = at < n ? ~static_cast<uint32_t>(entries[at]) : 0xFFFFFFFFu;
+  }
+  uint32_t lo = 0, hi = V - 1;
+#pragma unroll 1
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    own = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) own += place[j] <= mid ? w[j] : 0;
+    if (block_sum_u64(own) > aim) hi = mid;
+    else lo = mid + 1;
+  }
+  if (threadIdx.x == 0) *token = lo;
   return true;
 }
 
@@ -1109,7 +1125,7 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
 }
 
 template <typename T, int BLOCKS>
-__global__ void __launch_bounds__(kRowThreads, 2)
+__global__ void __launch_bounds__(kRowThreads, 4)
     sample_logits_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, const float* __restrict__ uniform,
                          SampleKnobs knobs, RowScan scan, RowWideRows wide, int64_t* __restrict__ tokens) {
   using K = RowKey<T>;
@@ -1169,7 +1185,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     const uint32_t bound = row_bound(scan.groups, knob.top_k, top_key);
     const int n = row_gather<T>(v.p, V, scan.groups, bound);
     if (n <= kRowList) {  // with fewer than top_k entries, all there are
-      row_pick_listed<T>(n, min(n, knob.top_k), knob.top_p, 0, least, u, weight, tokens + row);
+      row_pick_listed<T>(n, V, min(n, knob.top_k), knob.top_p, 0, least, u, weight, tokens + row);
       return;
     }
     filtered = true;
@@ -1218,7 +1234,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       const int n = row_gather<T>(v.p, V, scan.groups, bound);
       if (n <= kRowList) {
         const bool whole_row = n < kRowHead || bound == 1u;
-        if (row_pick_listed<T>(n, 0, knob.top_p, whole_row ? 0 : mass, least, u, weight, tokens + row)) return;
+        if (row_pick_listed<T>(n, V, 0, knob.top_p, whole_row ? 0 : mass, least, u, weight, tokens + row)) return;
         if (weight.top < INFINITY &&
             enlist(row_border_floor(V, T_, mass, target, weight.top, S), INFINITY, target, true))
           return;
@@ -1230,7 +1246,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   } else if (!filtered && floor_p > 0.f) {
     const int n = row_gather<T>(v.p, V, scan.groups, lowest);
     if (n <= kRowList) {
-      row_pick_listed<T>(n, 0, 1.f, 0, least, u, weight, tokens + row);
+      row_pick_listed<T>(n, V, 0, 1.f, 0, least, u, weight, tokens + row);
       return;
     }
     if (weight.top < INFINITY && enlist(K::value(lowest), K::value(lowest), 0, false)) return;
@@ -1416,7 +1432,7 @@ struct RowWideSlices {
 // One CTA per wide row at a time: the border among the window's entries, the slice that holds the
 // uniform's share of the kept weight, and in it the entry.
 template <typename T, int BLOCKS>
-__global__ void __launch_bounds__(kRowThreads, 2)
+__global__ void __launch_bounds__(kRowThreads, 4)
     row_wide_pick_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, const float* __restrict__ uniform,
                          SampleKnobs knobs, int slices, RowWideRows wide, int64_t* __restrict__ tokens) {
   using K = RowKey<T>;
@@ -1600,7 +1616,7 @@ inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned, bool wide)
   RowPlan p{};
   const int vec = 16 / elem;
   p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), 4 * kRowGroup)) * 4;
-  const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 19);
+  const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 18);
   p.blocks = (small ? 2048 : 8192) / vec / kScanThreads;
   p.slices = static_cast<int>(ceil_div(static_cast<int64_t>(p.groups) * kRowGroup, static_cast<int64_t>(p.blocks) * kScanThreads * vec));
   p.wide = wide ? static_cast<int>(std::min<int64_t>(R, kRowWideRows)) : 0;

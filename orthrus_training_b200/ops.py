@@ -7,6 +7,7 @@ import math
 from collections import defaultdict
 from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -766,6 +767,16 @@ def _vocab_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int]:
     return logits.shape[0], logits.shape[1], logits.stride(0)
 
 
+@lru_cache(maxsize=256)
+def _topk_rows_bytes(R: int, V: int, code: int) -> int:
+    return L.lib().orthrus_topk_rows_workspace_bytes(R, V, code)
+
+
+@lru_cache(maxsize=256)
+def _sample_logits_bytes(R: int, V: int, filters: bool, code: int) -> int:
+    return L.lib().orthrus_sample_logits_workspace_bytes(R, V, int(filters), code)
+
+
 def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
     """The k largest logits of each row [R, V] (fp32 or bf16, rows contiguous at any pitch):
     (values fp32 [R, k] descending, ids int64 [R, k], lse fp32 [R] = logsumexp(row / temperature)).
@@ -780,8 +791,7 @@ def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
     values = torch.empty(R, k, dtype=torch.float32, device=dev)
     ids = torch.empty(R, k, dtype=torch.int64, device=dev)
     lse = torch.empty(R, dtype=torch.float32, device=dev)
-    lib = L.lib()
-    nbytes = lib.orthrus_topk_rows_workspace_bytes(R, V, code)
+    lib, nbytes = L.lib(), _topk_rows_bytes(R, V, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
         L.check(lib.orthrus_topk_rows(logits.data_ptr(), pitch, R, V, k, float(temperature), values.data_ptr(),
@@ -823,10 +833,9 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     p, p1 = _knob(top_p, "top_p", R, dev, torch.float32, 0.0, 1.0)
     m, m1 = _knob(min_p, "min_p", R, dev, torch.float32, 0.0, 1.0)
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
-    lib = L.lib()
     filters = (k is not None or not 1 <= k1 <= TOPK_ROWS_MAX_K) and (
         p is not None or p1 < 1 or m is not None or m1 > 0)
-    nbytes = lib.orthrus_sample_logits_workspace_bytes(R, V, int(filters), code)
+    lib, nbytes = L.lib(), _sample_logits_bytes(R, V, filters, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on_device(dev):
         L.check(lib.orthrus_sample_logits(logits.data_ptr(), pitch, R, V, uniforms.data_ptr(), L.ptr(t), t1, L.ptr(k),
