@@ -241,8 +241,9 @@ struct RowWeight {
     constexpr double c = 0.6931471805599453;
     constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5, c6 = c5 * c / 6, c7 = c6 * c / 7,
                      c8 = c7 * c / 8, c9 = c8 * c / 9, c10 = c9 * c / 10;
-    const double y = x == top ? 0.0 : fma(-static_cast<double>(x), scale, at);
-    if (!(y < S + 2.0)) return 0;  // rounds to 0; also an infinite maximum's other entries
+    // at S + 2 the weight rounds to 0, so deeper entries count as that deep (no branch, so that the
+    // products of neighbouring entries interleave); also an infinite maximum's other entries
+    const double y = x == top ? 0.0 : fmin(fma(-static_cast<double>(x), scale, at), S + 2.0);
     const double r = y + kRound;
     const double f = (r - kRound) - y;
     double p = fma(c10, f, c9);
@@ -1296,13 +1297,15 @@ __device__ __forceinline__ void row_slice_entries(const RowView<T>& v, int b0, f
 }
 
 // Persistent over the slices of the wide rows with a nucleus: the weights from the maximum down to lo, in
-// bins even in x.
+// bins even in x. They only say where to look for the border, so fp32 does: an entry counts as
+// 2^18 times its weight over that of its bin's upper end, which keeps a slice's 8192 entries in 32
+// bits (whose shared-memory atomics cost a fifth of those on 64).
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kScanThreads)
-    row_wide_bins_kernel(const T* __restrict__ x, int64_t ldx, int V, int S, SampleKnobs knobs, int slices,
-                         RowWideRows wide) {
-  __shared__ uint2 queues[kScanThreads / 32][32 * (RowView<T>::VEC + 1)];  // (index, value)
-  __shared__ unsigned long long bins[kRowWideBins];
+    row_wide_bins_kernel(const T* __restrict__ x, int64_t ldx, int V, SampleKnobs knobs, int slices, RowWideRows wide) {
+  constexpr int VEC = RowView<T>::VEC;
+  static_assert(BLOCKS * kScanThreads * VEC <= 8192, "a slice's sums exceed 32 bits");
+  __shared__ uint32_t bins[kRowWideBins];
   griddep_launch_dependents();
   griddep_wait();
   const int64_t units = static_cast<int64_t>(min(*wide.count, static_cast<uint32_t>(wide.most))) * slices;
@@ -1312,24 +1315,32 @@ __global__ void __launch_bounds__(kScanThreads)
     for (int i = threadIdx.x; i < kRowWideBins; i += kScanThreads) bins[i] = 0;
     __syncthreads();
     const RowView<T> v(x + r.row * ldx, V);
-    const SampleRow knob(knobs, r.row);
-    const RowWeight weight = row_weight(r.top, knob.temperature, S);
-    const float top = r.top, inv = r.per_value();
-    row_slice_entries<T, BLOCKS>(v, static_cast<int>(unit % slices) * BLOCKS * kScanThreads, r.lo, queues[threadIdx.x >> 5],
-                                 [&](uint32_t, float xe, bool live) {
-                                   const uint64_t w = live ? weight(xe) : 0;
-                                   if (w) atomicAdd(&bins[min(kRowWideBins - 1, static_cast<int>((top - xe) * inv))], w);
-                                 });
+    const float top = r.top, lo = r.lo, inv = r.per_value();
+    const float bits = kLog2e / SampleRow(knobs, r.row).temperature / inv;  // of a bin
+    const int b0 = static_cast<int>(unit % slices) * BLOCKS * kScanThreads;
+#pragma unroll 1
+    for (int j = 0; j < BLOCKS; ++j) {
+      float xs[VEC];
+      v.values(b0 + j * kScanThreads + static_cast<int>(threadIdx.x), xs);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = (top - xs[e]) * inv;
+        const int b = min(kRowWideBins - 1, static_cast<int>(d));
+        const uint32_t w = __float2uint_rn(ex2_approx(18.f - (d - static_cast<float>(b)) * bits));
+        if (xs[e] >= lo) atomicAdd(&bins[b], w);
+      }
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < kRowWideBins; i += kScanThreads)
-      if (bins[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&r.bins[i]), bins[i]);
+      if (bins[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&r.bins[i]), static_cast<unsigned long long>(bins[i]));
     __syncthreads();
   }
 }
 
 // One warp per wide row: the window becomes the bin that holds the border, a little wider than the fp32
-// arithmetic needs.
-__global__ void __launch_bounds__(256) row_wide_window_kernel(RowWideRows wide) {
+// arithmetic needs, with the next bin where the border lies close to it. (Bins are off by 512 roundings
+// of a bin's part of at most 2^-3 bits, the sums that run over them by less than 2^-15 of themselves.)
+__global__ void __launch_bounds__(256) row_wide_window_kernel(int S, SampleKnobs knobs, RowWideRows wide) {
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
@@ -1338,27 +1349,40 @@ __global__ void __launch_bounds__(256) row_wide_window_kernel(RowWideRows wide) 
     RowWideRow& r = wide.rows[slot];
     if (!r.nucleus) continue;
     constexpr int PER = kRowWideBins / 32;
-    uint64_t sum = 0;
-    for (int j = 0; j < PER; ++j) sum += r.bins[lane * PER + j];
-    uint64_t run = sum;
+    const float lo = r.lo, inv = r.per_value();
+    const float bits = kLog2e / SampleRow(knobs, r.row).temperature / inv;
+    const double unit = static_cast<double>(1ull << (S - 18));
+    double h[PER], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      h[j] = static_cast<double>(r.bins[lane * PER + j]) * unit * exp2f(-bits * static_cast<float>(lane * PER + j));
+      sum += h[j];
+    }
+    double run = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, run, o);
+      const double u = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += u;
     }
     run -= sum;
-    const float lo = r.lo, inv = r.per_value();
-    __syncwarp();
+    const double target = static_cast<double>(r.target), near = target * 0x1p-15;
+    int first = kRowWideBins, last = -1;  // bins that may hold the border
+#pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const uint64_t h = r.bins[lane * PER + j];
-      if (run <= r.target && r.target < run + h) {
-        const int b = lane * PER + j;
-        const float slack = 1e-6f * (fabsf(r.top) + (r.top - lo));
-        r.hi = b == 0 ? INFINITY : r.top - static_cast<float>(b) / inv + slack;
-        r.lo = b == kRowWideBins - 1 ? lo : fmaxf(lo, r.top - static_cast<float>(b + 1) / inv - slack);
+      if (h[j] > 0.0 && run - near <= target && target <= run + h[j] + near) {
+        first = min(first, lane * PER + j);
+        last = lane * PER + j;
       }
-      run += h;
+      run += h[j];
     }
+    first = __reduce_min_sync(0xffffffffu, first);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && last >= 0) {
+      const float slack = 1e-6f * (fabsf(r.top) + (r.top - lo));
+      r.hi = first == 0 ? INFINITY : r.top - static_cast<float>(first) / inv + slack;
+      r.lo = last == kRowWideBins - 1 ? lo : fmaxf(lo, r.top - static_cast<float>(last + 1) / inv - slack);
+    }
+    __syncwarp();
   }
 }
 
@@ -1710,12 +1734,12 @@ int sample_finish_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, i
   const int64_t units = static_cast<int64_t>(p.wide) * p.slices;
   if (knobs.top_p || knobs.top_p1 < 1.f) {
     ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_bins_kernel<T, BLOCKS>,
-                                  dim3(static_cast<unsigned>(std::min<int64_t>(units, 6 * num_sms()))), dim3(kScanThreads),
-                                  0, stream, x, ldx, V, S, knobs, p.slices, wide));
+                                  dim3(static_cast<unsigned>(std::min<int64_t>(units, 8 * num_sms()))), dim3(kScanThreads),
+                                  0, stream, x, ldx, V, knobs, p.slices, wide));
     ORTHRUS_CHECK_LAUNCH();
     ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_window_kernel,
                                   dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(p.wide, 8), num_sms()))),
-                                  dim3(256), 0, stream, wide));
+                                  dim3(256), 0, stream, S, knobs, wide));
     ORTHRUS_CHECK_LAUNCH();
   }
   ORTHRUS_CHECK_CUDA(launch_pdl(row_wide_kernel<T, BLOCKS>,
@@ -1724,7 +1748,7 @@ int sample_finish_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, i
   ORTHRUS_CHECK_LAUNCH();
   auto pick = row_wide_pick_kernel<T, BLOCKS>;
   ORTHRUS_CHECK_CUDA(ensure_smem(pick, kRowWideSmem));
-  ORTHRUS_CHECK_CUDA(launch_pdl(pick, dim3(static_cast<unsigned>(std::min(p.wide, 2 * num_sms()))), dim3(kRowThreads),
+  ORTHRUS_CHECK_CUDA(launch_pdl(pick, dim3(static_cast<unsigned>(std::min(p.wide, 4 * num_sms()))), dim3(kRowThreads),
                                 kRowWideSmem, stream, x, ldx, V, S, uniform, knobs, p.slices, wide, tokens));
   ORTHRUS_CHECK_LAUNCH();
   return ORTHRUS_OK;
