@@ -227,37 +227,34 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& to
 // fall the same way on every path. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
 // 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
 //
-// The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f by its Taylor polynomial of
-// degree 10 (error below (ln2 / 2)^11 / 11! = 2.2e-13), 2^(S - n) by the exponent. A table would save
-// six of the fp64 products, but its lookups, of random banks, take longer.
+// The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f = 1 + f q(f) with q of degree
+// 8 through the Chebyshev nodes of [-1/2, 1/2] (error below 4e-14), 2^(S - n) by the exponent. A table
+// would save some of the fp64 products, but its lookups, of random banks, take longer. No branch, and
+// what can be is left to fp32: the loops over rows are bound by the instructions that they issue, some
+// 30 an entry here.
 struct RowWeight {
-  float top;         // the maximum the weights refer to
+  float top;            // the maximum the weights refer to
+  float floor;          // entries below are deeper than S + 3/2 bits: they weigh 0. +inf if top is
   int S;
-  double scale, at;  // log2(e) / T; top * scale
+  double from, scale;   // top, if finite; log2(e) / T
 
   __device__ __forceinline__ uint64_t operator()(float x) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     constexpr double kInt = 4503599627370496.0;    // 2^52
-    constexpr double c = 0.6931471805599453;
-    constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5, c6 = c5 * c / 6, c7 = c6 * c / 7,
-                     c8 = c7 * c / 8, c9 = c8 * c / 9, c10 = c9 * c / 10;
-    // at S + 2 the weight rounds to 0, so deeper entries count as that deep (no branch, so that the
-    // products of neighbouring entries interleave); also an infinite maximum's other entries
-    const double y = x == top ? 0.0 : fmin(fma(-static_cast<double>(x), scale, at), S + 2.0);
+    const double y = (from - static_cast<double>(fminf(x, 3.4028234663852886e38f))) * scale;
     const double r = y + kRound;
     const double f = (r - kRound) - y;
-    double p = fma(c10, f, c9);
-    p = fma(p, f, c8);
-    p = fma(p, f, c7);
-    p = fma(p, f, c6);
-    p = fma(p, f, c5);
-    p = fma(p, f, c4);
-    p = fma(p, f, c3);
-    p = fma(p, f, c2);
-    p = fma(p, f, c);
-    p = fma(p, f, 1.0);
+    double q = fma(1.0203121063391729e-07, f, 1.3255224878668817e-06);
+    q = fma(q, f, 1.525268684626772e-05);
+    q = fma(q, f, 1.5403455852453838e-04);
+    q = fma(q, f, 1.3333558179043112e-03);
+    q = fma(q, f, 9.618129159402558e-03);
+    q = fma(q, f, 5.5504108664760424e-02);
+    q = fma(q, f, 2.402265069581299e-01);
+    q = fma(q, f, 6.931471805599453e-01);
+    const double p = fma(q, f, 1.0);
     const double w = __hiloint2double(__double2hiint(p) + ((S - __double2loint(r)) << 20), __double2loint(p)) + kInt;
-    return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+    return x >= floor ? static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull : 0ull;
   }
 };
 
@@ -269,19 +266,22 @@ __host__ __device__ inline int row_weight_bits(int V) {
 
 __device__ __forceinline__ RowWeight row_weight(float top, float temperature, int S) {
   const double scale = 1.4426950408889634 / static_cast<double>(temperature);
-  return {top, S, scale, static_cast<double>(top) * scale};
+  if (top == INFINITY) return {top, top, S, 3.4028234663852886e38, scale};
+  const double from = static_cast<double>(top);
+  return {top, __double2float_ru(from - (S + 1.5) / scale), S, from, scale};
 }
 
 // The same out of line, for the finish, which has many places that weigh an entry.
-__device__ __noinline__ uint64_t row_weigh(float x, float top, int S, double scale, double at) {
-  return RowWeight{top, S, scale, at}(x);
+__device__ __noinline__ uint64_t row_weigh(float x, float floor, int S, double from, double scale) {
+  return RowWeight{0.f, floor, S, from, scale}(x);
 }
 struct RowWeigher {
-  float top;
+  float top, floor;
   int S;
-  double scale, at;
-  __device__ __forceinline__ explicit RowWeigher(const RowWeight& w) : top(w.top), S(w.S), scale(w.scale), at(w.at) {}
-  __device__ __forceinline__ uint64_t operator()(float x) const { return row_weigh(x, top, S, scale, at); }
+  double from, scale;
+  __device__ __forceinline__ explicit RowWeigher(const RowWeight& w)
+      : top(w.top), floor(w.floor), S(w.S), from(w.from), scale(w.scale) {}
+  __device__ __forceinline__ uint64_t operator()(float x) const { return row_weigh(x, floor, S, from, scale); }
 };
 
 // floor(f * z) for f in [0, 1) and z < 2^62, exactly (f is an integer of 24 bits times a power of
