@@ -151,8 +151,10 @@ struct RowView {
 // ------------------------------------------------------------------------------------------------
 
 struct RowScratch {
-  uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
-  uint32_t counts[kRowBins]; // histograms
+  union {
+    uint64_t list[kRowList];   // gathered entries, (key << 32 | ~index)
+    uint32_t counts[kRowBins]; // histograms; done with before entries are gathered
+  };
   uint64_t warp[kRowWarps];
   uint32_t top[kRowWarps];
   uint64_t found[2];         // result of a block-wide search
@@ -232,6 +234,10 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& to
 // would save some of the fp64 products, but its lookups, of random banks, take longer. No branch, and
 // what can be is left to fp32: the loops over rows are bound by the instructions that they issue, some
 // 30 an entry here.
+__constant__ double kRowExp2[9] = {6.931471805599453e-01,  2.402265069581299e-01,  5.5504108664760424e-02,
+                                   9.618129159402558e-03,  1.3333558179043112e-03, 1.5403455852453838e-04,
+                                   1.525268684626772e-05,  1.3255224878668817e-06, 1.0203121063391729e-07};
+
 struct RowWeight {
   float top;            // the maximum the weights refer to
   float floor;          // entries below are deeper than S + 3/2 bits: they weigh 0. +inf if top is
@@ -244,14 +250,9 @@ struct RowWeight {
     const double y = (from - static_cast<double>(fminf(x, 3.4028234663852886e38f))) * scale;
     const double r = y + kRound;
     const double f = (r - kRound) - y;
-    double q = fma(1.0203121063391729e-07, f, 1.3255224878668817e-06);
-    q = fma(q, f, 1.525268684626772e-05);
-    q = fma(q, f, 1.5403455852453838e-04);
-    q = fma(q, f, 1.3333558179043112e-03);
-    q = fma(q, f, 9.618129159402558e-03);
-    q = fma(q, f, 5.5504108664760424e-02);
-    q = fma(q, f, 2.402265069581299e-01);
-    q = fma(q, f, 6.931471805599453e-01);
+    double q = kRowExp2[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) q = fma(q, f, kRowExp2[i]);
     const double p = fma(q, f, 1.0);
     const double w = __hiloint2double(__double2hiint(p) + ((S - __double2loint(r)) << 20), __double2loint(p)) + kInt;
     return x >= floor ? static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull : 0ull;
