@@ -496,7 +496,7 @@ size_t orthrus_topk_rows_workspace_bytes(int64_t R, int64_t V, int dtype);
 
 /* The k largest candidates of each row (1 <= k <= 1024): values [R, k] fp32 and ids [R, k] in
  * order, (-inf, -1) past the last candidate, and lse [R] = log(sum exp(x / temperature)) over the
- * candidates (-inf without any, +inf if one is +inf). temperature > 0. */
+ * candidates (-inf without any, +inf if one is +inf). temperature from 1e-30 to 1e30. */
 int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
                       float* values, int64_t* ids, float* lse, void* workspace,
                       size_t workspace_bytes, int dtype, void* stream);
@@ -508,9 +508,10 @@ int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int
  * first always); and of these the ones with w_i >= min_p. The token is the first kept index at
  * which the running sum of kept weights, in index order, exceeds uniform * total. A uniform below 0
  * or NaN counts as 0, one of 1 or more picks the last kept token of positive weight. A temperature
- * below 1e-5 gives the row's first maximum; a row without candidates gives -1. Sums are exact
- * (integer weights of at least 42 fractional bits), so the token depends on the row and its knobs
- * alone. Each knob is a device array [R], or NULL and the value beside it for every row. The workspace
+ * below 1e-5 or NaN gives the row's first maximum; a row without candidates gives -1. Sums are of
+ * integer weights of at least 42 fractional bits, so they do not depend on their order; a row's
+ * slices are brought to one maximum in fp64, so a token can depend on how the call is launched
+ * only where the uniform, or top_p, falls within about 2^-40 of a border. Each knob is a device array [R], or NULL and the value beside it for every row. The workspace
  * is asked for with `filters` = 1 when top_p or min_p can filter a row whose top_k is off or above 1024
  * (either array given, or top_p1 < 1 or min_p1 > 0; top_k given, or top_k1 < 1 or > 1024): rows that
  * keep thousands of entries need about V bytes each, for up to 2048 of them. */

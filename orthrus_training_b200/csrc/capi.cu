@@ -928,7 +928,8 @@ extern "C" size_t orthrus_sample_logits_workspace_bytes(int64_t R, int64_t V, in
 extern "C" int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
                                  float* values, int64_t* ids, float* lse, void* workspace, size_t workspace_bytes,
                                  int dtype, void* stream) {
-  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V <= kRowMaxV && ldl >= 0 && k >= 1 && k <= kRowMaxK && temperature > 0.f);
+  ORTHRUS_CHECK_ARG(R >= 0 && V >= 1 && V <= kRowMaxV && ldl >= 0 && k >= 1 && k <= kRowMaxK);
+  ORTHRUS_CHECK_ARG(temperature >= 1e-30f && temperature <= 1e30f);
   ORTHRUS_CHECK_ARG(R < (1ll << 31) && (dtype == ORTHRUS_F32 || dtype == ORTHRUS_BF16));
   if (R == 0) return ORTHRUS_OK;
   ORTHRUS_CHECK_ARG(logits && values && ids && lse);

@@ -903,7 +903,8 @@ int lmhead_topk_kl_fwd_impl(const E* student, const E* weight, const TopkKlCall&
                             int num_offsets, float* total, E* grad, float* kl_by_offset, int64_t* agree_by_offset,
                             int64_t chunk_rows, void* ws_raw, size_t ws_bytes, cudaStream_t stream) {
   constexpr bool kBf16 = sizeof(E) == 2;
-  ORTHRUS_CHECK_ARG(a.n >= 0 && a.m >= 0 && a.V >= 1 && a.D >= 1 && a.k >= 1 && a.k <= kTopkKlMaxK && a.T > 0.f);
+  ORTHRUS_CHECK_ARG(a.n >= 0 && a.m >= 0 && a.V >= 1 && a.D >= 1 && a.k >= 1 && a.k <= kTopkKlMaxK);
+  ORTHRUS_CHECK_ARG(a.T >= 1e-30f && a.T <= 1e30f);
   ORTHRUS_CHECK_ARG(a.n < (1ll << 31) && a.m < (1ll << 31) && a.V < (1ll << 31) - 256 && a.D < (1ll << 30));
   ORTHRUS_CHECK_ARG(weight && total);
   ORTHRUS_CHECK_ARG(a.n == 0 || (student && a.values && a.ids && a.kl_rows && a.agree && a.m >= 1));

@@ -366,11 +366,11 @@ struct SampleRow {
   int top_k;
   bool greedy;
   __device__ __forceinline__ SampleRow(const SampleKnobs& k, int64_t row)
-      : temperature(k.temperature ? k.temperature[row] : k.temperature1),
+      : temperature(fminf(k.temperature ? k.temperature[row] : k.temperature1, 3e38f)),
         top_p(k.top_p ? k.top_p[row] : k.top_p1),
         min_p(k.min_p ? k.min_p[row] : k.min_p1),
         top_k(k.top_k ? k.top_k[row] : k.top_k1),
-        greedy(temperature < 1e-5f) {}
+        greedy(!((k.temperature ? k.temperature[row] : k.temperature1) >= 1e-5f)) {}
   // whether the slices' weights are asked for: no filter, or a nucleus of the whole row
   __device__ __forceinline__ bool wants_mass() const { return !greedy && top_k < 1 && (top_p < 1.f || !(min_p > 0.f)); }
 };
@@ -718,8 +718,9 @@ __device__ __forceinline__ void row_visit(const RowView<T>& v, F f) {
 
 // Finds, among the candidates with key >= floor_key in descending order of key, the key whose
 // entries hold position `target` of the running measure: the measure (MASS: the sum of weights;
-// otherwise the count) of all larger keys is `before` <= target < before + its own. The caller
-// makes sure that target is below the total. Every thread gets the result.
+// otherwise the count) of all larger keys is `before` <= target < before + its own; 1, less than any
+// candidate's key, if target is not below the total (a mass summed over slices can exceed it by its
+// rounding). Every thread gets the result.
 template <typename T, bool MASS>
 __device__ __noinline__ uint32_t row_radix_select(const RowView<T> v, uint32_t floor_key, uint64_t target,
                                                   const RowWeigher weight, uint64_t& before) {
@@ -737,6 +738,7 @@ __device__ __noinline__ uint32_t row_radix_select(const RowView<T> v, uint32_t f
       if constexpr (MASS) sh.hist[i] = 0;
       else counts[i] = 0;
     }
+    if (threadIdx.x == 0) sh.found[0] = ~0ull;
     __syncthreads();
     row_visit<T>(v, [&](int, uint32_t k) {
       if (k < floor_key || (shift < BITS && (k >> shift) != prefix)) return;
@@ -769,10 +771,12 @@ __device__ __noinline__ uint32_t row_radix_select(const RowView<T> v, uint32_t f
       run += h[j];
     }
     __syncthreads();
-    prefix = (prefix << width) | static_cast<uint32_t>(sh.found[0]);
+    const uint64_t bin = sh.found[0];
+    if (bin == ~0ull) return 1u;
+    prefix = (prefix << width) | static_cast<uint32_t>(bin);
     before = sh.found[1];
     shift = next;
-    __syncthreads();  // found is read before the next level sets it
+    __syncthreads();  // found is read before the next level clears it
   }
   return prefix;
 }
@@ -1244,7 +1248,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
       __syncthreads();
     }
     cut = row_radix_select<T, true>(v, cut, target, weight, before);
-    ties = (target - before) / weight(K::value(cut)) + 1;
+    ties = cut > 1u ? (target - before) / weight(K::value(cut)) + 1 : ~0ull;
   } else if (!filtered && floor_p > 0.f) {
     const int n = row_gather<T>(v.p, V, scan.groups, lowest);
     if (n <= kRowList) {
@@ -1568,7 +1572,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
         __syncthreads();
         uint64_t before;
         const uint32_t cut = row_radix_select<T, true>(v, 1u, r.target, weight, before);
-        const uint64_t ties = (r.target - before) / weight(K::value(cut)) + 1;
+        const uint64_t ties = cut > 1u ? (r.target - before) / weight(K::value(cut)) + 1 : ~0ull;
         row_pick_walk<T>(v, cut, ties, 1u, least, u, weight, tokens + r.row);
         continue;
       }

@@ -357,8 +357,8 @@ def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets
     if values.dim() != 2 or values.shape != ids.shape or not 1 <= values.shape[1] <= LMHEAD_TOPK_MAX_K:
         raise ValueError(f"values and ids must be [m, k] with 1 <= k <= {LMHEAD_TOPK_MAX_K}; got "
                          f"{tuple(values.shape)} and {tuple(ids.shape)}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"lmhead_topk_kl takes a finite temperature > 0 (got {temperature})")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"lmhead_topk_kl takes a temperature from 1e-30 to 1e30 (got {temperature})")
     (n, d), (m, k), V = student.shape, values.shape, weight.shape[0]
     if (index.shape != (n,)) if index is not None else n > m:
         raise ValueError("index must name a teacher row per student row")
@@ -785,8 +785,8 @@ def topk_rows(logits: torch.Tensor, k: int, temperature: float = 1.0):
     R, V, pitch = _vocab_rows(logits, "topk_rows")
     if not 1 <= k <= TOPK_ROWS_MAX_K:
         raise ValueError(f"topk_rows takes 1 <= k <= {TOPK_ROWS_MAX_K} (got {k})")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"topk_rows takes a finite temperature > 0 (got {temperature})")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"topk_rows takes a temperature from 1e-30 to 1e30 (got {temperature})")
     code, dev = L.dtype_code(logits.dtype), logits.device
     values = torch.empty(R, k, dtype=torch.float32, device=dev)
     ids = torch.empty(R, k, dtype=torch.int64, device=dev)
@@ -806,6 +806,8 @@ def _knob(value, name: str, rows: int, device, dtype, low, high):
     if isinstance(value, torch.Tensor):
         if value.shape != (rows,) or value.device != device:
             raise ValueError(f"{name} must be a number or a tensor [{rows}] on {device}")
+        if dtype == torch.int32 and value.dtype == torch.int64:
+            value = value.clamp(0, 2 ** 31 - 1)
         return value.to(dtype).contiguous(), low
     if not low <= value <= high or (name == "top_p" and value == 0):
         raise ValueError(f"{name} = {value} is out of range")
@@ -821,8 +823,9 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     top_p the smallest descending prefix whose probability exceeds it (1: off); min_p the entries
     at least min_p times as probable as the largest (0: off). Each knob is a number or a tensor [R].
     A temperature of 0 (below 1e-5) is greedy. -inf and NaN logits are never drawn; a row of
-    nothing else gives -1. The sums are exact, so a row's token depends on neither the other rows
-    nor the launch."""
+    nothing else gives -1. Weights and sums have 42 or more fractional bits and no order that
+    changes them: a row's token can depend on the other rows or the launch only where its uniform, or
+    top_p, falls within about 2^-40 of a border."""
     R, V, pitch = _vocab_rows(logits, "sample_logits")
     code, dev = L.dtype_code(logits.dtype), logits.device
     if uniforms.shape != (R,) or uniforms.dtype != torch.float32 or uniforms.device != dev:

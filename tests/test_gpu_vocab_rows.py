@@ -281,3 +281,91 @@ def test_refusals():
                   dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=1.1), dict(top_p=u[:1]), dict(min_p=u.cpu())):
         with pytest.raises(ValueError):
             ops.sample_logits(x, u, **knobs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [5003, 151936])
+def test_sample_wide_rows(dtype, V):
+    """Rows that keep thousands of entries: nuclei and min-p at high temperatures, top-k beyond a list."""
+    g = torch.Generator().manual_seed(V + 1)
+    x = _rows("normal", 12, V, dtype, seed=V)
+    x[10, : V // 2] = 1.0  # half a row of equals
+    x[11, 1::2] = -math.inf
+    for T in (1.5, 6.0, 40.0):
+        for f in (dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.9999), dict(min_p=0.001), dict(min_p=0.5),
+                  dict(top_p=0.8, min_p=0.3), dict(top_k=3000), dict(top_k=3000, top_p=0.9, min_p=0.01)):
+            u = torch.rand(12, generator=g).to(DEV)
+            args = dict(dict(temperature=T, top_k=0, top_p=1.0, min_p=0.0), **f)
+            assert torch.equal(_ops().sample_logits(x, u, **args), _sample64(x, u, **args)), (T, f)
+
+
+def test_sample_more_wide_rows_than_have_lists():
+    """Rows past the 2048 wide ones of a call are gone over one by one: the same tokens."""
+    R, V = 2100, 4099
+    x = _rows("normal", R, V, torch.float32)
+    u = torch.rand(R, generator=torch.Generator().manual_seed(3)).to(DEV)
+    args = (4.0, 0, 0.9, 0.0)
+    whole = _ops().sample_logits(x, u, *args)
+    assert torch.equal(whole[:1050], _ops().sample_logits(x[:1050], u[:1050], *args))
+    assert torch.equal(whole[1050:], _ops().sample_logits(x[1050:], u[1050:], *args))
+    assert torch.equal(whole[:20], _sample64(x[:20], u[:20], *args))
+
+
+def test_sample_wide_rows_replay():
+    """The wide rows' launches in a graph: their number is counted anew on every replay."""
+    R, V = 9, 151936
+    x, u = _rows("normal", R, V, torch.float32), torch.rand(R, device=DEV)
+    temperature = torch.full((R,), 3.0, device=DEV)
+    args = (temperature, 0, 0.95, 0.0)
+    _ops().sample_logits(x, u, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        token = _ops().sample_logits(x, u, *args)
+    for seed, sharp in ((1, 0), (2, 4), (3, 9)):  # that many rows are not wide
+        x.copy_(_rows("normal", R, V, torch.float32, seed))
+        temperature.fill_(3.0)[:sharp] = 0.2
+        graph.replay()
+        assert torch.equal(token, _sample64(x, u, *args))
+
+
+def test_sample_tail_of_lost_weights():
+    """A peak over a million entries whose weights round to nothing: a top-p near 1 asks for more than
+    the entries' own weights hold, which keeps them all."""
+    V = 2 ** 20
+    x = torch.full((2, V), -29.9, device=DEV)
+    x[0, 5] = x[1, V - 1] = 0.0
+    p = 1 - 2.0 ** -24
+    got = _ops().sample_logits(x, torch.tensor([0.5, 0.25], device=DEV), 1.0, 0, p, 0.0)
+    assert got.tolist() == [5, V - 1]
+
+
+def test_sample_knobs_beyond_their_ranges():
+    """Per-row knobs are not checked: NaN and low temperatures are greedy, +inf weighs all candidates
+    alike, top-k past 32 bits is off, top-p at or below 0 keeps the first, NaN filters are off."""
+    R, V = 8, 1000
+    x = _rows("normal", R, V, torch.float32)
+    x[1, 10:] = -math.inf
+    u = torch.full((R,), 0.55, device=DEV)
+    nan = math.nan
+    t = torch.tensor([nan, math.inf, -1.0, 1.0, 1.0, 1.0, 1.0, 1.0], device=DEV)
+    k = torch.tensor([0, 0, 0, 2 ** 32 + 1, -2 ** 40, 0, 0, 0], device=DEV)
+    p = torch.tensor([1.0, 1.0, 1.0, 1.0, 1.0, 0.0, -1.0, nan], device=DEV)
+    m = torch.tensor([0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, nan], device=DEV)
+    got = _ops().sample_logits(x, u, t, k, p, m)
+    best = x.argmax(1)
+    off = _ops().sample_logits(x, u)
+    want = [best[0], 5, best[2], off[3], off[4], best[5], best[6], off[7]]
+    assert got.tolist() == [int(w) for w in want]
+
+
+def test_temperature_range():
+    ops = _ops()
+    x = _rows("normal", 2, 50, torch.float32)
+    for t in (1e-31, 1e31):
+        with pytest.raises(ValueError):
+            ops.topk_rows(x, 2, t)
+    for t in (1e-30, 1e30):
+        lse = ops.topk_rows(x, 2, t)[2].double()
+        want = torch.logsumexp(x.double() / t, 1)
+        assert ((lse - want).abs() <= want.abs() * 2 ** -22 + 2 ** -20).all()
