@@ -776,12 +776,29 @@ def block_decode(model, prompts: list[list[int]], max_new_tokens: int, eos=(), *
                              steady_cycles=cycles_run - first_steady)
 
 
+class SampledBackend(ModelBackend):
+    """ModelBackend that draws its tokens from the whole filtered softmax (ops.sample_logits: any
+    top_k, top_p and min_p), with uniforms of torch's generator on the device, seeded by the sampler."""
+
+    def __init__(self, model, prompt_ids: list[int], sampler: ops.SamplingParams):
+        super().__init__(model, prompt_ids)
+        self.sampler = sampler
+        self.generator = torch.Generator(self.device).manual_seed(sampler.seed)
+
+    def _argmax(self, logits: torch.Tensor) -> torch.Tensor:
+        rows = logits.reshape(-1, logits.shape[-1])
+        uniforms = torch.rand(rows.shape[0], device=self.device, generator=self.generator)
+        s = self.sampler
+        return ops.sample_logits(rows, uniforms, s.temperature, s.top_k, s.top_p, s.min_p)
+
+
 @torch.inference_mode()
-def ar_generate_batch(model, input_ids: torch.Tensor, max_new_tokens: int, eos=()):
-    """Plain greedy decoding with the AR view (orthrus/evaluate.py:59-76), batch 1, on the device
-    path: one verification pass of one token per step."""
+def ar_generate_batch(model, input_ids: torch.Tensor, max_new_tokens: int, eos=(),
+                      sampler: ops.SamplingParams | None = None):
+    """Plain decoding with the AR view (orthrus/evaluate.py:59-76), batch 1, on the device path: one
+    verification pass of one token per step. Greedy, or with a sampler one draw per step."""
     eos = {eos} if isinstance(eos, int) else set(eos or ())
     prompt = input_ids[0].tolist()
-    backend = ModelBackend(model, prompt)
+    backend = ModelBackend(model, prompt) if sampler is None else SampledBackend(model, prompt, sampler)
     gen = ar_decode(backend, len(prompt), max_new_tokens, eos)
     return torch.tensor([prompt + gen.tokens], device=input_ids.device)

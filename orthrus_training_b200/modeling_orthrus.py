@@ -672,14 +672,18 @@ class OrthrusLM(nn.Module):
 
     @torch.inference_mode()
     def generate(self, input_ids, max_new_tokens=None, max_length=None, temperature=0.0, top_k=20,
-                 top_p=0.8, eos_token_id=None, streamer=None, use_diffusion_mode=True, **kwargs):
-        """OrthrusLM.generate (orthrus/modeling_orthrus.py:364-402), greedy."""
+                 top_p=0.8, eos_token_id=None, streamer=None, use_diffusion_mode=True, sampler=None, **kwargs):
+        """OrthrusLM.generate (orthrus/modeling_orthrus.py:364-402), greedy. Without the diffusion mode
+        the AR view alone decodes; a sampler (ops.SamplingParams) then draws its tokens from the whole
+        filtered softmax (any top_k, 0 for none; top_p; min_p) at the sampler's temperature and seed."""
         eos_token_id = eos_token_id if eos_token_id is not None else self.config.eos_token_id
         max_new_tokens = max_new_tokens or (max_length - input_ids.shape[1])
+        if sampler is not None and use_diffusion_mode:
+            raise ValueError("a sampler is for generation without the diffusion mode (use_diffusion_mode=False)")
         if not use_diffusion_mode:
             from orthrus_training_b200.decoding import ar_generate_batch
 
-            return ar_generate_batch(self, input_ids, max_new_tokens, eos_token_id)
+            return ar_generate_batch(self, input_ids, max_new_tokens, eos_token_id, sampler)
         output, _ = self.diffusion_generate(input_ids, max_new_tokens, temperature=temperature,
                                             top_k=top_k, top_p=top_p, eos_token_id=eos_token_id,
                                             streamer=streamer)

@@ -668,12 +668,14 @@ SAMPLE_MAX_TOP_K = 112  # top_k of the device sampler (candidates: top_k + 16 sp
 @dataclass(frozen=True)
 class SamplingParams:
     """The sampling knobs of diffusion_generate (orthrus/modeling_orthrus.py:405-449) and the seed
-    of the decode's Philox draws."""
+    of the decode's Philox draws. min_p (and a top_k of 0 or beyond the candidates) only for draws
+    from whole rows, sample_logits'."""
 
     temperature: float
     top_k: int = 20
     top_p: float = 0.8
     seed: int = 0
+    min_p: float = 0.0
 
     def candidates(self, vocab: int) -> int:
         """C: the top-k candidates kept per row, plus spares for ties at the k-th value."""
@@ -683,6 +685,8 @@ class SamplingParams:
             raise ValueError(f"the device sampler takes 1 <= top_k <= {SAMPLE_MAX_TOP_K} (got {self.top_k})")
         if not 0 < self.top_p <= 1:
             raise ValueError("top_p must be in (0, 1]")
+        if self.min_p != 0:
+            raise ValueError("the candidates' sampler has no min_p")
         k = min(self.top_k, vocab)
         return min(k + 16, vocab, 128)
 

@@ -369,3 +369,48 @@ def test_temperature_range():
         lse = ops.topk_rows(x, 2, t)[2].double()
         want = torch.logsumexp(x.double() / t, 1)
         assert ((lse - want).abs() <= want.abs() * 2 ** -22 + 2 ** -20).all()
+
+
+def _small_model():
+    from transformers import Qwen3Config
+
+    from orthrus_training_b200.modeling_orthrus import OrthrusLM, copy_diff_from_ar
+
+    cfg = Qwen3Config(vocab_size=1009, hidden_size=128, intermediate_size=256, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, head_dim=32, rms_norm_eps=1e-6,
+                      rope_theta=1e4, tie_word_embeddings=True, max_position_embeddings=512)
+    cfg.rope_parameters = {"rope_theta": 1e4, "rope_type": "default"}
+    cfg.block_size, cfg.mask_token_id = 8, 1008
+    torch.manual_seed(0)
+    with torch.device(DEV):
+        model = OrthrusLM(cfg)
+    copy_diff_from_ar(model)
+    return model
+
+
+def test_generate_draws_with_sample_logits():
+    """The AR view's sampled generation: each token is the draw from the logits of the sequence up to
+    it, the same seed gives the same tokens, and top_k = 1 decodes greedily."""
+    ops = _ops()
+    model = _small_model()
+    prompt = torch.randint(0, 1000, (1, 9), generator=torch.Generator().manual_seed(1)).to(DEV)
+    sampler = ops.SamplingParams(0.9, top_k=0, top_p=0.97, seed=11, min_p=0.01)
+    out = model.generate(prompt, max_new_tokens=12, use_diffusion_mode=False, sampler=sampler)
+    assert torch.equal(out, model.generate(prompt, max_new_tokens=12, use_diffusion_mode=False, sampler=sampler))
+    assert out.shape == (1, 21) and torch.equal(out[:, :9], prompt)
+    g = torch.Generator(DEV).manual_seed(11)
+    for i in range(9, 21):
+        with torch.inference_mode():
+            logits = model(input_ids=out[:, :i], use_cache=False).logits[0, -1:]
+        u = torch.rand(1, device=DEV, generator=g)
+        w = torch.softmax(logits[0].double() / 0.9, 0)
+        token = ops.sample_logits(logits.float().contiguous(), u, 0.9, 0, 0.97, 0.01)
+        assert token.item() == out[0, i].item() and w[token.item()] >= 0.01 * w.max()
+    greedy = model.generate(prompt, max_new_tokens=12, use_diffusion_mode=False)
+    one = model.generate(prompt, max_new_tokens=12, use_diffusion_mode=False,
+                         sampler=ops.SamplingParams(1.0, top_k=1, top_p=1.0, seed=3))
+    assert torch.equal(one, greedy)
+    with pytest.raises(ValueError):
+        model.generate(prompt, max_new_tokens=4, sampler=sampler)
+    with pytest.raises(ValueError):
+        ops.sample_candidates(torch.zeros(1, 1009, device=DEV), ops.SamplingParams(1.0, min_p=0.1))
