@@ -31,7 +31,7 @@
 #pragma once
 
 #include "gemm2_tc.cuh"
-#include "gemm_simt.cuh"
+#include "gemm_f32.cuh"
 #include "lmhead_kl.cuh"
 
 namespace orthrus {
@@ -766,7 +766,8 @@ inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64
     p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 12);
     p.off_scale = take(static_cast<size_t>(p.chunk) * 4);
   } else {
-    p.gemm_bytes = std::max(simt_ws_bytes(p.chunk, V, D), simt_ws_bytes(p.chunk, D, V));
+    for (int64_t rows : {std::min(n, p.chunk), n % p.chunk})  // a short last chunk may split deeper
+      if (rows > 0) p.gemm_bytes = std::max({p.gemm_bytes, f32_plan(rows, V, D).bytes, f32_plan(rows, D, V).bytes});
   }
   p.off_gemm = take(p.gemm_bytes);
   p.total = off;
@@ -791,15 +792,14 @@ inline int topk_kl_rows_f32(const TopkKlCall& a, const TopkKlPlan& p, const floa
   void* gws = ws + p.off_gemm;
   for (int64_t c0 = 0; c0 < a.n; c0 += p.chunk) {
     const int64_t rows = std::min<int64_t>(p.chunk, a.n - c0);
-    int rc = gemm_simt_impl<float, false>(student + c0 * a.D, a.D, W, a.D, buf, p.Vp, rows, a.V, a.D, gws, p.gemm_bytes,
-                                          stream);
+    int rc = f32_product<false>(student + c0 * a.D, a.D, W, a.D, buf, p.Vp, rows, a.V, a.D, gws, p.gemm_bytes, stream);
     if (rc != ORTHRUS_OK) return rc;
     topk_kl_rows_kernel<float><<<static_cast<unsigned>(rows), kTopkKlThreads, 0, stream>>>(
         buf, p.Vp, static_cast<int>(c0), static_cast<int>(a.V), a.values, a.ids, a.k, a.m, a.index, a.teacher_lse,
         a.row_weight, a.T, a.kl_rows, a.agree, grad ? buf : nullptr, p.Vp);
     ORTHRUS_CHECK_LAUNCH();
     if (grad == nullptr) continue;
-    rc = gemm_simt_impl<float, true>(buf, p.Vp, W, a.D, grad + c0 * a.D, a.D, rows, a.D, a.V, gws, p.gemm_bytes, stream);
+    rc = f32_product<true>(buf, p.Vp, W, a.D, grad + c0 * a.D, a.D, rows, a.D, a.V, gws, p.gemm_bytes, stream);
     if (rc != ORTHRUS_OK) return rc;
   }
   return ORTHRUS_OK;
