@@ -93,6 +93,25 @@ __device__ __noinline__ uint32_t row_key_at(const T* p, int V, int i) {
     return RowKey<T>::of_bits(__ldg(reinterpret_cast<const uint16_t*>(p) + i));
 }
 
+// The 16 bytes of a block that is not all within the row, with -inf outside it. Out of line, as above.
+template <typename T>
+__device__ __noinline__ uint4 row_raw_edge(const T* p, int V, int first) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      const int i = first + e;
+      w[e] = i < 0 || i >= V ? 0xFF800000u : __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    } else {
+      const int i = first + 2 * e;
+      const uint32_t a = i < 0 || i >= V ? 0xFF80u : __ldg(reinterpret_cast<const uint16_t*>(p) + i);
+      const uint32_t b = i + 1 < 0 || i + 1 >= V ? 0xFF80u : __ldg(reinterpret_cast<const uint16_t*>(p) + i + 1);
+      w[e] = a | b << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Block b of a row of any alignment covers the entries b * VEC - off .. + VEC - 1, where off is the
 // row's distance in entries from the 16-byte boundary before it; entries outside the row count as no
 // candidates and are never read.
@@ -109,6 +128,12 @@ struct RowView {
   __device__ __forceinline__ int first(int b) const { return b * VEC - off; }
   __device__ __forceinline__ bool whole(int b) const { return first(b) >= 0 && first(b) + VEC <= V; }
   __device__ __forceinline__ uint4 load(int b) const { return __ldg(reinterpret_cast<const uint4*>(p + first(b))); }
+  // block b as it is in memory, -inf outside the row
+  __device__ __forceinline__ uint4 raw(int b) const {
+    if (b < blocks) return whole(b) ? load(b) : row_raw_edge<T>(p, V, first(b));
+    constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+    return make_uint4(none, none, none, none);
+  }
   // the keys of a block loaded as 16 bytes
   __device__ __forceinline__ static void keys_of(const uint4& q, uint32_t (&k)[VEC]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -583,29 +608,6 @@ __device__ __forceinline__ void row_append(bool take, E entry, E* list, uint32_t
   if (take && at < kRowList) list[at] = entry;
 }
 
-// The same for the keys at or above `low` of each lane's block, whose first entry has index `first`.
-template <int VEC>
-__device__ __forceinline__ void row_append_block(const uint32_t (&k)[VEC], uint32_t low, int first, uint64_t* list,
-                                                 uint32_t* count) {
-  const uint32_t below = (1u << (threadIdx.x & 31)) - 1u;
-  uint32_t who[VEC], total = 0;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    who[e] = __ballot_sync(0xffffffffu, k[e] >= low);
-    total += __popc(who[e]);
-  }
-  if (total == 0) return;
-  uint32_t at = 0;
-  if ((threadIdx.x & 31) == 0) at = atomicAdd(count, total);
-  at = __shfl_sync(0xffffffffu, at, 0);
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const uint32_t mine = at + __popc(who[e] & below);
-    if (k[e] >= low && mine < kRowList) list[mine] = (static_cast<uint64_t>(k[e]) << 32) | ~static_cast<uint32_t>(first + e);
-    at += __popc(who[e]);
-  }
-}
-
 // Reads the groups at or above `low` again and lists their entries with low <= key; returns their
 // number, or more than kRowList if they do not fit. Ends with a barrier; listed is left at 0.
 template <typename T>
@@ -613,36 +615,53 @@ __device__ __noinline__ int row_gather(const T* row, int V, int groups, uint32_t
   RowScratch& sh = row_scratch();
   const uint32_t* maxima = row_maxima();
   const RowView<T> v(row, V);
-  constexpr int VEC = RowView<T>::VEC, LANES = kRowGroup / VEC;
+  constexpr int LANES = kRowGroup / RowView<T>::VEC;
   const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
-    const uint4 q = reinterpret_cast<const uint4*>(maxima)[i];
-    if (max(max(q.x, q.y), max(q.z, q.w)) < low) continue;
-    const uint32_t m[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (m[e] >= low) {
-        const uint32_t at = atomicAdd(&sh.ngroups, 1u);
-        if (at < kRowList) sh.groups[at] = 4 * i + e;
-      }
+  // each thread marks its groups, 32 at a time, and takes their places with one atomic
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < groups / 4; i0 += 8 * kRowThreads) {
+    uint32_t mine = 0;
+#pragma unroll 1
+    for (int j = 0; j < 8 && i0 + j * kRowThreads < groups / 4; ++j) {
+      const uint4 q = reinterpret_cast<const uint4*>(maxima)[i0 + j * kRowThreads];
+      mine |= ((q.x >= low) | (q.y >= low) << 1 | (q.z >= low) << 2 | (q.w >= low) << 3) << (4 * j);
+    }
+    uint32_t at = mine ? atomicAdd(&sh.ngroups, static_cast<uint32_t>(__popc(mine))) : 0u;
+#pragma unroll 1
+    for (; mine; mine &= mine - 1, ++at) {
+      const int bit = __ffs(mine) - 1;
+      if (at < kRowList) sh.groups[at] = 4 * (i0 + bit / 4 * kRowThreads) + bit % 4;
+    }
   }
   __syncthreads();
   const int ng = static_cast<int>(sh.ngroups);  // every group holds at least one entry
-  // LANES neighbouring lanes a group, the next load ahead of the one in hand
+  // LANES neighbouring lanes a group, four loads ahead; each thread marks its entries and takes their places
+  // with one atomic. Values compare as their keys do from the lowest number up.
   if (ng <= kRowList) {
+    using K = RowKey<T>;
+    constexpr int AHEAD = 4, STEP = kRowThreads / LANES, VEC = RowView<T>::VEC;
+    const float least = K::value(max(low, 0x00800000u >> (32 - K::BITS)));
     auto block = [&](int i) { return i < ng ? static_cast<int>(sh.groups[i]) * LANES + lane % LANES : v.blocks; };
-    int i = static_cast<int>(threadIdx.x) / LANES, b = block(i);
-    uint32_t k[VEC], next[VEC];
-    v.keys(b, k);
 #pragma unroll 1
-    for (int i0 = 0; i0 < ng; i0 += kRowThreads / LANES) {
-      const int bn = block(i += kRowThreads / LANES);
-      v.keys(bn, next);
-      __syncwarp();
-      row_append_block<VEC>(k, low, v.first(b), sh.list, &sh.listed);
-      b = bn;
+    for (int i0 = static_cast<int>(threadIdx.x) / LANES; i0 < ng; i0 += AHEAD * STEP) {
+      uint4 q[AHEAD];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) k[e] = next[e];
+      for (int j = 0; j < AHEAD; ++j) q[j] = v.raw(block(i0 + j * STEP));
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        float x[VEC];
+        RowView<T>::values_of(q[j], x);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) mine |= static_cast<uint32_t>(x[e] >= least) << (j * VEC + e);
+      }
+      uint32_t at = mine ? atomicAdd(&sh.listed, static_cast<uint32_t>(__popc(mine))) : 0u;
+#pragma unroll 1
+      for (; mine; mine &= mine - 1, ++at) {
+        const int bit = __ffs(mine) - 1;
+        const int i = v.first(block(i0 + bit / VEC * STEP)) + bit % VEC;
+        if (at < kRowList) sh.list[at] = (static_cast<uint64_t>(v.key(i)) << 32) | ~static_cast<uint32_t>(i);
+      }
     }
   }
   __syncthreads();
@@ -1478,7 +1497,8 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     const SampleRow knob(knobs, r.row);
     const RowWeigher weight{row_weight(r.top, knob.temperature, S)};
     const uint64_t least = row_least(knob.min_p, S);
-    const float u = uniform[r.row];
+    const float u = uniform[r.row], lo = r.lo;
+    const uint64_t border_at = r.target;
     uint64_t total;
     RowSums own{0, 0, 0};
     if (static_cast<int>(threadIdx.x) < slices) own = wide.sums[static_cast<int64_t>(slot) * slices + threadIdx.x];
@@ -1508,10 +1528,10 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     };
     if (r.nucleus) {
       const uint64_t above = block_sum_u64(own.above);
-      bool ok = !__syncthreads_or(own.listed > static_cast<uint32_t>(wide.room)) && above <= r.target;
+      bool ok = !__syncthreads_or(own.listed > static_cast<uint32_t>(wide.room)) && above <= border_at;
       if (ok) {
         // weights in 2048 bins even in x, the bin that holds the target, its entries in order
-        const float xhi = fminf(r.hi, r.top), inv = static_cast<float>(kRowBins) / fmaxf(xhi - r.lo, 1e-30f);
+        const float xhi = fminf(r.hi, r.top), inv = static_cast<float>(kRowBins) / fmaxf(xhi - lo, 1e-30f);
         auto bin = [&](float x) { return min(kRowBins - 1, max(0, static_cast<int>((xhi - x) * inv))); };
         each(
             [&](uint64_t e) {
@@ -1528,7 +1548,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
         uint64_t run = above + block_exclusive_u64(sum, total);
 #pragma unroll
         for (int j = 0; j < BINS; ++j) {
-          if (run <= r.target && r.target < run + h[j]) {
+          if (run <= border_at && border_at < run + h[j]) {
             sh.found[0] = threadIdx.x * BINS + j;
             sh.found[1] = run;
           }
@@ -1560,7 +1580,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
             run = before + block_exclusive_u64(mine, total);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-              if (run <= r.target && r.target < run + w[j]) sh.found[0] = sh.sorted[threadIdx.x * PER + j];
+              if (run <= border_at && border_at < run + w[j]) sh.found[0] = sh.sorted[threadIdx.x * PER + j];
               run += w[j];
             }
             __syncthreads();
@@ -1571,8 +1591,8 @@ __global__ void __launch_bounds__(kRowThreads, 4)
       if (!ok) {  // the border is not in the window, or the window holds too much: the whole row
         __syncthreads();
         uint64_t before;
-        const uint32_t cut = row_radix_select<T, true>(v, 1u, r.target, weight, before);
-        const uint64_t ties = cut > 1u ? (r.target - before) / weight(K::value(cut)) + 1 : ~0ull;
+        const uint32_t cut = row_radix_select<T, true>(v, 1u, border_at, weight, before);
+        const uint64_t ties = cut > 1u ? (border_at - before) / weight(K::value(cut)) + 1 : ~0ull;
         row_pick_walk<T>(v, cut, ties, 1u, least, u, weight, tokens + r.row);
         continue;
       }
@@ -1601,30 +1621,54 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     __syncthreads();
     const int b0 = static_cast<int>(sh.found[0]) * SLICE;
     const uint64_t rest = sh.found[1];
-    // the slice, a thread its neighbouring blocks
+    // The slice, a thread its neighbouring blocks, staged in the list's and the histogram's memory. (Loops
+    // that stay loops: unrolled code runs once here, at the speed of its instructions' fetches.)
     constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;
-    uint64_t sum = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-      uint64_t at = pass ? block_exclusive_u64(sum, total) : 0;
-      if (pass && !(at <= rest && rest < at + sum)) break;
+    static_assert(SLICE * 16 <= static_cast<int>(sizeof(sh.list) + sizeof(sh.hist)) && (PER & (PER - 1)) == 0 && PER * VEC <= 32, "");
+    auto place = [&](int thread, int j) {  // the exchange keeps a warp's 16-byte accesses off one another's banks
+      const int at = thread * PER + (j ^ (thread % PER));
+      return at < kRowList / 2 ? reinterpret_cast<uint4*>(sh.list) + at : reinterpret_cast<uint4*>(sh.hist) + at - kRowList / 2;
+    };
+    const int t = threadIdx.x;
+    if (t * PER < SLICE)
+#pragma unroll 4
+      for (int j = 0; j < PER; ++j) *place(t, j) = v.raw(b0 + t * PER + j);
+    uint32_t some = 0;  // the thread's entries at or above lo
+    if (t * PER < SLICE)
 #pragma unroll 1
       for (int j = 0; j < PER; ++j) {
-        const int k = threadIdx.x * PER + j;
         float xs[VEC];
-        v.values(k < SLICE ? b0 + k : v.blocks, xs);
+        RowView<T>::values_of(*place(t, j), xs);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          if (!(xs[e] >= r.lo)) continue;
-          const uint32_t i = v.first(b0 + k) + e;
-          if (((static_cast<uint64_t>(K::of(xs[e])) << 32) | ~i) < border) continue;
-          uint64_t w = weight(xs[e]);
-          w = w >= least ? w : 0;
-          if (pass && at <= rest && rest < at + w) tokens[r.row] = i;
-          at += w;
-        }
+        for (int e = 0; e < VEC; ++e) some |= static_cast<uint32_t>(xs[e] >= lo) << (j * VEC + e);
       }
-      if (!pass) sum = at;
+    auto kept = [&](int thread, int e) -> uint64_t {  // weight of a thread's e-th entry if it is kept
+      const T x = reinterpret_cast<const T*>(place(thread, e / VEC))[e % VEC];
+      const float xe = fmaxf(static_cast<float>(x), -INFINITY);
+      const uint32_t i = v.first(b0 + thread * PER) + e;
+      if (!(xe >= lo) || ((static_cast<uint64_t>(K::of(xe)) << 32) | ~i) < border) return 0;
+      const uint64_t w = weight(xe);
+      return w >= least ? w : 0;
+    };
+    uint64_t sum = 0;
+#pragma unroll 1
+    for (; some; some &= some - 1) sum += kept(t, __ffs(some) - 1);
+    const uint64_t at = block_exclusive_u64(sum, total);
+    if (at <= rest && rest < at + sum) {
+      sh.found[0] = t;
+      sh.found[1] = rest - at;
+    }
+    __syncthreads();
+    if (warp == 0) {  // that thread's entries, one a lane
+      const int owner = static_cast<int>(sh.found[0]);
+      const uint64_t w = lane < PER * VEC ? kept(owner, lane) : 0;
+      uint64_t inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      if (inc - w <= sh.found[1] && sh.found[1] < inc) tokens[r.row] = v.first(b0 + owner * PER) + lane;
     }
   }
 }
