@@ -918,11 +918,11 @@ extern "C" int orthrus_swiglu_bwd(const void* gate_up, const void* dout, int64_t
 // ------------------------------------------------------------------------------------------------
 
 extern "C" size_t orthrus_topk_rows_workspace_bytes(int64_t R, int64_t V, int dtype) {
-  return R < 1 || V < 1 || V > kRowMaxV ? 0 : row_ws_bytes(R, V, dtype == ORTHRUS_BF16 ? 2 : 4, false);
+  return R < 1 || V < 1 || V > kRowMaxV ? 0 : row_ws_bytes(R, V, dtype == ORTHRUS_BF16 ? 2 : 4, false, false);
 }
 
 extern "C" size_t orthrus_sample_logits_workspace_bytes(int64_t R, int64_t V, int filters, int dtype) {
-  return R < 1 || V < 1 || V > kRowMaxV ? 0 : row_ws_bytes(R, V, dtype == ORTHRUS_BF16 ? 2 : 4, filters != 0);
+  return R < 1 || V < 1 || V > kRowMaxV ? 0 : row_ws_bytes(R, V, dtype == ORTHRUS_BF16 ? 2 : 4, true, filters != 0);
 }
 
 extern "C" int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,

@@ -6,8 +6,12 @@
 // and goes through K in chunks of 16: the next chunk's elements are loaded into registers while this one's
 // are multiplied out of shared memory (two buffers, one barrier a chunk). The larger the tile the
 // fewer shared-memory reads a product takes (2 R for R^2); the smaller, the more SMs a small problem
-// fills, so R is the largest of 8, 4 and 2 that leaves no SM without a tile, counting parts of K of 128 or
-// more, which are summed in order by a second launch. Measured: see f32_plan.
+// fills, so R is the largest of 8, 4 and 2 with a tile for three SMs in four, counting parts of K of 128 or
+// more, which are summed in order by a second launch. Measured, us for the logits / the gradient with R =
+// 2, 4 and 8: 90 x 1024 x 256: 10 / 12, 13 / 14, 24 / 25; 300 x 4000 x 256: 43 / 119, 33 / 41, 37 / 35;
+// 600 x 8000 x 512: 289 / 426, 171 / 458, 193 / 156 (32 TFLOP/s); 2000 x 32000 x 1024: 7287 / 7319,
+// 3947 / 4776, 3506 / 4015 (37 and 33 TFLOP/s). What bounds the large ones is
+// the issue of FMAs beside one vector load of shared memory per 16.
 #pragma once
 
 #include "host_common.h"
@@ -109,7 +113,7 @@ inline F32Plan f32_plan(int64_t M, int64_t N, int64_t K) {
     p.tiles_m = ceil_div(M, 16 * p.R);
     p.tiles = p.tiles_m * ceil_div(N, 16 * p.R);
     p.splits = static_cast<int>(std::max<int64_t>(1, std::min(K / 128, num_sms() / p.tiles)));
-    if (p.R == 2 || p.tiles * p.splits * 2 > num_sms()) break;
+    if (p.R == 2 || p.tiles * p.splits * 4 >= 3 * num_sms()) break;
   }
   p.per_split = static_cast<int>(ceil_div(ceil_div(K, p.splits), kF32Chunk) * kF32Chunk);
   p.splits = static_cast<int>(ceil_div(K, p.per_split));

@@ -1091,6 +1091,56 @@ __device__ void row_pick_walk(const RowView<T>& v, uint32_t cut, uint64_t ties, 
   });
 }
 
+// A slice's values staged in the list's and the histogram's memory, a thread's blocks neighbours. What
+// goes over them are loops that stay loops: unrolled code would run once, at the speed of its
+// instructions' fetches.
+template <typename T, int BLOCKS>
+struct RowStage {
+  static constexpr int VEC = RowView<T>::VEC, SLICE = BLOCKS * kScanThreads;
+  static constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;  // blocks of a thread
+  static constexpr int ENTRIES = PER * VEC;
+  static_assert(SLICE * 16 <= static_cast<int>(sizeof(RowScratch::list) + sizeof(RowScratch::hist)) &&
+                (PER & (PER - 1)) == 0 && ENTRIES <= 32 && SLICE % kRowThreads == 0, "");
+  // block j of a thread; the exchange keeps a warp's 16-byte accesses off one another's banks
+  __device__ static __forceinline__ uint4* place(int thread, int j) {
+    RowScratch& sh = row_scratch();
+    const int at = thread * PER + (j ^ (thread % PER));
+    return at < kRowList / 2 ? reinterpret_cast<uint4*>(sh.list) + at : reinterpret_cast<uint4*>(sh.hist) + at - kRowList / 2;
+  }
+  __device__ static __forceinline__ void fill(const RowView<T>& v, int b0) {
+#pragma unroll 4
+    for (int j = 0; j < PER; ++j) *place(threadIdx.x, j) = v.raw(b0 + static_cast<int>(threadIdx.x) * PER + j);
+  }
+  __device__ static __forceinline__ float value(int thread, int e) {
+    return fmaxf(static_cast<float>(reinterpret_cast<const T*>(place(thread, e / VEC))[e % VEC]), -INFINITY);
+  }
+  // The index of the entry in which `aim` falls, given each thread's sum of weights w(thread, e); -1 where aim
+  // is not below their total. For the lanes of warp 0; the others get -1.
+  template <typename W>
+  __device__ static __forceinline__ int find(const RowView<T>& v, int b0, uint64_t sum, uint64_t aim, W w) {
+    RowScratch& sh = row_scratch();
+    const int lane = threadIdx.x & 31;
+    uint64_t total;
+    const uint64_t at = block_exclusive_u64(sum, total);
+    if (at <= aim && aim < at + sum) {
+      sh.found[0] = threadIdx.x;
+      sh.found[1] = aim - at;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32 || aim >= total) return -1;
+    const int owner = static_cast<int>(sh.found[0]);  // its entries, one a lane
+    const uint64_t rest = sh.found[1], own = lane < ENTRIES ? w(owner, lane) : 0;
+    uint64_t inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, inc - own <= rest && rest < inc);
+    return v.first(b0 + owner * PER) + __ffs(who) - 1;
+  }
+};
+
 // Picks the token of an unfiltered row from the slices' weights: the slice that holds the uniform's
 // share, and in it the entry, by the slice's own weights.
 template <typename T, int BLOCKS>
@@ -1099,7 +1149,8 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
                                int64_t* __restrict__ token) {
   RowScratch& sh = row_scratch();
   using K = RowKey<T>;
-  constexpr int VEC = RowView<T>::VEC, SLICE = BLOCKS * kScanThreads;
+  using View = RowView<T>;
+  constexpr int VEC = View::VEC, SLICE = BLOCKS * kScanThreads;
   RowSlice a{0u, 0u, 0ull};
   uint64_t own = 0, total;
   if (static_cast<int>(threadIdx.x) < scan.slices) {
@@ -1121,32 +1172,20 @@ __device__ void row_pick_slice(const RowView<T>& v, const RowScan& scan, int64_t
   const RowWeigher local{row_weight(K::value(static_cast<uint32_t>(sh.found[0] >> 32)), temperature, weight.S)};
   const int b0 = static_cast<int>(sh.found[0] & 0xFFFFFFFFu) * SLICE;
   aim = sh.found[1];
-  constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;  // blocks of a thread, neighbours
-  uint32_t key[PER][VEC];
-  uint64_t mine = 0;
+  __syncthreads();  // found is read
+  using Stage = RowStage<T, BLOCKS>;
+  Stage::fill(v, b0);
+  const RowWeight inline_local{local.top, local.floor, local.S, local.from, local.scale};
+  uint64_t sum = 0;
+#pragma unroll 1
+  for (int j = 0; j < Stage::PER; ++j) {
+    float x[VEC];
+    View::values_of(*Stage::place(threadIdx.x, j), x);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int at = threadIdx.x * PER + j;
-    if (at < SLICE) {
-      v.keys(b0 + at, key[j]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) key[j][e] = 0u;
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (key[j][e]) mine += local(K::value(key[j][e]));
+    for (int e = 0; e < VEC; ++e) sum += inline_local(x[e]);
   }
-  uint64_t at = block_exclusive_u64(mine, total);
-  if (at <= aim && aim < at + mine)
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint64_t w = key[j][e] ? local(K::value(key[j][e])) : 0;
-        if (at <= aim && aim < at + w) *token = v.first(b0 + threadIdx.x * PER + j) + e;
-        at += w;
-      }
+  const int i = Stage::find(v, b0, sum, aim, [&](int thread, int e) { return local(Stage::value(thread, e)); });
+  if (threadIdx.x == 0 && i >= 0) *token = i;
 }
 
 template <typename T, int BLOCKS>
@@ -1621,55 +1660,29 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     __syncthreads();
     const int b0 = static_cast<int>(sh.found[0]) * SLICE;
     const uint64_t rest = sh.found[1];
-    // The slice, a thread its neighbouring blocks, staged in the list's and the histogram's memory. (Loops
-    // that stay loops: unrolled code runs once here, at the speed of its instructions' fetches.)
-    constexpr int PER = SLICE > kRowThreads ? SLICE / kRowThreads : 1;
-    static_assert(SLICE * 16 <= static_cast<int>(sizeof(sh.list) + sizeof(sh.hist)) && (PER & (PER - 1)) == 0 && PER * VEC <= 32, "");
-    auto place = [&](int thread, int j) {  // the exchange keeps a warp's 16-byte accesses off one another's banks
-      const int at = thread * PER + (j ^ (thread % PER));
-      return at < kRowList / 2 ? reinterpret_cast<uint4*>(sh.list) + at : reinterpret_cast<uint4*>(sh.hist) + at - kRowList / 2;
-    };
-    const int t = threadIdx.x;
-    if (t * PER < SLICE)
-#pragma unroll 4
-      for (int j = 0; j < PER; ++j) *place(t, j) = v.raw(b0 + t * PER + j);
+    __syncthreads();
+    using Stage = RowStage<T, BLOCKS>;
+    Stage::fill(v, b0);
     uint32_t some = 0;  // the thread's entries at or above lo
-    if (t * PER < SLICE)
 #pragma unroll 1
-      for (int j = 0; j < PER; ++j) {
-        float xs[VEC];
-        RowView<T>::values_of(*place(t, j), xs);
+    for (int j = 0; j < Stage::PER; ++j) {
+      float xs[VEC];
+      RowView<T>::values_of(*Stage::place(threadIdx.x, j), xs);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) some |= static_cast<uint32_t>(xs[e] >= lo) << (j * VEC + e);
-      }
+      for (int e = 0; e < VEC; ++e) some |= static_cast<uint32_t>(xs[e] >= lo) << (j * VEC + e);
+    }
     auto kept = [&](int thread, int e) -> uint64_t {  // weight of a thread's e-th entry if it is kept
-      const T x = reinterpret_cast<const T*>(place(thread, e / VEC))[e % VEC];
-      const float xe = fmaxf(static_cast<float>(x), -INFINITY);
-      const uint32_t i = v.first(b0 + thread * PER) + e;
+      const float xe = Stage::value(thread, e);
+      const uint32_t i = v.first(b0 + thread * Stage::PER) + e;
       if (!(xe >= lo) || ((static_cast<uint64_t>(K::of(xe)) << 32) | ~i) < border) return 0;
       const uint64_t w = weight(xe);
       return w >= least ? w : 0;
     };
     uint64_t sum = 0;
 #pragma unroll 1
-    for (; some; some &= some - 1) sum += kept(t, __ffs(some) - 1);
-    const uint64_t at = block_exclusive_u64(sum, total);
-    if (at <= rest && rest < at + sum) {
-      sh.found[0] = t;
-      sh.found[1] = rest - at;
-    }
-    __syncthreads();
-    if (warp == 0) {  // that thread's entries, one a lane
-      const int owner = static_cast<int>(sh.found[0]);
-      const uint64_t w = lane < PER * VEC ? kept(owner, lane) : 0;
-      uint64_t inc = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-      }
-      if (inc - w <= sh.found[1] && sh.found[1] < inc) tokens[r.row] = v.first(b0 + owner * PER) + lane;
-    }
+    for (; some; some &= some - 1) sum += kept(threadIdx.x, __ffs(some) - 1);
+    const int i = Stage::find(v, b0, sum, rest, kept);
+    if (threadIdx.x == 0) tokens[r.row] = i;
   }
 }
 
@@ -1683,13 +1696,18 @@ struct RowPlan {
   size_t off_slice, off_count, off_rows, off_sums, off_lists, total;
 };
 
-// Slices of 8192 entries, 32 a thread in flight; of 2048 where that leaves SMs without a slice (a
-// few rows). `aligned`: every row starts on a 16-byte boundary. `wide`: rows can turn out wide.
-inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned, bool wide) {
+// Slices of 8192 entries, 32 a thread in flight, or of 2048 where those would leave SMs idle. (Top-64 of V =
+// 151936 fp32, us with slices of 8192 / 2048: 1 row 13.3 / 12.3, 16 rows 16.5 / 16.5, 64 rows 20.7 /
+// 22.8.) Sampling weighs each entry in fp64, which small slices spread better, and the finish weighs one
+// slice again: without filters that need more, 2048 up to some 120 such rows (1 row 16.5 / 10.3, 64 rows
+// 41.2 / 34.9, 128 rows 57.9 / 55.4, 256 rows 94.3 / 100.4); wide rows cost launches' work per slice
+// (top-p 0.95, 64 rows: 124 / 139, 256 rows: 251 / 324). `aligned`: every row starts on a 16-byte
+// boundary. `wide`: rows can turn out wide.
+inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned, bool sample, bool wide) {
   RowPlan p{};
   const int vec = 16 / elem;
   p.groups = static_cast<int>(ceil_div(V + (aligned ? 0 : vec - 1), 4 * kRowGroup)) * 4;
-  const bool small = R * ceil_div(V, 8192) < 2 * num_sms() && V <= (1 << 18);
+  const bool small = R * ceil_div(V, 8192) < (sample && !wide ? 16 : 2) * num_sms() && V <= (1 << 18);
   p.blocks = (small ? 2048 : 8192) / vec / kScanThreads;
   p.slices = static_cast<int>(ceil_div(static_cast<int64_t>(p.groups) * kRowGroup, static_cast<int64_t>(p.blocks) * kScanThreads * vec));
   p.wide = wide ? static_cast<int>(std::min<int64_t>(R, kRowWideRows)) : 0;
@@ -1711,8 +1729,8 @@ inline RowPlan row_plan(int64_t R, int64_t V, int elem, bool aligned, bool wide)
 }
 
 // Bytes that do for any alignment.
-inline size_t row_ws_bytes(int64_t R, int64_t V, int elem, bool wide) {
-  return std::max(row_plan(R, V, elem, true, wide).total, row_plan(R, V, elem, false, wide).total);
+inline size_t row_ws_bytes(int64_t R, int64_t V, int elem, bool sample, bool wide) {
+  return std::max(row_plan(R, V, elem, true, sample, wide).total, row_plan(R, V, elem, false, sample, wide).total);
 }
 
 template <typename T, bool SAMPLE>
@@ -1729,9 +1747,9 @@ int row_scan_launch(const RowPlan& p, const T* x, int64_t ldx, int64_t R, int V,
 }
 
 template <typename T>
-inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, bool wide, void* ws, size_t ws_bytes, RowPlan& p,
+inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, bool sample, bool wide, void* ws, size_t ws_bytes, RowPlan& p,
                        RowScan& scan) {
-  p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0, wide);
+  p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0, sample, wide);
   ORTHRUS_CHECK_ARG(R * p.slices < (1ll << 31) && (reinterpret_cast<uintptr_t>(x) & (sizeof(T) - 1)) == 0);
   if (ws == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
   uint8_t* w = static_cast<uint8_t*>(ws);
@@ -1750,7 +1768,7 @@ int topk_rows_impl(const T* x, int64_t ldx, int64_t R, int64_t V, int k, float t
                    float* lse, void* ws, size_t ws_bytes, cudaStream_t stream) {
   RowPlan p;
   RowScan scan;
-  int rc = row_prepare(x, ldx, R, V, false, ws, ws_bytes, p, scan);
+  int rc = row_prepare(x, ldx, R, V, false, false, ws, ws_bytes, p, scan);
   if (rc != ORTHRUS_OK) return rc;
   rc = row_scan_launch<T, false>(p, x, ldx, R, static_cast<int>(V), temperature, 0, SampleKnobs{}, scan, stream);
   if (rc != ORTHRUS_OK) return rc;
@@ -1808,7 +1826,7 @@ int sample_logits_impl(const T* x, int64_t ldx, int64_t R, int64_t V, const floa
                        int64_t* tokens, void* ws, size_t ws_bytes, cudaStream_t stream) {
   RowPlan p;
   RowScan scan;
-  int rc = row_prepare(x, ldx, R, V, sample_can_be_wide(knobs), ws, ws_bytes, p, scan);
+  int rc = row_prepare(x, ldx, R, V, true, sample_can_be_wide(knobs), ws, ws_bytes, p, scan);
   if (rc != ORTHRUS_OK) return rc;
   const int n = static_cast<int>(V), S = row_weight_bits(n);
   rc = row_scan_launch<T, true>(p, x, ldx, R, n, 1.f, S, knobs, scan, stream);
