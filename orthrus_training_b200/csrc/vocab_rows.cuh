@@ -16,6 +16,24 @@
 // even that does not do (rows of equal values), a CTA goes over the whole row again: a radix selection
 // that is right for every row, and a walk in index order.
 //
+// What bounds it, and what it measured (us; V = 151936 where not given; floor: each logit read once at
+// 6540 GB/s):
+//   top-64, 1024 rows fp32           137 (floor 95): the scan 107 (5.8 TB/s), then the finish, whose one
+//                                    and a half waves of CTAs wait for memory and barriers, 28
+//   top-300, 333 x 50257 bf16         37 (5.3): the finish
+//   top-8, 2 x 1024; top-64, 32 rows  18, 18: the call's host time (7 and 18 on the device)
+//   plain sampling, 1 row             16: the call's host time (10 on the device)
+//   top-p 0.95, 256 rows fp32        254 (24), every row wide: scan 76, finish 38, bins 43, window 6, sums 50,
+//                                    pick 25. The scan is bound by the instructions of the integer
+//                                    weights (48 an entry, 15 of them fp64 at half rate), the bins
+//                                    and sums by those of passing over the entries (26 each)
+//   mixed filters, 1024 rows bf16    270 (48): scan 106, finish 58, wide rows the rest
+//   min-p 0.05, 77 x 32003 fp32       23 (1.5): latency of two dependent launches
+// One CTA per row for all of it (a cluster, or a CTA going over its row again) took 576 us for the first,
+// and 1490 against 254 for the wide nuclei: few bytes in flight. The finish is mostly code that runs once
+// per row, so that fetching instructions costs more than executing them: what is not a hot loop is kept
+// rolled and out of line.
+//
 // Candidates are the entries that are neither -inf nor NaN. Entries are ordered by (descending
 // value, ascending index); -0 counts as +0.
 #pragma once
@@ -211,7 +229,7 @@ struct uint2x64 {
   uint64_t x, y;
 };
 
-// Block-wide sum; every thread gets it. Leaves warp_u64 free for reuse.
+// Block-wide sum; every thread gets it.
 __device__ __noinline__ uint64_t block_sum_u64(uint64_t v) {
   RowScratch& sh = row_scratch();
   v = warp_sum_u64(v);
@@ -249,10 +267,10 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& to
 // Softmax weights as 64-bit integers
 // ------------------------------------------------------------------------------------------------
 
-// w(x) = round(2^S exp((x - top) / T)). Integer weights make every sum exact, so running sums do not
-// depend on how a row is split over threads, and comparisons with a uniform's share of the total
-// fall the same way on every path. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
-// 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
+// w(x) = round(2^S exp((x - top) / T)). Integer weights make sums exact, so running sums do not
+// depend on how a slice is split over threads. (Slices whose maximum is below the row's are brought down
+// in fp64, the one rounding that depends on where slices end.) S = min(44, 62 - ceil(log2 V)) keeps a
+// row's sum below 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
 //
 // The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f = 1 + f q(f) with q of degree
 // 8 through the Chebyshev nodes of [-1/2, 1/2] (error below 4e-14), 2^(S - n) by the exponent. A table
@@ -520,7 +538,7 @@ __device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row) {
 // A key with at least k entries of the row at or above it, and not many more: between the k-th largest
 // maximum of a group (of four groups where k is a small part of their number) and a little below it;
 // 1 if fewer than k of them hold a candidate. Histograms of the maxima over the range of keys that
-// can hold the bound, 1024 bins at a time.
+// can hold the bound, 512 bins at a time.
 __device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) {
   RowScratch& sh = row_scratch();
   const uint32_t* maxima = row_maxima();
@@ -1758,7 +1776,7 @@ inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, bool sampl
   return ORTHRUS_OK;
 }
 
-// The scratch and the group maxima, of the longest row or of these; the scratch and a window.
+// Shared memory of a finish: the scratch and the group maxima (kRowSmem: of the longest row); of a pick.
 constexpr int kRowScratch = (sizeof(RowScratch) + 15) / 16 * 16;
 constexpr int kRowSmem = kRowScratch + (kRowMaxV + 8) / kRowGroup * 4 + 512;
 constexpr int kRowWideSmem = kRowScratch + static_cast<int>(sizeof(RowWideSlices));
