@@ -536,8 +536,7 @@ __device__ __forceinline__ uint32_t row_open(const RowScan& scan, int64_t row) {
 }
 
 // A key with at least k entries of the row at or above it, and not many more: between the k-th largest
-// maximum of a group (of four groups where k is a small part of their number) and a little below it;
-// 1 if fewer than k of them hold a candidate. Histograms of the maxima over the range of keys that
+// maximum of a group and a little below it; 1 if fewer than k groups hold a candidate. Histograms of the maxima over the range of keys that
 // can hold the bound, 512 bins at a time.
 __device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) {
   RowScratch& sh = row_scratch();
@@ -547,16 +546,10 @@ __device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t* counts = sh.counts;
   const uint4* m4 = reinterpret_cast<const uint4*>(maxima);
-  const bool quads = k <= groups / 16;
   // the smallest candidate maximum
   uint32_t least = top_key;
   for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
     const uint4 q = m4[i];
-    if (quads) {
-      const uint32_t m = max(max(q.x, q.y), max(q.z, q.w));
-      least = min(least, m ? m : top_key);
-      continue;
-    }
     least = min(min(least, q.x ? q.x : top_key), min(min(q.y ? q.y : top_key, q.z ? q.z : top_key), q.w ? q.w : top_key));
   }
   least = __reduce_min_sync(0xffffffffu, least);
@@ -572,8 +565,7 @@ __device__ __noinline__ uint32_t row_bound(int groups, int k, uint32_t top_key) 
     const int shift = max(0, 32 - __clz(hi - lo) - BIN_BITS);
     for (int i = threadIdx.x; i < groups / 4; i += kRowThreads) {
       const uint4 q = m4[i];
-      const uint32_t m[4] = {quads ? max(max(q.x, q.y), max(q.z, q.w)) : q.x, quads ? 0u : q.y, quads ? 0u : q.z,
-                             quads ? 0u : q.w};
+      const uint32_t m[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (m[e] >= lo && m[e] <= hi) atomicAdd(&counts[(hi - m[e]) >> shift], 1u);
@@ -708,10 +700,11 @@ __device__ __forceinline__ void row_sort_desc(uint64_t* a, int n2) {
 }
 
 // Orders the scratch's list (n <= kRowList different entries) descending into `sorted`: by rank
-// counting for a few entries, several threads an entry; else by a sorting network.
+// counting for a few entries, several threads an entry; else by a sorting network (top-64 of 16 rows of V
+// = 151936 16.4 us by ranks, 18.5 by the network; top-120 18.8, 20.5; top-200 24.6, 22.6).
 __device__ __noinline__ void row_order(int n) {
   uint64_t *in = row_scratch().list, *out = row_scratch().sorted;
-  if (n <= kRowThreads) {
+  if (n <= 160) {
     int parts = 32;
     while (parts > 1 && parts * n > kRowThreads) parts >>= 1;
     const int e = threadIdx.x / parts, part = threadIdx.x % parts;
@@ -977,17 +970,20 @@ __device__ __noinline__ bool row_pick_listed(int n, int V, int top_k, float top_
   }
   const uint64_t aim = floor_share(uniform, block_sum_u64(own));
   // the token: the lowest index up to which the kept entries weigh more than `aim`
-  if (n <= kRowThreads / 2) {  // a few: the running sum before each, two threads an entry
+  // Up to 256 entries: the running sum before each, over all pairs (16 rows of V = 151936, us: top-k 60 20.5,
+  // by bisection 31; top-k 200 35 and 39; top-k 400 71 and 47).
+  if (n <= kRowThreads) {
     uint64_t* kept = order ? sh.list : sh.sorted;
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (threadIdx.x * PER + j < n) kept[threadIdx.x * PER + j] = w[j];
     __syncthreads();
-    const int e = min(static_cast<int>(threadIdx.x) / 2, n - 1);
+    const int parts = n <= kRowThreads / 2 ? 2 : 1;  // threads an entry
+    const int e = min(static_cast<int>(threadIdx.x) / parts, n - 1);
     const uint32_t place = static_cast<uint32_t>(entries[e]);
     uint64_t run = 0;
-    for (int j = threadIdx.x % 2; j < n; j += 2) run += static_cast<uint32_t>(entries[j]) > place ? kept[j] : 0;
-    run += __shfl_xor_sync(0xffffffffu, run, 1);
+    for (int j = threadIdx.x % parts; j < n; j += parts) run += static_cast<uint32_t>(entries[j]) > place ? kept[j] : 0;
+    if (parts == 2) run += __shfl_xor_sync(0xffffffffu, run, 1);
     if (run <= aim && aim < run + kept[e]) *token = ~place;
     return true;
   }
