@@ -587,7 +587,9 @@ class FusedLinearTopKKL:
     the teacher's whole row / temperature, the teacher's own probabilities, whose sum falls short
     of 1 by what was not kept. teacher_top_logits gives all three. Returns (total, kl_rows, agree),
     total differentiable w.r.t. the student rows (the LM head is frozen). The chunk_size rows whose
-    probabilities are held at a time cost 2 V bytes each for bf16, 4 V for fp32."""
+    probabilities are held at a time cost 2 V bytes each for bf16, 4 V for fp32. Forward and backward
+    can be captured into a CUDA graph; as with every torch function, not while an eager graph of the
+    same leaves lives."""
 
     @staticmethod
     def apply(student, values, ids, index, weight, chunk_size, row_weight=None, temperature=1.0,

@@ -94,3 +94,14 @@ def test_distillation_status(bad, status):
         ctypes.c_float(a["T"]), None, a["offsets"], a["num"], a["total"], a["kl"], a["agree"], a["grad"], None, None,
         4096, a["ws"], a["ws_bytes"], a["dtype"], None)
     assert got == getattr(_lib(), status)
+
+
+@pytest.mark.parametrize("t", [0.0, 1e-31, 1e31, float("inf"), float("nan"), -1.0])
+def test_temperatures_out_of_range(t):
+    lib, f = _lib().lib(), ctypes.c_float
+    assert lib.orthrus_topk_rows(64, 8, 2, 8, 3, f(t), 64, 64, 64, 64, 1 << 50, 1, None) == _lib().EINVAL
+    a = dict(GOOD, T=t)
+    assert lib.orthrus_lmhead_topk_kl_fwd(
+        a["student"], a["n"], a["values"], a["ids"], a["m"], a["k"], a["index"], a["lse"], a["weight"], a["V"], a["d"],
+        f(t), None, a["offsets"], a["num"], a["total"], a["kl"], a["agree"], a["grad"], None, None, 4096, a["ws"],
+        a["ws_bytes"], a["dtype"], None) == _lib().EINVAL

@@ -358,3 +358,11 @@ def test_trainer_steps_on_top_logits():
         out = trainer.step([(ids.to(DEV), mask.to(DEV))])
         assert torch.isfinite(out["loss"]) and not bool(out["skipped"])
     assert any(not torch.equal(p, q) for p, q in zip(trainer.params, before))
+
+
+@pytest.mark.parametrize("n,V,d,chunk", [(600, 8001, 100, 4096), (300, 4000, 33, 4096), (97, 1009, 513, 4096),
+                                         (600, 2500, 257, 256), (33, 20011, 7, 4096)])
+def test_fp32_product_tiles(n, V, d, chunk):
+    """Every tile size of the fp32 products, with and without parts of the long axis, ragged in all three."""
+    a, lse = _inputs(n, 40, V, d, 9, torch.float32, seed=n)
+    _check(a, 1.5, lse, chunk=chunk)
