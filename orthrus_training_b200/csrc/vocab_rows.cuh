@@ -455,20 +455,38 @@ __global__ void __launch_bounds__(kScanThreads)
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) v.values(b0 + j * kScanThreads + threadIdx.x, val[j]);
   }
-  float top = -INFINITY;
+  float m[BLOCKS], top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < BLOCKS; ++j) {
-    float m = val[j][0];
+    m[j] = val[j][0];
 #pragma unroll
-    for (int e = 1; e < VEC; ++e) m = fmaxf(m, val[j][e]);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    top = fmaxf(top, m);
-    const int g = (b0 + j * kScanThreads + static_cast<int>(threadIdx.x)) / LANES;
-    if (lane % LANES == 0 && g < out.groups) out.group[row * out.groups + g] = K::of(m);
+    for (int e = 1; e < VEC; ++e) m[j] = fmaxf(m[j], val[j][e]);
+    top = fmaxf(top, m[j]);
   }
+  // the groups' maxima: halves of a group's lanes exchange halves of the blocks while there are several,
+  // so that a lane ends with one group (block `held`) rather than every lane with all of its
+  static_assert(BLOCKS <= LANES, "");
+  int held = 0;
 #pragma unroll
-  for (int o = 16; o >= LANES; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = LANES / 2, n = BLOCKS; o > 0; o >>= 1) {
+    if (n > 1) {
+      n /= 2;
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < BLOCKS / 2; ++i)
+        if (i < n) {
+          const float other = __shfl_xor_sync(0xffffffffu, up ? m[i] : m[i + n], o);
+          m[i] = fmaxf(up ? m[i + n] : m[i], other);
+        }
+      held += up ? n : 0;
+    } else {
+      m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+    }
+  }
+  const int g = (b0 + held * kScanThreads + static_cast<int>(threadIdx.x)) / LANES;
+  if (lane % (LANES / BLOCKS) == 0 && g < out.groups) out.group[row * out.groups + g] = K::of(m[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) wtop[warp] = top;
   __syncthreads();
 #pragma unroll
