@@ -18,16 +18,16 @@
 //
 // What bounds it, and what it measured (us; V = 151936 where not given; floor: each logit read once at
 // 6540 GB/s):
-//   top-64, 1024 rows fp32           137 (floor 95): the scan 107 (5.8 TB/s), then the finish, whose one
-//                                    and a half waves of CTAs wait for memory and barriers, 28
+//   top-64, 1024 rows fp32           127 (floor 95): the scan 96 (6.5 TB/s), then the finish, whose one and a
+//                                    half waves of CTAs wait for memory and barriers, 25
 //   top-300, 333 x 50257 bf16         37 (5.3): the finish
 //   top-8, 2 x 1024; top-64, 32 rows  18, 18: the call's host time (7 and 18 on the device)
 //   plain sampling, 1 row             16: the call's host time (10 on the device)
-//   top-p 0.95, 256 rows fp32        254 (24), every row wide: scan 76, finish 38, bins 43, window 6, sums 50,
+//   top-p 0.95, 256 rows fp32        247 (24), every row wide: scan 69, finish 38, bins 43, window 6, sums 50,
 //                                    pick 25. The scan is bound by the instructions of the integer
-//                                    weights (48 an entry, 15 of them fp64 at half rate), the bins
+//                                    weights (45 an entry, 15 of them fp64 at half rate), the bins
 //                                    and sums by those of passing over the entries (26 each)
-//   mixed filters, 1024 rows bf16    270 (48): scan 106, finish 58, wide rows the rest
+//   mixed filters, 1024 rows bf16    258 (48): scan 96, finish 54, wide rows the rest
 //   min-p 0.05, 77 x 32003 fp32       23 (1.5): latency of two dependent launches
 // One CTA per row for all of it (a cluster, or a CTA going over its row again) took 576 us for the first,
 // and 1490 against 254 for the wide nuclei: few bytes in flight. The finish is mostly code that runs once
