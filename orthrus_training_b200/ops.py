@@ -339,6 +339,15 @@ def _kernel_operand(t: torch.Tensor, pad: int = 0) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _dense(t, dtype):
+    return t if t is None or (t.dtype == dtype and t.is_contiguous()) else t.to(dtype).contiguous()
+
+
+@lru_cache(maxsize=256)
+def _lmhead_topk_kl_bytes(n, m, V, d, k, chunk_rows, code):
+    return L.lib().orthrus_lmhead_topk_kl_workspace_bytes(n, m, V, d, k, chunk_rows, code)
+
+
 def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets=None, num_offsets=0,
                    temperature=1.0, teacher_lse=None, need_grad=True, chunk_rows=4096):
     """Distillation from a teacher's top logits through the LM head: sum_r w_r sum_j q_j (log q_j -
@@ -370,23 +379,20 @@ def lmhead_topk_kl(student, values, ids, index, weight, row_weight=None, offsets
             raise ValueError("lmhead_topk_kl takes tensors of one device")
     pad = (-d) % 8 if student.dtype == torch.bfloat16 else 0  # TMA rows are multiples of 16 bytes
     student, weight = _kernel_operand(student, pad), _kernel_operand(weight, pad)
-    values, ids = values.to(torch.float32).contiguous(), ids.to(torch.int64).contiguous()
-    index = None if index is None else index.to(torch.int64).contiguous()
-    row_weight = None if row_weight is None else row_weight.to(torch.float32).contiguous()
-    teacher_lse = None if teacher_lse is None else teacher_lse.to(torch.float32).contiguous()
+    values, ids, index = _dense(values, torch.float32), _dense(ids, torch.int64), _dense(index, torch.int64)
+    row_weight, teacher_lse = _dense(row_weight, torch.float32), _dense(teacher_lse, torch.float32)
     total = torch.empty((), dtype=torch.float32, device=dev)
     kl_rows = torch.empty(n, dtype=torch.float32, device=dev)
     agree = torch.empty(n, dtype=torch.bool, device=dev)  # the kernel writes bytes 0 and 1
     grad = torch.empty(n, d + pad, dtype=student.dtype, device=dev) if need_grad else None
     kbo = abo = None
     if offsets is not None:
-        offsets = offsets.to(torch.int64).contiguous()
+        offsets = _dense(offsets, torch.int64)
         kbo = torch.empty(num_offsets, dtype=torch.float32, device=dev)
         abo = torch.empty(num_offsets, dtype=torch.int64, device=dev)
     lib = L.lib()
     with _on_device(dev):
-        ws = torch.empty(max(lib.orthrus_lmhead_topk_kl_workspace_bytes(n, m, V, d + pad, k, chunk_rows, code), 1),
-                         dtype=torch.uint8, device=dev)
+        ws = torch.empty(max(_lmhead_topk_kl_bytes(n, m, V, d + pad, k, chunk_rows, code), 1), dtype=torch.uint8, device=dev)
         t0 = TIMER.begin() if TIMER is not None else None
         L.check(lib.orthrus_lmhead_topk_kl_fwd(
             L.ptr(student), n, L.ptr(values), L.ptr(ids), m, k, L.ptr(index), L.ptr(teacher_lse), L.ptr(weight), V,
