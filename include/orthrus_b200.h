@@ -496,7 +496,8 @@ size_t orthrus_topk_rows_workspace_bytes(int64_t R, int64_t V, int dtype);
 
 /* The k largest candidates of each row (1 <= k <= 1024): values [R, k] fp32 and ids [R, k] in
  * order, (-inf, -1) past the last candidate, and lse [R] = log(sum exp(x / temperature)) over the
- * candidates (-inf without any, +inf if one is +inf). temperature from 1e-30 to 1e30. */
+ * candidates (-inf without any, +inf if one is +inf; infinite too where it leaves fp32). temperature
+ * from 1e-30 to 1e30. */
 int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int k, float temperature,
                       float* values, int64_t* ids, float* lse, void* workspace,
                       size_t workspace_bytes, int dtype, void* stream);
