@@ -719,7 +719,8 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) {
     kl_rows[g] = kl;
     agree[g] = t >= 0 && top_id[t] >= 0 && top_id[t] == at;
-    scale[r] = (row_weight ? row_weight[g] : 1.f) / T * (Q / z);
+    // a row of padding has no reference near its logits, so its z may be 0 (or anything)
+    scale[r] = Q == 0.f ? 0.f : (row_weight ? row_weight[g] : 1.f) / T * (Q / z);
   }
 }
 

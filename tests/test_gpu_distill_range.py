@@ -1,0 +1,108 @@
+"""Distillation from a teacher's top logits (GPU) over the range its arguments may take: rows of padding
+with any student, temperatures from 1e-30, operands of any distribution.
+
+The operands are small integers, so that every logit is a sum of integers below 2^24 and exact in fp32
+in whatever order and with whatever cutting it is formed. What is left are roundings that do not grow
+with 1 / T: an exponent (x - c) / T carries three of its own size (8 U with the constants beside it),
+ex2 errs by 2^-22, a sum of exponentials is formed over fewer than 64 additions in a row, expf and logf
+are off by two units."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def _rows(n, V, d, k, dtype, seed, near=True):
+    """Integer operands; each teacher row keeps the k largest logits of an integer student of its own,
+    near the student's (near) or not."""
+    g = torch.Generator().manual_seed(seed)
+    W = torch.randint(-3, 4, (V, d), generator=g).float()
+    h = torch.randint(-2, 3, (n, d), generator=g).float()
+    t = h + (torch.rand(n, d, generator=g) < 0.05).float() if near else torch.randint(-2, 3, (n, d), generator=g).float()
+    values, ids = (t @ W.T).topk(k)
+    return dict(student=h.to(DEV, dtype), values=values.to(DEV), ids=ids.to(DEV), index=None, weight=W.to(DEV, dtype),
+                row_weight=(0.5 + torch.rand(n, generator=g)).to(DEV))
+
+
+def _formula(a, T):
+    """kl, gradient and agreement in 64 bits, and the bounds of the first two (see above)."""
+    T = float(torch.tensor(T, dtype=torch.float32))
+    h, W, w = a["student"].double(), a["weight"].double(), a["row_weight"].double()
+    live = (a["ids"] >= 0) & (a["values"] > -math.inf)
+    some = live.any(1, keepdim=True)
+    v, ids = torch.where(live, a["values"].double(), -math.inf), a["ids"].clamp_min(0)
+    v = torch.where(some, (v - v.max(1, keepdim=True).values) / T, -math.inf)
+    lq = torch.where(live, v - torch.where(some, v.logsumexp(1, keepdim=True), 0.0), -math.inf)
+    q = torch.where(live, lq.exp(), 0.0)
+    s = h @ W.T
+    y = (s - s.max(1, keepdim=True).values) / T
+    lp = y.log_softmax(1)
+    lpk = lp.gather(1, ids)
+    taken = q > 0
+    kl = torch.where(taken, q * (lq - lpk), 0.0).sum(1)
+    zerr = 2.0 ** -22 + 64 * U
+    step = 16 * U * (1 + lq.abs()) * (lq - lpk).abs() + 8 * U * (lq.abs() + lpk.abs() + 1) + zerr
+    klb = torch.where(taken, q * step, 0.0).sum(1)
+    qs = torch.zeros_like(lp).scatter_add_(1, ids, q)
+    c = (w / T)[:, None]
+    Qp = q.sum(1, keepdim=True) * lp.exp()
+    diff = c * (Qp - qs)
+    half = 2.0 ** -8 if a["student"].dtype == torch.bfloat16 else U
+    lqs = torch.where(taken, 16 * U * (1 + lq.abs()), 0.0).max(1, keepdim=True).values
+    dd = c * (Qp * (zerr + 8 * U * lp.abs().clamp_max(1e3) + lqs) + qs * (lqs + zerr)) + diff.abs() * half
+    grad = diff @ W
+    gb = (dd + diff.abs() * W.shape[0] * 2.0 ** -23) @ W.abs() + half * grad.abs()
+    top = torch.where(live, a["values"].double(), -math.inf).argmax(1, keepdim=True)
+    agree = some[:, 0] & (s.argmax(1) == ids.gather(1, top)[:, 0])
+    return kl, grad, agree, klb, gb
+
+
+def _check(a, T):
+    from orthrus_training_b200.objective import FusedLinearTopKKL
+
+    student = a["student"].detach().requires_grad_()
+    total, kl, agree = FusedLinearTopKKL.apply(student, a["values"], a["ids"], a["index"], a["weight"], 4096,
+                                               a["row_weight"], T)
+    total.backward()
+    grad = student.grad
+    want_kl, want_grad, want_agree, klb, gb = _formula(a, T)
+    assert torch.isfinite(kl).all() and torch.isfinite(grad).all()
+    assert ((kl.double() - want_kl).abs() <= klb).all(), ((kl.double() - want_kl).abs() / klb).max()
+    assert ((grad.double() - want_grad).abs() <= gb).all(), ((grad.double() - want_grad).abs() / gb).max()
+    assert torch.equal(agree, want_agree)
+    return total, kl, grad
+
+
+@pytest.mark.parametrize("T", [1.0, 0.3, 0.02])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_padding_rows_of_low_logits_are_nothing(dtype, T):
+    """Rows whose teacher kept nothing (no ids, ids past the vocabulary, an index out of range), all of
+    whose logits lie near -240: kl 0 and gradient 0, beside rows that kept something."""
+    from orthrus_training_b200 import _lib, ops
+
+    n, m = 300, 200
+    a = _rows(n, 900, 64, 6, dtype, seed=1)
+    a["student"][:, 0] = 2
+    a["weight"][:, 0] = -120
+    a["values"], a["ids"] = a["values"][:m] - 240, a["ids"][:m].clone()
+    a["index"] = torch.arange(n, device=DEV) % m
+    a["ids"][10:20] = -1
+    a["index"][30:40] = 12
+    _lib.device_error(0)
+    clean = ops.lmhead_topk_kl(**a, temperature=T)
+    none = (a["ids"] < 0).all(1)[a["index"]]
+    assert _lib.device_error(0) == 0 and 10 <= int(none.sum()) < n
+    a["ids"][15:20] = 900
+    a["index"][35:40] = torch.tensor([m, -1, 2 ** 40, m + 1, -2 ** 40], device=DEV)
+    got = ops.lmhead_topk_kl(**a, temperature=T)
+    assert _lib.device_error(0) == _lib.ERR_BOUNDS
+    for total, kl, agree, grad, _, _ in (clean, got):
+        assert (kl[none] == 0).all() and (grad[none] == 0).all() and not agree[none].any()
+        assert torch.isfinite(total) and torch.isfinite(kl).all() and torch.isfinite(grad).all()
+        assert (grad[~none] != 0).any()
