@@ -16,7 +16,8 @@
 // SwiGLU backward, where acc = dact = dy @ W_down of the MLP and R = [gate | up] [M, 2N] kept by the
 // forward: the epilogue writes C = [dgate | dup] [M, 2N] (the arithmetic and roundings of
 // swiglu_bwd_kernel), so dact never goes through HBM. Row scale: C = s[row] * acc with fp32 factors
-// s [M] (passed in place of R), one rounding (the LM-head gradient of lmhead_topk_kl.cuh).
+// s [M] (passed in place of R), one rounding; a factor of 0 gives 0 for any acc, NaN and infinities among
+// them (the LM-head gradient of lmhead_topk_kl.cuh, whose rows of padding may hold anything).
 //
 // Persistent: one cluster per SM pair loops over pair tiles (n fastest). 320 threads per CTA:
 //   warp 0     TMA producer (both CTAs): this CTA's A and B k-blocks of 64 into a 6-stage ring;
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(Gemm2Base::THREADS, 1)
           if constexpr (EPI == kGemm2RowScale) {
             const float f = row < g.M ? reinterpret_cast<const float*>(R)[row] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= f;
+            for (int i = 0; i < 32; ++i) v[i] = f == 0.f ? 0.f : v[i] * f;  // 0 whatever the row holds
           }
           if constexpr (EPI == kGemm2Residual) {
 #pragma unroll
@@ -478,6 +479,7 @@ __global__ void gemm2_reduce_scaled_kernel(const float* __restrict__ part, int s
       acc.w += p.w;
     }
     const float f = scale[m];
+    if (f == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // whatever the row holds
     __nv_bfloat16* c = C + m * ldc + n;
     *reinterpret_cast<__nv_bfloat162*>(c) = __floats2bfloat162_rn(f * acc.x, f * acc.y);
     *reinterpret_cast<__nv_bfloat162*>(c + 2) = __floats2bfloat162_rn(f * acc.z, f * acc.w);

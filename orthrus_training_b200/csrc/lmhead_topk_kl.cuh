@@ -174,6 +174,11 @@ __global__ void __launch_bounds__(kTopkKlThreads)
   if (diff == nullptr) return;
   // the kept entries' differences first (they read the logits), then the sweep, then their stores
   const float w = (row_weight ? row_weight[r] : 1.f) / T;
+  D* d = diff + blockIdx.x * ldd;
+  if (w * Q == 0.f) {  // no mass or no weight: 0 whatever the row holds (the sum above is past its last reads)
+    for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = from_f32<D>(0.f);
+    return;
+  }
   constexpr int PER = kTopkKlMaxK / kTopkKlThreads;
   float fix[PER];
 #pragma unroll
@@ -185,7 +190,6 @@ __global__ void __launch_bounds__(kTopkKlThreads)
     fix[u] = w * (Q * (expf((x[sh.id[j]] - top) / T) / z) - q);
   }
   __syncthreads();
-  D* d = diff + blockIdx.x * ldd;
   const float scale = w * Q / z;
   for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = from_f32<D>(scale * expf((x[i] - top) / T));
   __syncthreads();

@@ -106,3 +106,21 @@ def test_padding_rows_of_low_logits_are_nothing(dtype, T):
         assert (kl[none] == 0).all() and (grad[none] == 0).all() and not agree[none].any()
         assert torch.isfinite(total) and torch.isfinite(kl).all() and torch.isfinite(grad).all()
         assert (grad[~none] != 0).any()
+
+
+@pytest.mark.parametrize("V", [900, 5003])  # the gradient's product in one and in several parts
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_padding_rows_of_any_student_are_nothing(dtype, V):
+    """What stands in the student's row has no effect where the teacher kept nothing: NaN and
+    infinities there leave kl and gradient 0, and the other rows as they are."""
+    from orthrus_training_b200 import ops
+
+    a = _rows(300, V, 64, 6, dtype, seed=2)
+    a["ids"][5:280:3] = -1
+    none = (a["ids"] < 0).all(1)
+    clean = ops.lmhead_topk_kl(**a)
+    for junk in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
+        a["student"][none] = junk
+        for x, y in zip(ops.lmhead_topk_kl(**a)[:4], clean[:4]):
+            assert torch.equal(x, y)
+    assert (clean[1][none] == 0).all() and (clean[3][none] == 0).all() and (clean[3][~none] != 0).any()
