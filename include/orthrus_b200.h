@@ -364,6 +364,7 @@ int orthrus_lmhead_kl_bwd(const void* grad, const float* grad_total, void* grad_
 /* Distillation from a teacher's top logits through the LM head. Per student row r with teacher row
  * t = index[r] (index NULL: t = r) and its kept logits (values[t, j], ids[t, j]), j < k <= 1024:
  *   q_j = softmax over the kept values / temperature, or exp(value_j / temperature - teacher_lse[t])
+ *         (an fp32 number: its rounding, up to 2^-24 of it, goes into every log q_j)
  *   p = softmax(weight student[r] / temperature) over all V entries
  *   kl_rows[r] = sum_j q_j (log q_j - log p[id_j]);  total = sum_r row_weight[r] kl_rows[r];
  *   grad[r] = (row_weight[r] / temperature) ((sum_j q_j) p - q) weight, the gradient of total;

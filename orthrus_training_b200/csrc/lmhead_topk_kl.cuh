@@ -111,7 +111,7 @@ __device__ inline float tk_load_teacher(const float* __restrict__ values, const 
     if (past) record_error(ORTHRUS_ERR_BOUNDS);
     const bool live = row_ok && id >= 0 && !past && v != -INFINITY;
     sh.id[j] = live ? static_cast<int>(id) : -1;
-    sh.logq[j] = live ? v / T : -INFINITY;
+    sh.logq[j] = live ? v : -INFINITY;
     if (live && v > best) {
       best = v;
       at = j;
@@ -119,18 +119,21 @@ __device__ inline float tk_load_teacher(const float* __restrict__ values, const 
   }
   tk_block_argmax(best, at, sh);
   top_id = at == INT_MAX ? -1 : sh.id[at];
-  float norm;
+  // log q from the distance to the largest value: v / T - (best / T + log z) would lose log z where
+  // best / T is large
+  float base = 0.f, norm;
   if (teacher_lse != nullptr) {
     norm = teacher_lse[t];
   } else {
     float z = 0.f;
+    base = best;
     for (int j = threadIdx.x; j < k; j += kTopkKlThreads)
-      if (sh.id[j] >= 0) z += expf(sh.logq[j] - best / T);
-    norm = best / T + logf(tk_block_sum(z, sh));
+      if (sh.id[j] >= 0) z += expf((sh.logq[j] - base) / T);
+    norm = logf(tk_block_sum(z, sh));
   }
   float Q = 0.f;
   for (int j = threadIdx.x; j < k; j += kTopkKlThreads) {
-    const float lq = sh.id[j] >= 0 ? sh.logq[j] - norm : -INFINITY;
+    const float lq = sh.id[j] >= 0 ? (sh.logq[j] - base) / T - norm : -INFINITY;
     sh.logq[j] = lq;
     sh.q[j] = expf(lq);
     Q += sh.q[j];
@@ -282,18 +285,19 @@ __global__ void __launch_bounds__(128)
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
   };
-  float norm;
+  float base = 0.f, norm;  // as tk_load_teacher
   if (teacher_lse != nullptr) {
     norm = teacher_lse[t];
   } else {
     float z = 0.f;
+    base = best;
     for (int j = threadIdx.x; j < k; j += 128)
-      if (id[j] != INT_MAX) z += expf(val[j] / T - best / T);
-    norm = best / T + logf(sum(z));
+      if (id[j] != INT_MAX) z += expf((val[j] - base) / T);
+    norm = logf(sum(z));
   }
   float q = 0.f;
   for (int j = threadIdx.x; j < k; j += 128) {
-    const float lq = id[j] != INT_MAX ? val[j] / T - norm : -INFINITY;
+    const float lq = id[j] != INT_MAX ? (val[j] - base) / T - norm : -INFINITY;
     sid[t * k + j] = id[j];
     slogq[t * k + j] = lq;
     q += expf(lq);

@@ -55,7 +55,8 @@ def _formula(a, T):
     diff = c * (Qp - qs)
     half = 2.0 ** -8 if a["student"].dtype == torch.bfloat16 else U
     lqs = torch.where(taken, 16 * U * (1 + lq.abs()), 0.0).max(1, keepdim=True).values
-    dd = c * (Qp * (zerr + 8 * U * lp.abs().clamp_max(1e3) + lqs) + qs * (lqs + zerr)) + diff.abs() * half
+    # exponentials below 2^-126 are 0, and the largest of a row is 2^-60 or more: 2^-66 of p
+    dd = c * 2.0 ** -66 + c * (Qp * (zerr + 8 * U * lp.abs().clamp_max(1e3) + lqs) + qs * (lqs + zerr)) + diff.abs() * half
     grad = diff @ W
     gb = (dd + diff.abs() * W.shape[0] * 2.0 ** -23) @ W.abs() + half * grad.abs()
     top = torch.where(live, a["values"].double(), -math.inf).argmax(1, keepdim=True)
@@ -124,3 +125,16 @@ def test_padding_rows_of_any_student_are_nothing(dtype, V):
         for x, y in zip(ops.lmhead_topk_kl(**a)[:4], clean[:4]):
             assert torch.equal(x, y)
     assert (clean[1][none] == 0).all() and (clean[3][none] == 0).all() and (clean[3][~none] != 0).any()
+
+
+@pytest.mark.parametrize("dtype,T", [(t, T) for t in DTYPES for T in (1e-2, 1e-3, 1e-5)] +
+                         [(torch.float32, T) for T in (1e-8, 1e-30)])
+def test_teacher_ties_at_low_temperatures(dtype, T):
+    """Equal kept logits share the teacher's mass however large the logits are beside the temperature: a
+    student with the same ties has kl 0 and no gradient but of roundings."""
+    a = _rows(200, 700, 64, 4, dtype, seed=3)
+    W = a["weight"]
+    W[1::2] = W[::2]  # every logit stands twice
+    values, ids = (a["student"].double() @ W.double().T).sort(dim=1, descending=True, stable=True)
+    a["values"], a["ids"] = values[:, :4].float(), ids[:, :4].contiguous()
+    _check(a, T)
