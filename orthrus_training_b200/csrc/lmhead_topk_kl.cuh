@@ -22,9 +22,10 @@
 //          and the row factor;
 //   grad   row factor * (chunk buffer @ W) on CTA pairs (gemm2_tc.cuh).
 // The reference c is the student's logit at the teacher's first id. bf16 has fp32's exponent range, so
-// a c up to 2^60 below the maximum loses nothing; rows with a larger logit are clamped, noticed by
-// their maximum and swept again with c = maximum (whole tiles of 256 rows; that launch ends at once
-// where there are none).
+// a c within 60 bits of the row's maximum loses nothing. Rows where it is further below (another
+// logit is the student's) or above (T so low that the roundings of that logit, over T, are many bits)
+// are noticed, and swept again relative to their maximum, subtracted before the division by T, where
+// nothing is lost at any T (whole tiles of 256 rows; that launch ends at once where there are none).
 //
 // fp32 rows run on CUDA cores: logits = student @ W^T, a row kernel that turns a row of logits into
 // its kl and the difference (w / T) (Q p - q), and grad = difference @ W.
@@ -310,11 +311,11 @@ __global__ void __launch_bounds__(128)
 }
 
 // One warp per student row: its teacher row (-1 if the index is out of range) and its reference
-// c = log2(e) / T * (student . W[top_id]); clears the second sweep's references and flags.
+// c = log2(e) / T * (student . W[top_id]); clears the rows' maxima and the second sweep's flags.
 __global__ void __launch_bounds__(256)
     topk_student_kernel(const __nv_bfloat16* __restrict__ student, const __nv_bfloat16* __restrict__ W, int64_t n,
                         int64_t m, int D, const int64_t* __restrict__ index, const int* __restrict__ top_id,
-                        float alpha, int* __restrict__ trow, float* __restrict__ ref, unsigned* __restrict__ over,
+                        float alpha, int* __restrict__ trow, float* __restrict__ ref, unsigned* __restrict__ rowmax,
                         int* __restrict__ again) {
   const int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -346,19 +347,27 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) {
     trow[r] = static_cast<int>(t);
     ref[r] = dot * alpha;
-    over[r] = 0;
+    rowmax[r] = 0;
     if (r % 256 == 0) again[r / 256] = 0;
   }
 }
 
-// The reference of a row: its largest logit where the first sweep left one in `over` (as an ordered
-// integer, 0: none), else the logit at the teacher's first id.
-__device__ __forceinline__ unsigned topk_over_key(float x) {
+// A row's largest logit as an ordered integer (0: none yet).
+__device__ __forceinline__ unsigned topk_max_key(float x) {
   const unsigned b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float topk_reference(float ref, unsigned over) {
-  return over == 0 ? ref : __uint_as_float((over & 0x80000000u) ? (over & 0x7FFFFFFFu) : ~over);
+
+// How a row's exponents are formed: (x - shift) * alpha - ref. In the first sweep shift is 0; once the
+// row's maximum is known, a reference too far from it (of a row with teacher entries) gives way to it.
+struct TopkReference {
+  float shift, ref;
+  __device__ __forceinline__ float operator()(float x, float alpha) const { return fmaf(x - shift, alpha, -ref); }
+};
+__device__ __forceinline__ TopkReference topk_reference(float ref, unsigned max_key, float alpha, bool kept) {
+  if (!kept || max_key == 0u) return {0.f, ref};
+  const float m = __uint_as_float((max_key & 0x80000000u) ? (max_key & 0x7FFFFFFFu) : ~max_key);
+  return fabsf(fmaf(m, alpha, -ref)) > kTopkExpLimit ? TopkReference{m, 0.f} : TopkReference{0.f, ref};
 }
 
 struct TopkExpTile {
@@ -381,8 +390,9 @@ struct TopkExpArgs {
   const int* trow;        // [n]
   const float* ref;       // [n]
   const int* sid;         // [m, k]
-  unsigned* over;         // [n]
-  int* again;             // [ceil(n / 256)]: tiles with a row above the exponent limit
+  const int* top_id;      // [m]
+  unsigned* rowmax;       // [n]: topk_max_key of the row's maximum, from the first sweep
+  int* again;             // [ceil(n / 256)]: tiles that may hold a row whose reference is too far off
   bool second;            // the second sweep takes the flagged tiles only
   float* kept;            // [chunk, k] student logits at the sorted ids
   float* part_z;          // [2 splits, chunk], as part_m and part_i
@@ -537,8 +547,11 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
       if (ntiles == 0) continue;
       const int crow = row0 + quarter * 32 + lane;  // row in the chunk
       const bool live = crow < a.rows;
-      const float ref = live ? topk_reference(a.ref[a.c0 + crow], a.second ? a.over[a.c0 + crow] : 0u) : 0.f;
       const int trow = live ? a.trow[a.c0 + crow] : -1;
+      const int top = trow < 0 ? -1 : a.top_id[trow];
+      const TopkReference ref = topk_reference(live ? a.ref[a.c0 + crow] : 0.f,
+                                               live && a.second ? a.rowmax[a.c0 + crow] : 0u, a.alpha, top >= 0);
+      bool far = false;  // the row's largest logit may be too far from its reference
       // the row's sorted ids from this unit's first column on
       const int* sid = a.sid + static_cast<int64_t>(trow < 0 ? 0 : trow) * a.k;
       int p = 0;
@@ -571,6 +584,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
           tmem_wait_ld();
           while (next == col) {  // an id kept twice stands twice
             a.kept[static_cast<int64_t>(crow) * a.k + p] = x;
+            far |= col == top && ref(x, a.alpha) < -kTopkExpLimit;
             next = ++p < a.k ? sid[p] : INT_MAX;
           }
           __syncwarp();
@@ -615,7 +629,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
           uint32_t packed[16];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            float y = fmaf(x[j], a.alpha, -ref);
+            float y = ref(x[j], a.alpha);
             y = y > kTopkExpLimit ? kTopkExpLimit : y;  // NaN stays
             x[j] = j < nvalid ? ex2_approx(y) : 0.f;
             zv[j & 3] += x[j];
@@ -651,9 +665,9 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
         a.part_z[o] = z;
         a.part_m[o] = m;
         a.part_i[o] = idx;
-        if (!a.second && fmaf(m, a.alpha, -ref) > kTopkExpLimit) {
-          atomicMax(&a.over[a.c0 + crow], topk_over_key(m * a.alpha));
-          a.again[(a.c0 + crow) / 256] = 1;
+        if (!a.second && top >= 0) {
+          atomicMax(&a.rowmax[a.c0 + crow], topk_max_key(m));
+          if (far || ref(m, a.alpha) > kTopkExpLimit) a.again[(a.c0 + crow) / 256] = 1;
         }
       }
     }
@@ -673,7 +687,7 @@ __global__ void __launch_bounds__(256)
     topk_finish_kernel(const float* __restrict__ part_z, const float* __restrict__ part_m,
                        const int* __restrict__ part_i, int parts, int64_t part_ld, int rows, int c0, int k, float alpha,
                        float T, const int* __restrict__ trow, const float* __restrict__ ref,
-                       const unsigned* __restrict__ over, const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
+                       const unsigned* __restrict__ rowmax, const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
                        const float* __restrict__ mass, const float* __restrict__ kept,
                        const float* __restrict__ row_weight, float* __restrict__ kl_rows, uint8_t* __restrict__ agree,
                        __nv_bfloat16* __restrict__ e, int64_t lde, float* __restrict__ scale) {
@@ -705,7 +719,8 @@ __global__ void __launch_bounds__(256)
   }
   const int t = trow[g];
   const float Q = t >= 0 ? mass[t] : 0.f;
-  const float logz = logf(z), c = topk_reference(ref[g], over[g]);
+  const float logz = logf(z);
+  const TopkReference c = topk_reference(ref[g], rowmax[g], alpha, t >= 0 && top_id[t] >= 0);
   float kl = 0.f;
   if (t >= 0 && Q != 0.f) {
     const int* id = sid + static_cast<int64_t>(t) * k;
@@ -713,7 +728,7 @@ __global__ void __launch_bounds__(256)
     for (int j = lane; j < k; j += 32) {
       const int i = id[j];
       if (i == INT_MAX) continue;
-      const float y = fmaf(kept[static_cast<int64_t>(r) * k + j], alpha, -c);
+      const float y = c(kept[static_cast<int64_t>(r) * k + j], alpha);
       const float q = expf(lq[j]);
       if (q != 0.f) kl += q * (lq[j] - (y * kLn2 - logz));
       if (e == nullptr || (j > 0 && id[j - 1] == i)) continue;
@@ -740,7 +755,7 @@ struct TopkKlPlan {
   int64_t chunk, Vp;
   int splits;  // most vocabulary ranges of a chunk's sweep
   size_t off_buf, off_gemm, gemm_bytes;
-  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_over, off_again, off_kept, off_part, off_scale;
+  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_rowmax, off_again, off_kept, off_part, off_scale;
   size_t total;
 };
 
@@ -769,7 +784,7 @@ inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64
     p.off_mass = take(static_cast<size_t>(m) * 4);
     p.off_trow = take(static_cast<size_t>(n) * 4);
     p.off_ref = take(static_cast<size_t>(n) * 4);
-    p.off_over = take(static_cast<size_t>(n) * 4);
+    p.off_rowmax = take(static_cast<size_t>(n) * 4);
     p.off_again = take(static_cast<size_t>(ceil_div(n, 256)) * 4);
     p.off_kept = take(static_cast<size_t>(p.chunk) * k * 4);
     p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 12);
@@ -850,10 +865,10 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
                                                                       i(p.off_sid), f(p.off_logq), i(p.off_top),
                                                                       f(p.off_mass));
   ORTHRUS_CHECK_LAUNCH();
-  auto* over = reinterpret_cast<unsigned*>(ws + p.off_over);
+  auto* rowmax = reinterpret_cast<unsigned*>(ws + p.off_rowmax);
   ORTHRUS_CHECK_CUDA(launch_pdl(topk_student_kernel, dim3(static_cast<unsigned>(ceil_div(a.n, 8))), dim3(256), 0, stream,
                                 student, W, a.n, a.m, D, a.index, static_cast<const int*>(i(p.off_top)), alpha,
-                                i(p.off_trow), f(p.off_ref), over, i(p.off_again)));
+                                i(p.off_trow), f(p.off_ref), rowmax, i(p.off_again)));
   ORTHRUS_CHECK_LAUNCH();
   CUtensorMap th, tw, te{};
   if (!make_tmap_2d_bf16(&th, student, a.D, a.n, a.D, 64, 128)) return ORTHRUS_ECUDA;
@@ -866,7 +881,8 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   x.alpha = alpha;
   x.trow = i(p.off_trow);
   x.ref = f(p.off_ref);
-  x.over = over;
+  x.top_id = i(p.off_top);
+  x.rowmax = rowmax;
   x.again = i(p.off_again);
   x.sid = i(p.off_sid);
   x.kept = f(p.off_kept);
@@ -894,7 +910,7 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
     ORTHRUS_CHECK_CUDA(launch_pdl(
         topk_finish_kernel, dim3(static_cast<unsigned>(ceil_div(x.rows, 8))), dim3(256), 0, stream,
         static_cast<const float*>(x.part_z), static_cast<const float*>(x.part_m), static_cast<const int*>(x.part_i),
-        2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, static_cast<const unsigned*>(over), x.sid,
+        2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, static_cast<const unsigned*>(rowmax), x.sid,
         static_cast<const float*>(f(p.off_logq)), static_cast<const int*>(i(p.off_top)),
         static_cast<const float*>(f(p.off_mass)), static_cast<const float*>(x.kept), a.row_weight, a.kl_rows, a.agree,
         grad ? e : nullptr, p.Vp, f(p.off_scale)));

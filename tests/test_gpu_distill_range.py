@@ -138,3 +138,25 @@ def test_teacher_ties_at_low_temperatures(dtype, T):
     values, ids = (a["student"].double() @ W.double().T).sort(dim=1, descending=True, stable=True)
     a["values"], a["ids"] = values[:, :4].float(), ids[:, :4].contiguous()
     _check(a, T)
+
+
+@pytest.mark.parametrize("T", [1e-6, 1e-7, 1e-8, 1e-12, 1e-30])
+@pytest.mark.parametrize("near", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_low_temperatures(dtype, near, T):
+    """The lowest temperatures the loss takes, where a logit over T has no fraction left: softmax is one
+    entry or a tie, kl the largest logit's distance over T, everything finite."""
+    a = _rows(300, 700, 64, 5, dtype, seed=4, near=near)
+    a["ids"][7] = -1
+    _, _, grad = _check(a, T)
+    assert (grad[7] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_low_temperatures_beside_large_logits(dtype):
+    """Rows whose largest logit is far above, at, or far below every kept one, in one tile."""
+    a = _rows(300, 700, 64, 5, dtype, seed=5)
+    a["student"][::5] *= 64
+    a["student"][1::5] *= -32
+    for T in (1.0, 1e-3, 1e-9):
+        _check(a, T)
