@@ -16,7 +16,8 @@
 // finished product, and only the k kept entries are rewritten in between. bf16 passes, a chunk of rows
 // at a time:
 //   exp    logits tile in tensor memory (CTA pairs), e in bf16 to the chunk buffer [rows, V],
-//          per-row partial z and maximum, and the fp32 logits at the kept ids picked out of the tile;
+//          per-row partial z, sum of e times its exponent and maximum, and the fp32 logits at the kept
+//          ids picked out of the tile;
 //   finish z, kl, agreement, the kept entries e_j - q_j z / Q (one rounding of the difference, so
 //          the gradient of a student near its teacher is not the difference of rounded numbers),
 //          and the row factor;
@@ -26,6 +27,15 @@
 // logit is the student's) or above (T so low that the roundings of that logit, over T, are many bits)
 // are noticed, and swept again relative to their maximum, subtracted before the division by T, where
 // nothing is lost at any T (whole tiles of 256 rows; that launch ends at once where there are none).
+//
+// The tensor cores' adder cuts where fp32 rounds, so a logit comes out short by a part delta of itself:
+// with normal operands about 8e-10 d, up to 2.3e-9 d for products of one sign, nothing where the sums
+// are exact. A common factor of the logits is to kl what its derivative says,
+//   kl(s (1 + delta)) = kl(s) + delta (Q sum_i p_i s_i - sum_j q_j s_j) / T + O(delta^2),
+// and delta is measured for each row, by least squares over the two logits whose fp32 products are at
+// hand: the teacher's first and the student's largest. Relative error of kl_rows against 64 bits: 6.4e-7 at
+// 1999 x 50257 x 768 (3.7e-6 without; torch's fp32 products 6.1e-7), 2.8e-7 at 512 x 151936 x 1024 (9e-7;
+// 5.3e-7). It costs one more fp32 product per row and one FMA per exponential, 1 % of 512 rows.
 //
 // fp32 rows run on CUDA cores: logits = student @ W^T, a row kernel that turns a row of logits into
 // its kl and the difference (w / T) (Q p - q), and grad = difference @ W.
@@ -310,12 +320,32 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// One warp per student row: its teacher row (-1 if the index is out of range) and its reference
-// c = log2(e) / T * (student . W[top_id]); clears the rows' maxima and the second sweep's flags.
+// The product of two rows of D bf16 numbers in fp32, by a warp; lane 0 has it.
+__device__ __forceinline__ float topk_dot(const __nv_bfloat16* h, const __nv_bfloat16* w, int D) {
+  const uint4* h4 = reinterpret_cast<const uint4*>(h);
+  const uint4* w4 = reinterpret_cast<const uint4*>(w);
+  float dot = 0.f;
+  for (int i = threadIdx.x & 31; i < D / 8; i += 32) {
+    const uint4 a = h4[i], b = w4[i];
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dot = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), dot);
+      dot = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), dot);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  return dot;
+}
+
+// One warp per student row: its teacher row (-1 if the index is out of range) and its logit at the
+// teacher's first id, whose log2(e) / T fold is the reference c; clears the rows' maxima and the second
+// sweep's flags.
 __global__ void __launch_bounds__(256)
     topk_student_kernel(const __nv_bfloat16* __restrict__ student, const __nv_bfloat16* __restrict__ W, int64_t n,
                         int64_t m, int D, const int64_t* __restrict__ index, const int* __restrict__ top_id,
-                        float alpha, int* __restrict__ trow, float* __restrict__ ref, unsigned* __restrict__ rowmax,
+                        int* __restrict__ trow, float* __restrict__ top_logit, unsigned* __restrict__ rowmax,
                         int* __restrict__ again) {
   const int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -328,25 +358,10 @@ __global__ void __launch_bounds__(256)
     t = -1;
   }
   const int id = t < 0 ? -1 : top_id[t];
-  float dot = 0.f;
-  if (id >= 0) {
-    const uint4* h4 = reinterpret_cast<const uint4*>(student + r * D);
-    const uint4* w4 = reinterpret_cast<const uint4*>(W + static_cast<int64_t>(id) * D);
-    for (int i = lane; i < D / 8; i += 32) {
-      const uint4 a = h4[i], b = w4[i];
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dot = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), dot);
-        dot = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), dot);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-  }
+  const float dot = id < 0 ? 0.f : topk_dot(student + r * D, W + static_cast<int64_t>(id) * D, D);
   if (lane == 0) {
     trow[r] = static_cast<int>(t);
-    ref[r] = dot * alpha;
+    top_logit[r] = dot;
     rowmax[r] = 0;
     if (r % 256 == 0) again[r / 256] = 0;
   }
@@ -364,7 +379,8 @@ struct TopkReference {
   float shift, ref;
   __device__ __forceinline__ float operator()(float x, float alpha) const { return fmaf(x - shift, alpha, -ref); }
 };
-__device__ __forceinline__ TopkReference topk_reference(float ref, unsigned max_key, float alpha, bool kept) {
+__device__ __forceinline__ TopkReference topk_reference(float top_logit, unsigned max_key, float alpha, bool kept) {
+  const float ref = top_logit * alpha;
   if (!kept || max_key == 0u) return {0.f, ref};
   const float m = __uint_as_float((max_key & 0x80000000u) ? (max_key & 0x7FFFFFFFu) : ~max_key);
   return fabsf(fmaf(m, alpha, -ref)) > kTopkExpLimit ? TopkReference{m, 0.f} : TopkReference{0.f, ref};
@@ -388,14 +404,15 @@ struct TopkExpArgs {
   int vtiles, tiles_per_split, rtiles, units;
   float alpha;            // log2(e) / T
   const int* trow;        // [n]
-  const float* ref;       // [n]
+  const float* top_logit; // [n]
   const int* sid;         // [m, k]
   const int* top_id;      // [m]
   unsigned* rowmax;       // [n]: topk_max_key of the row's maximum, from the first sweep
   int* again;             // [ceil(n / 256)]: tiles that may hold a row whose reference is too far off
   bool second;            // the second sweep takes the flagged tiles only
   float* kept;            // [chunk, k] student logits at the sorted ids
-  float* part_z;          // [2 splits, chunk], as part_m and part_i
+  float* part_z;          // [2 splits, chunk], as the three below
+  float* part_y;          // sum of e_i times its exponent
   float* part_m;
   int* part_i;
   int64_t part_ld;
@@ -549,7 +566,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
       const bool live = crow < a.rows;
       const int trow = live ? a.trow[a.c0 + crow] : -1;
       const int top = trow < 0 ? -1 : a.top_id[trow];
-      const TopkReference ref = topk_reference(live ? a.ref[a.c0 + crow] : 0.f,
+      const TopkReference ref = topk_reference(live ? a.top_logit[a.c0 + crow] : 0.f,
                                                live && a.second ? a.rowmax[a.c0 + crow] : 0u, a.alpha, top >= 0);
       bool far = false;  // the row's largest logit may be too far from its reference
       // the row's sorted ids from this unit's first column on
@@ -562,7 +579,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
           else hi = mid;
         }
       int next = trow >= 0 && p < a.k ? sid[p] : INT_MAX;
-      float z = 0.f, m = -INFINITY;
+      float z = 0.f, zy = 0.f, m = -INFINITY;
       int idx = INT_MAX;
       for (int t = 0; t < ntiles; ++t, ++tt) {
         const int b = tt & 1;
@@ -625,7 +642,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
             m = cmv[0];
             idx = col0 + civ[0];
           }
-          float zv[4] = {0.f, 0.f, 0.f, 0.f};
+          float zv[4] = {0.f, 0.f, 0.f, 0.f}, yv[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t packed[16];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -633,8 +650,10 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
             y = y > kTopkExpLimit ? kTopkExpLimit : y;  // NaN stays
             x[j] = j < nvalid ? ex2_approx(y) : 0.f;
             zv[j & 3] += x[j];
+            yv[j & 3] = fmaf(x[j], y, yv[j & 3]);
           }
           z += (zv[0] + zv[1]) + (zv[2] + zv[3]);
+          zy += (yv[0] + yv[1]) + (yv[2] + yv[3]);
 #pragma unroll
           for (int j = 0; j < 16; ++j) packed[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
           if (a.write_e) {
@@ -663,6 +682,7 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
       if (live) {
         const int64_t o = static_cast<int64_t>(2 * split + half) * a.part_ld + crow;
         a.part_z[o] = z;
+        a.part_y[o] = zy;
         a.part_m[o] = m;
         a.part_i[o] = idx;
         if (!a.second && top >= 0) {
@@ -684,10 +704,12 @@ __global__ void __launch_bounds__(TopkExpTile::THREADS, 1)
 // One warp per row of the chunk: z and the first maximum from the partials (a fixed order), the row's
 // kl and agreement, the kept entries of the chunk buffer and the row factor of the gradient.
 __global__ void __launch_bounds__(256)
-    topk_finish_kernel(const float* __restrict__ part_z, const float* __restrict__ part_m,
+    topk_finish_kernel(const float* __restrict__ part_z, const float* __restrict__ part_y, const float* __restrict__ part_m,
                        const int* __restrict__ part_i, int parts, int64_t part_ld, int rows, int c0, int k, float alpha,
-                       float T, const int* __restrict__ trow, const float* __restrict__ ref,
-                       const unsigned* __restrict__ rowmax, const int* __restrict__ sid, const float* __restrict__ slogq, const int* __restrict__ top_id,
+                       float T, const __nv_bfloat16* __restrict__ student, const __nv_bfloat16* __restrict__ W, int D,
+                       const int* __restrict__ trow, const float* __restrict__ top_logit,
+                       const unsigned* __restrict__ rowmax, const int* __restrict__ sid,
+                       const float* __restrict__ slogq, const int* __restrict__ top_id,
                        const float* __restrict__ mass, const float* __restrict__ kept,
                        const float* __restrict__ row_weight, float* __restrict__ kl_rows, uint8_t* __restrict__ agree,
                        __nv_bfloat16* __restrict__ e, int64_t lde, float* __restrict__ scale) {
@@ -696,10 +718,11 @@ __global__ void __launch_bounds__(256)
   griddep_wait();  // launched as a programmatic dependent
   if (r >= rows) return;
   const int64_t g = c0 + r;
-  float z = 0.f, m = -INFINITY;
+  float z = 0.f, zy = 0.f, m = -INFINITY;
   int at = INT_MAX;
   for (int s = lane; s < parts; s += 32) {
     z += part_z[s * part_ld + r];
+    zy += part_y[s * part_ld + r];
     const float pm = part_m[s * part_ld + r];
     const int pi = part_i[s * part_ld + r];
     if (pm > m || (pm == m && pi < at)) {
@@ -710,6 +733,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
+    zy += __shfl_xor_sync(0xffffffffu, zy, o);
     const float om = __shfl_xor_sync(0xffffffffu, m, o);
     const int oi = __shfl_xor_sync(0xffffffffu, at, o);
     if (om > m || (om == m && oi < at)) {
@@ -717,31 +741,48 @@ __global__ void __launch_bounds__(256)
       at = oi;
     }
   }
-  const int t = trow[g];
+  const int t = trow[g], top = t >= 0 ? top_id[t] : -1;
   const float Q = t >= 0 ? mass[t] : 0.f;
   const float logz = logf(z);
-  const TopkReference c = topk_reference(ref[g], rowmax[g], alpha, t >= 0 && top_id[t] >= 0);
+  const TopkReference c = topk_reference(top_logit[g], rowmax[g], alpha, top >= 0);
   float kl = 0.f;
-  if (t >= 0 && Q != 0.f) {
+  if (top >= 0 && Q != 0.f) {
     const int* id = sid + static_cast<int64_t>(t) * k;
     const float* lq = slogq + static_cast<int64_t>(t) * k;
+    float qy = 0.f, first = -INFINITY;  // sum of q_j times its exponent; the swept logit at the first id
     for (int j = lane; j < k; j += 32) {
       const int i = id[j];
       if (i == INT_MAX) continue;
-      const float y = c(kept[static_cast<int64_t>(r) * k + j], alpha);
+      const float x = kept[static_cast<int64_t>(r) * k + j], y = c(x, alpha);
+      if (i == top) first = x;
       const float q = expf(lq[j]);
-      if (q != 0.f) kl += q * (lq[j] - (y * kLn2 - logz));
+      if (q != 0.f) {
+        kl += q * (lq[j] - (y * kLn2 - logz));
+        qy += q * y;
+      }
       if (e == nullptr || (j > 0 && id[j - 1] == i)) continue;
       float all = q;  // an id kept twice counts with its whole mass
       for (int o = j + 1; o < k && id[o] == i; ++o) all += expf(lq[o]);
       e[r * lde + i] = __float2bfloat16_rn(ex2_approx(y > kTopkExpLimit ? kTopkExpLimit : y) - (all / Q) * z);
     }
-  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      kl += __shfl_xor_sync(0xffffffffu, kl, o);
+      qy += __shfl_xor_sync(0xffffffffu, qy, o);
+      first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, o));
+    }
+    if (at != INT_MAX) {
+      // what the sweep's sums cut off (see the top of this file): at most a unit of fp32 every 16
+      // products. More is no cut but logits that cancel, or NaN, and says nothing about the others.
+      const float exact = at == top ? top_logit[g] : topk_dot(student + g * D, W + static_cast<int64_t>(at) * D, D);
+      const float delta = ((exact - m) * m + (top_logit[g] - first) * first) / (m * m + first * first);
+      const float add = fabsf(delta) <= static_cast<float>(D) * 0x1p-27f ? delta * kLn2 * (Q * (zy / z) - qy) : 0.f;
+      if (fabsf(add) < INFINITY) kl += add;
+    }
+  }
   if (lane == 0) {
     kl_rows[g] = kl;
-    agree[g] = t >= 0 && top_id[t] >= 0 && top_id[t] == at;
+    agree[g] = top >= 0 && top == at;
     // a row of padding has no reference near its logits, so its z may be 0 (or anything)
     scale[r] = Q == 0.f ? 0.f : (row_weight ? row_weight[g] : 1.f) / T * (Q / z);
   }
@@ -755,7 +796,7 @@ struct TopkKlPlan {
   int64_t chunk, Vp;
   int splits;  // most vocabulary ranges of a chunk's sweep
   size_t off_buf, off_gemm, gemm_bytes;
-  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_ref, off_rowmax, off_again, off_kept, off_part, off_scale;
+  size_t off_sid, off_logq, off_top, off_mass, off_trow, off_logit, off_rowmax, off_again, off_kept, off_part, off_scale;
   size_t total;
 };
 
@@ -783,11 +824,11 @@ inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64
     p.off_top = take(static_cast<size_t>(m) * 4);
     p.off_mass = take(static_cast<size_t>(m) * 4);
     p.off_trow = take(static_cast<size_t>(n) * 4);
-    p.off_ref = take(static_cast<size_t>(n) * 4);
+    p.off_logit = take(static_cast<size_t>(n) * 4);
     p.off_rowmax = take(static_cast<size_t>(n) * 4);
     p.off_again = take(static_cast<size_t>(ceil_div(n, 256)) * 4);
     p.off_kept = take(static_cast<size_t>(p.chunk) * k * 4);
-    p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 12);
+    p.off_part = take(static_cast<size_t>(p.chunk) * 2 * p.splits * 16);
     p.off_scale = take(static_cast<size_t>(p.chunk) * 4);
   } else {
     for (int64_t rows : {std::min(n, p.chunk), n % p.chunk})  // a short last chunk may split deeper
@@ -856,10 +897,7 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   auto* e = reinterpret_cast<__nv_bfloat16*>(ws + p.off_buf);
   auto f = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   auto i = [&](size_t off) { return reinterpret_cast<int*>(ws + off); };
-  // log2(e) / T, and what the tensor cores' adder takes away: it cuts instead of rounding, so a logit
-  // of d products comes out short by about 8.7e-10 d of itself (measured with normal operands: 9.0e-7
-  // at d = 1024, 6.6e-7 at 768, 2.0e-7 at 256). Left in, that is the larger part of the error of kl.
-  const float alpha = static_cast<float>(1.4426950408889634 / a.T * (1.0 + 8.7e-10 * a.D));
+  const float alpha = static_cast<float>(1.4426950408889634 / a.T);
   const int D = static_cast<int>(a.D), V = static_cast<int>(a.V);
   topk_teacher_kernel<<<static_cast<unsigned>(a.m), 128, 0, stream>>>(a.values, a.ids, a.k, V, a.T, a.teacher_lse,
                                                                       i(p.off_sid), f(p.off_logq), i(p.off_top),
@@ -867,8 +905,8 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   ORTHRUS_CHECK_LAUNCH();
   auto* rowmax = reinterpret_cast<unsigned*>(ws + p.off_rowmax);
   ORTHRUS_CHECK_CUDA(launch_pdl(topk_student_kernel, dim3(static_cast<unsigned>(ceil_div(a.n, 8))), dim3(256), 0, stream,
-                                student, W, a.n, a.m, D, a.index, static_cast<const int*>(i(p.off_top)), alpha,
-                                i(p.off_trow), f(p.off_ref), rowmax, i(p.off_again)));
+                                student, W, a.n, a.m, D, a.index, static_cast<const int*>(i(p.off_top)),
+                                i(p.off_trow), f(p.off_logit), rowmax, i(p.off_again)));
   ORTHRUS_CHECK_LAUNCH();
   CUtensorMap th, tw, te{};
   if (!make_tmap_2d_bf16(&th, student, a.D, a.n, a.D, 64, 128)) return ORTHRUS_ECUDA;
@@ -880,7 +918,7 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   x.vtiles = static_cast<int>(ceil_div(a.V, 256));
   x.alpha = alpha;
   x.trow = i(p.off_trow);
-  x.ref = f(p.off_ref);
+  x.top_logit = f(p.off_logit);
   x.top_id = i(p.off_top);
   x.rowmax = rowmax;
   x.again = i(p.off_again);
@@ -888,7 +926,8 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
   x.kept = f(p.off_kept);
   const size_t part = static_cast<size_t>(p.chunk) * 2 * p.splits;
   x.part_z = f(p.off_part);
-  x.part_m = x.part_z + part;
+  x.part_y = x.part_z + part;
+  x.part_m = x.part_y + part;
   x.part_i = reinterpret_cast<int*>(x.part_m + part);
   x.part_ld = p.chunk;
   x.write_e = grad != nullptr;
@@ -909,9 +948,9 @@ inline int topk_kl_rows_bf16(const TopkKlCall& a, const TopkKlPlan& p, const __n
     if (rc != ORTHRUS_OK) return rc;
     ORTHRUS_CHECK_CUDA(launch_pdl(
         topk_finish_kernel, dim3(static_cast<unsigned>(ceil_div(x.rows, 8))), dim3(256), 0, stream,
-        static_cast<const float*>(x.part_z), static_cast<const float*>(x.part_m), static_cast<const int*>(x.part_i),
-        2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, x.trow, x.ref, static_cast<const unsigned*>(rowmax), x.sid,
-        static_cast<const float*>(f(p.off_logq)), static_cast<const int*>(i(p.off_top)),
+        static_cast<const float*>(x.part_z), static_cast<const float*>(x.part_y), static_cast<const float*>(x.part_m),
+        static_cast<const int*>(x.part_i), 2 * splits, x.part_ld, x.rows, x.c0, a.k, alpha, a.T, student, W, D, x.trow,
+        x.top_logit, static_cast<const unsigned*>(rowmax), x.sid, static_cast<const float*>(f(p.off_logq)), x.top_id,
         static_cast<const float*>(f(p.off_mass)), static_cast<const float*>(x.kept), a.row_weight, a.kl_rows, a.agree,
         grad ? e : nullptr, p.Vp, f(p.off_scale)));
     ORTHRUS_CHECK_LAUNCH();

@@ -160,3 +160,54 @@ def test_low_temperatures_beside_large_logits(dtype):
     a["student"][1::5] *= -32
     for T in (1.0, 1e-3, 1e-9):
         _check(a, T)
+
+
+@pytest.mark.parametrize("kind", ["one", "integers", "positive"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [256, 1024, 8192])
+def test_operands_of_any_distribution(dtype, d, kind):
+    """Logits of one product, of many small integers, and of one sign: the sums are exact, so kl is right
+    to its own roundings at any width."""
+    g = torch.Generator().manual_seed(d)
+    n, V, k = 200, 600, 4
+    W = torch.randint(-4, 5, (V, d), generator=g).float()
+    h = torch.zeros(n, d)
+    if kind == "integers":
+        h = torch.randint(-1, 2, (n, d), generator=g).float() * (torch.rand(n, d, generator=g) < 64 / d)
+    elif kind == "positive":
+        W, h = W.abs(), (torch.rand(n, d, generator=g) < 32 / d).float()
+    else:
+        h.scatter_(1, torch.randint(0, d, (n, 1), generator=g), 16.0)
+    ids = torch.randint(0, V, (n, k), generator=g)
+    a = dict(student=h.to(DEV, dtype), values=torch.randint(0, 3, (n, k), generator=g).float().to(DEV), ids=ids.to(DEV),
+             index=None, weight=W.to(DEV, dtype), row_weight=torch.ones(n, device=DEV))
+    _check(a, 1.0)
+
+
+@pytest.mark.parametrize("d", [64, 768, 1024, 4096])
+@pytest.mark.parametrize("kind", ["normal", "positive", "same"])
+def test_kl_of_sums_that_are_cut(kind, d):
+    """The tensor cores' adder cuts where fp32 rounds: every 16 products up to a unit of the partial sum, half
+    of one on average, which is d / 32 units of a logit whose partial sums grow evenly to it, halved for
+    their growth. The loss measures and puts back what was cut: in sum over the rows it is off by no more
+    than a quarter of the like."""
+    from orthrus_training_b200 import ops
+
+    g = torch.Generator().manual_seed(d)
+    n, V, k = 512, 5003, 32
+    W, t = torch.randn(V, d, generator=g) * 3 / math.sqrt(d), torch.randn(n, d, generator=g)
+    h = t if kind == "same" else 0.6 * t + 0.4 * torch.randn(n, d, generator=g)
+    if kind == "positive":
+        W, t, h = W.abs(), t.abs(), h.abs()
+    W, t, h = W.to(DEV).bfloat16(), t.to(DEV).bfloat16(), h.to(DEV).bfloat16()
+    values, ids = (t.double() @ W.double().T).topk(k)
+    values = values.float()
+    kl = ops.lmhead_topk_kl(h, values, ids, None, W, need_grad=False)[1].double()
+    lq, s = values.double().log_softmax(1), h.double() @ W.double().T
+    q, p = lq.exp(), s.softmax(1)
+    want = (q * (lq - s.log_softmax(1).gather(1, ids))).sum(1)
+    slope = (p * s).sum(1) - (q * s.gather(1, ids)).sum(1)  # of kl by a common part of the logits
+    # roundings of kl itself, of either sign: log q, the exponents, log z, the sums (see the top)
+    noise = (8 * U * (q * lq.abs()).sum(1) + 8 * U * (q * s.log_softmax(1).gather(1, ids).abs()).sum(1) + 2.0 ** -22).sum()
+    noise = noise / math.sqrt(n)
+    assert (kl - want).sum().abs() <= d / 64 * 2 * U / 4 * slope.abs().sum() + noise
