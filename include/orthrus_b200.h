@@ -510,11 +510,15 @@ int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int
  * first always); and of these the ones with w_i >= min_p. The token is the first kept index at
  * which the running sum of kept weights, in index order, exceeds uniform * total. A uniform below 0
  * or NaN counts as 0, one of 1 or more picks the last kept token of positive weight. A temperature
- * below 1e-5 or NaN gives the row's first maximum; a row without candidates gives -1. Sums are of
- * integer weights of at least 42 fractional bits, so they do not depend on their order; a row's
- * slices are brought to one maximum in fp64, so a token can depend on how the call is launched
- * only where the uniform, or top_p, falls within about 2^-40 of a border. Each knob is a device array [R], or NULL and the value beside it for every row. The workspace
- * is asked for with `filters` = 1 when top_p or min_p can filter a row whose top_k is off or above 1024
+ * below 1e-5 or NaN gives the row's first maximum; a row without candidates gives -1. Weights are
+ * rounded to multiples of 2^-S of the largest, S = min(44, 62 - ceil(log2 V)), and summed as integers,
+ * so sums do not depend on their order. Up to V roundings of half a unit, and the fp64 that brings a
+ * slice of the row from its own maximum to the row's, move a border by at most V 2^-(S+1) + 2^-42 of
+ * the total (2^-27.8 at V = 151936, 2^-23 at V = 2^20; about sqrt(V / 12) 2^-S where the roundings are
+ * of either sign): only a uniform or a top_p that near to one, or a min_p within 2^-S of a
+ * weight, can give another token than the definition, or than the same row in another batch, whose
+ * slices may be of another size. Each knob is a device array [R], or NULL and the value beside it for
+ * every row. The workspace is asked for with `filters` = 1 when top_p or min_p can filter a row whose top_k is off or above 1024
  * (either array given, or top_p1 < 1 or min_p1 > 0; top_k given, or top_k1 < 1 or > 1024): rows that
  * keep thousands of entries need about V bytes each, for up to 2048 of them. */
 size_t orthrus_sample_logits_workspace_bytes(int64_t R, int64_t V, int filters, int dtype);

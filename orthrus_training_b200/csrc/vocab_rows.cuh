@@ -268,9 +268,10 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& to
 // ------------------------------------------------------------------------------------------------
 
 // w(x) = round(2^S exp((x - top) / T)). Integer weights make sums exact, so running sums do not
-// depend on how a slice is split over threads. (Slices whose maximum is below the row's are brought down
-// in fp64, the one rounding that depends on where slices end.) S = min(44, 62 - ceil(log2 V)) keeps a
-// row's sum below 2^62; a weight is off by at most half a unit plus 2^-44 of itself.
+// depend on how a slice is split over threads. S = min(44, 62 - ceil(log2 V)) keeps a row's sum below
+// 2^62; a weight is off by at most half a unit plus 2^-44 of itself, V of them by V / 2 units of a total
+// of 2^S or more. What depends on where slices end: the scan weighs a slice against its own maximum,
+// so that its units are finer than the row's, and brings its sum down in fp64.
 //
 // The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f = 1 + f q(f) with q of degree
 // 8 through the Chebyshev nodes of [-1/2, 1/2] (error below 4e-14), 2^(S - n) by the exponent. A table

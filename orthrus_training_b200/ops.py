@@ -833,9 +833,15 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     top_p the smallest descending prefix whose probability exceeds it (1: off); min_p the entries
     at least min_p times as probable as the largest (0: off). Each knob is a number or a tensor [R].
     A temperature of 0 (below 1e-5) is greedy. -inf and NaN logits are never drawn; a row of
-    nothing else gives -1. Weights and sums have 42 or more fractional bits and no order that
-    changes them: a row's token can depend on the other rows or the launch only where its uniform, or
-    top_p, falls within about 2^-40 of a border."""
+    nothing else gives -1. Weights are rounded to multiples of 2^-S of the largest, S = min(44, 62 -
+    ceil(log2 V)), and summed exactly, so no order changes a sum. The token is the 64-bit
+    definition's, and the same for the row in any other batch, unless the uniform or top_p falls
+    within V 2^-(S+1) + 2^-42 of a border (2^-27.8 at V = 151936, 2^-23 at V = 2^20: the case of
+    a peak over entries that all round to nothing; roundings of either sign come to about
+    sqrt(V / 12) 2^-S, 2^-37 and 2^-34), or min_p within 2^-S of a weight. Nuclei (top_p) and
+    min_p without a top_k up to 1024 take a workspace of about V bytes a row, for up to 2048 rows
+    (311 MB at V = 151936), and the rows past the first 2048 that keep thousands of entries are
+    gone over one by one, several times slower; so are rows with a top_k above 1024."""
     R, V, pitch = _vocab_rows(logits, "sample_logits")
     code, dev = L.dtype_code(logits.dtype), logits.device
     if uniforms.shape != (R,) or uniforms.dtype != torch.float32 or uniforms.device != dev:
