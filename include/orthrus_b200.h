@@ -518,9 +518,9 @@ int orthrus_topk_rows(const void* logits, int64_t ldl, int64_t R, int64_t V, int
  * of either sign): only a uniform or a top_p that near to one, or a min_p within 2^-S of a
  * weight, can give another token than the definition, or than the same row in another batch, whose
  * slices may be of another size. Each knob is a device array [R], or NULL and the value beside it for
- * every row. The workspace is asked for with `filters` = 1 when top_p or min_p can filter a row whose top_k is off or above 1024
- * (either array given, or top_p1 < 1 or min_p1 > 0; top_k given, or top_k1 < 1 or > 1024): rows that
- * keep thousands of entries need about V bytes each, for up to 2048 of them. */
+ * every row. The workspace is asked for with `filters` = 1 when top_p or min_p can filter a row whose
+ * top_k is off or above 1024 (either array given, or top_p1 < 1 or min_p1 > 0; top_k given, or top_k1 < 1
+ * or > 1024): rows that keep thousands of entries need about V bytes each, for up to 2048 of them. */
 size_t orthrus_sample_logits_workspace_bytes(int64_t R, int64_t V, int filters, int dtype);
 int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R, int64_t V, const float* uniform,
                           const float* temperature, float temperature1, const int32_t* top_k,

@@ -65,6 +65,9 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, b_kn: bool = False, out_dtype=None
          out: torch.Tensor | None = None) -> torch.Tensor:
     """a [M, K] @ (b [N, K])^T (or a @ b for b [K, N] with b_kn). bf16 inputs run on tcgen05 tensor
     cores, fp32 inputs on the exact CUDA-core kernel; fp32 accumulation either way."""
+    if a.dtype != b.dtype or a.device != b.device:
+        raise ValueError(f"gemm takes operands of one dtype on one device; got {a.dtype} on {a.device} and "
+                         f"{b.dtype} on {b.device}")
     _require_cuda(a, b)
     if a.dim() != 2 or b.dim() != 2 or a.stride(1) != 1 or b.stride(1) != 1:
         raise ValueError("gemm takes row-major 2-D operands")
@@ -72,6 +75,9 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, b_kn: bool = False, out_dtype=None
     N = b.shape[1] if b_kn else b.shape[0]
     if (b.shape[0] if b_kn else b.shape[1]) != K:
         raise ValueError(f"gemm shape mismatch {tuple(a.shape)} x {tuple(b.shape)}")
+    if out is not None and (out.shape != (M, N) or out.stride(1) != 1 or out.device != a.device or
+                            out.dtype not in (a.dtype, torch.float32)):
+        raise ValueError(f"gemm writes a row-major [{M}, {N}] of {a.dtype} or float32 on {a.device}")
     lib = L.lib()
     stream = L.stream_of(a.device)
     if a.dtype == torch.bfloat16 and b.dtype == torch.bfloat16:
