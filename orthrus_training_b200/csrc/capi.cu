@@ -959,6 +959,8 @@ extern "C" int orthrus_sample_logits(const void* logits, int64_t ldl, int64_t R,
 
 extern "C" size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,
                                                          int64_t chunk_rows, int dtype) {
+  // what the entry refuses needs none (and has no plan: its tiles may be 0)
+  if (!topk_kl_sizes_ok(n, m, V, d, k) || (dtype != ORTHRUS_BF16 && dtype != ORTHRUS_F32)) return 0;
   return topk_kl_plan(n, m, V, d, k, chunk_rows, dtype).total;
 }
 

@@ -800,6 +800,11 @@ struct TopkKlPlan {
   size_t total;
 };
 
+inline bool topk_kl_sizes_ok(int64_t n, int64_t m, int64_t V, int64_t D, int64_t k) {
+  return n >= 0 && m >= 0 && V >= 1 && D >= 1 && k >= 1 && k <= kTopkKlMaxK && n < (1ll << 31) && m < (1ll << 31) &&
+         V < (1ll << 31) - 256 && D < (1ll << 30);
+}
+
 // The chunk buffer holds fp32 logits (fp32 rows) or bf16 exponentials of p.chunk rows.
 inline TopkKlPlan topk_kl_plan(int64_t n, int64_t m, int64_t V, int64_t D, int64_t k, int64_t chunk_rows, int dtype) {
   TopkKlPlan p{};
@@ -967,9 +972,8 @@ int lmhead_topk_kl_fwd_impl(const E* student, const E* weight, const TopkKlCall&
                             int num_offsets, float* total, E* grad, float* kl_by_offset, int64_t* agree_by_offset,
                             int64_t chunk_rows, void* ws_raw, size_t ws_bytes, cudaStream_t stream) {
   constexpr bool kBf16 = sizeof(E) == 2;
-  ORTHRUS_CHECK_ARG(a.n >= 0 && a.m >= 0 && a.V >= 1 && a.D >= 1 && a.k >= 1 && a.k <= kTopkKlMaxK);
+  ORTHRUS_CHECK_ARG(topk_kl_sizes_ok(a.n, a.m, a.V, a.D, a.k));
   ORTHRUS_CHECK_ARG(a.T >= 1e-30f && a.T <= 1e30f);
-  ORTHRUS_CHECK_ARG(a.n < (1ll << 31) && a.m < (1ll << 31) && a.V < (1ll << 31) - 256 && a.D < (1ll << 30));
   ORTHRUS_CHECK_ARG(weight && total);
   ORTHRUS_CHECK_ARG(a.n == 0 || (student && a.values && a.ids && a.kl_rows && a.agree && a.m >= 1));
   ORTHRUS_CHECK_ARG(a.index != nullptr || a.n <= a.m);

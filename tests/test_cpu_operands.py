@@ -1,5 +1,8 @@
 """Operands that a kernel would read or write out of range are refused before anything is launched (no GPU)."""
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -19,3 +22,20 @@ def test_gemm_refuses_operands_of_two_devices():
 
     with pytest.raises(ValueError, match="one dtype on one device"):
         ops.gemm(torch.zeros(4, 8), torch.zeros(6, 8, device="meta"))
+
+
+def test_distillation_workspace_of_refused_sizes():
+    """Sizes that the distillation refuses need no workspace; asking for it does not end the process (in one
+    of its own, which a division by no tiles would end)."""
+    from orthrus_training_b200 import _lib as L
+
+    calls = []
+    for bad in (dict(V=0), dict(d=0), dict(V=-7), dict(d=-1), dict(n=-1), dict(m=-1), dict(k=0), dict(k=1025),
+                dict(n=2 ** 31), dict(V=2 ** 31), dict(dtype=7)):
+        for dtype in (L.F32, L.BF16):
+            a = dict(dict(n=4, m=4, V=10, d=8, k=2, chunk=4096, dtype=dtype), **bad)
+            calls.append(tuple(a.values()))
+    code = ("from orthrus_training_b200 import _lib as L\n"
+            f"print([L.lib().orthrus_lmhead_topk_kl_workspace_bytes(*c) for c in {calls}])")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == str([0] * len(calls)), (run.returncode, run.stdout, run.stderr[-500:])

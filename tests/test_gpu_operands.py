@@ -20,3 +20,14 @@ def test_gemm_refusals():
                 torch.zeros(4, 24, device=DEV, dtype=torch.bfloat16), torch.zeros(4, 24)):
         with pytest.raises(ValueError, match="writes a row-major"):
             ops.gemm(h, W, out=out)
+
+
+def test_distillation_refuses_an_empty_head():
+    from orthrus_training_b200 import ops
+
+    for dtype in (torch.float32, torch.bfloat16):
+        h, v, i = torch.zeros(4, 8, device=DEV, dtype=dtype), torch.zeros(4, 2, device=DEV), torch.zeros(4, 2, device=DEV).long()
+        with pytest.raises(ValueError):
+            ops.lmhead_topk_kl(h, v, i, None, torch.zeros(0, 8, device=DEV, dtype=dtype))
+        with pytest.raises(ValueError):
+            ops.lmhead_topk_kl(h[:, :0], v, i, None, torch.zeros(6, 0, device=DEV, dtype=dtype))
