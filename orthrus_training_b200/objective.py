@@ -609,7 +609,7 @@ def teacher_top_logits(hidden: torch.Tensor, weight: torch.Tensor, k: int, tempe
     ids = torch.empty(m, k, dtype=torch.int64, device=hidden.device)
     lse = torch.empty(m, dtype=torch.float32, device=hidden.device)
     pad = (-hidden.shape[1]) % 8
-    hidden, weight = (F.pad(t, (0, pad)) if pad else t.contiguous() for t in (hidden, weight))
+    hidden, weight = (ops._kernel_operand(t, pad) for t in (hidden, weight))
     rows = min(max(int(chunk_rows), 1), max(m, 1))
     logits = torch.empty(rows, V + (-V) % 8, dtype=torch.float32, device=hidden.device)[:, :V]
     with torch.cuda.device(hidden.device):

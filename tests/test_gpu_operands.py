@@ -31,3 +31,19 @@ def test_distillation_refuses_an_empty_head():
             ops.lmhead_topk_kl(h, v, i, None, torch.zeros(0, 8, device=DEV, dtype=dtype))
         with pytest.raises(ValueError):
             ops.lmhead_topk_kl(h[:, :0], v, i, None, torch.zeros(6, 0, device=DEV, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 33])
+def test_teacher_top_logits_of_views(dtype, d):
+    """Rows and an LM head that start off a 16-byte boundary, or are strided, give what their copies give."""
+    from orthrus_training_b200 import objective
+
+    g = torch.Generator().manual_seed(d)
+    flat = torch.randn(70 * d + 3, generator=g).to(DEV, dtype)
+    wide = torch.randn(200, d + 5, generator=g).to(DEV, dtype)
+    head = torch.randn(200 * d + 1, generator=g).to(DEV, dtype)
+    for h, W in ((flat[3:].view(70, d), wide[:, 2 : d + 2]), (wide[::3, 1 : d + 1], head[1:].view(200, d))):
+        got = objective.teacher_top_logits(h, W, 9, chunk_rows=32)
+        want = objective.teacher_top_logits(h.clone().contiguous(), W.clone().contiguous(), 9, chunk_rows=32)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
