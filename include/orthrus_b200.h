@@ -374,8 +374,9 @@ int orthrus_lmhead_kl_bwd(const void* grad, const float* grad_total, void* grad_
  * kept twice counts with its whole mass. student [n, d], weight [V, d], grad [n, d] (NULL: not
  * computed) in dtype, bf16 with d a multiple of 8 and 16-byte alignment; values, teacher_lse and
  * row_weight fp32, ids and index int64; row_weight, teacher_lse and offsets may be NULL. total and
- * the per-offset sums as orthrus_lmhead_kl_fwd. temperature from 1e-30 to 1e30. The probabilities of
- * chunk_rows rows at a time live in the workspace. orthrus_lmhead_kl_bwd scales grad by the gradient of total. */
+ * the per-offset sums as orthrus_lmhead_kl_fwd. temperature from 1e-30 to 1e30; n, V and d at most 2^30
+ * (ORTHRUS_EINVAL beyond, and a workspace of 0 bytes). The probabilities of chunk_rows rows at a time
+ * live in the workspace. orthrus_lmhead_kl_bwd scales grad by the gradient of total. */
 size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,
                                               int64_t chunk_rows, int dtype);
 int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values,

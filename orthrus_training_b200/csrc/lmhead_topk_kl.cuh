@@ -800,9 +800,10 @@ struct TopkKlPlan {
   size_t total;
 };
 
+// n, V and d up to 2^30: loops step past them in 32 bits.
 inline bool topk_kl_sizes_ok(int64_t n, int64_t m, int64_t V, int64_t D, int64_t k) {
-  return n >= 0 && m >= 0 && V >= 1 && D >= 1 && k >= 1 && k <= kTopkKlMaxK && n < (1ll << 31) && m < (1ll << 31) &&
-         V < (1ll << 31) - 256 && D < (1ll << 30);
+  return n >= 0 && m >= 0 && V >= 1 && D >= 1 && k >= 1 && k <= kTopkKlMaxK && n <= (1ll << 30) && m < (1ll << 31) &&
+         V <= (1ll << 30) && D <= (1ll << 30);
 }
 
 // The chunk buffer holds fp32 logits (fp32 rows) or bf16 exponentials of p.chunk rows.

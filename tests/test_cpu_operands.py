@@ -39,3 +39,18 @@ def test_distillation_workspace_of_refused_sizes():
             f"print([L.lib().orthrus_lmhead_topk_kl_workspace_bytes(*c) for c in {calls}])")
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip() == str([0] * len(calls)), (run.returncode, run.stdout, run.stderr[-500:])
+
+
+@pytest.mark.parametrize("size", ["n", "V", "d"])
+@pytest.mark.parametrize("dtype", ["F32", "BF16"])
+def test_distillation_refuses_sizes_past_its_loops(size, dtype):
+    """Loops over rows, entries and columns step past their end in 32 bits: near 2^31 they would wrap around."""
+    import ctypes
+
+    from orthrus_training_b200 import _lib as L
+
+    a = dict(dict(n=4, V=10, d=8), **{size: 2 ** 31 - 512})
+    got = L.lib().orthrus_lmhead_topk_kl_fwd(64, a["n"], 64, 64, 2 ** 31 - 1, 2, 64, None, 64, a["V"], a["d"], ctypes.c_float(1.0),
+                                             None, None, 0, 64, 64, 64, 64, None, None, 128, 64, 1 << 62, getattr(L, dtype),
+                                             None)
+    assert got == L.EINVAL
