@@ -982,6 +982,7 @@ int lmhead_topk_kl_fwd_impl(const E* student, const E* weight, const TopkKlCall&
   if (kBf16) ORTHRUS_CHECK_ARG(a.D % 8 == 0 && aligned16(student) && aligned16(weight) && (!grad || aligned16(grad)));
   const TopkKlPlan p = topk_kl_plan(a.n, a.m, a.V, a.D, a.k, chunk_rows, kBf16 ? ORTHRUS_BF16 : ORTHRUS_F32);
   if (ws_raw == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
+  ORTHRUS_CHECK_ARG(aligned16(ws_raw));
   if (a.n == 0) {
     ORTHRUS_CHECK_CUDA(cudaMemsetAsync(total, 0, sizeof(float), stream));
     if (kl_by_offset && agree_by_offset) {  // an empty offsets array may be NULL

@@ -1785,6 +1785,7 @@ inline int row_prepare(const T* x, int64_t ldx, int64_t R, int64_t V, bool sampl
   p = row_plan(R, V, sizeof(T), aligned16(x) && (ldx * sizeof(T)) % 16 == 0, sample, wide);
   ORTHRUS_CHECK_ARG(R * p.slices < (1ll << 31) && (reinterpret_cast<uintptr_t>(x) & (sizeof(T) - 1)) == 0);
   if (ws == nullptr || ws_bytes < p.total) return ORTHRUS_EWORKSPACE;
+  ORTHRUS_CHECK_ARG(aligned16(ws));
   uint8_t* w = static_cast<uint8_t*>(ws);
   scan = {reinterpret_cast<uint32_t*>(w), reinterpret_cast<RowSlice*>(w + p.off_slice), p.groups, p.slices,
           wide ? reinterpret_cast<uint32_t*>(w + p.off_count) : nullptr};

@@ -54,3 +54,18 @@ def test_distillation_refuses_sizes_past_its_loops(size, dtype):
                                              None, None, 0, 64, 64, 64, 64, None, None, 128, 64, 1 << 62, getattr(L, dtype),
                                              None)
     assert got == L.EINVAL
+
+
+@pytest.mark.parametrize("at", [65, 66, 68, 72])
+@pytest.mark.parametrize("dtype", ["F32", "BF16"])
+def test_workspaces_off_their_boundary(dtype, at):
+    import ctypes
+
+    from orthrus_training_b200 import _lib as L
+
+    lib, f, code = L.lib(), ctypes.c_float, getattr(L, dtype)
+    assert lib.orthrus_topk_rows(64, 8, 2, 8, 2, f(1), 64, 64, 64, at, 1 << 50, code, None) == L.EINVAL
+    assert lib.orthrus_sample_logits(64, 8, 2, 8, 64, None, f(1), None, 0, None, f(1), None, f(0), 64, at, 1 << 50, code,
+                                     None) == L.EINVAL
+    assert lib.orthrus_lmhead_topk_kl_fwd(64, 4, 64, 64, 4, 2, 64, None, 64, 10, 8, f(1), None, None, 0, 64, 64, 64, 64, None,
+                                          None, 128, at, 1 << 50, code, None) == L.EINVAL
