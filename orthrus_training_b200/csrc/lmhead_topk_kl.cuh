@@ -153,13 +153,12 @@ __device__ inline float tk_load_teacher(const float* __restrict__ values, const 
 }
 
 // One CTA per row of a chunk: logits [rows, ld] fp32 of student rows c0.. -> kl_rows, agree and, with
-// `diff`, the difference (w / T) (Q p - q) in T's type (which may overwrite the logits).
-template <typename D>
+// `diff`, the difference (w / T) (Q p - q) (which may overwrite the logits).
 __global__ void __launch_bounds__(kTopkKlThreads)
     topk_kl_rows_kernel(const float* logits, int64_t ld, int c0, int V, const float* __restrict__ values,
                         const int64_t* __restrict__ ids, int k, int64_t m, const int64_t* __restrict__ index,
                         const float* __restrict__ teacher_lse, const float* __restrict__ row_weight, float T,
-                        float* __restrict__ kl_rows, uint8_t* __restrict__ agree, D* diff, int64_t ldd) {
+                        float* __restrict__ kl_rows, uint8_t* __restrict__ agree, float* diff, int64_t ldd) {
   __shared__ TopkTeacherRow sh;
   const int64_t r = c0 + static_cast<int64_t>(blockIdx.x);
   const float* x = logits + blockIdx.x * ld;
@@ -188,9 +187,9 @@ __global__ void __launch_bounds__(kTopkKlThreads)
   if (diff == nullptr) return;
   // the kept entries' differences first (they read the logits), then the sweep, then their stores
   const float w = (row_weight ? row_weight[r] : 1.f) / T;
-  D* d = diff + blockIdx.x * ldd;
+  float* d = diff + blockIdx.x * ldd;
   if (w * Q == 0.f) {  // no mass or no weight: 0 whatever the row holds (the sum above is past its last reads)
-    for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = from_f32<D>(0.f);
+    for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = 0.f;
     return;
   }
   constexpr int PER = kTopkKlMaxK / kTopkKlThreads;
@@ -205,12 +204,12 @@ __global__ void __launch_bounds__(kTopkKlThreads)
   }
   __syncthreads();
   const float scale = w * Q / z;
-  for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = from_f32<D>(scale * expf((x[i] - top) / T));
+  for (int i = threadIdx.x; i < V; i += kTopkKlThreads) d[i] = scale * expf((x[i] - top) / T);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int j = threadIdx.x + u * kTopkKlThreads;
-    if (j < k && sh.id[j] >= 0) d[sh.id[j]] = from_f32<D>(fix[u]);
+    if (j < k && sh.id[j] >= 0) d[sh.id[j]] = fix[u];
   }
 }
 
@@ -865,7 +864,7 @@ inline int topk_kl_rows_f32(const TopkKlCall& a, const TopkKlPlan& p, const floa
     const int64_t rows = std::min<int64_t>(p.chunk, a.n - c0);
     int rc = f32_product<false>(student + c0 * a.D, a.D, W, a.D, buf, p.Vp, rows, a.V, a.D, gws, p.gemm_bytes, stream);
     if (rc != ORTHRUS_OK) return rc;
-    topk_kl_rows_kernel<float><<<static_cast<unsigned>(rows), kTopkKlThreads, 0, stream>>>(
+    topk_kl_rows_kernel<<<static_cast<unsigned>(rows), kTopkKlThreads, 0, stream>>>(
         buf, p.Vp, static_cast<int>(c0), static_cast<int>(a.V), a.values, a.ids, a.k, a.m, a.index, a.teacher_lse,
         a.row_weight, a.T, a.kl_rows, a.agree, grad ? buf : nullptr, p.Vp);
     ORTHRUS_CHECK_LAUNCH();
