@@ -13,8 +13,12 @@
 // Sampled rows that keep more than fits a CTA's shared memory (wide rows: nuclei of thousands of entries)
 // get more launches: a scan that bins their weights and so finds a narrow window of values with the
 // nucleus' border, one that sums what lies above the window and lists what lies in it, and a pick. Where
-// even that does not do (rows of equal values), a CTA goes over the whole row again: a radix selection
-// that is right for every row, and a walk in index order.
+// even that does not do, a CTA goes over the whole row again: a radix selection that is right for every
+// row, and a walk in index order. Those are rows of many equal values, wide rows past the first 2048 of a
+// call (50257 entries, top-p 0.95 at T = 1.5: 2048 rows 750 us, 2100 rows 1113), a top-k above 1024, and
+// rows with more than 2048 candidates in fewer than k groups, which give no bound: k = 300 with V from
+// 2049 to 9600, k = 1024 to 32768, a nucleus (k = 256) to 8192, longer rows whose candidates stand
+// together (256 rows fp32: top-300 at V = 8000 80 us, at 12000 43; top-p 0.9 at V = 8000 125, at 9000 99).
 //
 // What bounds it, and what it measured (us; V = 151936 where not given; floor: each logit read once at
 // 6540 GB/s):
@@ -24,9 +28,9 @@
 //   top-8, 2 x 1024; top-64, 32 rows  18, 18: the call's host time (7 and 18 on the device)
 //   plain sampling, 1 row             16: the call's host time (10 on the device)
 //   top-p 0.95, 256 rows fp32        247 (24), every row wide: scan 69, finish 38, bins 43, window 6, sums 50,
-//                                    pick 25. The scan is bound by the instructions of the integer
-//                                    weights (45 an entry, 15 of them fp64 at half rate), the bins
-//                                    and sums by those of passing over the entries (26 each)
+//                                    pick 25. The scan is bound by instructions, 42 an entry, 15 of them
+//                                    fp64 at half rate for the integer weight, the bins and sums by
+//                                    those of passing over the entries (28 and 31)
 //   mixed filters, 1024 rows bf16    258 (48): scan 96, finish 54, wide rows the rest
 //   min-p 0.05, 77 x 32003 fp32       23 (1.5): latency of two dependent launches
 // One CTA per row for all of it (a cluster, or a CTA going over its row again) took 576 us for the first,
@@ -276,8 +280,7 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, uint64_t& to
 // The exponential: y = (top - x) log2(e) / T = n - f with |f| <= 1/2, 2^f = 1 + f q(f) with q of degree
 // 8 through the Chebyshev nodes of [-1/2, 1/2] (error below 4e-14), 2^(S - n) by the exponent. A table
 // would save some of the fp64 products, but its lookups, of random banks, take longer. No branch, and
-// what can be is left to fp32: the loops over rows are bound by the instructions that they issue, some
-// 30 an entry here.
+// what can be is left to fp32: the loops over rows are bound by the instructions that they issue.
 __constant__ double kRowExp2[9] = {6.931471805599453e-01,  2.402265069581299e-01,  5.5504108664760424e-02,
                                    9.618129159402558e-03,  1.3333558179043112e-03, 1.5403455852453838e-04,
                                    1.525268684626772e-05,  1.3255224878668817e-06, 1.0203121063391729e-07};
