@@ -376,7 +376,8 @@ int orthrus_lmhead_kl_bwd(const void* grad, const float* grad_total, void* grad_
  * row_weight fp32, ids and index int64; row_weight, teacher_lse and offsets may be NULL. total and
  * the per-offset sums as orthrus_lmhead_kl_fwd. temperature from 1e-30 to 1e30; n, V and d at most 2^30
  * (ORTHRUS_EINVAL beyond, and a workspace of 0 bytes). The probabilities of chunk_rows rows at a time
- * live in the workspace, which starts on a 16-byte boundary. orthrus_lmhead_kl_bwd scales grad by the gradient of total. */
+ * live in the workspace, which starts on a 16-byte boundary. orthrus_lmhead_kl_bwd scales grad by the
+ * gradient of total. */
 size_t orthrus_lmhead_topk_kl_workspace_bytes(int64_t n, int64_t m, int64_t V, int64_t d, int k,
                                               int64_t chunk_rows, int dtype);
 int orthrus_lmhead_topk_kl_fwd(const void* student, int64_t n, const float* values,

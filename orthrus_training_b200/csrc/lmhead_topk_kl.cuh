@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// The product of two rows of D bf16 numbers in fp32, by a warp; lane 0 has it.
+// The product of two rows of D bf16 numbers in fp32, by a warp; every lane has it.
 __device__ __forceinline__ float topk_dot(const __nv_bfloat16* h, const __nv_bfloat16* w, int D) {
   const uint4* h4 = reinterpret_cast<const uint4*>(h);
   const uint4* w4 = reinterpret_cast<const uint4*>(w);
